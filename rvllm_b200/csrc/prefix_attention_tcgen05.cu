@@ -1,0 +1,409 @@
+// Attention of a step's one-token sequences over the cached tokens that groups of them share (bfloat16): the keys of a
+// group's prefix are read once for all of its sequences, on the fifth-generation tensor cores.
+//
+// The queries of a group for one key/value head are n G rows (n sequences, G = nh / nkv heads) against the same P keys:
+//   S = scale Q K^T [n G x P],   m = max_j S,   l = sum_j e^(S - m),   O = e^(S - m) V
+// a matrix product of the size of a prompt's attention, without a triangle.  A CTA owns up to 128 rows (floor(128 / G)
+// whole sequences) of one kv head and one range of the keys and leaves (O, m, l) unnormalised; the kernel that has the keys
+// behind the prefix leaves the same, and shared_prefix.cu merges them.  Which rows and ranges there are is a list that the
+// host makes once for a set of sequences (they change when a request comes or goes, not from step to step).
+//
+// Inside a CTA: S = Q K^T of 64 keys into one of two buffers of tensor memory, one thread per row of softmax, P written back
+// over S as bfloat16 pairs and read from there as the A operand of O += P V; two loader warps (keys, values: TMA boxes
+// through the block table) and two warps that issue, as in attention_tcgen05.cu, which has the measurements behind this cut.
+// What differs: rows come from sequences that lie anywhere in the batch (fetched by plain loads and swizzled by hand), keys
+// behind the end of a prefix inside its last page belong to somebody else (their values are set to zero, so that a NaN there
+// does not meet a probability of zero), and warps whose rows are all empty skip the softmax.
+// P is rounded to bfloat16 (2^-9 relative), as both attention kernels of this library do: the tensor core takes no wider A
+// beside a bfloat16 V; sums and maxima are float.
+// Cache layer layout: [num_pages, 2 (k, v), nkv, page_size, HEAD_DIM].
+#include "common.cuh"
+#include "shared_prefix.cuh"
+#include "tcgen05_attention.cuh"
+
+#ifndef HEAD_DIM
+#define HEAD_DIM 128
+#endif
+static_assert(HEAD_DIM == 64 || HEAD_DIM == 128, "this kernel is built for head sizes 64 and 128");
+
+#define ROWS SP_ROWS
+#define KV_TILE 64
+#define SOFTMAX_WARPS 4
+#define LOADER_WARP SOFTMAX_WARPS               // the keys (and the tensor memory's allocation)
+#define VLOADER_WARP (SOFTMAX_WARPS + 1)        // the values
+#define QK_WARP (SOFTMAX_WARPS + 2)             // issues S = Q K^T
+#define PV_WARP (SOFTMAX_WARPS + 3)             // issues O += P V
+#define HALVES (HEAD_DIM / 64)
+#define Q_BYTES (ROWS * HEAD_DIM * 2)
+#define TILE_BYTES (KV_TILE * HEAD_DIM * 2)
+#define NUM_THREADS (32 * (SOFTMAX_WARPS + 4))
+// two CTAs an SM: 128 registers a thread at launch, (200 + 56) x 128 = 128 x 256 after the split
+#define REGS_SOFTMAX 200
+#define REGS_OTHERS 56
+#define TMEM_COLS 256
+#define S_COL 0
+#define O_COL 128
+#define NK (HEAD_DIM == 128 ? 3 : 4)
+#define NV (HEAD_DIM == 128 ? 2 : 4)
+// mbarriers, by their index
+#define B_K 0
+#define B_KFREE (B_K + NK)
+#define B_V (B_KFREE + NK)
+#define B_VFREE (B_V + NV)
+#define B_SFULL (B_VFREE + NV)     // [2] each from here on
+#define B_OFULL (B_SFULL + 2)
+#define B_PFULL (B_OFULL + 2)
+#define NUM_BARS (B_PFULL + 2)
+static_assert(NUM_BARS <= 30, "the barriers, the tensor-memory address and the abort flag share 256 bytes");
+#define RESCALE_LOG2 8.0f
+
+struct PrefixParams {
+    SharedPlan plan;
+    const __nv_bfloat16* q;        // [num_seqs, nh, HEAD_DIM]: sequence b brings row b
+    const int* block_tables;       // [num_seqs, max_blocks]
+    const int* ctx_lens;
+    float* part_o;                 // [items, nkv, ROWS, HEAD_DIM]
+    float* part_ml;                // [items, nkv, ROWS, 2]
+    int* status;
+    int nh, nkv, page_shift, page_size, max_blocks, num_pages;
+    float scale_log2e, cap_log2e, scale_over_cap;
+};
+
+__global__ void __launch_bounds__(NUM_THREADS, 2)
+prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const PrefixParams p) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* q_s = smem_raw;                           // [HALVES][128 rows x 128 B]
+    unsigned char* k_s = q_s + Q_BYTES;                      // [NK stages][HALVES][KV_TILE keys x 128 B]
+    unsigned char* v_s = k_s + NK * TILE_BYTES;              // [NV stages][HALVES][KV_TILE keys x 128 B]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + NV * TILE_BYTES);
+    uint32_t& tmem_base_slot = *reinterpret_cast<uint32_t*>(bars + 30);
+    volatile int& abort_flag = *reinterpret_cast<volatile int*>(bars + 31);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) tma_prefetch_descriptor(&map_kv);
+    const uint32_t bar_k0 = smem_u32(&bars[B_K]), bar_kfree0 = smem_u32(&bars[B_KFREE]);
+    const uint32_t bar_v0 = smem_u32(&bars[B_V]), bar_vfree0 = smem_u32(&bars[B_VFREE]);
+    const uint32_t bar_s_full0 = smem_u32(&bars[B_SFULL]), bar_o_full0 = smem_u32(&bars[B_OFULL]), bar_p_full0 = smem_u32(&bars[B_PFULL]);
+
+    const int kvh = blockIdx.x, item = blockIdx.y;
+    const int G = p.nh / p.nkv;
+    rv_pdl_wait();
+    if (item >= p.plan.items_used()) return;
+    const SharedItem it_ = p.plan.item(item);
+    const SharedTile tile = p.plan.tile(it_.tile);
+    const int key_lo = it_.key_begin, key_hi = it_.key_end;                 // a multiple of KV_TILE; the end may lie inside a page
+    const int tile_rows = min(tile.count, ROWS / G) * G;
+    if (key_hi <= key_lo || tile_rows <= 0) return;
+    const int t_begin = key_lo / KV_TILE, n_it = (key_hi + KV_TILE - 1) / KV_TILE - t_begin;
+    const int* table = p.block_tables + (size_t)tile.table_seq * p.max_blocks;
+
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < NK; ++i) { mbar_init(bar_k0 + 8 * i, 1); mbar_init(bar_kfree0 + 8 * i, 1); }
+        for (int i = 0; i < NV; ++i) { mbar_init(bar_v0 + 8 * i, 1); mbar_init(bar_vfree0 + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar_s_full0 + 8 * i, 1);
+            mbar_init(bar_o_full0 + 8 * i, 1);
+            mbar_init(bar_p_full0 + 8 * i, SOFTMAX_WARPS);                  // one arrival per warp
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == LOADER_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(TMEM_COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    // value tiles start as zeros: what a box does not bring must not meet a probability of zero with a NaN
+    for (int i = tid; i < NV * TILE_BYTES / 16; i += NUM_THREADS) reinterpret_cast<uint4*>(v_s)[i] = make_uint4(0, 0, 0, 0);
+    // the rows' queries, 16 bytes at a time, to their places in the 128-byte swizzle; rows without a sequence are zeros
+    for (int i = tid; i < ROWS * (HEAD_DIM / 8); i += NUM_THREADS) {
+        const int row = i / (HEAD_DIM / 8), chunk = i - row * (HEAD_DIM / 8);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < tile_rows) {
+            const int m = row / G, seq = p.plan.member(tile.first + m);
+            v = *reinterpret_cast<const uint4*>(p.q + ((size_t)seq * p.nh + kvh * G + (row - m * G)) * HEAD_DIM + chunk * 8);
+        }
+        *reinterpret_cast<uint4*>(q_s + (chunk >> 3) * (ROWS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = v;
+    }
+    fence_async_smem();
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = tmem_base_slot;
+    // (only now that this CTA holds its tensor memory: a kernel behind this one might allocate before it waits)
+    rv_pdl_launch_dependents();
+
+    const int box_keys = p.page_size < KV_TILE ? p.page_size : KV_TILE;     // keys one TMA box brings
+    const int boxes = KV_TILE / box_keys;
+    int tiles_issued = 0;             // by this warp, if it is a loader
+    if (warp == LOADER_WARP || warp == VLOADER_WARP) {
+        // ------------------------------------------------------------ loader warps: TMA, one for keys, one for values
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
+        const int which = warp == LOADER_WARP ? 0 : 1;
+        const int stages = which == 0 ? NK : NV;
+        const uint32_t bar_full0 = which == 0 ? bar_k0 : bar_v0, bar_free0 = which == 0 ? bar_kfree0 : bar_vfree0;
+        const uint32_t ring = smem_u32(which == 0 ? k_s : v_s);
+        auto lookup = [&](int t) -> int {               // this lane's page of tile t, or -1
+            const int key = t * KV_TILE + lane * box_keys;
+            if (lane >= boxes || key >= key_hi || (key >> p.page_shift) >= p.max_blocks) return -1;
+            const int page = __ldg(table + (key >> p.page_shift));
+            return page < p.num_pages ? page : -1;
+        };
+        auto issue = [&](int t, int stage, int page) {
+            const uint32_t bar = bar_full0 + 8 * stage;
+            const int key = t * KV_TILE + lane * box_keys;
+            const unsigned mask = __ballot_sync(0xffffffffu, page >= 0);
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)__popc(mask) * HALVES * (uint32_t)box_keys * 128u);
+            __syncwarp();
+            if (page >= 0) {
+                const int row = ((page * 2 + which) * p.nkv + kvh) * p.page_size + (key & (p.page_size - 1));
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h)
+                    tma_load_2d(ring + (uint32_t)stage * TILE_BYTES + (uint32_t)h * (KV_TILE * 128) + (uint32_t)lane * box_keys * 128,
+                                &map_kv, h * 64, row, bar);
+            }
+            __syncwarp();
+        };
+        for (int i = 0; i < stages && i < n_it; ++i, ++tiles_issued) issue(t_begin + i, i, lookup(t_begin + i));
+        int page = stages < n_it ? lookup(t_begin + stages) : -1;
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int e = 0; e + stages < n_it; ++e) {
+            const int next = e + 1 + stages < n_it ? lookup(t_begin + e + 1 + stages) : -1;     // a turn before it is needed
+            int ok_l = 1;
+            if (lane == 0) ok_l = mbar_wait(bar_free0 + 8 * stage, phase, &abort_flag, 3 + which) ? 1 : 0;
+            if (!__shfl_sync(0xffffffffu, ok_l, 0)) break;
+            issue(t_begin + e + stages, stage, page);
+            ++tiles_issued;
+            page = next;
+            if (++stage == stages) { stage = 0; phase ^= 1; }
+        }
+    } else if (warp == QK_WARP) {
+        // ------------------------------------------------------------ S = Q K^T, over P(i - 2) once that product has finished
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
+        if (lane == 0) {
+            const uint32_t idesc_s = umma_idesc_bf16(ROWS, KV_TILE);
+            int k_stage = 0;
+            uint32_t k_phase = 0;
+            for (int i = 0; i < n_it; ++i) {
+                const int buf = i & 1;
+                if (!mbar_wait(bar_k0 + 8 * k_stage, k_phase, &abort_flag, 5)) break;
+                if (i >= 2 && !mbar_wait(bar_o_full0 + 8 * buf, ((i - 2) >> 1) & 1, &abort_flag, 6)) break;
+                tcgen05_fence_after();
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) {
+                    const uint64_t dq = umma_desc(smem_u32(q_s) + h * (ROWS * 128));
+                    const uint64_t dk = umma_desc(smem_u32(k_s) + k_stage * TILE_BYTES + h * (KV_TILE * 128));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        tcgen05_mma_bf16(tmem_base + S_COL + buf * KV_TILE, dq + (uint64_t)(2 * j), dk + (uint64_t)(2 * j), idesc_s, (h | j) != 0);
+                }
+                tcgen05_commit(bar_s_full0 + 8 * buf);
+                tcgen05_commit(bar_kfree0 + 8 * k_stage);
+                if (++k_stage == NK) { k_stage = 0; k_phase ^= 1; }
+            }
+        }
+    } else if (warp == PV_WARP) {
+        // ------------------------------------------------------------ O += P V
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
+        if (lane == 0) {
+            const uint32_t idesc_o = umma_idesc_bf16(ROWS, HEAD_DIM) | (1u << 16);          // B is MN-major
+            int v_stage = 0;
+            uint32_t v_phase = 0;
+            for (int i = 0; i < n_it; ++i) {
+                const int b = i & 1;
+                if (!mbar_wait(bar_v0 + 8 * v_stage, v_phase, &abort_flag, 7)) break;
+                if (!mbar_wait(bar_p_full0 + 8 * b, (i >> 1) & 1, &abort_flag, 8)) break;
+                tcgen05_fence_after();
+                const uint32_t tp = tmem_base + S_COL + b * KV_TILE;
+                const uint64_t dv = umma_desc_mn(smem_u32(v_s) + v_stage * TILE_BYTES, KV_TILE * 128);
+#pragma unroll
+                for (int j = 0; j < KV_TILE / 16; ++j)
+                    tcgen05_mma_bf16_ts(tmem_base + O_COL, tp + 8 * j, dv + (uint64_t)(128 * j), idesc_o, (i | j) != 0);
+                tcgen05_commit(bar_vfree0 + 8 * v_stage);
+                tcgen05_commit(bar_o_full0 + 8 * b);
+                if (++v_stage == NV) { v_stage = 0; v_phase ^= 1; }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ softmax warps: one thread per row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+        const int row = warp * 32 + lane;                            // row of the tile = lane of tensor memory
+        const bool rows_here = warp * 32 < tile_rows;                // (a warp without rows only hands its buffers on)
+        const bool in_range = row < tile_rows;
+        // a row sees the keys of the range that its sequence has
+        const int limit = in_range ? min(key_hi, p.ctx_lens[p.plan.member(tile.first + row / G)]) : 0;
+        const uint32_t t_lane = tmem_base + ((uint32_t)(warp * 32) << 16);
+        float m_ref = -INFINITY, l_run = 0.f;
+        bool ok = true;
+        for (int it = 0; it < n_it; ++it) {
+            const int sb = it & 1;
+            const int key0 = (t_begin + it) * KV_TILE;
+            if (!mbar_wait(bar_s_full0 + 8 * sb, (it >> 1) & 1, &abort_flag, 9)) { ok = false; break; }
+            tcgen05_fence_after();
+            if (key0 + KV_TILE > key_hi) {
+                // values of keys behind the range's end: zeros, before the product may read them (it waits for P of all four warps)
+                if (!mbar_wait(bar_v0 + 8 * (it % NV), (it / NV) & 1, &abort_flag, 12)) { ok = false; break; }
+                const int from = key_hi - key0, n = (KV_TILE - from) * 8;
+                unsigned char* vt = v_s + (it % NV) * TILE_BYTES;
+                for (int i = tid; i < HALVES * n; i += 32 * SOFTMAX_WARPS) {
+                    const int h = i / n;
+                    reinterpret_cast<uint4*>(vt + h * (KV_TILE * 128) + from * 128)[i - h * n] = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();
+            }
+            if (rows_here) {
+                uint32_t s0[32], s1[32];
+                tmem_ld_32x32(t_lane + S_COL + sb * KV_TILE, s0);
+                tmem_ld_32x32(t_lane + S_COL + sb * KV_TILE + 32, s1);
+                tmem_ld_wait();
+                tcgen05_fence_before();
+                __syncwarp();
+                // with a cap the scores become c log2(e) tanh(scale s / c) here (tanh as 1 - 2 / (e^2x + 1)), and the scale below is 1
+                const float eff_scale = p.cap_log2e > 0.f ? 1.f : p.scale_log2e;
+                if (p.cap_log2e > 0.f) {
+                    const float k2 = p.scale_over_cap * 2.885390081777927f;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float ea = fast_exp2(__uint_as_float(s0[e]) * k2), eb = fast_exp2(__uint_as_float(s1[e]) * k2);
+                        s0[e] = __float_as_uint(p.cap_log2e * (1.f - __fdividef(2.f, ea + 1.f)));
+                        s1[e] = __float_as_uint(p.cap_log2e * (1.f - __fdividef(2.f, eb + 1.f)));
+                    }
+                }
+                if (key0 + KV_TILE > limit) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        if (key0 + e >= limit) s0[e] = 0xff800000u;               // -inf
+                        if (key0 + 32 + e >= limit) s1[e] = 0xff800000u;
+                    }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    mx[0] = max3(mx[0], __uint_as_float(s0[e]), __uint_as_float(s0[e + 1]));
+                    mx[1] = max3(mx[1], __uint_as_float(s0[e + 2]), __uint_as_float(s0[e + 3]));
+                    mx[2] = max3(mx[2], __uint_as_float(s1[e]), __uint_as_float(s1[e + 1]));
+                    mx[3] = max3(mx[3], __uint_as_float(s1[e + 2]), __uint_as_float(s1[e + 3]));
+                }
+                const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * eff_scale;
+                // the reference maximum is raised only when it is far behind: O then needs a pass
+                const bool first_data = m_ref == -INFINITY && m_tile > -INFINITY;
+                const bool raise = first_data || m_tile > m_ref + RESCALE_LOG2;
+                float factor = 1.f;
+                if (raise) {
+                    factor = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_tile);
+                    m_ref = m_tile;
+                    l_run *= factor;
+                }
+                if (__any_sync(0xffffffffu, raise && it > 0)) {
+                    // the product of the tile before must have finished; the one after waits for this warp's P
+                    if (!mbar_wait(bar_o_full0 + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &abort_flag, 11)) { ok = false; break; }
+                    tcgen05_fence_after();
+#pragma unroll
+                    for (int c = 0; c < HEAD_DIM; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(t_lane + O_COL + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                        tmem_st_32x32(t_lane + O_COL + c, o);
+                    }
+                    tmem_st_wait();
+                    tcgen05_fence_before();
+                }
+                const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
+                float l_tile = 0.f, l_tile2 = 0.f;
+                uint32_t pk[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {                   // keys 2j and 2j + 1 of the tile: one column of P
+                    const int e = 2 * j;
+                    float a0, a1;
+                    fma2(a0, a1, __uint_as_float(e < 32 ? s0[e] : s1[e - 32]), __uint_as_float(e + 1 < 32 ? s0[e + 1] : s1[e + 1 - 32]),
+                         eff_scale, neg_m);
+                    const float x0 = fast_exp2(a0), x1 = fast_exp2(a1);
+                    add2(l_tile, l_tile2, x0, x1);
+                    __nv_bfloat162 h2 = __floats2bfloat162_rn(x0, x1);
+                    pk[j] = *reinterpret_cast<uint32_t*>(&h2);
+                }
+                l_run += l_tile + l_tile2;
+                tmem_st_32x32(t_lane + S_COL + sb * KV_TILE, pk);
+                tmem_st_wait();
+            }
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_p_full0 + 8 * sb);
+        }
+        if (ok) {
+            ok = mbar_wait(bar_o_full0 + 8 * ((n_it - 1) & 1), ((n_it - 1) >> 1) & 1, &abort_flag, 10);
+            tcgen05_fence_after();
+            if (ok && rows_here) {
+                const size_t prow = ((size_t)item * p.nkv + kvh) * ROWS + row;
+                if (in_range) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m_ref, l_run);
+#pragma unroll
+                for (int c = 0; c < HEAD_DIM; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld_32x32(t_lane + O_COL + c, o);
+                    tmem_ld_wait();
+                    if (in_range) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<uint4*>(p.part_o + prow * HEAD_DIM + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                }
+            }
+        }
+    }
+
+    tcgen05_fence_before();
+    __syncthreads();
+    if (abort_flag != 0) {
+        // A wait gave up somewhere: tiles may still be on their way into this CTA's shared memory with nobody left to wait for
+        // them.  Their loaders do (bounded, without touching the flag) before the CTA ends.
+        if ((warp == LOADER_WARP || warp == VLOADER_WARP) && lane == 0) {
+            volatile int ignore = 0;
+            const int stages = warp == LOADER_WARP ? NK : NV;
+            const uint32_t full0 = warp == LOADER_WARP ? bar_k0 : bar_v0;
+            for (int i = max(0, tiles_issued - stages); i < tiles_issued; ++i)
+                mbar_wait(full0 + 8 * (i % stages), (i / stages) & 1, &ignore, 0);
+        }
+        __syncthreads();
+    }
+    if (warp == LOADER_WARP)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
+    if (tid == 0 && abort_flag != 0 && p.status) atomicCAS(p.status, 0, abort_flag);
+}
+
+// ---------------------------------------------------------------- host side
+RV_EXPORT int rv_prefix_attention_tcgen05(const void* q, const void* cache, long long num_pages, const int* block_tables, const int* ctx_lens,
+                                          const int* plan, int num_seqs, int cap_tiles, int cap_items, float* part_o, float* part_ml, int nh, int nkv, int hd, int page_size, int max_blocks, float scale,
+                                          float softcap, int* status, cudaStream_t stream) {
+    if (hd != HEAD_DIM) return RV_ERR_UNSUPPORTED;
+    if (num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 ||
+        num_pages > 0x7fffffffLL || cap_tiles < 0 || cap_items < 0 || !plan || !part_o || !part_ml)
+        return RV_ERR_BAD_SIZE;
+    if (nh / nkv > ROWS || (page_size & (page_size - 1)) || page_size < 8) return RV_ERR_UNSUPPORTED;
+    // a row of the tensor map is an int in the kernel
+    if (num_pages * 2 * nkv * page_size > 0x7fffffffLL) return RV_ERR_UNSUPPORTED;
+    if (nkv > 65535 || cap_items > 65535) return RV_ERR_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(part_o) |
+         reinterpret_cast<uintptr_t>(plan)) % 16 || reinterpret_cast<uintptr_t>(part_ml) % 8)
+        return RV_ERR_ALIGNMENT;
+    if (num_seqs == 0 || cap_items == 0) return RV_OK;
+    alignas(64) CUtensorMap map_kv;
+    int st = rv_make_bf16_map(&map_kv, cache, num_pages * 2 * nkv * page_size, HEAD_DIM, page_size < KV_TILE ? page_size : KV_TILE);
+    if (st != RV_OK) return st;
+    PrefixParams p;
+    p.plan = shared_plan(plan, num_seqs, cap_tiles, cap_items);
+    p.q = (const __nv_bfloat16*)q; p.block_tables = block_tables; p.ctx_lens = ctx_lens;
+    p.part_o = part_o; p.part_ml = part_ml; p.status = status;
+    p.nh = nh; p.nkv = nkv; p.page_size = page_size; p.max_blocks = max_blocks; p.num_pages = (int)num_pages;
+    p.page_shift = 0;
+    while ((1 << p.page_shift) < page_size) ++p.page_shift;
+    p.scale_log2e = scale * 1.4426950408889634f;
+    p.cap_log2e = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
+    p.scale_over_cap = softcap > 0.f ? scale / softcap : 0.f;
+    const int smem = Q_BYTES + NK * TILE_BYTES + NV * TILE_BYTES + 256;
+    static RvPerDevice configured;
+    if (int e = rv_configure_smem(configured, prefix_attention_kernel, smem)) return e;
+    RV_LAUNCH_ST = rv_launch(prefix_attention_kernel, dim3(nkv, cap_items), dim3(NUM_THREADS), smem, stream, map_kv, p);
+    return rv_launch_status();
+}

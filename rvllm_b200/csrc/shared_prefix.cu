@@ -1,0 +1,325 @@
+// Attention over a prefix that sequences share: the plain kernels (any type, head size and page size) and the merge.
+//
+// With the keys of a sequence cut at its prefix's end, (m1, l1, o1) over the prefix and (m2, l2, o2) over what lies behind it, each
+// (maximum, sum of e^(s - m), sum of e^(s - m) v), the attention is (o1 e^(m1 - m) + o2 e^(m2 - m)) / (l1 e^(m1 - m) + l2 e^(m2 - m)),
+// m = max(m1, m2); cutting either part into further ranges changes nothing.  Maxima are in units of log2 throughout.
+#include "common.cuh"
+#include "shared_prefix.cuh"
+
+// ---------------------------------------------------------------------------------------------
+// The plain kernel of both parts: 32-bit products and sums, one CTA per (row block, kv head, range of keys).  The rows of a CTA share
+// the keys, so a tile of 32 keys and values goes to shared memory once and meets 4 * RPW rows: a warp owns RPW rows, its lanes the
+// 32 keys of the tile for the scores and hd / 32 columns for the sums.  In float32 the arithmetic bounds it (no tensor core takes
+// 32 bits); RPW = 8 reads a shared word per four multiply-adds, RPW = 2 serves the few rows of one sequence.
+#define PLAIN_THREADS 128
+#define PLAIN_TILE 32
+#define PLAIN_MAX_DIM 256
+
+struct PlainParams {
+    SharedPlan plan;
+    const void* q;                 // [num_seqs, nh, hd]: sequence b brings row b
+    const void* cache;             // [num_pages, 2, nkv, page_size, hd]
+    const int* block_tables;       // [num_seqs, max_blocks]
+    const int* ctx_lens;
+    float* part_o;                 // prefixes: [items, nkv, SP_ROWS, hd]; own keys: [splits, num_seqs, nh, hd]
+    float* part_ml;                // ... and the same with 2 in place of hd
+    long long num_pages;
+    int num_seqs, nh, nkv, hd, page_size, max_blocks, splits;
+    float scale, softcap;          // softcap 0: none
+};
+
+// OWN: the keys behind the prefix, one sequence a CTA (blockIdx: kv head x row block, split, sequence);
+// else a range of a group's prefix (kv head x row block, item)
+template <typename T, int RPW, int DPL, bool OWN>
+__global__ void __launch_bounds__(PLAIN_THREADS)
+shared_plain_kernel(const PlainParams p) {
+    extern __shared__ __align__(16) float sh[];
+    constexpr int R = 4 * RPW;
+    const int stride = p.hd + 4;                            // (a multiple of four that is odd in units of 16 bytes for hd a multiple of 8)
+    float* q_s = sh;                                        // [R][hd]
+    float* k_s = q_s + R * p.hd;                            // [PLAIN_TILE][stride]
+    float* v_s = k_s + PLAIN_TILE * stride;                 // [PLAIN_TILE][stride]
+    float* p_s = v_s + PLAIN_TILE * stride;                 // [R][PLAIN_TILE]
+    int* tok_s = reinterpret_cast<int*>(p_s + R * PLAIN_TILE);   // [R] token of a row, -1 without one
+    int* lim_s = tok_s + R;                                 // [R] keys that a row sees end here
+
+    rv_pdl_launch_dependents();
+    rv_pdl_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kvh = blockIdx.x % p.nkv, row0 = blockIdx.x / p.nkv * R;
+    const int G = p.nh / p.nkv;
+    int key_lo, key_hi, table_seq, rows, first = 0, item = 0;
+    if (OWN) {
+        table_seq = blockIdx.z;
+        rows = G;
+        const int ctx = p.ctx_lens[table_seq], start = p.plan.own_start(table_seq);
+        const int tiles = ctx > start ? (ctx - start + PLAIN_TILE - 1) / PLAIN_TILE : 0;
+        const int per = (tiles + p.splits - 1) / p.splits;
+        key_lo = start + (int)blockIdx.y * per * PLAIN_TILE;
+        key_hi = min(ctx, key_lo + per * PLAIN_TILE);
+    } else {
+        item = blockIdx.y;
+        if (item >= p.plan.items_used()) return;
+        const SharedItem it = p.plan.item(item);
+        const SharedTile tile = p.plan.tile(it.tile);
+        table_seq = tile.table_seq; first = tile.first;
+        rows = min(tile.count, SP_ROWS / G) * G;
+        key_lo = it.key_begin; key_hi = it.key_end;
+    }
+    if (row0 >= rows) return;
+    if (tid < R) {
+        int tok = -1, lim = 0;
+        if (row0 + tid < rows) {
+            const int seq = OWN ? table_seq : p.plan.member(first + (row0 + tid) / G);
+            tok = seq;
+            lim = min(key_hi, p.ctx_lens[seq]);
+        }
+        tok_s[tid] = tok; lim_s[tid] = lim;
+    }
+    __syncthreads();
+    const T* q = (const T*)p.q;
+    for (int i = tid; i < R * p.hd; i += PLAIN_THREADS) {
+        const int r = i / p.hd, d = i - r * p.hd;
+        q_s[i] = tok_s[r] >= 0 ? rv_to_float(q[((size_t)tok_s[r] * p.nh + kvh * G + (row0 + r) % G) * p.hd + d]) * p.scale : 0.f;
+    }
+    const T* cache = (const T*)p.cache;
+    const int* table = p.block_tables + (size_t)table_seq * p.max_blocks;
+    float m[RPW], l[RPW], acc[RPW][DPL];
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+        m[i] = -INFINITY; l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) acc[i][d] = 0.f;
+    }
+    const int per_row = p.hd / 4;
+    for (int key0 = key_lo; key0 < key_hi; key0 += PLAIN_TILE) {
+        __syncthreads();                                    // the tile before has been read
+        for (int i = tid; i < PLAIN_TILE * per_row; i += PLAIN_THREADS) {
+            const int k = i / per_row, d = (i - k * per_row) * 4, key = key0 + k;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+            if (key < key_hi && key / p.page_size < p.max_blocks) {
+                const int page = table[key / p.page_size];
+                if (page >= 0 && page < p.num_pages) {
+                    const size_t at = (((size_t)page * 2 * p.nkv + kvh) * p.page_size + key % p.page_size) * p.hd + d;
+                    constexpr int dt = sizeof(T) == 4 ? RV_DTYPE_F32 : RV_DTYPE_BF16;
+                    a = rv_load4(cache, dt, at);
+                    b = rv_load4(cache, dt, at + (size_t)p.nkv * p.page_size * p.hd);
+                }
+            }
+            *reinterpret_cast<float4*>(k_s + k * stride + d) = a;
+            *reinterpret_cast<float4*>(v_s + k * stride + d) = b;
+        }
+        __syncthreads();
+        float s[RPW];
+#pragma unroll
+        for (int i = 0; i < RPW; ++i) s[i] = 0.f;
+        for (int d = 0; d < p.hd; d += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(k_s + lane * stride + d);
+#pragma unroll
+            for (int i = 0; i < RPW; ++i) {
+                const float4 b = *reinterpret_cast<const float4*>(q_s + (warp * RPW + i) * p.hd + d);
+                s[i] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s[i]))));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RPW; ++i) {
+            const int r = warp * RPW + i;
+            float v = s[i];
+            if (p.softcap > 0.f) v = p.softcap * tanhf(v / p.softcap);
+            v = key0 + lane < lim_s[r] ? v * 1.4426950408889634f : -INFINITY;
+            const float m_new = fmaxf(m[i], rv_warp_max(v));
+            const float m_s = m_new == -INFINITY ? 0.f : m_new;
+            const float keep = exp2f(m[i] - m_s), e = exp2f(v - m_s);
+            l[i] = l[i] * keep + rv_warp_sum(e);
+            m[i] = m_new;
+#pragma unroll
+            for (int d = 0; d < DPL; ++d) acc[i][d] *= keep;
+            p_s[r * PLAIN_TILE + lane] = e;
+        }
+        __syncwarp();
+#pragma unroll 4
+        for (int k = 0; k < PLAIN_TILE; ++k) {
+#pragma unroll
+            for (int c = 0; c < DPL; c += 4) {
+                const int d = c * 32 + lane * 4;
+                if (d >= p.hd) continue;
+                const float4 v = *reinterpret_cast<const float4*>(v_s + k * stride + d);
+#pragma unroll
+                for (int i = 0; i < RPW; ++i) {
+                    const float e = p_s[(warp * RPW + i) * PLAIN_TILE + k];
+                    acc[i][c] = fmaf(e, v.x, acc[i][c]); acc[i][c + 1] = fmaf(e, v.y, acc[i][c + 1]);
+                    acc[i][c + 2] = fmaf(e, v.z, acc[i][c + 2]); acc[i][c + 3] = fmaf(e, v.w, acc[i][c + 3]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+        const int r = warp * RPW + i;
+        if (row0 + r >= rows || tok_s[r] < 0) continue;
+        const size_t prow = OWN ? ((size_t)blockIdx.y * p.num_seqs + tok_s[r]) * p.nh + kvh * G + row0 + r
+                                : ((size_t)item * p.nkv + kvh) * SP_ROWS + row0 + r;
+#pragma unroll
+        for (int c = 0; c < DPL; c += 4) {
+            const int d = c * 32 + lane * 4;
+            if (d < p.hd) *reinterpret_cast<float4*>(p.part_o + prow * p.hd + d) = make_float4(acc[i][c], acc[i][c + 1], acc[i][c + 2], acc[i][c + 3]);
+        }
+        if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m[i], l[i]);
+    }
+}
+
+template <typename T, int RPW, int DPL, bool OWN>
+static int launch_plain(const PlainParams& p, dim3 grid, cudaStream_t stream) {
+    const int R = 4 * RPW;
+    const int smem = (R * p.hd + 2 * PLAIN_TILE * (p.hd + 4) + R * PLAIN_TILE + 2 * R) * 4;
+    const int most = (R * PLAIN_MAX_DIM + 2 * PLAIN_TILE * (PLAIN_MAX_DIM + 4) + R * PLAIN_TILE + 2 * R) * 4;
+    static RvPerDevice configured;
+    if (int e = rv_configure_smem(configured, shared_plain_kernel<T, RPW, DPL, OWN>, most)) return e;
+    RV_LAUNCH_ST = rv_launch(shared_plain_kernel<T, RPW, DPL, OWN>, grid, dim3(PLAIN_THREADS), smem, stream, p);
+    return rv_launch_status();
+}
+
+template <typename T, int RPW, bool OWN>
+static int launch_plain_dim(const PlainParams& p, dim3 grid, cudaStream_t stream) {
+    return p.hd <= 128 ? launch_plain<T, RPW, 4, OWN>(p, grid, stream) : launch_plain<T, RPW, 8, OWN>(p, grid, stream);
+}
+
+// part 0: the ranges of the prefixes (part_o [cap_items, nkv, SP_ROWS, hd]); part 1: the keys behind them, cut into `splits` ranges
+// (part_o [splits, num_seqs, nh, hd])
+RV_EXPORT int rv_shared_plain(const void* q, const void* cache, long long num_pages, const int* block_tables, const int* ctx_lens,
+                              const int* plan, int num_seqs, int cap_tiles, int cap_items, float* part_o, float* part_ml,
+                              int nh, int nkv, int hd, int page_size, int max_blocks, float scale, float softcap, int part,
+                              int splits, int dtype, cudaStream_t stream) {
+    if (num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 ||
+        cap_tiles < 0 || cap_items < 0 || splits < 1 || !plan || !part_o || !part_ml)
+        return RV_ERR_BAD_SIZE;
+    if (dtype != RV_DTYPE_F32 && dtype != RV_DTYPE_BF16) return RV_ERR_BAD_DTYPE;
+    if (hd % 4 || hd > PLAIN_MAX_DIM || nh / nkv > SP_ROWS) return RV_ERR_UNSUPPORTED;
+    if (num_seqs > 65535 || splits > 65535 || cap_items > 65535) return RV_ERR_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(part_o) | reinterpret_cast<uintptr_t>(plan)) % 16 ||
+        reinterpret_cast<uintptr_t>(part_ml) % 8)
+        return RV_ERR_ALIGNMENT;
+    if (num_seqs == 0 || (part == 0 && cap_items == 0)) return RV_OK;
+    PlainParams p;
+    p.plan = shared_plan(plan, num_seqs, cap_tiles, cap_items);
+    p.q = q; p.cache = cache; p.block_tables = block_tables; p.ctx_lens = ctx_lens;
+    p.part_o = part_o; p.part_ml = part_ml; p.num_pages = num_pages; p.num_seqs = num_seqs;
+    p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = page_size; p.max_blocks = max_blocks; p.splits = splits;
+    p.scale = scale; p.softcap = softcap;
+    const int G = nh / nkv;
+    if (part == 0) {
+        const dim3 grid(nkv * ((SP_ROWS / G * G + 31) / 32), cap_items);
+        return dtype == RV_DTYPE_F32 ? launch_plain_dim<float, 8, false>(p, grid, stream) : launch_plain_dim<__nv_bfloat16, 8, false>(p, grid, stream);
+    }
+    const dim3 grid(nkv * ((G + 7) / 8), splits, num_seqs);
+    return dtype == RV_DTYPE_F32 ? launch_plain_dim<float, 2, true>(p, grid, stream) : launch_plain_dim<__nv_bfloat16, 2, true>(p, grid, stream);
+}
+
+// ---------------------------------------------------------------------------------------------
+// The merge: hd / 4 threads per (token, head) row, four neighbouring elements each, eight ranges' loads in flight at a time.
+struct MergeParams {
+    SharedPlan plan;
+    const float* pre_o;            // [cap_items, nkv, SP_ROWS, hd]
+    const float* pre_ml;
+    const float* own_o;            // [splits, num_seqs, nh, hd]
+    const float* own_ml;
+    const int* own_count;          // [num_seqs, nkv] ranges of the own keys, or null: `splits` of them
+    const float* sinks;            // [nh] or null
+    const float* gate;             // [num_seqs, nh] or null
+    void* out;                     // [num_seqs, nh, hd]
+    int num_seqs, nh, nkv, hd, splits, rows_per_block;
+};
+
+struct Running {
+    float m, l;
+    float4 o;
+};
+
+// Takes up `n` ranges, `step` rows apart from `row` on.
+__device__ __forceinline__ void merge_ranges(Running& r, const float* __restrict__ part_o, const float* __restrict__ part_ml, size_t row,
+                                             size_t step, int n, int hd, int d) {
+    for (int s0 = 0; s0 < n; s0 += 8) {
+        float m[8], l[8];
+        float4 o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool have = s0 + i < n;
+            const size_t at = row + (size_t)(have ? s0 + i : s0) * step;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml) + at);
+            m[i] = have ? ml.x : -INFINITY;
+            l[i] = have ? ml.y : 0.f;
+            o[i] = __ldcg(reinterpret_cast<const float4*>(part_o + at * hd + d));
+        }
+        float m_new = r.m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m_new = fmaxf(m_new, m[i]);
+        const float m_s = m_new == -INFINITY ? 0.f : m_new;
+        const float keep = exp2f(r.m - m_s);             // 0 while nothing has been seen
+        r.l *= keep;
+        r.o.x *= keep; r.o.y *= keep; r.o.z *= keep; r.o.w *= keep;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = exp2f(m[i] - m_s);           // 0 for an empty or absent range, whose sum may hold anything
+            r.l += l[i] * f;
+            if (f > 0.f) { r.o.x += o[i].x * f; r.o.y += o[i].y * f; r.o.z += o[i].z * f; r.o.w += o[i].w * f; }
+        }
+        r.m = m_new;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(128)
+shared_merge_kernel(const MergeParams p) {
+    rv_pdl_launch_dependents();
+    const int per = p.hd / 4;
+    const int r = threadIdx.x / per, d = (threadIdx.x - r * per) * 4;
+    const long long row = (long long)blockIdx.x * p.rows_per_block + r;           // (sequence, head)
+    const bool live = r < p.rows_per_block && row < (long long)p.num_seqs * p.nh;
+    const int seq = live ? (int)(row / p.nh) : 0, head = live ? (int)(row - (long long)seq * p.nh) : 0;
+    const int G = p.nh / p.nkv, kvh = head / G;
+    rv_pdl_wait();
+    if (!live) return;
+    Running v;
+    v.m = -INFINITY; v.l = 0.f; v.o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int place = p.plan.place(seq);
+    if (place >= 0) {
+        const int2 parts = p.plan.parts(place / SP_ROWS);
+        merge_ranges(v, p.pre_o, p.pre_ml, ((size_t)parts.x * p.nkv + kvh) * SP_ROWS + place % SP_ROWS + (head - kvh * G),
+                     (size_t)p.nkv * SP_ROWS, parts.y, p.hd, d);
+    }
+    const size_t out_row = (size_t)seq * p.nh + head;
+    merge_ranges(v, p.own_o, p.own_ml, out_row, (size_t)p.num_seqs * p.nh, p.own_count ? p.own_count[seq * p.nkv + kvh] : p.splits, p.hd, d);
+    float num = 1.f, den = v.l;
+    if (p.sinks) {                                       // exp(sink) joins the denominator; it has no value
+        const float sk = p.sinks[head] * 1.4426950408889634f;
+        const float m_new = fmaxf(v.m, sk);
+        num = exp2f(v.m - m_new);
+        den = v.l * num + exp2f(sk - m_new);
+    }
+    float inv = den > 0.f ? num / den : 0.f;
+    if (p.gate) inv *= p.gate[out_row];
+    constexpr int dt = sizeof(T) == 4 ? RV_DTYPE_F32 : RV_DTYPE_BF16;
+    rv_store4(p.out, dt, out_row * p.hd + d, make_float4(v.o.x * inv, v.o.y * inv, v.o.z * inv, v.o.w * inv));
+}
+
+RV_EXPORT int rv_shared_merge(const int* plan, int num_seqs, int cap_tiles, int cap_items, const float* pre_o, const float* pre_ml,
+                              const float* own_o, const float* own_ml, const int* own_count, int splits, void* out,
+                              const float* sinks, const float* gate, int nh, int nkv, int hd, int dtype, cudaStream_t stream) {
+    if (num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || cap_tiles < 0 || cap_items < 0 || splits < 1 || !plan ||
+        !own_o || !own_ml)
+        return RV_ERR_BAD_SIZE;
+    if (dtype != RV_DTYPE_F32 && dtype != RV_DTYPE_BF16) return RV_ERR_BAD_DTYPE;
+    if (hd % 4 || hd > PLAIN_MAX_DIM) return RV_ERR_UNSUPPORTED;
+    if (num_seqs == 0) return RV_OK;
+    MergeParams p;
+    p.plan = shared_plan(plan, num_seqs, cap_tiles, cap_items);
+    p.pre_o = pre_o; p.pre_ml = pre_ml; p.own_o = own_o; p.own_ml = own_ml; p.own_count = own_count; 
+    p.sinks = sinks; p.gate = gate; p.out = out;
+    p.num_seqs = num_seqs; p.nh = nh; p.nkv = nkv; p.hd = hd; p.splits = splits;
+    p.rows_per_block = 128 / (hd / 4);
+    const long long blocks = ((long long)num_seqs * nh + p.rows_per_block - 1) / p.rows_per_block;
+    if (blocks > 0x7fffffffLL) return RV_ERR_UNSUPPORTED;
+    if (dtype == RV_DTYPE_F32) RV_LAUNCH_ST = rv_launch(shared_merge_kernel<float>, dim3((unsigned)blocks), dim3(128), 0, stream, p);
+    else RV_LAUNCH_ST = rv_launch(shared_merge_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(128), 0, stream, p);
+    return rv_launch_status();
+}

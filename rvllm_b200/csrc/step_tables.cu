@@ -1,0 +1,139 @@
+// Block tables, slot maps and positions of a step, built on the device from the requests' lengths.
+//
+// A table of pages stays on the device, one row per request slot and cache group: [groups, table_rows, table_width].  A step
+// brings, per sequence b, the row it owns, how many of that row's entries are already there (`held`), the position of its first
+// token and how many tokens it brings; and one flat list of the pages that were handed out for the step, group by group and
+// sequence by sequence.  With u(b) = ceil((start + q) / page) blocks in use, sequence b of group g takes the next
+// max(0, u - held) pages of the list for the entries [held, u) of its row, and
+//   block_tables[g][b][j] = row[j] for live <= j < u, else -1   (live: the first block that a window or chunk still sees)
+//   slot_mapping[g][t]    = row[pos / page] * page + pos % page  for token t at position pos
+//   positions, token_seq, cu_seqlens, ctx_lens                   as the step's kernels read them.
+// A sequence without a row (-1) stands for no request: its context length is 0, its entries and slots are -1.
+//
+// One launch, no order between its CTAs: where a sequence's pages begin in the list, and its tokens in the step, are sums over
+// the sequences before it, which every CTA forms for itself (integers: any order gives the same), and an entry that is new in
+// this step is read from the list, never from the row that another CTA may be writing.  A CTA takes one sequence of
+// one group; the lengths are read once per CTA (a few KB from L2), the entries once in the whole grid.  Every index that
+// comes from device memory is checked against its bound; an entry that would lie outside counts as absent (-1).
+#include "common.cuh"
+
+#define TABLE_THREADS 256
+
+struct TableParams {
+    int* page_table;               // [groups, table_rows, table_width]
+    const int* rows;               // [num_seqs]
+    const int* held;               // [groups, num_seqs]
+    const int* starts;             // [num_seqs]
+    const int* q_lens;             // [num_seqs]
+    const int* new_pages;          // [num_new]
+    const int* spans;              // [groups, 2]: window, chunk (0: none)
+    int* block_tables;             // [groups, num_seqs, max_blocks]
+    int* slot_mapping;             // [groups, num_tokens]
+    int* positions;                // [num_tokens]
+    int* token_seq;                // [num_tokens]
+    int* cu_seqlens;               // [num_seqs + 1]
+    int* ctx_lens;                 // [num_seqs]
+    int groups, num_seqs, table_rows, table_width, num_new, num_tokens, max_blocks, page_size;
+};
+
+__device__ __forceinline__ int blocks_in_use(const TableParams& p, int b) {
+    const int row = p.rows[b];
+    if (row < 0 || row >= p.table_rows) return 0;
+    const long long end = (long long)max(p.starts[b], 0) + max(p.q_lens[b], 0);
+    const long long u = (end + p.page_size - 1) / p.page_size;
+    return (int)(u < p.table_width ? u : p.table_width);
+}
+
+// Sum over the block of a pair of integers; every thread gets both.  `scratch` holds 2 * 8 integers.
+__device__ __forceinline__ void block_sum2(int& a, int& b, int* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    if (lane == 0) { scratch[warp] = a; scratch[8 + warp] = b; }
+    __syncthreads();
+    a = b = 0;
+#pragma unroll
+    for (int w = 0; w < TABLE_THREADS / 32; ++w) { a += scratch[w]; b += scratch[8 + w]; }
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(TABLE_THREADS)
+step_tables_kernel(const TableParams p) {
+    __shared__ int scratch[16];
+    rv_pdl_wait();
+    const int tid = threadIdx.x;
+    const int b = blockIdx.x, g = blockIdx.y;
+    // pages taken before this sequence (all groups before g, then the sequences before b), tokens before it
+    int pages = 0, tokens = 0;
+    for (long long i = tid; i < (long long)g * p.num_seqs + b; i += TABLE_THREADS) {
+        const int s = (int)(i % p.num_seqs);
+        pages += max(0, blocks_in_use(p, s) - max(p.held[i], 0));
+    }
+    for (int s = tid; s < b; s += TABLE_THREADS) tokens += max(p.q_lens[s], 0);
+    block_sum2(pages, tokens, scratch);
+
+    const int row = p.rows[b];
+    const bool real = row >= 0 && row < p.table_rows;
+    const int start = max(p.starts[b], 0), q = max(p.q_lens[b], 0);
+    const int used = blocks_in_use(p, b);
+    const int held = max(p.held[(size_t)g * p.num_seqs + b], 0);
+    int* mine = p.page_table + ((size_t)g * p.table_rows + (real ? row : 0)) * p.table_width;
+    auto entry = [&](int j) -> int {                 // j < used
+        if (j < held) return mine[j];
+        const int at = pages + (j - held);
+        return at < p.num_new ? p.new_pages[at] : -1;
+    };
+    for (int j = held + tid; j < used; j += TABLE_THREADS) mine[j] = entry(j);
+    const int window = p.spans[2 * g], chunk = p.spans[2 * g + 1];
+    int first = window > 0 ? max(0, start - window + 1) : 0;
+    if (chunk > 0) first = max(first, start / chunk * chunk);
+    const int live = first / p.page_size;
+    int* out = p.block_tables + ((size_t)g * p.num_seqs + b) * p.max_blocks;
+    for (int j = tid; j < p.max_blocks; j += TABLE_THREADS) out[j] = (j >= live && j < used) ? entry(j) : -1;
+    for (int i = tid; i < q; i += TABLE_THREADS) {
+        const int t = tokens + i;
+        if (t >= p.num_tokens) break;
+        const int pos = real ? start + i : 0;
+        const int block = pos / p.page_size;
+        int slot = -1;
+        if (real && block < used) {
+            const int page = entry(block);
+            if (page >= 0) slot = page * p.page_size + (pos - block * p.page_size);
+        }
+        p.slot_mapping[(size_t)g * p.num_tokens + t] = slot;
+        if (g == 0) { p.positions[t] = pos; p.token_seq[t] = b; }
+    }
+    if (b == p.num_seqs - 1)                         // places behind the last sequence's tokens belong to none
+        for (int t = tokens + q + tid; t < p.num_tokens; t += TABLE_THREADS) {
+            p.slot_mapping[(size_t)g * p.num_tokens + t] = -1;
+            if (g == 0) { p.positions[t] = 0; p.token_seq[t] = -1; }
+        }
+    if (g == 0 && tid == 0) {
+        p.cu_seqlens[b] = tokens;
+        if (b == p.num_seqs - 1) p.cu_seqlens[p.num_seqs] = tokens + q;
+        p.ctx_lens[b] = real ? start + q : 0;
+    }
+    // The step's other kernels may read this metadata before they wait for their predecessor, so nothing behind this kernel may
+    // start before all of it is written: it gives no early signal, and what it wrote is out when a CTA ends.
+    __threadfence();
+}
+
+RV_EXPORT int rv_step_tables(int* page_table, const int* rows, const int* held, const int* starts, const int* q_lens, const int* new_pages,
+                             const int* spans, int* block_tables, int* slot_mapping, int* positions, int* token_seq, int* cu_seqlens,
+                             int* ctx_lens, int groups, int num_seqs, int table_rows, int table_width, int num_new, int num_tokens,
+                             int max_blocks, int page_size, cudaStream_t stream) {
+    if (groups < 1 || num_seqs < 1 || table_rows < 1 || table_width < 1 || num_new < 0 || num_tokens < 0 || max_blocks < 1 || page_size < 1)
+        return RV_ERR_BAD_SIZE;
+    if (groups > 65535) return RV_ERR_UNSUPPORTED;
+    TableParams p;
+    p.page_table = page_table; p.rows = rows; p.held = held; p.starts = starts; p.q_lens = q_lens; p.new_pages = new_pages; p.spans = spans;
+    p.block_tables = block_tables; p.slot_mapping = slot_mapping; p.positions = positions; p.token_seq = token_seq;
+    p.cu_seqlens = cu_seqlens; p.ctx_lens = ctx_lens;
+    p.groups = groups; p.num_seqs = num_seqs; p.table_rows = table_rows; p.table_width = table_width; p.num_new = num_new;
+    p.num_tokens = num_tokens; p.max_blocks = max_blocks; p.page_size = page_size;
+    RV_LAUNCH_ST = rv_launch(step_tables_kernel, dim3(num_seqs, groups), dim3(TABLE_THREADS), 0, stream, p);
+    return rv_launch_status();
+}

@@ -20,6 +20,7 @@ import torch
 
 from ..errors import KernelError
 from . import build
+from .shared import SharedPrefixes, StepTables, KEY_TILE, TILE_ROWS
 
 _DT = {torch.float32: 0, torch.bfloat16: 1}
 _GATED_PREFILL, _GATED_DECODE = {"silu": 2, "gelu_tanh": 4, "swiglu_clamp": 5}, {"silu": 1, "gelu_tanh": 2, "swiglu_clamp": 3}
@@ -386,10 +387,13 @@ class CudaKernels:
         of the memory), the merge kernel 2.5 us.  The split count with the least modelled time is
         taken: it fills one wave when the batch is small and keeps the last wave full when it is
         large."""
+        return self._splits(meta.num_seqs, meta.max_ctx_len, num_heads, num_kv_heads)
+
+    def _splits(self, num_seqs: int, longest: int, num_heads: int, num_kv_heads: int) -> int:
         self_max_splits = 64          # a long context at a small batch still fills the GPU (one sequence of 32,768 keys: 55)
         group = num_heads // num_kv_heads
-        ctas = meta.num_seqs * num_kv_heads * ((group + 15) // 16)
-        tiles = max(1, (meta.max_ctx_len + 63) // 64)
+        ctas = num_seqs * num_kv_heads * ((group + 15) // 16)
+        tiles = max(1, (longest + 63) // 64)
         best, best_t = 1, float("inf")
         for s in range(1, min(self_max_splits, tiles) + 1):
             per = -(-tiles // s)
@@ -497,6 +501,141 @@ class CudaKernels:
             c_float(scale), c_int(window or 0), c_int(meta.max_q_len), _ptr(status if status is not None else self._status),
             c_float(softcap or 0.0), _ptr(sinks), _ptr(gate), *self._distance_args(distance_bias), self._stream())
         _check("attention_tcgen05", st)
+        return out
+
+    # ------------------------------------------------------------------ tokens that requests share
+    def _on_this_device(self, *named):
+        """Every tensor lies on the device that is current, whose stream the kernels are launched on."""
+        here = torch.cuda.current_device()
+        for t, name in named:
+            if t is not None and (not t.is_cuda or t.device.index != here):
+                raise KernelError(f"{name} lies on {t.device}, but the current device is cuda:{here}")
+
+    def shared_prefix_attention(self, q, cache_layer, meta: AttentionMeta, shared: SharedPrefixes, num_heads, num_kv_heads, head_dim,
+                                scale: float, softcap: Optional[float] = None, sinks: Optional[torch.Tensor] = None,
+                                gate: Optional[torch.Tensor] = None, max_own: Optional[int] = None) -> torch.Tensor:
+        """`paged_attention` of a step whose sequences bring one token each, for groups of sequences that begin with the same
+        cached tokens (`shared`): the keys and values of a group's prefix are read once for all its sequences, the keys behind
+        it sequence by sequence, and both are merged under one softmax.  A sequence outside every group is all its own.
+
+        `softcap`, `sinks`, `gate` as in `paged_attention`.  There is no window: where one is set, sequences of different
+        lengths see different parts of a prefix.  `max_own`: no sequence has more keys behind its prefix (sizes the launch
+        only; without it the longest context less the shortest prefix is taken).
+
+        bfloat16 with heads of 64 or 128, up to 128 query heads on a key/value head and pages of a power of two from 8 on: the prefixes on the
+        tcgen05 kernel, the rest on the TMA-fed decode kernels.  float32, and other sizes whose head is a multiple of 4 up to
+        256: the plain kernels.  What neither takes, and steps without a group, go to `paged_attention`, to which every table
+        is whole."""
+        _need(q, "q", dims=2); _need(cache_layer, "cache_layer", q.dtype, 5)
+        _need(meta.block_tables, "block_tables", torch.int32, 2); _need(meta.ctx_lens, "ctx_lens", torch.int32, 1)
+        dt = self._dt(q, "q")
+        B = meta.num_seqs
+        if meta.max_q_len > 1 or q.shape[0] != B:
+            raise KernelError(f"shared_prefix_attention: {q.shape[0]} tokens of {B} sequences, the longest of {meta.max_q_len}: every sequence "
+                              "brings one")
+        if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or q.shape[1] != num_heads * head_dim:
+            raise KernelError(f"shared_prefix_attention: rows of {q.shape[1]} for {num_heads} heads of {head_dim} on {num_kv_heads}")
+        if tuple(cache_layer.shape[1:3]) != (2, num_kv_heads) or cache_layer.shape[4] != head_dim:
+            raise KernelError(f"shared_prefix_attention: a cache layer of shape {tuple(cache_layer.shape)} for {num_kv_heads} key/value heads of {head_dim}")
+        if (shared.num_seqs, shared.num_heads, shared.num_kv_heads) != (B, num_heads, num_kv_heads):
+            raise KernelError(f"shared_prefix_attention: prefixes laid out for {shared.num_seqs} sequences of {shared.num_heads} heads on "
+                              f"{shared.num_kv_heads}, a step of {B} of {num_heads} on {num_kv_heads}")
+        if meta.block_tables.shape[0] < B or meta.ctx_lens.shape[0] < B:
+            raise KernelError(f"shared_prefix_attention: tables of {meta.block_tables.shape[0]} and lengths of {meta.ctx_lens.shape[0]} sequences for {B}")
+        self._check_attention_extras(q, num_heads, sinks, gate)
+        self._on_this_device((q, "q"), (cache_layer, "cache_layer"), (meta.block_tables, "block_tables"), (meta.ctx_lens, "ctx_lens"),
+                             (shared.device_ints, "shared"), (sinks, "sinks"), (gate, "gate"))
+        page, group = cache_layer.shape[3], num_heads // num_kv_heads
+        power = page & (page - 1) == 0
+        fast = q.dtype == torch.bfloat16 and head_dim in (64, 128) and power and page >= 8 and cache_layer.shape[0] * 2 * num_kv_heads * page < 2 ** 31
+        if shared.capacity[1] == 0 or B == 0 or group > TILE_ROWS or not (fast or (head_dim % 4 == 0 and head_dim <= 256)):
+            return self.paged_attention(q, cache_layer, meta, num_heads, num_kv_heads, head_dim, scale, None, softcap, sinks, gate)
+        if max_own is None:
+            max_own = meta.max_ctx_len - (min(t for _, t in shared.groups) if sum(len(m) for m, _ in shared.groups) == B else 0)
+        max_own = max(1, min(max_own, meta.max_ctx_len))
+        tiles, items = shared.capacity
+        out = torch.empty_like(q)
+        row = head_dim + 2
+        pre = torch.empty((items * num_kv_heads * TILE_ROWS * row,), dtype=torch.float32, device=q.device)
+        pre_ml = pre[items * num_kv_heads * TILE_ROWS * head_dim:]
+        counts, pieces = None, 1
+        layout = (c_int(num_heads), c_int(num_kv_heads), c_int(head_dim), c_int(page), c_int(meta.max_blocks), c_float(scale))
+        plan = (_ptr(shared.device_ints), c_int(B), c_int(tiles), c_int(items))
+        pages = ctypes.c_longlong(cache_layer.shape[0])
+        lib = self._lib("shared_prefix.cu")
+        if fast:
+            st = self._lib("prefix_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",)).rv_prefix_attention_tcgen05(
+                _ptr(q), _ptr(cache_layer), pages, _ptr(meta.block_tables), _ptr(meta.ctx_lens), *plan, _ptr(pre), _ptr(pre_ml), *layout,
+                c_float(softcap or 0.0), _ptr(self._status), self._stream())
+            _check("prefix_attention_tcgen05", st)
+            flash = self._lib("attention_flash.cu", (f"-DHEAD_DIM={head_dim}",))
+            common = (_ptr(q), _ptr(cache_layer), pages, _ptr(meta.block_tables), _ptr(meta.cu_seqlens), _ptr(meta.ctx_lens), _ptr(shared.own_start))
+            if softcap is None and self.BALANCED_DECODE and group <= 16 and B <= 240 and B * num_kv_heads >= self.BALANCED_MIN_PAIRS:
+                ctas = self._balanced_tma_ctas(flash, num_heads, num_kv_heads)
+                pieces = flash.rv_flash_balanced_max_pieces(c_int(meta.max_ctx_len + KEY_TILE), c_int(num_kv_heads), c_int(ctas))
+                own = torch.empty((pieces * B * num_heads * row,), dtype=torch.float32, device=q.device)
+                counts = torch.empty((B * num_kv_heads,), dtype=torch.int32, device=q.device)
+                st = flash.rv_flash_decode_balanced_parts(*common, _ptr(own), _ptr(counts), c_int(pieces), c_int(B), c_int(B), *layout,
+                                                          c_int(ctas), _ptr(self._status), self._stream())
+                _check("flash_decode_balanced_parts", st)
+            else:
+                pieces = self._splits(B, max_own + KEY_TILE - 1, num_heads, num_kv_heads)
+                own = torch.empty((pieces * B * num_heads * row,), dtype=torch.float32, device=q.device)
+                st = flash.rv_flash_decode_tma_parts(*common, _ptr(own), c_int(B), c_int(B), *layout, c_int(pieces), _ptr(self._status),
+                                                     c_int(1 if (self.TMA_DECODE_EARLY and self.pdl) else 0), c_float(softcap or 0.0),
+                                                     self._stream())
+                _check("flash_decode_tma_parts", st)
+        else:
+            pieces = max(1, min(64, -(-max_own // 64), 4 * self.num_sms // max(1, B * num_kv_heads)))
+            own = torch.empty((pieces * B * num_heads * row,), dtype=torch.float32, device=q.device)
+            for part, buf, ml in ((0, pre, pre_ml), (1, own, own[pieces * B * num_heads * head_dim:])):
+                st = lib.rv_shared_plain(_ptr(q), _ptr(cache_layer), pages, _ptr(meta.block_tables), _ptr(meta.ctx_lens), *plan, _ptr(buf),
+                                         _ptr(ml), *layout, c_float(softcap or 0.0), c_int(part), c_int(pieces), c_int(dt), self._stream())
+                _check("shared_plain", st)
+        st = lib.rv_shared_merge(*plan, _ptr(pre), _ptr(pre_ml), _ptr(own), _ptr(own[pieces * B * num_heads * head_dim:]), _ptr(counts),
+                                 c_int(pieces), _ptr(out), _ptr(sinks), _ptr(gate), c_int(num_heads), c_int(num_kv_heads), c_int(head_dim),
+                                 c_int(dt), self._stream())
+        _check("shared_merge", st)
+        return out
+
+    def step_tables(self, page_table: torch.Tensor, rows: torch.Tensor, held: torch.Tensor, starts: torch.Tensor, q_lens: torch.Tensor,
+                    new_pages: torch.Tensor, spans: torch.Tensor, num_tokens: int, max_blocks: int, page_size: int,
+                    out: Optional[StepTables] = None) -> StepTables:
+        """The block tables, slot map and positions of a step from its requests' lengths; all tensors int32 on the device.
+
+        page_table [groups, table rows, table width]: the pages of every request, kept by the caller and brought up to date
+        here.  Per sequence of the step: `rows` the row it owns (-1: none, a sequence that stands for no request; no row twice),
+        `held` [groups, sequences] the entries its row has already, `starts` and `q_lens` the position of its first token and
+        its tokens.  `new_pages`: the pages handed out for the step, group by group and sequence by sequence, each sequence as
+        many as its ceil((start + q_len) / page_size) blocks exceed what it holds.  `spans` [groups, 2]: the window and the chunk
+        of a group (0: none); blocks that no later token can see are -1 in its block tables.
+
+        `num_tokens` = the sum of q_lens and `max_blocks` >= the most blocks of a sequence, as the caller knows them.  With `out`
+        the tables are written into tensors of the caller (those a captured graph reads)."""
+        tensors = ((page_table, "page_table", 3), (rows, "rows", 1), (held, "held", 2), (starts, "starts", 1), (q_lens, "q_lens", 1),
+                   (new_pages, "new_pages", 1), (spans, "spans", 2))
+        for t, name, dims in tensors:
+            _need(t, name, torch.int32, dims)
+        G, R, width = page_table.shape
+        B = rows.shape[0]
+        if held.shape != (G, B) or starts.shape[0] != B or q_lens.shape[0] != B or spans.shape != (G, 2):
+            raise KernelError(f"step_tables: {B} rows in {G} groups, but held {tuple(held.shape)}, starts {tuple(starts.shape)}, q_lens "
+                              f"{tuple(q_lens.shape)}, spans {tuple(spans.shape)}")
+        if num_tokens < 0 or max_blocks < 1 or page_size < 1 or min(G, B, R, width) < 1:
+            raise KernelError(f"step_tables: {num_tokens} tokens of {B} sequences, {max_blocks} blocks of {page_size}, a page table of {(G, R, width)}")
+        shapes = ((G, B, max_blocks), (G, num_tokens), (num_tokens,), (num_tokens,), (B + 1,), (B,))
+        if out is None:
+            out = StepTables(*(torch.empty(s, dtype=torch.int32, device=page_table.device) for s in shapes))
+        made = (out.block_tables, out.slot_mapping, out.positions, out.token_seq, out.cu_seqlens, out.ctx_lens)
+        for t, s in zip(made, shapes):
+            _need(t, "out", torch.int32)
+            if tuple(t.shape) != s:
+                raise KernelError(f"step_tables: an output of shape {tuple(t.shape)} where {s} is written")
+        self._on_this_device(*((t, name) for t, name, _ in tensors), *((t, "out") for t in made))
+        st = self._lib("step_tables.cu").rv_step_tables(
+            *(_ptr(t) for t, _, _ in tensors), *(_ptr(t) for t in made), c_int(G), c_int(B), c_int(R), c_int(width),
+            c_int(new_pages.shape[0]), c_int(num_tokens), c_int(max_blocks), c_int(page_size), self._stream())
+        _check("step_tables", st)
         return out
 
     def paged_attention_plain(self, q, cache_layer, meta, num_heads, num_kv_heads, head_dim, scale, window,

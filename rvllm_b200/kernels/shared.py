@@ -1,0 +1,127 @@
+"""Which sequences of a step begin with the same cached tokens, and the step's tables as the kernels read them."""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from ..errors import KernelError
+
+TILE_ROWS = 128            # rows of a row tile (SP_ROWS of csrc/shared_prefix.cuh)
+KEY_TILE = 64              # keys of a tile: ranges of keys begin at multiples of it
+
+
+def _cut(tiles_of: Sequence[int], kv_heads: int, places: int) -> int:
+    """Key tiles of a range so that the ranges of all row tiles and kv heads come closest to filling `places` CTAs once (at
+    least two: a CTA costs about as much as three tiles to set up and to merge)."""
+    lo, hi = 2, max(max(tiles_of), 2)
+    while lo < hi:
+        mid = (lo + hi) // 2
+        if sum(-(-n // mid) for n in tiles_of) * kv_heads <= places:
+            hi = mid
+        else:
+            lo = mid + 1
+    return lo
+
+
+class SharedPrefixes:
+    """The groups of a step's sequences whose first tokens are the same cached ones, laid out for the kernels.
+
+    `groups`: (members, tokens) per group: the places of its sequences in the step and how many leading tokens they share.
+    Their block tables must lead to the same keys and values there (as a rule the same pages; the page in which the shared
+    tokens end may be a copy).  A sequence belongs to one group at most; groups of one and groups without tokens share nothing
+    and are left out.  The object depends on neither the tokens behind the prefixes nor the layer: a program keeps it while
+    its set of sequences stays.  It takes part in no computation but `CudaKernels.shared_prefix_attention`.
+
+    `capacity` = (row tiles, ranges of keys): fixes the size of the arrays, so that a captured graph serves other groups of
+    the same number of sequences ."""
+
+    def __init__(self, groups, num_seqs: int, num_heads: int, num_kv_heads: int, device, capacity: Optional[Tuple[int, int]] = None,
+                 num_sms: int = 148):
+        if num_seqs < 0 or num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads:
+            raise KernelError(f"shared prefixes: {num_seqs} sequences of {num_heads} heads on {num_kv_heads} key/value heads")
+        self.num_seqs, self.num_heads, self.num_kv_heads = num_seqs, num_heads, num_kv_heads
+        self.num_sms = num_sms
+        self.capacity = None
+        host = self._lay_out(groups, capacity)
+        self.device_ints = torch.from_numpy(host).to(device)
+
+    @staticmethod
+    def ints(num_seqs: int, capacity: Tuple[int, int]) -> int:
+        """32-bit integers of the array."""
+        tiles, items = capacity
+        return (4 + 3 * num_seqs + 2 * tiles + 3) // 4 * 4 + 4 * tiles + 4 * items
+
+    @property
+    def own_start(self) -> torch.Tensor:
+        """int32 [num_seqs] on the device: the first token of each sequence that lies behind its prefix."""
+        return self.device_ints[4:4 + self.num_seqs]
+
+    def _lay_out(self, groups, capacity) -> np.ndarray:
+        B, per = self.num_seqs, self.num_heads // self.num_kv_heads
+        seen = set()
+        kept = []
+        for members, tokens in groups:
+            members = [int(m) for m in members]
+            for m in members:
+                if not 0 <= m < B:
+                    raise KernelError(f"shared prefixes: sequence {m} of a step of {B}")
+                if m in seen:
+                    raise KernelError(f"shared prefixes: sequence {m} is in two groups, or twice in one")
+                seen.add(m)
+            if tokens < 0 or tokens > 0x7fffffff - KEY_TILE:
+                raise KernelError(f"shared prefixes: a prefix of {tokens} tokens")
+            if len(members) > 1 and tokens > 0:
+                kept.append((members, int(tokens)))
+        if per > TILE_ROWS and kept:
+            raise KernelError(f"shared prefixes: {per} query heads on a key/value head are more than the {TILE_ROWS} rows of a tile")
+        tile_members = max(1, TILE_ROWS // per)
+        tiles = []                                   # (sequence whose table is read, first member, how many, tokens)
+        flat, own_start, place = [], np.zeros(B, np.int32), np.full(B, -1, np.int32)
+        for members, tokens in kept:
+            for at in range(0, len(members), tile_members):
+                part = members[at:at + tile_members]
+                for i, m in enumerate(part):
+                    own_start[m] = tokens
+                    place[m] = len(tiles) * TILE_ROWS + i * per
+                tiles.append((members[0], len(flat), len(part), tokens))
+                flat.extend(part)
+        key_tiles = [-(-t[3] // KEY_TILE) for t in tiles]
+        items, parts = [], []
+        if tiles:
+            step = _cut(key_tiles, self.num_kv_heads, 2 * self.num_sms)
+            for i, n in enumerate(key_tiles):
+                k = -(-n // step)
+                edges = [n * j // k for j in range(k + 1)]
+                parts.append((len(items), k))
+                items += [(i, a * KEY_TILE, min(b * KEY_TILE, tiles[i][3]), 0) for a, b in zip(edges, edges[1:])]
+        capacity = capacity or (len(tiles), len(items))
+        if len(tiles) > capacity[0] or len(items) > capacity[1]:
+            raise KernelError(f"shared prefixes: {len(tiles)} row tiles and {len(items)} ranges of keys do not fit a capacity of {capacity}")
+        host = np.zeros(self.ints(B, capacity), np.int32)
+        host[0], host[1] = len(items), len(tiles)
+        host[4:4 + B] = own_start
+        host[4 + B:4 + 2 * B] = place
+        host[4 + 2 * B:4 + 2 * B + len(flat)] = flat
+        if tiles:
+            host[4 + 3 * B:4 + 3 * B + 2 * len(tiles)] = np.asarray(parts, np.int32).ravel()
+            at = (4 + 3 * B + 2 * capacity[0] + 3) // 4 * 4
+            host[at:at + 4 * len(tiles)] = np.asarray(tiles, np.int32).ravel()
+            at += 4 * capacity[0]
+            host[at:at + 4 * len(items)] = np.asarray(items, np.int32).ravel()
+        self.capacity, self.num_items, self.num_tiles = capacity, len(items), len(tiles)
+        self.groups = kept
+        return host
+
+
+@dataclass
+class StepTables:
+    """What `CudaKernels.step_tables` writes (int32, on the device)."""
+    block_tables: torch.Tensor         # [groups, sequences, max_blocks]
+    slot_mapping: torch.Tensor         # [groups, tokens]
+    positions: torch.Tensor            # [tokens]
+    token_seq: torch.Tensor            # [tokens]
+    cu_seqlens: torch.Tensor           # [sequences + 1]
+    ctx_lens: torch.Tensor             # [sequences]
