@@ -100,9 +100,6 @@ struct FlashParams {
     // ... and a bias per (distance, head) in units of log2, [nkv][dist_n][nh / nkv]; a distance beyond the last reads the last
     const float* dist;             // or null
     int dist_n;
-    // ... and, for sequences whose first keys another kernel has (rv_flash_decode_tma_parts): the first key of each sequence that this
-    // one looks at; the result is then left as partial sums whatever the number of splits
-    const int* key_start;          // [num_seqs] or null
 };
 
 // What the bias adds to the score of a row of head `in_group` of kv head `kvh` (of G heads), `distance` >= 0 positions back.
@@ -573,8 +570,7 @@ flash_decode_tma_kernel(const __grid_constant__ CUtensorMap map_kv, const FlashP
     // key range of the row tile and this split's share of its key tiles (as in the kernel above)
     const int last_row = min(rows_total, row0 + 16) - 1;
     const int pos_first = ctx - q_len + row0 / G, pos_last = ctx - q_len + last_row / G;
-    const int start = p.key_start ? p.key_start[seq] : 0;
-    const int key_lo = max(start, (p.window > 0 && pos_first - p.window + 1 > 0) ? pos_first - p.window + 1 : 0);
+    const int key_lo = (p.window > 0 && pos_first - p.window + 1 > 0) ? pos_first - p.window + 1 : 0;
     const int key_hi = ctx > 0 ? pos_last + 1 : 0;
     const int tile_lo = key_lo / KV_TILE, tile_hi = (key_hi + KV_TILE - 1) / KV_TILE;
     const int per_split = (tile_hi - tile_lo + p.num_splits - 1) / p.num_splits;
@@ -659,7 +655,7 @@ flash_decode_tma_kernel(const __grid_constant__ CUtensorMap map_kv, const FlashP
             head[i] = kvh * G + (in_range ? r[i] - t * G : 0);
             valid[i] = in_range && ctx > 0;
             pos[i] = valid[i] ? ctx - q_len + t : -1;
-            lo[i] = max(start, (p.window > 0 && pos[i] - p.window + 1 > 0) ? pos[i] - p.window + 1 : 0);
+            lo[i] = (p.window > 0 && pos[i] - p.window + 1 > 0) ? pos[i] - p.window + 1 : 0;
         }
         float o[HD / 8][4];
 #pragma unroll
@@ -737,18 +733,6 @@ flash_decode_tma_kernel(const __grid_constant__ CUtensorMap map_kv, const FlashP
                 o[n][0] *= alpha[0]; o[n][1] *= alpha[0];
                 o[n][2] *= alpha[1]; o[n][3] *= alpha[1];
             }
-            if (p.key_start && (t + 1) * KV_TILE > key_hi) {
-                // slots behind the newest key hold what an earlier request left: a NaN there must not meet a probability of zero
-                // (a warp reads the values of its own 16 keys only)
-                const int key = t * KV_TILE + warp_n * 16 + (lane >> 1);
-                if (key >= key_hi) {
-                    unsigned char* row = v_s + (size_t)stage * TMA_TILE_BYTES + (warp_n * 16 + (lane >> 1)) * 128 + (lane & 1) * 64;
-#pragma unroll
-                    for (int i = 0; i < 4 * TMA_HALVES; ++i)
-                        *reinterpret_cast<uint4*>(row + (i >> 2) * TMA_SLAB + (i & 3) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                __syncwarp();
-            }
             // O += P V
             uint32_t pa[4];
             pa[0] = pack_bf16(s[0][0], s[0][1]);
@@ -810,7 +794,7 @@ flash_decode_tma_kernel(const __grid_constant__ CUtensorMap map_kv, const FlashP
                 const int rr = row0 + row;
                 const int t = rr / G;
                 const size_t row_out = (size_t)(q_start + t) * p.nh + kvh * G + (rr - t * G);
-                if (p.num_splits == 1 && !p.key_start) {
+                if (p.num_splits == 1) {
                     p.out[row_out * HD + d] = __float2bfloat16_rn(acc * flash_final(m_all, l_all, p.sinks, p.gate, row_out, kvh * G + (rr - t * G)));
                 } else {
                     const size_t prow = (size_t)split * p.n_tokens * p.nh + row_out;
@@ -850,7 +834,6 @@ struct BalancedParams {
     int n_tokens, num_seqs, nh, nkv, page_shift, page_size, max_blocks, max_pieces;
     float scale_log2e;
     int window;
-    const int* key_start;          // [num_seqs] or null: the first key of each sequence that is looked at (the TMA-fed kernel)
 };
 
 template <int NSTAGES>
@@ -1158,9 +1141,9 @@ flash_decode_balanced_tma_kernel(const __grid_constant__ CUtensorMap map_kv, con
         int lo = 0, n = 0;
         if (q_len == 1 && ctx > 0) {
             const int pos = ctx - 1;
-            const int key_lo = max(p.key_start ? p.key_start[s] : 0, (p.window > 0 && pos - p.window + 1 > 0) ? pos - p.window + 1 : 0);
+            const int key_lo = (p.window > 0 && pos - p.window + 1 > 0) ? pos - p.window + 1 : 0;
             lo = key_lo / KV_TILE;
-            n = key_lo < ctx ? (ctx + KV_TILE - 1) / KV_TILE - lo : 0;
+            n = (ctx + KV_TILE - 1) / KV_TILE - lo;
         }
         s_first[s + 1] = n;
     }
@@ -1216,7 +1199,7 @@ flash_decode_balanced_tma_kernel(const __grid_constant__ CUtensorMap map_kv, con
                 if (!ok) break;
             }
             const int ctx = p.ctx_lens[seq];
-            const int key_lo = max(p.key_start ? p.key_start[seq] : 0, (p.window > 0 && ctx - p.window > 0) ? ctx - p.window : 0);
+            const int key_lo = (p.window > 0 && ctx - p.window > 0) ? ctx - p.window : 0;
             const int t = key_lo / KV_TILE + (in_seq - kvh * n_seq);
             // the newest key of a sequence was written by the kernel before this one
             if (!waited && (t + 1) * KV_TILE >= ctx) { rv_pdl_wait(); waited = true; }
@@ -1263,7 +1246,7 @@ flash_decode_balanced_tma_kernel(const __grid_constant__ CUtensorMap map_kv, con
                 const int u_pair = s_first[s] * p.nkv + kvh * n;
                 count = (u_pair + n - 1) / W - u_pair / W + 1;
             }
-            p.piece_count[pair] = min(count, p.max_pieces);
+            p.piece_count[pair] = count;
         }
         const size_t rows_all = (size_t)p.n_tokens * p.nh;
         float* mml = mo + 4 * G * (HD / (G <= 4 ? 1 : (G <= 8 ? 2 : 4)));
@@ -1281,7 +1264,7 @@ flash_decode_balanced_tma_kernel(const __grid_constant__ CUtensorMap map_kv, con
             const int piece = u / W - u_pair / W;                           // its place among the pair's pieces
             const int ctx = p.ctx_lens[seq];
             const int pos = ctx - 1;
-            const int key_lo = max(p.key_start ? p.key_start[seq] : 0, (p.window > 0 && pos - p.window + 1 > 0) ? pos - p.window + 1 : 0);
+            const int key_lo = (p.window > 0 && pos - p.window + 1 > 0) ? pos - p.window + 1 : 0;
             const int t_begin = key_lo / KV_TILE + t_rel, t_end = t_begin + n_here;
             const int tok = p.cu_seqlens[seq];
             bool valid[2];
@@ -1363,15 +1346,6 @@ flash_decode_balanced_tma_kernel(const __grid_constant__ CUtensorMap map_kv, con
                     o[n][0] *= alpha[0]; o[n][1] *= alpha[0];
                     o[n][2] *= alpha[1]; o[n][3] *= alpha[1];
                 }
-                if (p.key_start && (t + 1) * KV_TILE > ctx) {        // as in the kernel above
-                    if (t * KV_TILE + warp_n * 16 + (lane >> 1) >= ctx) {
-                        unsigned char* row = v_s + (size_t)stage * TMA_TILE_BYTES + (warp_n * 16 + (lane >> 1)) * 128 + (lane & 1) * 64;
-#pragma unroll
-                        for (int i = 0; i < 4 * TMA_HALVES; ++i)
-                            *reinterpret_cast<uint4*>(row + (i >> 2) * TMA_SLAB + (i & 3) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    __syncwarp();
-                }
                 uint32_t pa[4];
                 pa[0] = pack_bf16(s[0][0], s[0][1]);
                 pa[1] = pack_bf16(s[0][2], s[0][3]);
@@ -1422,7 +1396,7 @@ flash_decode_balanced_tma_kernel(const __grid_constant__ CUtensorMap map_kv, con
                 }
                 consumer_sync();
                 if (abort_flag != 0 || !ok) { gave_up = true; break; }
-                for (int idx = tid; piece < p.max_pieces && idx < G * HDP; idx += 128) {      // (a sequence longer than the caller said)
+                for (int idx = tid; idx < G * HDP; idx += 128) {
                     const int row = idx / HDP, dd = idx - row * HDP, d = ps * HDP + dd;
                     float m_all = -INFINITY;
 #pragma unroll
@@ -1510,7 +1484,6 @@ RV_EXPORT int rv_flash_decode_balanced(const void* q, const void* cache, const i
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     p.scale_log2e = scale * 1.4426950408889634f;
     p.window = window;
-    p.key_start = nullptr;
     if (ctas <= 0) ctas = 3 * rv_sm_count();
     const int merge_bytes = 4 * 16 * (HEAD_DIM + 2) * 4;
     const int smem = max(DECODE_STAGES * 2 * TILE_BYTES, merge_bytes);
@@ -1582,7 +1555,6 @@ RV_EXPORT int rv_flash_attention_ex(const void* q, const void* cache, const int*
     p.scale_over_cap = softcap > 0.f ? scale / softcap : 0.f;
     p.sinks = sinks; p.gate = gate;
     p.dist = dist; p.dist_n = dist_n;
-    p.key_start = nullptr;
     const int G = nh / nkv;
     const int m_tile = mode == 1 ? 16 : 64;
     p.row_tiles = (max_q_len * G + m_tile - 1) / m_tile;
@@ -1614,12 +1586,12 @@ RV_EXPORT int rv_flash_attention(const void* q, const void* cache, const int* bl
 // plus the number of pages of the cache layer (for the tensor map), the status word of bounded
 // waits and `early` (request keys before griddepcontrol.wait).  Refuses (RV_ERR_UNSUPPORTED) head
 // sizes other than 64 and 128 and pages of fewer than 8 keys: the caller falls back to rv_flash_attention.
-static int flash_decode_tma_launch(const void* q, const void* cache, long long num_pages, const int* block_tables,
-                                   const int* cu_seqlens, const int* ctx_lens, void* out, float* scratch, int n_tokens,
-                                   int num_seqs, int nh, int nkv, int hd, int page_size, int max_blocks, float scale,
-                                   int window, int max_q_len, int num_splits, int q_filter, int* status, int early,
-                                   float softcap, const float* sinks, const float* gate, const float* dist, int dist_n,
-                                   const int* key_start, cudaStream_t stream) {
+RV_EXPORT int rv_flash_decode_tma_ex(const void* q, const void* cache, long long num_pages, const int* block_tables,
+                                     const int* cu_seqlens, const int* ctx_lens, void* out, float* scratch, int n_tokens,
+                                     int num_seqs, int nh, int nkv, int hd, int page_size, int max_blocks, float scale,
+                                     int window, int max_q_len, int num_splits, int q_filter, int* status, int early,
+                                     float softcap, const float* sinks, const float* gate, const float* dist, int dist_n,
+                                     cudaStream_t stream) {
 #ifdef RV_HAVE_TMA_DECODE
     if (dist && dist_n <= 0) return RV_ERR_BAD_SIZE;
     if (hd != HEAD_DIM) return RV_ERR_UNSUPPORTED;
@@ -1629,7 +1601,7 @@ static int flash_decode_tma_launch(const void* q, const void* cache, long long n
     if ((page_size & (page_size - 1)) || page_size < 8) return RV_ERR_UNSUPPORTED;
     if (num_seqs > 65535 || nkv > 65535) return RV_ERR_BAD_SIZE;
     if (n_tokens == 0 || num_seqs == 0) return RV_OK;
-    if ((num_splits > 1 || key_start) && scratch == nullptr) return RV_ERR_BAD_SIZE;
+    if (num_splits > 1 && scratch == nullptr) return RV_ERR_BAD_SIZE;
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) % 16)
         return RV_ERR_ALIGNMENT;
     alignas(64) CUtensorMap map_kv;
@@ -1650,7 +1622,6 @@ static int flash_decode_tma_launch(const void* q, const void* cache, long long n
     p.scale_over_cap = softcap > 0.f ? scale / softcap : 0.f;
     p.sinks = sinks; p.gate = gate;
     p.dist = dist; p.dist_n = dist_n;
-    p.key_start = key_start;
     const int G = nh / nkv;
     p.row_tiles = (max_q_len * G + 15) / 16;
     const int smem = 2 * TMA_STAGES * TMA_TILE_BYTES + 1024;
@@ -1662,7 +1633,7 @@ static int flash_decode_tma_launch(const void* q, const void* cache, long long n
     RV_LAUNCH_ST = rv_launch(kernel, grid, dim3(TMA_THREADS), smem, stream, map_kv, p, status, early);
     st = rv_launch_status();
     if (st != RV_OK) return st;
-    if (num_splits > 1 && !key_start) {
+    if (num_splits > 1) {
         RV_LAUNCH_ST = rv_launch(flash_combine_kernel, dim3((n_tokens * nh + COMBINE_ROWS - 1) / COMBINE_ROWS), dim3(128), 0, stream,
                                  p.part_o, p.part_ml, p.out, n_tokens * nh, num_splits, p.sinks, p.gate, nh);
         return rv_launch_status();
@@ -1671,30 +1642,6 @@ static int flash_decode_tma_launch(const void* q, const void* cache, long long n
 #else
     return RV_ERR_UNSUPPORTED;
 #endif
-}
-
-RV_EXPORT int rv_flash_decode_tma_ex(const void* q, const void* cache, long long num_pages, const int* block_tables,
-                                     const int* cu_seqlens, const int* ctx_lens, void* out, float* scratch, int n_tokens,
-                                     int num_seqs, int nh, int nkv, int hd, int page_size, int max_blocks, float scale,
-                                     int window, int max_q_len, int num_splits, int q_filter, int* status, int early,
-                                     float softcap, const float* sinks, const float* gate, const float* dist, int dist_n,
-                                     cudaStream_t stream) {
-    return flash_decode_tma_launch(q, cache, num_pages, block_tables, cu_seqlens, ctx_lens, out, scratch, n_tokens, num_seqs, nh, nkv, hd,
-                                   page_size, max_blocks, scale, window, max_q_len, num_splits, q_filter, status, early, softcap, sinks,
-                                   gate, dist, dist_n, nullptr, stream);
-}
-
-// The keys from key_start[seq] on of sequences that bring one token each, for a caller that has the keys before them elsewhere and
-// merges both: `scratch` (floats of rv_flash_scratch_floats for two splits, times num_splits / 2) receives the sums
-// [num_splits, n_tokens, nh, HEAD_DIM], unnormalised, and behind them maxima (in units of log2) and denominators [.., 2].
-RV_EXPORT int rv_flash_decode_tma_parts(const void* q, const void* cache, long long num_pages, const int* block_tables,
-                                        const int* cu_seqlens, const int* ctx_lens, const int* key_start, float* scratch, int n_tokens,
-                                        int num_seqs, int nh, int nkv, int hd, int page_size, int max_blocks, float scale,
-                                        int num_splits, int* status, int early, float softcap, cudaStream_t stream) {
-    if (!key_start) return RV_ERR_BAD_SIZE;
-    return flash_decode_tma_launch(q, cache, num_pages, block_tables, cu_seqlens, ctx_lens, scratch, scratch, n_tokens, num_seqs, nh, nkv, hd,
-                                   page_size, max_blocks, scale, 0, 1, num_splits, 0, status, early, softcap, nullptr, nullptr, nullptr, 0,
-                                   key_start, stream);
 }
 
 RV_EXPORT int rv_flash_decode_tma(const void* q, const void* cache, long long num_pages, const int* block_tables,
@@ -1733,11 +1680,11 @@ RV_EXPORT int rv_flash_balanced_tma_ctas(int nh, int nkv) {
     return 0;
 #endif
 }
-static int flash_balanced_tma_launch(const void* q, const void* cache, long long num_pages, const int* block_tables,
-                                     const int* cu_seqlens, const int* ctx_lens, void* out, float* scratch,
-                                     int* piece_count, int max_pieces, int n_tokens, int num_seqs, int nh, int nkv,
-                                     int hd, int page_size, int max_blocks, float scale, int window, int ctas,
-                                     int* status, const int* key_start, cudaStream_t stream) {
+RV_EXPORT int rv_flash_decode_balanced_tma(const void* q, const void* cache, long long num_pages, const int* block_tables,
+                                           const int* cu_seqlens, const int* ctx_lens, void* out, float* scratch,
+                                           int* piece_count, int max_pieces, int n_tokens, int num_seqs, int nh, int nkv,
+                                           int hd, int page_size, int max_blocks, float scale, int window, int ctas,
+                                           int* status, cudaStream_t stream) {
 #ifdef RV_HAVE_TMA_DECODE
     if (hd != HEAD_DIM) return RV_ERR_UNSUPPORTED;
     if (n_tokens < 0 || num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size <= 0 || max_blocks <= 0 || max_pieces < 1 ||
@@ -1767,13 +1714,12 @@ static int flash_balanced_tma_launch(const void* q, const void* cache, long long
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     p.scale_log2e = scale * 1.4426950408889634f;
     p.window = window;
-    p.key_start = key_start;
     const int smem = balanced_tma_smem(nh / nkv);
     static RvPerDevice configured;
     if (int e = rv_configure_smem(configured, flash_decode_balanced_tma_kernel<TMA_STAGES>, balanced_tma_smem(16))) return e;
     RV_LAUNCH_ST = rv_launch(flash_decode_balanced_tma_kernel<TMA_STAGES>, dim3(ctas), dim3(TMA_THREADS), smem, stream, map_kv, p, status);
     st = rv_launch_status();
-    if (st != RV_OK || key_start) return st;
+    if (st != RV_OK) return st;
     RV_LAUNCH_ST = rv_launch(flash_balanced_combine_kernel, dim3((num_seqs * nh + COMBINE_ROWS - 1) / COMBINE_ROWS), dim3(128), 0, stream,
                              (const float*)p.part_o, (const float*)p.part_ml, (const int*)piece_count, cu_seqlens, p.out,
                              n_tokens, nh, nkv, num_seqs);
@@ -1781,26 +1727,6 @@ static int flash_balanced_tma_launch(const void* q, const void* cache, long long
 #else
     return RV_ERR_UNSUPPORTED;
 #endif
-}
-
-RV_EXPORT int rv_flash_decode_balanced_tma(const void* q, const void* cache, long long num_pages, const int* block_tables,
-                                           const int* cu_seqlens, const int* ctx_lens, void* out, float* scratch,
-                                           int* piece_count, int max_pieces, int n_tokens, int num_seqs, int nh, int nkv,
-                                           int hd, int page_size, int max_blocks, float scale, int window, int ctas,
-                                           int* status, cudaStream_t stream) {
-    return flash_balanced_tma_launch(q, cache, num_pages, block_tables, cu_seqlens, ctx_lens, out, scratch, piece_count, max_pieces, n_tokens,
-                                     num_seqs, nh, nkv, hd, page_size, max_blocks, scale, window, ctas, status, nullptr, stream);
-}
-
-// The keys from key_start[seq] on, left as partial sums (see rv_flash_decode_tma_parts): scratch [max_pieces, n_tokens, nh, ..] as above,
-// piece_count [num_seqs * nkv] says how many pieces of a (sequence, kv head) there are.
-RV_EXPORT int rv_flash_decode_balanced_parts(const void* q, const void* cache, long long num_pages, const int* block_tables,
-                                             const int* cu_seqlens, const int* ctx_lens, const int* key_start, float* scratch,
-                                             int* piece_count, int max_pieces, int n_tokens, int num_seqs, int nh, int nkv,
-                                             int hd, int page_size, int max_blocks, float scale, int ctas, int* status, cudaStream_t stream) {
-    if (!key_start) return RV_ERR_BAD_SIZE;
-    return flash_balanced_tma_launch(q, cache, num_pages, block_tables, cu_seqlens, ctx_lens, scratch, scratch, piece_count, max_pieces, n_tokens,
-                                     num_seqs, nh, nkv, hd, page_size, max_blocks, scale, 0, ctas, status, key_start, stream);
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -4,8 +4,8 @@
 // The queries of a group for one key/value head are n G rows (n sequences, G = nh / nkv heads) against the same P keys:
 //   S = scale Q K^T [n G x P],   m = max_j S,   l = sum_j e^(S - m),   O = e^(S - m) V
 // a matrix product of the size of a prompt's attention, without a triangle.  A CTA owns up to 128 rows (floor(128 / G)
-// whole sequences) of one kv head and one range of the keys and leaves (O, m, l) unnormalised; the kernel that has the keys
-// behind the prefix leaves the same, and shared_prefix.cu merges them.  Which rows and ranges there are is a list that the
+// whole sequences) of one kv head and one range of the keys and leaves (O, m, l) unnormalised; a second kernel walks the keys behind
+// the prefix, sequence by sequence, takes up what the first has left and writes the result.  Which rows and ranges there are is a list that the
 // host makes once for a set of sequences (they change when a request comes or goes, not from step to step).
 //
 // Inside a CTA: S = Q K^T of 64 keys into one of two buffers of tensor memory, one thread per row of softmax, P written back
@@ -372,38 +372,339 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
     if (tid == 0 && abort_flag != 0 && p.status) atomicCAS(p.status, 0, abort_flag);
 }
 
+// ---------------------------------------------------------------------------------------------
+// The keys behind the prefix, and the merge.  One token per sequence: G rows against each key, so the bytes bound it (hd x 4 bytes
+// a key and kv head) and the tensor cores only save instructions.  A warp works alone, on 16 keys at a time, without shared memory
+// or barriers: keys and values go from global memory straight into the operands of mma.sync.  For that the products are turned
+// over - S^T [16 keys x 8 heads] = K Q^T and O^T [16 dims x 8 heads] += V^T P^T, so that a group of up to eight heads fills the
+// narrow side - and the order of what is summed over is chosen by what a lane can load in 16 bytes: its eight neighbouring elements
+// of a key serve two steps of the product; of two neighbouring keys' values it takes the same columns, and byte permutes pair them.
+// P^T gets from the layout of a result to that of an operand by two 8 x 8 transposes (movmatrix).
+// The loads of a chunk's values and of the next chunk's keys are in flight while its scores are formed.
+// A CTA has four warps of one (sequence, kv head), which take chunks in turn; a cluster of 1 to 8 CTAs shares a long sequence, and
+// each of them ends up with a part of the columns (through distributed shared memory).  This kernel does not wait for the one with
+// the prefixes before its last part: it may begin as soon as that one's CTAs have all been placed - each of them only lets it
+// begin after its own wait, so that what both read has been written - and it waits for its end only to take up the partial sums.
+// Keys outside a sequence, and pages that do not exist, are not loaded and count as not there.
+#define OWN_WARPS 4
+#define OWN_THREADS (32 * OWN_WARPS)
+#define KEY_CHUNKS (HEAD_DIM / 32)            // 16-byte loads of a lane per key
+#define VAL_CHUNKS (HEAD_DIM / 64)            // ... per value row
+#define DIM_BLOCKS (HEAD_DIM / 16)
+
+struct OwnParams {
+    SharedPlan plan;
+    const __nv_bfloat16* q;        // [num_seqs, nh, HEAD_DIM]
+    const __nv_bfloat16* cache;
+    const int* block_tables;       // [num_seqs, max_blocks]
+    const int* ctx_lens;
+    const float* pre_o;            // what the prefixes' kernel left
+    const float* pre_ml;
+    const float* sinks;            // [nh] or null
+    const float* gate;             // [num_seqs, nh] or null
+    __nv_bfloat16* out;            // [num_seqs, nh, HEAD_DIM]
+    int nh, nkv, page_shift, page_size, max_blocks, num_pages, row_blocks;
+    float scale_log2e, cap_log2e, scale_over_cap;
+};
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+// (by way of L2 alone: this kernel reads before it waits, and what is read may have been written on another SM just before)
+__device__ __forceinline__ uint4 load_16(const __nv_bfloat16* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ uint32_t cluster_smem(uint32_t addr, uint32_t rank) {
+    uint32_t out;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+    return out;
+}
+__device__ __forceinline__ float4 load_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 load_cluster2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// NB: blocks of eight heads (a group of up to 8 or up to 16)
+template <int NB>
+__global__ void __launch_bounds__(OWN_THREADS, NB == 1 ? 3 : 2)
+own_attention_kernel(const OwnParams p) {
+    rv_pdl_launch_dependents();
+    constexpr int HD = HEAD_DIM;
+    __shared__ __align__(16) float part_o[OWN_WARPS][8 * NB][HD + 4];      // (rows four floats apart: the columns of a block in turn)
+    __shared__ __align__(8) float part_ml[OWN_WARPS][8 * NB][2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int g = lane >> 2, tq = lane & 3;
+    const int rank = blockIdx.x, ctas = gridDim.x;                         // of the cluster
+    const int kvh = blockIdx.y / p.row_blocks, seq = blockIdx.z;
+    const int G = p.nh / p.nkv;
+    const int head0 = (blockIdx.y - kvh * p.row_blocks) * 8 * NB;          // of the group
+    const int heads = min(8 * NB, G - head0);
+    const int ctx = p.ctx_lens[seq], start = min(p.plan.own_start(seq), max(ctx, 0));
+    const int* table = p.block_tables + (size_t)seq * p.max_blocks;
+
+    // this lane's queries: head g of a block, elements (4 j + tq) * 8 .. + 7
+    uint4 qf[NB][KEY_CHUNKS];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int j = 0; j < KEY_CHUNKS; ++j) {
+            qf[n][j] = make_uint4(0, 0, 0, 0);
+            if (8 * n + g < heads)
+                qf[n][j] = load_16(p.q + ((size_t)seq * p.nh + kvh * G + head0 + 8 * n + g) * HD + (4 * j + tq) * 8);
+        }
+    float o[NB][DIM_BLOCKS][4];
+    float m_run[NB][2], l_run[NB][2];                                      // heads 2 tq, 2 tq + 1 of a block
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+        for (int i = 0; i < DIM_BLOCKS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+        m_run[n][0] = m_run[n][1] = -INFINITY;
+        l_run[n][0] = l_run[n][1] = 0.f;
+    }
+    const size_t plane = (size_t)p.nkv * p.page_size * HD;                 // from a key to its value
+    // the row of `key`, or null where the sequence has no such key
+    auto row_of = [&](int key) -> const __nv_bfloat16* {
+        if (key < start || key >= ctx || (key >> p.page_shift) >= p.max_blocks) return nullptr;
+        const int page = __ldg(table + (key >> p.page_shift));
+        if (page < 0 || page >= p.num_pages) return nullptr;
+        return p.cache + (((size_t)page * 2 * p.nkv + kvh) * p.page_size + (key & (p.page_size - 1))) * HD;
+    };
+    const int step = OWN_WARPS * ctas;
+    const int chunk_end = (ctx + 15) / 16;
+    int chunk = start / 16 + rank * OWN_WARPS + warp;
+    uint4 kf[2][KEY_CHUNKS];                                               // keys g and g + 8 of the chunk
+    bool seen[2];
+    auto load_keys = [&](int c) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const __nv_bfloat16* row = c < chunk_end ? row_of(c * 16 + g + 8 * r) : nullptr;
+            seen[r] = row != nullptr;
+#pragma unroll
+            for (int j = 0; j < KEY_CHUNKS; ++j) kf[r][j] = row ? load_16(row + (4 * j + tq) * 8) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    load_keys(chunk);
+    for (; chunk < chunk_end; chunk += step) {
+        // values of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9: columns 64 c + 8 g .. + 7
+        uint4 vf[4][VAL_CHUNKS];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const __nv_bfloat16* row = row_of(chunk * 16 + 2 * tq + (r & 1) + 8 * (r >> 1));
+#pragma unroll
+            for (int c = 0; c < VAL_CHUNKS; ++c) vf[r][c] = row ? load_16(row + plane + 64 * c + 8 * g) : make_uint4(0, 0, 0, 0);
+        }
+        float s[NB][4];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < KEY_CHUNKS; ++j) {
+            const uint32_t a0[4] = {kf[0][j].x, kf[1][j].x, kf[0][j].y, kf[1][j].y};
+            const uint32_t a1[4] = {kf[0][j].z, kf[1][j].z, kf[0][j].w, kf[1][j].w};
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                mma_16816(s[n], a0, qf[n][j].x, qf[n][j].y);
+                mma_16816(s[n], a1, qf[n][j].z, qf[n][j].w);
+            }
+        }
+        const bool see[2] = {seen[0], seen[1]};
+        load_keys(chunk + step);
+        uint32_t pt[NB][2];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            float alpha[2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {                                  // e: key g + 8 (e >> 1), head 2 tq + (e & 1)
+                float v = s[n][e] * p.scale_log2e;
+                if (p.cap_log2e > 0.f) {
+                    const float x = fast_exp2(s[n][e] * p.scale_over_cap * 2.885390081777927f);
+                    v = p.cap_log2e * (1.f - __fdividef(2.f, x + 1.f));
+                }
+                s[n][e] = see[e >> 1] ? v : -INFINITY;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float mx = fmaxf(s[n][h], s[n][h + 2]);
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                const float m_new = fmaxf(m_run[n][h], mx);
+                const float m_s = m_new == -INFINITY ? 0.f : m_new;
+                alpha[h] = fast_exp2(m_run[n][h] - m_s);                   // 0 while nothing has been seen
+                m_run[n][h] = m_new;
+                s[n][h] = fast_exp2(s[n][h] - m_s);
+                s[n][h + 2] = fast_exp2(s[n][h + 2] - m_s);
+                l_run[n][h] = l_run[n][h] * alpha[h] + s[n][h] + s[n][h + 2];      // this lane's keys; the lanes are added at the end
+            }
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(s[n][0], s[n][1]), hi = __floats2bfloat162_rn(s[n][2], s[n][3]);
+            pt[n][0] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&lo));     // keys 2 tq, 2 tq + 1 of head g
+            pt[n][1] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&hi));     // ... + 8
+#pragma unroll
+            for (int i = 0; i < DIM_BLOCKS; ++i) {
+                o[n][i][0] *= alpha[0]; o[n][i][1] *= alpha[1];
+                o[n][i][2] *= alpha[0]; o[n][i][3] *= alpha[1];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < DIM_BLOCKS; ++i) {                             // rows g, g + 8 of a block: columns 64 c + 8 g + 2 w, + 1
+            const int c = i >> 2, w = i & 3;
+            auto word = [&](int r) -> uint32_t {
+                const uint4& v = vf[r][c];
+                return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w;
+            };
+            const uint32_t a[4] = {__byte_perm(word(0), word(1), 0x5410), __byte_perm(word(0), word(1), 0x7632),
+                                   __byte_perm(word(2), word(3), 0x5410), __byte_perm(word(2), word(3), 0x7632)};
+#pragma unroll
+            for (int n = 0; n < NB; ++n) mma_16816(o[n][i], a, pt[n][0], pt[n][1]);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l_run[n][h] += __shfl_xor_sync(0xffffffffu, l_run[n][h], x);
+            const int row = 8 * n + 2 * tq + h;
+            if (g == 0) { part_ml[warp][row][0] = m_run[n][h]; part_ml[warp][row][1] = l_run[n][h]; }
+#pragma unroll
+            for (int i = 0; i < DIM_BLOCKS; ++i)
+                *reinterpret_cast<float2*>(&part_o[warp][row][64 * (i >> 2) + 8 * g + 2 * (i & 3)]) = make_float2(o[n][i][h], o[n][i][h + 2]);
+        }
+    __syncthreads();
+    const bool together = ctas > 1;
+    if (together) cluster_sync();
+    rv_pdl_wait();                                   // the prefixes' sums are there
+
+    // ---- the merge: every CTA of the cluster takes its share of the (head, four columns)
+    const int place = p.plan.place(seq);
+    int2 parts = make_int2(0, 0);
+    if (place >= 0) parts = p.plan.parts(place / SP_ROWS);
+    const size_t pre_step = (size_t)p.nkv * SP_ROWS;
+    for (int i = rank * OWN_THREADS + tid; i < heads * (HD / 4); i += ctas * OWN_THREADS) {
+        const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
+        const int head = kvh * G + head0 + row;
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto take = [&](float pm, float pl, const float4& po) {            // one more part; one without keys may hold any sum
+            if (pm == -INFINITY) return;
+            const float m_new = fmaxf(m, pm);
+            const float keep = fast_exp2(m - m_new), f = fast_exp2(pm - m_new);
+            m = m_new;
+            l = l * keep + pl * f;
+            acc.x = acc.x * keep + po.x * f; acc.y = acc.y * keep + po.y * f;
+            acc.z = acc.z * keep + po.z * f; acc.w = acc.w * keep + po.w * f;
+        };
+        if (place >= 0) {
+            const size_t at = ((size_t)parts.x * p.nkv + kvh) * SP_ROWS + place % SP_ROWS + head0 + row;
+            for (int s0 = 0; s0 < parts.y; s0 += 8) {                      // eight parts' loads in flight at a time
+                float2 ml[8];
+                float4 v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const size_t r = at + (size_t)min(s0 + k, parts.y - 1) * pre_step;
+                    ml[k] = __ldcg(reinterpret_cast<const float2*>(p.pre_ml) + r);
+                    v[k] = __ldcg(reinterpret_cast<const float4*>(p.pre_o + r * HD + d));
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (s0 + k < parts.y) take(ml[k].x, ml[k].y, v[k]);
+            }
+        }
+        for (int c = 0; c < ctas; ++c) {
+#pragma unroll
+            for (int w = 0; w < OWN_WARPS; ++w) {
+                if (together) {
+                    const float2 ml = load_cluster2(cluster_smem(smem_u32(&part_ml[w][row][0]), c));
+                    take(ml.x, ml.y, load_cluster4(cluster_smem(smem_u32(&part_o[w][row][d]), c)));
+                } else {
+                    take(part_ml[w][row][0], part_ml[w][row][1], *reinterpret_cast<const float4*>(&part_o[w][row][d]));
+                }
+            }
+        }
+        float num = 1.f, den = l;
+        if (p.sinks) {                               // exp(sink) joins the denominator; it has no value
+            const float sk = p.sinks[head] * 1.4426950408889634f;
+            const float m_new = fmaxf(m, sk);
+            num = m == -INFINITY ? 0.f : fast_exp2(m - m_new);
+            den = l * num + fast_exp2(sk - m_new);
+        }
+        float inv = den > 0.f ? num / den : 0.f;
+        const size_t row_out = (size_t)seq * p.nh + head;
+        if (p.gate) inv *= p.gate[row_out];
+        rv_store4(p.out, RV_DTYPE_BF16, row_out * HD + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    }
+    if (together) cluster_sync();                    // nobody leaves while its sums are being read
+}
+
 // ---------------------------------------------------------------- host side
-RV_EXPORT int rv_prefix_attention_tcgen05(const void* q, const void* cache, long long num_pages, const int* block_tables, const int* ctx_lens,
-                                          const int* plan, int num_seqs, int cap_tiles, int cap_items, float* part_o, float* part_ml, int nh, int nkv, int hd, int page_size, int max_blocks, float scale,
-                                          float softcap, int* status, cudaStream_t stream) {
-    if (hd != HEAD_DIM) return RV_ERR_UNSUPPORTED;
-    if (num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 ||
-        num_pages > 0x7fffffffLL || cap_tiles < 0 || cap_items < 0 || !plan || !part_o || !part_ml)
+// The arguments, packed by the caller in this order (a step makes this call once a layer).
+struct SharedArgs {
+    const void* q; const void* cache; const int* block_tables; const int* ctx_lens; const int* plan;
+    float* pre_o; float* pre_ml; void* out; const float* sinks; const float* gate; int* status; cudaStream_t stream; long long num_pages;
+    int num_seqs, cap_tiles, cap_items, nh, nkv, hd, page_size, max_blocks, ctas;
+    float scale, softcap;
+};
+
+template <int NB>
+static int launch_own(const OwnParams& p, int num_seqs, int ctas, cudaStream_t stream) {
+    const dim3 grid(ctas, p.nkv * p.row_blocks, num_seqs);
+    if (ctas == 1) RV_LAUNCH_ST = rv_launch(own_attention_kernel<NB>, grid, dim3(OWN_THREADS), 0, stream, p);
+    else RV_LAUNCH_ST = rv_launch_cluster(own_attention_kernel<NB>, grid, dim3(OWN_THREADS), 0, stream, (unsigned)ctas, p);
+    return rv_launch_status();
+}
+
+// part_o [cap_items, nkv, SP_ROWS, HEAD_DIM] and part_ml [.., 2] receive the prefixes' sums; `ctas`: 1, 2, 4 or 8 CTAs share the own
+// keys of a (sequence, kv head).
+RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
+    if (a->hd != HEAD_DIM) return RV_ERR_UNSUPPORTED;
+    const int nh = a->nh, nkv = a->nkv, page_size = a->page_size;
+    if (a->num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size <= 0 || a->max_blocks <= 0 || a->num_pages <= 0 || a->cap_tiles < 0 ||
+        a->cap_items <= 0 || !a->plan || !a->pre_o || !a->pre_ml || a->num_pages > 0x7fffffffLL)
         return RV_ERR_BAD_SIZE;
-    if (nh / nkv > ROWS || (page_size & (page_size - 1)) || page_size < 8) return RV_ERR_UNSUPPORTED;
+    if (a->ctas != 1 && a->ctas != 2 && a->ctas != 4 && a->ctas != 8) return RV_ERR_BAD_SIZE;
+    const int G = nh / nkv;
+    if (G > SP_ROWS || (page_size & (page_size - 1)) || page_size < 8) return RV_ERR_UNSUPPORTED;
     // a row of the tensor map is an int in the kernel
-    if (num_pages * 2 * nkv * page_size > 0x7fffffffLL) return RV_ERR_UNSUPPORTED;
-    if (nkv > 65535 || cap_items > 65535) return RV_ERR_UNSUPPORTED;
-    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(part_o) |
-         reinterpret_cast<uintptr_t>(plan)) % 16 || reinterpret_cast<uintptr_t>(part_ml) % 8)
+    if (a->num_pages * 2 * nkv * page_size > 0x7fffffffLL) return RV_ERR_UNSUPPORTED;
+    const int row_blocks = G <= 8 ? 1 : (G + 15) / 16;
+    if ((long long)nkv * row_blocks > 65535 || a->cap_items > 65535 || a->num_seqs > 65535) return RV_ERR_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->cache) | reinterpret_cast<uintptr_t>(a->pre_o) |
+         reinterpret_cast<uintptr_t>(a->plan) | reinterpret_cast<uintptr_t>(a->out)) % 16 || reinterpret_cast<uintptr_t>(a->pre_ml) % 8)
         return RV_ERR_ALIGNMENT;
-    if (num_seqs == 0 || cap_items == 0) return RV_OK;
+    if (a->num_seqs == 0) return RV_OK;
     alignas(64) CUtensorMap map_kv;
-    int st = rv_make_bf16_map(&map_kv, cache, num_pages * 2 * nkv * page_size, HEAD_DIM, page_size < KV_TILE ? page_size : KV_TILE);
+    int st = rv_make_bf16_map(&map_kv, a->cache, a->num_pages * 2 * nkv * page_size, HEAD_DIM, page_size < KV_TILE ? page_size : KV_TILE);
     if (st != RV_OK) return st;
     PrefixParams p;
-    p.plan = shared_plan(plan, num_seqs, cap_tiles, cap_items);
-    p.q = (const __nv_bfloat16*)q; p.block_tables = block_tables; p.ctx_lens = ctx_lens;
-    p.part_o = part_o; p.part_ml = part_ml; p.status = status;
-    p.nh = nh; p.nkv = nkv; p.page_size = page_size; p.max_blocks = max_blocks; p.num_pages = (int)num_pages;
+    p.plan = shared_plan(a->plan, a->num_seqs, a->cap_tiles, a->cap_items);
+    p.q = (const __nv_bfloat16*)a->q; p.block_tables = a->block_tables; p.ctx_lens = a->ctx_lens;
+    p.part_o = a->pre_o; p.part_ml = a->pre_ml; p.status = a->status;
+    p.nh = nh; p.nkv = nkv; p.page_size = page_size; p.max_blocks = a->max_blocks; p.num_pages = (int)a->num_pages;
     p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
-    p.scale_log2e = scale * 1.4426950408889634f;
-    p.cap_log2e = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
-    p.scale_over_cap = softcap > 0.f ? scale / softcap : 0.f;
+    p.scale_log2e = a->scale * 1.4426950408889634f;
+    p.cap_log2e = a->softcap > 0.f ? a->softcap * 1.4426950408889634f : 0.f;
+    p.scale_over_cap = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
     const int smem = Q_BYTES + NK * TILE_BYTES + NV * TILE_BYTES + 256;
     static RvPerDevice configured;
     if (int e = rv_configure_smem(configured, prefix_attention_kernel, smem)) return e;
-    RV_LAUNCH_ST = rv_launch(prefix_attention_kernel, dim3(nkv, cap_items), dim3(NUM_THREADS), smem, stream, map_kv, p);
-    return rv_launch_status();
+    RV_LAUNCH_ST = rv_launch(prefix_attention_kernel, dim3(nkv, a->cap_items), dim3(NUM_THREADS), smem, a->stream, map_kv, p);
+    if ((st = rv_launch_status()) != RV_OK) return st;
+    OwnParams o;
+    o.plan = p.plan; o.q = p.q; o.cache = (const __nv_bfloat16*)a->cache; o.block_tables = p.block_tables; o.ctx_lens = p.ctx_lens;
+    o.pre_o = p.part_o; o.pre_ml = p.part_ml; o.sinks = a->sinks; o.gate = a->gate; o.out = (__nv_bfloat16*)a->out;
+    o.nh = nh; o.nkv = nkv; o.page_shift = p.page_shift; o.page_size = page_size; o.max_blocks = a->max_blocks; o.num_pages = p.num_pages;
+    o.row_blocks = row_blocks; o.scale_log2e = p.scale_log2e; o.cap_log2e = p.cap_log2e; o.scale_over_cap = p.scale_over_cap;
+    return G <= 8 ? launch_own<1>(o, a->num_seqs, a->ctas, a->stream) : launch_own<2>(o, a->num_seqs, a->ctas, a->stream);
 }

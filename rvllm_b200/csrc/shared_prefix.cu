@@ -42,6 +42,7 @@ shared_plain_kernel(const PlainParams p) {
     float* p_s = v_s + PLAIN_TILE * stride;                 // [R][PLAIN_TILE]
     int* tok_s = reinterpret_cast<int*>(p_s + R * PLAIN_TILE);   // [R] token of a row, -1 without one
     int* lim_s = tok_s + R;                                 // [R] keys that a row sees end here
+    int* there_s = lim_s + R;                               // [PLAIN_TILE] whether a key's page exists
 
     rv_pdl_launch_dependents();
     rv_pdl_wait();
@@ -77,13 +78,23 @@ shared_plain_kernel(const PlainParams p) {
         tok_s[tid] = tok; lim_s[tid] = lim;
     }
     __syncthreads();
-    const T* q = (const T*)p.q;
-    for (int i = tid; i < R * p.hd; i += PLAIN_THREADS) {
-        const int r = i / p.hd, d = i - r * p.hd;
-        q_s[i] = tok_s[r] >= 0 ? rv_to_float(q[((size_t)tok_s[r] * p.nh + kvh * G + (row0 + r) % G) * p.hd + d]) * p.scale : 0.f;
+    // a quarter of the columns of key tid / 4 (of row tid / 4) per thread
+    constexpr int dt = sizeof(T) == 4 ? RV_DTYPE_F32 : RV_DTYPE_BF16;
+    const int mine = tid >> 2, quarter = (tid & 3) * 4;
+    if (mine < R) {
+        const int tok = tok_s[mine];
+        const size_t at = ((size_t)max(tok, 0) * p.nh + kvh * G + (row0 + mine) % G) * p.hd;
+#pragma unroll 4
+        for (int d = quarter; d < p.hd; d += 16) {
+            const float4 v = rv_load4(p.q, dt, at + d);
+            *reinterpret_cast<float4*>(q_s + mine * p.hd + d) =
+                tok >= 0 ? make_float4(v.x * p.scale, v.y * p.scale, v.z * p.scale, v.w * p.scale) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
     }
-    const T* cache = (const T*)p.cache;
     const int* table = p.block_tables + (size_t)table_seq * p.max_blocks;
+    auto page_of = [&](int key) -> int {
+        return key < key_hi && key / p.page_size < p.max_blocks ? table[key / p.page_size] : -1;
+    };
     float m[RPW], l[RPW], acc[RPW][DPL];
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
@@ -91,24 +102,21 @@ shared_plain_kernel(const PlainParams p) {
 #pragma unroll
         for (int d = 0; d < DPL; ++d) acc[i][d] = 0.f;
     }
-    const int per_row = p.hd / 4;
+    const size_t plane = (size_t)p.nkv * p.page_size * p.hd;
+    int page = page_of(key_lo + mine);
     for (int key0 = key_lo; key0 < key_hi; key0 += PLAIN_TILE) {
         __syncthreads();                                    // the tile before has been read
-        for (int i = tid; i < PLAIN_TILE * per_row; i += PLAIN_THREADS) {
-            const int k = i / per_row, d = (i - k * per_row) * 4, key = key0 + k;
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-            if (key < key_hi && key / p.page_size < p.max_blocks) {
-                const int page = table[key / p.page_size];
-                if (page >= 0 && page < p.num_pages) {
-                    const size_t at = (((size_t)page * 2 * p.nkv + kvh) * p.page_size + key % p.page_size) * p.hd + d;
-                    constexpr int dt = sizeof(T) == 4 ? RV_DTYPE_F32 : RV_DTYPE_BF16;
-                    a = rv_load4(cache, dt, at);
-                    b = rv_load4(cache, dt, at + (size_t)p.nkv * p.page_size * p.hd);
-                }
-            }
-            *reinterpret_cast<float4*>(k_s + k * stride + d) = a;
-            *reinterpret_cast<float4*>(v_s + k * stride + d) = b;
+        const bool there = page >= 0 && page < p.num_pages;
+        const size_t at = (((size_t)max(page, 0) * 2 * p.nkv + kvh) * p.page_size + (key0 + mine) % p.page_size) * p.hd;
+#pragma unroll 4
+        for (int d = quarter; d < p.hd; d += 16) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+            if (there) { x = rv_load4(p.cache, dt, at + d); y = rv_load4(p.cache, dt, at + plane + d); }
+            *reinterpret_cast<float4*>(k_s + mine * stride + d) = x;
+            *reinterpret_cast<float4*>(v_s + mine * stride + d) = y;
         }
+        if (quarter == 0) there_s[mine] = there;
+        page = page_of(key0 + PLAIN_TILE + mine);
         __syncthreads();
         float s[RPW];
 #pragma unroll
@@ -126,7 +134,7 @@ shared_plain_kernel(const PlainParams p) {
             const int r = warp * RPW + i;
             float v = s[i];
             if (p.softcap > 0.f) v = p.softcap * tanhf(v / p.softcap);
-            v = key0 + lane < lim_s[r] ? v * 1.4426950408889634f : -INFINITY;
+            v = key0 + lane < lim_s[r] && there_s[lane] ? v * 1.4426950408889634f : -INFINITY;
             const float m_new = fmaxf(m[i], rv_warp_max(v));
             const float m_s = m_new == -INFINITY ? 0.f : m_new;
             const float keep = exp2f(m[i] - m_s), e = exp2f(v - m_s);
@@ -171,8 +179,8 @@ shared_plain_kernel(const PlainParams p) {
 template <typename T, int RPW, int DPL, bool OWN>
 static int launch_plain(const PlainParams& p, dim3 grid, cudaStream_t stream) {
     const int R = 4 * RPW;
-    const int smem = (R * p.hd + 2 * PLAIN_TILE * (p.hd + 4) + R * PLAIN_TILE + 2 * R) * 4;
-    const int most = (R * PLAIN_MAX_DIM + 2 * PLAIN_TILE * (PLAIN_MAX_DIM + 4) + R * PLAIN_TILE + 2 * R) * 4;
+    const int smem = (R * p.hd + 2 * PLAIN_TILE * (p.hd + 4) + R * PLAIN_TILE + 2 * R + PLAIN_TILE) * 4;
+    const int most = (R * PLAIN_MAX_DIM + 2 * PLAIN_TILE * (PLAIN_MAX_DIM + 4) + R * PLAIN_TILE + 2 * R + PLAIN_TILE) * 4;
     static RvPerDevice configured;
     if (int e = rv_configure_smem(configured, shared_plain_kernel<T, RPW, DPL, OWN>, most)) return e;
     RV_LAUNCH_ST = rv_launch(shared_plain_kernel<T, RPW, DPL, OWN>, grid, dim3(PLAIN_THREADS), smem, stream, p);
@@ -184,37 +192,6 @@ static int launch_plain_dim(const PlainParams& p, dim3 grid, cudaStream_t stream
     return p.hd <= 128 ? launch_plain<T, RPW, 4, OWN>(p, grid, stream) : launch_plain<T, RPW, 8, OWN>(p, grid, stream);
 }
 
-// part 0: the ranges of the prefixes (part_o [cap_items, nkv, SP_ROWS, hd]); part 1: the keys behind them, cut into `splits` ranges
-// (part_o [splits, num_seqs, nh, hd])
-RV_EXPORT int rv_shared_plain(const void* q, const void* cache, long long num_pages, const int* block_tables, const int* ctx_lens,
-                              const int* plan, int num_seqs, int cap_tiles, int cap_items, float* part_o, float* part_ml,
-                              int nh, int nkv, int hd, int page_size, int max_blocks, float scale, float softcap, int part,
-                              int splits, int dtype, cudaStream_t stream) {
-    if (num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 ||
-        cap_tiles < 0 || cap_items < 0 || splits < 1 || !plan || !part_o || !part_ml)
-        return RV_ERR_BAD_SIZE;
-    if (dtype != RV_DTYPE_F32 && dtype != RV_DTYPE_BF16) return RV_ERR_BAD_DTYPE;
-    if (hd % 4 || hd > PLAIN_MAX_DIM || nh / nkv > SP_ROWS) return RV_ERR_UNSUPPORTED;
-    if (num_seqs > 65535 || splits > 65535 || cap_items > 65535) return RV_ERR_UNSUPPORTED;
-    if ((reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(part_o) | reinterpret_cast<uintptr_t>(plan)) % 16 ||
-        reinterpret_cast<uintptr_t>(part_ml) % 8)
-        return RV_ERR_ALIGNMENT;
-    if (num_seqs == 0 || (part == 0 && cap_items == 0)) return RV_OK;
-    PlainParams p;
-    p.plan = shared_plan(plan, num_seqs, cap_tiles, cap_items);
-    p.q = q; p.cache = cache; p.block_tables = block_tables; p.ctx_lens = ctx_lens;
-    p.part_o = part_o; p.part_ml = part_ml; p.num_pages = num_pages; p.num_seqs = num_seqs;
-    p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = page_size; p.max_blocks = max_blocks; p.splits = splits;
-    p.scale = scale; p.softcap = softcap;
-    const int G = nh / nkv;
-    if (part == 0) {
-        const dim3 grid(nkv * ((SP_ROWS / G * G + 31) / 32), cap_items);
-        return dtype == RV_DTYPE_F32 ? launch_plain_dim<float, 8, false>(p, grid, stream) : launch_plain_dim<__nv_bfloat16, 8, false>(p, grid, stream);
-    }
-    const dim3 grid(nkv * ((G + 7) / 8), splits, num_seqs);
-    return dtype == RV_DTYPE_F32 ? launch_plain_dim<float, 2, true>(p, grid, stream) : launch_plain_dim<__nv_bfloat16, 2, true>(p, grid, stream);
-}
-
 // ---------------------------------------------------------------------------------------------
 // The merge: hd / 4 threads per (token, head) row, four neighbouring elements each, eight ranges' loads in flight at a time.
 struct MergeParams {
@@ -223,7 +200,6 @@ struct MergeParams {
     const float* pre_ml;
     const float* own_o;            // [splits, num_seqs, nh, hd]
     const float* own_ml;
-    const int* own_count;          // [num_seqs, nkv] ranges of the own keys, or null: `splits` of them
     const float* sinks;            // [nh] or null
     const float* gate;             // [num_seqs, nh] or null
     void* out;                     // [num_seqs, nh, hd]
@@ -288,7 +264,7 @@ shared_merge_kernel(const MergeParams p) {
                      (size_t)p.nkv * SP_ROWS, parts.y, p.hd, d);
     }
     const size_t out_row = (size_t)seq * p.nh + head;
-    merge_ranges(v, p.own_o, p.own_ml, out_row, (size_t)p.num_seqs * p.nh, p.own_count ? p.own_count[seq * p.nkv + kvh] : p.splits, p.hd, d);
+    merge_ranges(v, p.own_o, p.own_ml, out_row, (size_t)p.num_seqs * p.nh, p.splits, p.hd, d);
     float num = 1.f, den = v.l;
     if (p.sinks) {                                       // exp(sink) joins the denominator; it has no value
         const float sk = p.sinks[head] * 1.4426950408889634f;
@@ -302,24 +278,52 @@ shared_merge_kernel(const MergeParams p) {
     rv_store4(p.out, dt, out_row * p.hd + d, make_float4(v.o.x * inv, v.o.y * inv, v.o.z * inv, v.o.w * inv));
 }
 
-RV_EXPORT int rv_shared_merge(const int* plan, int num_seqs, int cap_tiles, int cap_items, const float* pre_o, const float* pre_ml,
-                              const float* own_o, const float* own_ml, const int* own_count, int splits, void* out,
-                              const float* sinks, const float* gate, int nh, int nkv, int hd, int dtype, cudaStream_t stream) {
-    if (num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || cap_tiles < 0 || cap_items < 0 || splits < 1 || !plan ||
-        !own_o || !own_ml)
+// The arguments, packed by the caller in this order (a step makes this call once a layer).
+struct PlainArgs {
+    const void* q; const void* cache; const int* block_tables; const int* ctx_lens; const int* plan;
+    float* pre_o; float* pre_ml; float* own_o; float* own_ml; void* out; const float* sinks; const float* gate; cudaStream_t stream;
+    long long num_pages;
+    int num_seqs, cap_tiles, cap_items, nh, nkv, hd, page_size, max_blocks, splits, dtype;
+    float scale, softcap;
+};
+
+// pre_o [cap_items, nkv, SP_ROWS, hd], own_o [splits, num_seqs, nh, hd] and the same with 2 in place of hd receive the parts' sums.
+RV_EXPORT int rv_shared_attention_plain(const PlainArgs* a) {
+    const int nh = a->nh, nkv = a->nkv, hd = a->hd;
+    if (a->num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || a->page_size <= 0 || a->max_blocks <= 0 || a->num_pages <= 0 ||
+        a->cap_tiles < 0 || a->cap_items <= 0 || a->splits < 1 || !a->plan || !a->pre_o || !a->pre_ml || !a->own_o || !a->own_ml)
         return RV_ERR_BAD_SIZE;
-    if (dtype != RV_DTYPE_F32 && dtype != RV_DTYPE_BF16) return RV_ERR_BAD_DTYPE;
-    if (hd % 4 || hd > PLAIN_MAX_DIM) return RV_ERR_UNSUPPORTED;
-    if (num_seqs == 0) return RV_OK;
-    MergeParams p;
-    p.plan = shared_plan(plan, num_seqs, cap_tiles, cap_items);
-    p.pre_o = pre_o; p.pre_ml = pre_ml; p.own_o = own_o; p.own_ml = own_ml; p.own_count = own_count; 
-    p.sinks = sinks; p.gate = gate; p.out = out;
-    p.num_seqs = num_seqs; p.nh = nh; p.nkv = nkv; p.hd = hd; p.splits = splits;
-    p.rows_per_block = 128 / (hd / 4);
-    const long long blocks = ((long long)num_seqs * nh + p.rows_per_block - 1) / p.rows_per_block;
+    if (a->dtype != RV_DTYPE_F32 && a->dtype != RV_DTYPE_BF16) return RV_ERR_BAD_DTYPE;
+    if (hd % 4 || hd > PLAIN_MAX_DIM || nh / nkv > SP_ROWS) return RV_ERR_UNSUPPORTED;
+    if (a->num_seqs > 65535 || a->splits > 65535 || a->cap_items > 65535) return RV_ERR_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->cache) | reinterpret_cast<uintptr_t>(a->pre_o) |
+         reinterpret_cast<uintptr_t>(a->own_o) | reinterpret_cast<uintptr_t>(a->plan) | reinterpret_cast<uintptr_t>(a->out)) % 16 ||
+        (reinterpret_cast<uintptr_t>(a->pre_ml) | reinterpret_cast<uintptr_t>(a->own_ml)) % 8)
+        return RV_ERR_ALIGNMENT;
+    if (a->num_seqs == 0) return RV_OK;
+    PlainParams p;
+    p.plan = shared_plan(a->plan, a->num_seqs, a->cap_tiles, a->cap_items);
+    p.q = a->q; p.cache = a->cache; p.block_tables = a->block_tables; p.ctx_lens = a->ctx_lens;
+    p.num_pages = a->num_pages; p.num_seqs = a->num_seqs;
+    p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = a->page_size; p.max_blocks = a->max_blocks; p.splits = a->splits;
+    p.scale = a->scale; p.softcap = a->softcap;
+    const int G = nh / nkv;
+    const bool wide = a->dtype == RV_DTYPE_F32;
+    const dim3 grid(nkv * ((SP_ROWS / G * G + 31) / 32), a->cap_items), own_grid(nkv * ((G + 7) / 8), a->splits, a->num_seqs);
+    p.part_o = a->pre_o; p.part_ml = a->pre_ml;
+    int st = wide ? launch_plain_dim<float, 8, false>(p, grid, a->stream) : launch_plain_dim<__nv_bfloat16, 8, false>(p, grid, a->stream);
+    if (st != RV_OK) return st;
+    p.part_o = a->own_o; p.part_ml = a->own_ml;
+    st = wide ? launch_plain_dim<float, 2, true>(p, own_grid, a->stream) : launch_plain_dim<__nv_bfloat16, 2, true>(p, own_grid, a->stream);
+    if (st != RV_OK) return st;
+    MergeParams m;
+    m.plan = p.plan; m.pre_o = a->pre_o; m.pre_ml = a->pre_ml; m.own_o = a->own_o; m.own_ml = a->own_ml;
+    m.sinks = a->sinks; m.gate = a->gate; m.out = a->out;
+    m.num_seqs = a->num_seqs; m.nh = nh; m.nkv = nkv; m.hd = hd; m.splits = a->splits;
+    m.rows_per_block = 128 / (hd / 4);
+    const long long blocks = ((long long)a->num_seqs * nh + m.rows_per_block - 1) / m.rows_per_block;
     if (blocks > 0x7fffffffLL) return RV_ERR_UNSUPPORTED;
-    if (dtype == RV_DTYPE_F32) RV_LAUNCH_ST = rv_launch(shared_merge_kernel<float>, dim3((unsigned)blocks), dim3(128), 0, stream, p);
-    else RV_LAUNCH_ST = rv_launch(shared_merge_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(128), 0, stream, p);
+    if (wide) RV_LAUNCH_ST = rv_launch(shared_merge_kernel<float>, dim3((unsigned)blocks), dim3(128), 0, a->stream, m);
+    else RV_LAUNCH_ST = rv_launch(shared_merge_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(128), 0, a->stream, m);
     return rv_launch_status();
 }

@@ -121,19 +121,18 @@ step_tables_kernel(const TableParams p) {
     __threadfence();
 }
 
-RV_EXPORT int rv_step_tables(int* page_table, const int* rows, const int* held, const int* starts, const int* q_lens, const int* new_pages,
-                             const int* spans, int* block_tables, int* slot_mapping, int* positions, int* token_seq, int* cu_seqlens,
-                             int* ctx_lens, int groups, int num_seqs, int table_rows, int table_width, int num_new, int num_tokens,
-                             int max_blocks, int page_size, cudaStream_t stream) {
-    if (groups < 1 || num_seqs < 1 || table_rows < 1 || table_width < 1 || num_new < 0 || num_tokens < 0 || max_blocks < 1 || page_size < 1)
-        return RV_ERR_BAD_SIZE;
-    if (groups > 65535) return RV_ERR_UNSUPPORTED;
+// The arguments, packed by the caller in the order of TableParams, then the stream.
+struct TableArgs {
     TableParams p;
-    p.page_table = page_table; p.rows = rows; p.held = held; p.starts = starts; p.q_lens = q_lens; p.new_pages = new_pages; p.spans = spans;
-    p.block_tables = block_tables; p.slot_mapping = slot_mapping; p.positions = positions; p.token_seq = token_seq;
-    p.cu_seqlens = cu_seqlens; p.ctx_lens = ctx_lens;
-    p.groups = groups; p.num_seqs = num_seqs; p.table_rows = table_rows; p.table_width = table_width; p.num_new = num_new;
-    p.num_tokens = num_tokens; p.max_blocks = max_blocks; p.page_size = page_size;
-    RV_LAUNCH_ST = rv_launch(step_tables_kernel, dim3(num_seqs, groups), dim3(TABLE_THREADS), 0, stream, p);
+    cudaStream_t stream;
+};
+
+RV_EXPORT int rv_step_tables(const TableArgs* a) {
+    const TableParams& p = a->p;
+    if (p.groups < 1 || p.num_seqs < 1 || p.table_rows < 1 || p.table_width < 1 || p.num_new < 0 || p.num_tokens < 0 || p.max_blocks < 1 ||
+        p.page_size < 1)
+        return RV_ERR_BAD_SIZE;
+    if (p.groups > 65535) return RV_ERR_UNSUPPORTED;
+    RV_LAUNCH_ST = rv_launch(step_tables_kernel, dim3(p.num_seqs, p.groups), dim3(TABLE_THREADS), 0, a->stream, p);
     return rv_launch_status();
 }

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_void_p, c_int, c_float
 from typing import Optional
 
@@ -20,7 +21,7 @@ import torch
 
 from ..errors import KernelError
 from . import build
-from .shared import SharedPrefixes, StepTables, KEY_TILE, TILE_ROWS
+from .shared import SharedPrefixes, StepTables, TILE_ROWS
 
 _DT = {torch.float32: 0, torch.bfloat16: 1}
 _GATED_PREFILL, _GATED_DECODE = {"silu": 2, "gelu_tanh": 4, "swiglu_clamp": 5}, {"silu": 1, "gelu_tanh": 2, "swiglu_clamp": 3}
@@ -51,6 +52,21 @@ def _need(t: torch.Tensor, name: str, dtype=None, dims=None):
         raise KernelError(f"{name} must be {dtype}, got {t.dtype}")
     if dims is not None and t.dim() != dims:
         raise KernelError(f"{name} must have {dims} dimensions, got shape {tuple(t.shape)}")
+
+
+# arguments of the entry points that take them as one block (the structures of the same names in csrc/)
+_SHARED_ARGS = struct.Struct("=13q9i2f")       # shared_attention_tcgen05.cu
+_PLAIN_ARGS = struct.Struct("=14q10i2f")       # shared_prefix.cu
+_TABLE_ARGS = struct.Struct("=13q8iq")         # step_tables.cu
+
+
+def _same_device(here: int, named) -> None:
+    """Every tensor is contiguous and lies on the current CUDA device, on whose stream the kernels are launched."""
+    for t, name in named:
+        if t.get_device() != here:
+            raise KernelError(f"{name} must be a CUDA tensor on the current device, cuda:{here}; it lies on {t.device}")
+        if not t.is_contiguous():
+            raise KernelError(f"{name} must be contiguous, got strides {t.stride()} for shape {tuple(t.shape)}")
 
 
 class AttentionMeta:
@@ -136,6 +152,7 @@ class CudaKernels:
         torch.backends.cudnn.allow_tf32 = False
         self.num_sms = torch.cuda.get_device_properties(self.device).multi_processor_count
         self._libs = {}
+        self._entries = {}
         self._pdl_allowed = True     # a model may switch programmatic dependent launch off for its steps (`set_pdl`)
         self._decode_counters = None
         # one status word for every tcgen05 launch of the engine: a kernel whose bounded wait on an
@@ -387,13 +404,10 @@ class CudaKernels:
         of the memory), the merge kernel 2.5 us.  The split count with the least modelled time is
         taken: it fills one wave when the batch is small and keeps the last wave full when it is
         large."""
-        return self._splits(meta.num_seqs, meta.max_ctx_len, num_heads, num_kv_heads)
-
-    def _splits(self, num_seqs: int, longest: int, num_heads: int, num_kv_heads: int) -> int:
         self_max_splits = 64          # a long context at a small batch still fills the GPU (one sequence of 32,768 keys: 55)
         group = num_heads // num_kv_heads
-        ctas = num_seqs * num_kv_heads * ((group + 15) // 16)
-        tiles = max(1, (longest + 63) // 64)
+        ctas = meta.num_seqs * num_kv_heads * ((group + 15) // 16)
+        tiles = max(1, (meta.max_ctx_len + 63) // 64)
         best, best_t = 1, float("inf")
         for s in range(1, min(self_max_splits, tiles) + 1):
             per = -(-tiles // s)
@@ -504,12 +518,16 @@ class CudaKernels:
         return out
 
     # ------------------------------------------------------------------ tokens that requests share
-    def _on_this_device(self, *named):
-        """Every tensor lies on the device that is current, whose stream the kernels are launched on."""
-        here = torch.cuda.current_device()
-        for t, name in named:
-            if t is not None and (not t.is_cuda or t.device.index != here):
-                raise KernelError(f"{name} lies on {t.device}, but the current device is cuda:{here}")
+    def _entry(self, source: str, defines, name: str):
+        """An exported function that takes its arguments packed into one block of bytes, looked up once (twenty arguments as ctypes
+        objects were half of what such a call cost the host)."""
+        key = (source, defines, name)
+        fn = self._entries.get(key)
+        if fn is None:
+            fn = getattr(self._lib(source, defines), name)
+            fn.argtypes = [ctypes.c_char_p]
+            self._entries[key] = fn
+        return fn
 
     def shared_prefix_attention(self, q, cache_layer, meta: AttentionMeta, shared: SharedPrefixes, num_heads, num_kv_heads, head_dim,
                                 scale: float, softcap: Optional[float] = None, sinks: Optional[torch.Tensor] = None,
@@ -522,81 +540,79 @@ class CudaKernels:
         lengths see different parts of a prefix.  `max_own`: no sequence has more keys behind its prefix (sizes the launch
         only; without it the longest context less the shortest prefix is taken).
 
-        bfloat16 with heads of 64 or 128, up to 128 query heads on a key/value head and pages of a power of two from 8 on: the prefixes on the
-        tcgen05 kernel, the rest on the TMA-fed decode kernels.  float32, and other sizes whose head is a multiple of 4 up to
-        256: the plain kernels.  What neither takes, and steps without a group, go to `paged_attention`, to which every table
-        is whole."""
-        _need(q, "q", dims=2); _need(cache_layer, "cache_layer", q.dtype, 5)
-        _need(meta.block_tables, "block_tables", torch.int32, 2); _need(meta.ctx_lens, "ctx_lens", torch.int32, 1)
+        bfloat16 with heads of 64 or 128 and pages of a power of two from 8 on: the prefixes on the tcgen05 kernel, the rest on
+        the TMA-fed decode kernels.  float32, and other sizes whose head is a multiple of 4 up to 256: the plain kernels.  What
+        neither takes (more than 128 query heads on a key/value head among it), and steps without a group, go to
+        `paged_attention`, to which every table is whole."""
+        tables, lens = meta.block_tables, meta.ctx_lens
+        here = torch._C._cuda_getDevice()
+        _same_device(here, ((q, "q"), (cache_layer, "cache_layer"), (tables, "block_tables"), (lens, "ctx_lens"), (shared.device_ints, "shared")))
         dt = self._dt(q, "q")
+        if q.dim() != 2 or cache_layer.dim() != 5 or cache_layer.dtype != q.dtype or tables.dim() != 2 or tables.dtype != torch.int32 \
+                or lens.dim() != 1 or lens.dtype != torch.int32:
+            raise KernelError(f"shared_prefix_attention: q {tuple(q.shape)} of {q.dtype}, a cache layer {tuple(cache_layer.shape)} of "
+                              f"{cache_layer.dtype}, block tables {tuple(tables.shape)} of {tables.dtype}, lengths {tuple(lens.shape)} of {lens.dtype}")
         B = meta.num_seqs
-        if meta.max_q_len > 1 or q.shape[0] != B:
-            raise KernelError(f"shared_prefix_attention: {q.shape[0]} tokens of {B} sequences, the longest of {meta.max_q_len}: every sequence "
+        tokens, width = q.shape
+        pages, planes, kv_heads, page, size = cache_layer.shape
+        if meta.max_q_len > 1 or tokens != B:
+            raise KernelError(f"shared_prefix_attention: {tokens} tokens of {B} sequences, the longest of {meta.max_q_len}: every sequence "
                               "brings one")
-        if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or q.shape[1] != num_heads * head_dim:
-            raise KernelError(f"shared_prefix_attention: rows of {q.shape[1]} for {num_heads} heads of {head_dim} on {num_kv_heads}")
-        if tuple(cache_layer.shape[1:3]) != (2, num_kv_heads) or cache_layer.shape[4] != head_dim:
+        if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or width != num_heads * head_dim:
+            raise KernelError(f"shared_prefix_attention: rows of {width} for {num_heads} heads of {head_dim} on {num_kv_heads}")
+        if planes != 2 or kv_heads != num_kv_heads or size != head_dim:
             raise KernelError(f"shared_prefix_attention: a cache layer of shape {tuple(cache_layer.shape)} for {num_kv_heads} key/value heads of {head_dim}")
         if (shared.num_seqs, shared.num_heads, shared.num_kv_heads) != (B, num_heads, num_kv_heads):
             raise KernelError(f"shared_prefix_attention: prefixes laid out for {shared.num_seqs} sequences of {shared.num_heads} heads on "
                               f"{shared.num_kv_heads}, a step of {B} of {num_heads} on {num_kv_heads}")
-        if meta.block_tables.shape[0] < B or meta.ctx_lens.shape[0] < B:
-            raise KernelError(f"shared_prefix_attention: tables of {meta.block_tables.shape[0]} and lengths of {meta.ctx_lens.shape[0]} sequences for {B}")
-        self._check_attention_extras(q, num_heads, sinks, gate)
-        self._on_this_device((q, "q"), (cache_layer, "cache_layer"), (meta.block_tables, "block_tables"), (meta.ctx_lens, "ctx_lens"),
-                             (shared.device_ints, "shared"), (sinks, "sinks"), (gate, "gate"))
-        page, group = cache_layer.shape[3], num_heads // num_kv_heads
-        power = page & (page - 1) == 0
-        fast = q.dtype == torch.bfloat16 and head_dim in (64, 128) and power and page >= 8 and cache_layer.shape[0] * 2 * num_kv_heads * page < 2 ** 31
-        if shared.capacity[1] == 0 or B == 0 or group > TILE_ROWS or not (fast or (head_dim % 4 == 0 and head_dim <= 256)):
+        if tables.shape[0] < B or lens.shape[0] < B:
+            raise KernelError(f"shared_prefix_attention: tables of {tables.shape[0]} and lengths of {lens.shape[0]} sequences for {B}")
+        if sinks is not None or gate is not None:
+            self._check_attention_extras(q, num_heads, sinks, gate)
+            _same_device(here, tuple((t, name) for t, name in ((sinks, "sinks"), (gate, "gate")) if t is not None))
+        group = num_heads // num_kv_heads
+        fast = dt == 1 and head_dim in (64, 128) and page & (page - 1) == 0 and page >= 8 and pages * 2 * num_kv_heads * page < 2 ** 31
+        tiles, items = shared.capacity
+        if items == 0 or B == 0 or group > TILE_ROWS or not (fast or (head_dim % 4 == 0 and head_dim <= 256)):
             return self.paged_attention(q, cache_layer, meta, num_heads, num_kv_heads, head_dim, scale, None, softcap, sinks, gate)
         if max_own is None:
-            max_own = meta.max_ctx_len - (min(t for _, t in shared.groups) if sum(len(m) for m, _ in shared.groups) == B else 0)
-        max_own = max(1, min(max_own, meta.max_ctx_len))
-        tiles, items = shared.capacity
+            max_own = meta.max_ctx_len - shared.shortest
+        pre_rows = items * num_kv_heads * TILE_ROWS
         out = torch.empty_like(q)
-        row = head_dim + 2
-        pre = torch.empty((items * num_kv_heads * TILE_ROWS * row,), dtype=torch.float32, device=q.device)
-        pre_ml = pre[items * num_kv_heads * TILE_ROWS * head_dim:]
-        counts, pieces = None, 1
-        layout = (c_int(num_heads), c_int(num_kv_heads), c_int(head_dim), c_int(page), c_int(meta.max_blocks), c_float(scale))
-        plan = (_ptr(shared.device_ints), c_int(B), c_int(tiles), c_int(items))
-        pages = ctypes.c_longlong(cache_layer.shape[0])
-        lib = self._lib("shared_prefix.cu")
+        plan_at, q_at, cache_at, tables_at, lens_at, out_at = (shared.device_ints.data_ptr(), q.data_ptr(), cache_layer.data_ptr(), tables.data_ptr(),
+                                                               lens.data_ptr(), out.data_ptr())
+        sinks_at, gate_at = 0 if sinks is None else sinks.data_ptr(), 0 if gate is None else gate.data_ptr()
+        stream, cap = torch._C._cuda_getCurrentRawStream(here), softcap or 0.0
         if fast:
-            st = self._lib("prefix_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",)).rv_prefix_attention_tcgen05(
-                _ptr(q), _ptr(cache_layer), pages, _ptr(meta.block_tables), _ptr(meta.ctx_lens), *plan, _ptr(pre), _ptr(pre_ml), *layout,
-                c_float(softcap or 0.0), _ptr(self._status), self._stream())
-            _check("prefix_attention_tcgen05", st)
-            flash = self._lib("attention_flash.cu", (f"-DHEAD_DIM={head_dim}",))
-            common = (_ptr(q), _ptr(cache_layer), pages, _ptr(meta.block_tables), _ptr(meta.cu_seqlens), _ptr(meta.ctx_lens), _ptr(shared.own_start))
-            if softcap is None and self.BALANCED_DECODE and group <= 16 and B <= 240 and B * num_kv_heads >= self.BALANCED_MIN_PAIRS:
-                ctas = self._balanced_tma_ctas(flash, num_heads, num_kv_heads)
-                pieces = flash.rv_flash_balanced_max_pieces(c_int(meta.max_ctx_len + KEY_TILE), c_int(num_kv_heads), c_int(ctas))
-                own = torch.empty((pieces * B * num_heads * row,), dtype=torch.float32, device=q.device)
-                counts = torch.empty((B * num_kv_heads,), dtype=torch.int32, device=q.device)
-                st = flash.rv_flash_decode_balanced_parts(*common, _ptr(own), _ptr(counts), c_int(pieces), c_int(B), c_int(B), *layout,
-                                                          c_int(ctas), _ptr(self._status), self._stream())
-                _check("flash_decode_balanced_parts", st)
-            else:
-                pieces = self._splits(B, max_own + KEY_TILE - 1, num_heads, num_kv_heads)
-                own = torch.empty((pieces * B * num_heads * row,), dtype=torch.float32, device=q.device)
-                st = flash.rv_flash_decode_tma_parts(*common, _ptr(own), c_int(B), c_int(B), *layout, c_int(pieces), _ptr(self._status),
-                                                     c_int(1 if (self.TMA_DECODE_EARLY and self.pdl) else 0), c_float(softcap or 0.0),
-                                                     self._stream())
-                _check("flash_decode_tma_parts", st)
-        else:
-            pieces = max(1, min(64, -(-max_own // 64), 4 * self.num_sms // max(1, B * num_kv_heads)))
-            own = torch.empty((pieces * B * num_heads * row,), dtype=torch.float32, device=q.device)
-            for part, buf, ml in ((0, pre, pre_ml), (1, own, own[pieces * B * num_heads * head_dim:])):
-                st = lib.rv_shared_plain(_ptr(q), _ptr(cache_layer), pages, _ptr(meta.block_tables), _ptr(meta.ctx_lens), *plan, _ptr(buf),
-                                         _ptr(ml), *layout, c_float(softcap or 0.0), c_int(part), c_int(pieces), c_int(dt), self._stream())
-                _check("shared_plain", st)
-        st = lib.rv_shared_merge(*plan, _ptr(pre), _ptr(pre_ml), _ptr(own), _ptr(own[pieces * B * num_heads * head_dim:]), _ptr(counts),
-                                 c_int(pieces), _ptr(out), _ptr(sinks), _ptr(gate), c_int(num_heads), c_int(num_kv_heads), c_int(head_dim),
-                                 c_int(dt), self._stream())
-        _check("shared_merge", st)
+            scratch = torch.empty((pre_rows * (head_dim + 2),), dtype=torch.float32, device=q.device)
+            pre = scratch.data_ptr()
+            st = self._entry("shared_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",), "rv_shared_attention_tcgen05")(_SHARED_ARGS.pack(
+                q_at, cache_at, tables_at, lens_at, plan_at, pre, pre + 4 * pre_rows * head_dim, out_at, sinks_at, gate_at,
+                self._status.data_ptr(), stream, pages, B, tiles, items, num_heads, num_kv_heads, head_dim, page, tables.shape[1],
+                self._own_ctas(B * num_kv_heads * (1 if group <= 8 else -(-group // 16)), max_own), scale, cap))
+            _check("shared_attention_tcgen05", st)
+            COUNTERS['launches'] += 1
+            return out
+        splits = max(1, min(64, -(-max_own // 64), 4 * self.num_sms // (B * num_kv_heads)))
+        own_rows = splits * B * num_heads
+        scratch = torch.empty(((pre_rows + own_rows) * (head_dim + 2),), dtype=torch.float32, device=q.device)
+        pre = scratch.data_ptr()
+        pre_ml = pre + 4 * pre_rows * head_dim
+        own = pre_ml + 8 * pre_rows
+        st = self._entry("shared_prefix.cu", (), "rv_shared_attention_plain")(_PLAIN_ARGS.pack(
+            q_at, cache_at, tables_at, lens_at, plan_at, pre, pre_ml, own, own + 4 * own_rows * head_dim, out_at, sinks_at, gate_at, stream, pages,
+            B, tiles, items, num_heads, num_kv_heads, head_dim, page, tables.shape[1], splits, dt, scale, cap))
+        _check("shared_attention_plain", st)
+        COUNTERS['launches'] += 2
         return out
+
+    def _own_ctas(self, pairs: int, max_own: int) -> int:
+        """CTAs that share the keys of a sequence and kv head behind its prefix (a cluster): as many as there is room for, while each
+        still has four chunks of 16 keys for its warps."""
+        ctas = 1
+        while ctas < 8 and pairs * ctas * 2 <= 3 * self.num_sms and max_own > 64 * ctas:
+            ctas *= 2
+        return ctas
 
     def step_tables(self, page_table: torch.Tensor, rows: torch.Tensor, held: torch.Tensor, starts: torch.Tensor, q_lens: torch.Tensor,
                     new_pages: torch.Tensor, spans: torch.Tensor, num_tokens: int, max_blocks: int, page_size: int,
@@ -612,29 +628,37 @@ class CudaKernels:
 
         `num_tokens` = the sum of q_lens and `max_blocks` >= the most blocks of a sequence, as the caller knows them.  With `out`
         the tables are written into tensors of the caller (those a captured graph reads)."""
-        tensors = ((page_table, "page_table", 3), (rows, "rows", 1), (held, "held", 2), (starts, "starts", 1), (q_lens, "q_lens", 1),
-                   (new_pages, "new_pages", 1), (spans, "spans", 2))
-        for t, name, dims in tensors:
-            _need(t, name, torch.int32, dims)
+        here = torch._C._cuda_getDevice()
+        given = (page_table, rows, held, starts, q_lens, new_pages, spans)
+        for t in given:
+            if t.dtype is not torch.int32 or t.get_device() != here or not t.is_contiguous():
+                raise KernelError(f"step_tables: the inputs are contiguous int32 tensors on the current device, cuda:{here}; one is {t.dtype} of "
+                                  f"shape {tuple(t.shape)} with strides {t.stride()} on {t.device}")
+        if page_table.dim() != 3 or rows.dim() != 1 or new_pages.dim() != 1:
+            raise KernelError(f"step_tables: a page table of shape {tuple(page_table.shape)}, rows {tuple(rows.shape)}, new pages {tuple(new_pages.shape)}")
         G, R, width = page_table.shape
         B = rows.shape[0]
-        if held.shape != (G, B) or starts.shape[0] != B or q_lens.shape[0] != B or spans.shape != (G, 2):
+        if held.shape != (G, B) or starts.shape != (B,) or q_lens.shape != (B,) or spans.shape != (G, 2):
             raise KernelError(f"step_tables: {B} rows in {G} groups, but held {tuple(held.shape)}, starts {tuple(starts.shape)}, q_lens "
                               f"{tuple(q_lens.shape)}, spans {tuple(spans.shape)}")
-        if num_tokens < 0 or max_blocks < 1 or page_size < 1 or min(G, B, R, width) < 1:
+        if num_tokens < 0 or max_blocks < 1 or page_size < 1 or G < 1 or B < 1 or R < 1 or width < 1:
             raise KernelError(f"step_tables: {num_tokens} tokens of {B} sequences, {max_blocks} blocks of {page_size}, a page table of {(G, R, width)}")
-        shapes = ((G, B, max_blocks), (G, num_tokens), (num_tokens,), (num_tokens,), (B + 1,), (B,))
         if out is None:
-            out = StepTables(*(torch.empty(s, dtype=torch.int32, device=page_table.device) for s in shapes))
-        made = (out.block_tables, out.slot_mapping, out.positions, out.token_seq, out.cu_seqlens, out.ctx_lens)
-        for t, s in zip(made, shapes):
-            _need(t, "out", torch.int32)
-            if tuple(t.shape) != s:
-                raise KernelError(f"step_tables: an output of shape {tuple(t.shape)} where {s} is written")
-        self._on_this_device(*((t, name) for t, name, _ in tensors), *((t, "out") for t in made))
-        st = self._lib("step_tables.cu").rv_step_tables(
-            *(_ptr(t) for t, _, _ in tensors), *(_ptr(t) for t in made), c_int(G), c_int(B), c_int(R), c_int(width),
-            c_int(new_pages.shape[0]), c_int(num_tokens), c_int(max_blocks), c_int(page_size), self._stream())
+            # one allocation: block tables, slots, positions, sequences of the tokens, their starts, context lengths
+            parts = torch.empty((G * (B * max_blocks + num_tokens) + 2 * num_tokens + 2 * B + 1,), dtype=torch.int32, device=page_table.device
+                                ).split_with_sizes((G * B * max_blocks, G * num_tokens, num_tokens, num_tokens, B + 1, B))
+            out = StepTables(parts[0].view(G, B, max_blocks), parts[1].view(G, num_tokens), parts[2], parts[3], parts[4], parts[5])
+        else:
+            for t, shape in ((out.block_tables, (G, B, max_blocks)), (out.slot_mapping, (G, num_tokens)), (out.positions, (num_tokens,)),
+                             (out.token_seq, (num_tokens,)), (out.cu_seqlens, (B + 1,)), (out.ctx_lens, (B,))):
+                if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != here or not t.is_contiguous():
+                    raise KernelError(f"step_tables: an output of shape {tuple(t.shape)} and {t.dtype} on {t.device} where contiguous int32 {shape} "
+                                      f"on cuda:{here} is written")
+        st = self._entry("step_tables.cu", (), "rv_step_tables")(_TABLE_ARGS.pack(
+            page_table.data_ptr(), rows.data_ptr(), held.data_ptr(), starts.data_ptr(), q_lens.data_ptr(), new_pages.data_ptr(), spans.data_ptr(),
+            out.block_tables.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.token_seq.data_ptr(),
+            out.cu_seqlens.data_ptr(), out.ctx_lens.data_ptr(), G, B, R, width, new_pages.shape[0], num_tokens, max_blocks, page_size,
+            torch._C._cuda_getCurrentRawStream(here)))
         _check("step_tables", st)
         return out
 

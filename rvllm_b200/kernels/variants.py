@@ -22,7 +22,7 @@ def all_variants() -> List[Tuple[str, Sequence[str]]]:
         elif src == "attention_tcgen05.cu":
             out.extend((src, (f"-DHEAD_DIM={hd}",)) for hd in (64, 128))
             out.extend((src, (f"-DLATENT_ROW={row}", f"-DV_DIM={vd}")) for row, vd in FLASH_LATENT_ROWS)
-        elif src == "prefix_attention_tcgen05.cu":
+        elif src == "shared_attention_tcgen05.cu":
             out.extend((src, (f"-DHEAD_DIM={hd}",)) for hd in (64, 128))
         elif src == "gemm_tcgen05.cu":
             # one CTA per tile and pairs of CTAs, each with tiles of 256 and of 128 columns
