@@ -29,9 +29,9 @@ static_assert(HEAD_DIM == 64 || HEAD_DIM == 128, "this kernel is built for head 
 #define ROWS SP_ROWS
 #define KV_TILE 64
 #define SOFTMAX_WARPS 4
-#define LOADER_WARP SOFTMAX_WARPS               // the keys (and the tensor memory's allocation)
+#define LOADER_WARP SOFTMAX_WARPS               // the keys
 #define VLOADER_WARP (SOFTMAX_WARPS + 1)        // the values
-#define QK_WARP (SOFTMAX_WARPS + 2)             // issues S = Q K^T
+#define QK_WARP (SOFTMAX_WARPS + 2)             // issues S = Q K^T (and allocates the tensor memory)
 #define PV_WARP (SOFTMAX_WARPS + 3)             // issues O += P V
 #define HALVES (HEAD_DIM / 64)
 #define Q_BYTES (ROWS * HEAD_DIM * 2)
@@ -46,7 +46,8 @@ static_assert(HEAD_DIM == 64 || HEAD_DIM == 128, "this kernel is built for head 
 #define NK (HEAD_DIM == 128 ? 3 : 4)
 #define NV (HEAD_DIM == 128 ? 2 : 4)
 // mbarriers, by their index
-#define B_K 0
+#define B_Q 0
+#define B_K 1
 #define B_KFREE (B_K + NK)
 #define B_V (B_KFREE + NK)
 #define B_VFREE (B_V + NV)
@@ -54,6 +55,7 @@ static_assert(HEAD_DIM == 64 || HEAD_DIM == 128, "this kernel is built for head 
 #define B_OFULL (B_SFULL + 2)
 #define B_PFULL (B_OFULL + 2)
 #define NUM_BARS (B_PFULL + 2)
+static_assert(SOFTMAX_WARPS * 32 * 36 * 4 <= NK * TILE_BYTES, "the softmax warps turn their rows over in the keys' ring");
 static_assert(NUM_BARS <= 30, "the barriers, the tensor-memory address and the abort flag share 256 bytes");
 #define RESCALE_LOG2 8.0f
 
@@ -65,6 +67,8 @@ struct PrefixParams {
     float* part_o;                 // [items, nkv, ROWS, HEAD_DIM]
     float* part_ml;                // [items, nkv, ROWS, 2]
     int* status;
+    int* arrivals;                 // [num_arrivals]: set to zero here for the kernel behind this one
+    int num_arrivals;
     int nh, nkv, page_shift, page_size, max_blocks, num_pages;
     float scale_log2e, cap_log2e, scale_over_cap;
 };
@@ -81,6 +85,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) tma_prefetch_descriptor(&map_kv);
+    const uint32_t bar_q = smem_u32(&bars[B_Q]);
     const uint32_t bar_k0 = smem_u32(&bars[B_K]), bar_kfree0 = smem_u32(&bars[B_KFREE]);
     const uint32_t bar_v0 = smem_u32(&bars[B_V]), bar_vfree0 = smem_u32(&bars[B_VFREE]);
     const uint32_t bar_s_full0 = smem_u32(&bars[B_SFULL]), bar_o_full0 = smem_u32(&bars[B_OFULL]), bar_p_full0 = smem_u32(&bars[B_PFULL]);
@@ -88,6 +93,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
     const int kvh = blockIdx.x, item = blockIdx.y;
     const int G = p.nh / p.nkv;
     rv_pdl_wait();
+    for (int i = (item * gridDim.x + kvh) * NUM_THREADS + tid; i < p.num_arrivals; i += gridDim.x * gridDim.y * NUM_THREADS) p.arrivals[i] = 0;
     if (item >= p.plan.items_used()) return;
     const SharedItem it_ = p.plan.item(item);
     const SharedTile tile = p.plan.tile(it_.tile);
@@ -99,6 +105,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
 
     if (tid == 0) {
         abort_flag = 0;
+        mbar_init(bar_q, SOFTMAX_WARPS);
         for (int i = 0; i < NK; ++i) { mbar_init(bar_k0 + 8 * i, 1); mbar_init(bar_kfree0 + 8 * i, 1); }
         for (int i = 0; i < NV; ++i) { mbar_init(bar_v0 + 8 * i, 1); mbar_init(bar_vfree0 + 8 * i, 1); }
         for (int i = 0; i < 2; ++i) {
@@ -108,23 +115,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == LOADER_WARP) {
+    if (warp == QK_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
-    // value tiles start as zeros: what a box does not bring must not meet a probability of zero with a NaN
-    for (int i = tid; i < NV * TILE_BYTES / 16; i += NUM_THREADS) reinterpret_cast<uint4*>(v_s)[i] = make_uint4(0, 0, 0, 0);
-    // the rows' queries, 16 bytes at a time, to their places in the 128-byte swizzle; rows without a sequence are zeros
-    for (int i = tid; i < ROWS * (HEAD_DIM / 8); i += NUM_THREADS) {
-        const int row = i / (HEAD_DIM / 8), chunk = i - row * (HEAD_DIM / 8);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < tile_rows) {
-            const int m = row / G, seq = p.plan.member(tile.first + m);
-            v = *reinterpret_cast<const uint4*>(p.q + ((size_t)seq * p.nh + kvh * G + (row - m * G)) * HEAD_DIM + chunk * 8);
-        }
-        *reinterpret_cast<uint4*>(q_s + (chunk >> 3) * (ROWS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = v;
-    }
-    fence_async_smem();
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -184,7 +178,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
             const uint32_t idesc_s = umma_idesc_bf16(ROWS, KV_TILE);
             int k_stage = 0;
             uint32_t k_phase = 0;
-            for (int i = 0; i < n_it; ++i) {
+            const bool ready = mbar_wait(bar_q, 0, &abort_flag, 1);
+            for (int i = 0; i < n_it && ready; ++i) {
                 const int buf = i & 1;
                 if (!mbar_wait(bar_k0 + 8 * k_stage, k_phase, &abort_flag, 5)) break;
                 if (i >= 2 && !mbar_wait(bar_o_full0 + 8 * buf, ((i - 2) >> 1) & 1, &abort_flag, 6)) break;
@@ -230,6 +225,20 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
         const int row = warp * 32 + lane;                            // row of the tile = lane of tensor memory
         const bool rows_here = warp * 32 < tile_rows;                // (a warp without rows only hands its buffers on)
         const bool in_range = row < tile_rows;
+        // the rows' queries, 16 bytes at a time, to their places in the 128-byte swizzle; rows without a sequence are zeros
+#pragma unroll 8
+        for (int i = tid; i < ROWS * (HEAD_DIM / 8); i += 32 * SOFTMAX_WARPS) {
+            const int r = i / (HEAD_DIM / 8), chunk = i - r * (HEAD_DIM / 8);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < tile_rows) {
+                const int m = r / G;
+                v = *reinterpret_cast<const uint4*>(p.q + ((size_t)p.plan.member(tile.first + m) * p.nh + kvh * G + (r - m * G)) * HEAD_DIM + chunk * 8);
+            }
+            *reinterpret_cast<uint4*>(q_s + (chunk >> 3) * (ROWS * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = v;
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_q);
         // a row sees the keys of the range that its sequence has
         const int limit = in_range ? min(key_hi, p.ctx_lens[p.plan.member(tile.first + row / G)]) : 0;
         const uint32_t t_lane = tmem_base + ((uint32_t)(warp * 32) << 16);
@@ -336,18 +345,28 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
             ok = mbar_wait(bar_o_full0 + 8 * ((n_it - 1) & 1), ((n_it - 1) >> 1) & 1, &abort_flag, 10);
             tcgen05_fence_after();
             if (ok && rows_here) {
-                const size_t prow = ((size_t)item * p.nkv + kvh) * ROWS + row;
-                if (in_range) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m_ref, l_run);
+                // A thread holds a row, so its stores would be 16 bytes here and there: the warp turns 32 x 32 floats over in shared
+                // memory (its share of the keys' ring, which no product reads any more) and stores whole lines of four rows.
+                const size_t prow0 = ((size_t)item * p.nkv + kvh) * ROWS + warp * 32;
+                if (in_range) *reinterpret_cast<float2*>(p.part_ml + (prow0 + lane) * 2) = make_float2(m_ref, l_run);
+                float* turn = reinterpret_cast<float*>(k_s) + warp * (32 * 36);
+                const int last = min(32, tile_rows - warp * 32);
 #pragma unroll
                 for (int c = 0; c < HEAD_DIM; c += 32) {
                     uint32_t o[32];
                     tmem_ld_32x32(t_lane + O_COL + c, o);
                     tmem_ld_wait();
-                    if (in_range) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<uint4*>(p.part_o + prow * HEAD_DIM + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<uint4*>(turn + lane * 36 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int r0 = 0; r0 < 32; r0 += 4) {
+                        const int r = r0 + (lane >> 3);
+                        const uint4 v = *reinterpret_cast<const uint4*>(turn + r * 36 + (lane & 7) * 4);
+                        if (r < last) *reinterpret_cast<uint4*>(p.part_o + (prow0 + r) * HEAD_DIM + c + (lane & 7) * 4) = v;
                     }
+                    __syncwarp();
                 }
             }
         }
@@ -367,7 +386,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
         }
         __syncthreads();
     }
-    if (warp == LOADER_WARP)
+    if (warp == QK_WARP)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
     if (tid == 0 && abort_flag != 0 && p.status) atomicCAS(p.status, 0, abort_flag);
 }
@@ -381,16 +400,20 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
 // of a key serve two steps of the product; of two neighbouring keys' values it takes the same columns, and byte permutes pair them.
 // P^T gets from the layout of a result to that of an operand by two 8 x 8 transposes (movmatrix).
 // The loads of a chunk's values and of the next chunk's keys are in flight while its scores are formed.
-// A CTA has four warps of one (sequence, kv head), which take chunks in turn; a cluster of 1 to 8 CTAs shares a long sequence, and
-// each of them ends up with a part of the columns (through distributed shared memory).  This kernel does not wait for the one with
-// the prefixes before its last part: it may begin as soon as that one's CTAs have all been placed - each of them only lets it
-// begin after its own wait, so that what both read has been written - and it waits for its end only to take up the partial sums.
+// A CTA has four warps of one (sequence, kv head), which take chunks in turn.  Sequences with more than `piece` keys of their own are
+// shared by several CTAs, as many as their own length asks for (the grid is laid out for the longest, the rest leave at once): each
+// leaves its sums, the one that arrives last adds all of them up, in the order of the pieces.  (Clusters that merge through distributed
+// shared memory were measured first: 512 pairs with lengths of 1 to 700 in clusters of 1, 2, 4 took 46, 48 and 68 us.)
+// This kernel does not wait for the one with the prefixes before its last part: it may begin as soon as that one's CTAs have all been
+// placed - each of them only lets it begin after its own wait, so that what both read has been written - and it waits for its end only
+// to take up the partial sums and to count arrivals, in counters that the other kernel has set to zero.
 // Keys outside a sequence, and pages that do not exist, are not loaded and count as not there.
 #define OWN_WARPS 4
 #define OWN_THREADS (32 * OWN_WARPS)
 #define KEY_CHUNKS (HEAD_DIM / 32)            // 16-byte loads of a lane per key
 #define VAL_CHUNKS (HEAD_DIM / 64)            // ... per value row
 #define DIM_BLOCKS (HEAD_DIM / 16)
+#define MERGE_BATCH 12
 
 struct OwnParams {
     SharedPlan plan;
@@ -403,7 +426,10 @@ struct OwnParams {
     const float* sinks;            // [nh] or null
     const float* gate;             // [num_seqs, nh] or null
     __nv_bfloat16* out;            // [num_seqs, nh, HEAD_DIM]
-    int nh, nkv, page_shift, page_size, max_blocks, num_pages, row_blocks;
+    float* own_o;                  // [pieces, num_seqs, nh, HEAD_DIM]: sums of sequences in several pieces
+    float* own_ml;                 // [pieces, num_seqs, nh, 2]
+    int* arrivals;                 // [num_seqs, nkv, row_blocks]
+    int num_seqs, nh, nkv, page_shift, page_size, max_blocks, num_pages, row_blocks, piece;
     float scale_log2e, cap_log2e, scale_over_cap;
 };
 
@@ -418,24 +444,37 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 }
 // (by way of L2 alone: this kernel reads before it waits, and what is read may have been written on another SM just before)
 __device__ __forceinline__ uint4 load_16(const __nv_bfloat16* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); }
-__device__ __forceinline__ uint32_t cluster_smem(uint32_t addr, uint32_t rank) {
-    uint32_t out;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
-    return out;
-}
-__device__ __forceinline__ float4 load_cluster4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ float2 load_cluster2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
+
+// The running (maximum, denominator, four columns) of a row, and one more part's taken up into it; one without keys may hold any sum.
+struct Merged {
+    float m, l;
+    float4 o;
+    __device__ __forceinline__ void take(float pm, float pl, const float4& po) {
+        if (pm == -INFINITY) return;
+        const float m_new = fmaxf(m, pm);
+        const float keep = fast_exp2(m - m_new), f = fast_exp2(pm - m_new);
+        m = m_new;
+        l = l * keep + pl * f;
+        o.x = o.x * keep + po.x * f; o.y = o.y * keep + po.y * f;
+        o.z = o.z * keep + po.z * f; o.w = o.w * keep + po.w * f;
+    }
+    // `n` parts, `step` rows apart from row `at` on; MERGE_BATCH parts' loads in flight at a time
+    __device__ __forceinline__ void take_rows(const float* part_o, const float* part_ml, size_t at, size_t step, int n, int d) {
+        for (int s0 = 0; s0 < n; s0 += MERGE_BATCH) {
+            float2 ml[MERGE_BATCH];
+            float4 v[MERGE_BATCH];
+#pragma unroll
+            for (int k = 0; k < MERGE_BATCH; ++k) {
+                const size_t r = at + (size_t)min(s0 + k, n - 1) * step;
+                ml[k] = __ldcg(reinterpret_cast<const float2*>(part_ml) + r);
+                v[k] = __ldcg(reinterpret_cast<const float4*>(part_o + r * HEAD_DIM + d));
+            }
+#pragma unroll
+            for (int k = 0; k < MERGE_BATCH; ++k)
+                if (s0 + k < n) take(ml[k].x, ml[k].y, v[k]);
+        }
+    }
+};
 
 // NB: blocks of eight heads (a group of up to 8 or up to 16)
 template <int NB>
@@ -445,14 +484,21 @@ own_attention_kernel(const OwnParams p) {
     constexpr int HD = HEAD_DIM;
     __shared__ __align__(16) float part_o[OWN_WARPS][8 * NB][HD + 4];      // (rows four floats apart: the columns of a block in turn)
     __shared__ __align__(8) float part_ml[OWN_WARPS][8 * NB][2];
+    __shared__ int last_one;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, tq = lane & 3;
-    const int rank = blockIdx.x, ctas = gridDim.x;                         // of the cluster
     const int kvh = blockIdx.y / p.row_blocks, seq = blockIdx.z;
     const int G = p.nh / p.nkv;
     const int head0 = (blockIdx.y - kvh * p.row_blocks) * 8 * NB;          // of the group
     const int heads = min(8 * NB, G - head0);
     const int ctx = p.ctx_lens[seq], start = min(p.plan.own_start(seq), max(ctx, 0));
+    // the pieces of this sequence, at most as many as the grid has
+    const int rank = blockIdx.x;
+    const int pieces = max(1, min((int)gridDim.x, (ctx - start + p.piece - 1) / p.piece));
+    if (rank >= pieces) {
+        rv_pdl_wait();
+        return;
+    }
     const int* table = p.block_tables + (size_t)seq * p.max_blocks;
 
     // this lane's queries: head g of a block, elements (4 j + tq) * 8 .. + 7
@@ -475,36 +521,47 @@ own_attention_kernel(const OwnParams p) {
         l_run[n][0] = l_run[n][1] = 0.f;
     }
     const size_t plane = (size_t)p.nkv * p.page_size * HD;                 // from a key to its value
-    // the row of `key`, or null where the sequence has no such key
-    auto row_of = [&](int key) -> const __nv_bfloat16* {
-        if (key < start || key >= ctx || (key >> p.page_shift) >= p.max_blocks) return nullptr;
+    // the page of `key`, or -1 where the sequence has no such key
+    auto page_of = [&](int key) -> int {
+        if (key < start || key >= ctx || (key >> p.page_shift) >= p.max_blocks) return -1;
         const int page = __ldg(table + (key >> p.page_shift));
-        if (page < 0 || page >= p.num_pages) return nullptr;
+        return page < p.num_pages ? page : -1;
+    };
+    auto row_at = [&](int page, int key) -> const __nv_bfloat16* {
         return p.cache + (((size_t)page * 2 * p.nkv + kvh) * p.page_size + (key & (p.page_size - 1))) * HD;
     };
-    const int step = OWN_WARPS * ctas;
+    const int step = OWN_WARPS * pieces;
     const int chunk_end = (ctx + 15) / 16;
     int chunk = start / 16 + rank * OWN_WARPS + warp;
+    // Pages of the chunk's keys, looked up a chunk ahead of the keys themselves: of keys g and g + 8 by every lane; with pages of 16
+    // keys or more that is the page of all of them, with pages of 8 one for each half.
+    int pk[2], next[2];
     uint4 kf[2][KEY_CHUNKS];                                               // keys g and g + 8 of the chunk
-    bool seen[2];
+    auto look_up = [&](int c, int (&to)[2]) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) to[r] = page_of(c * 16 + g + 8 * r);
+    };
     auto load_keys = [&](int c) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const __nv_bfloat16* row = c < chunk_end ? row_of(c * 16 + g + 8 * r) : nullptr;
-            seen[r] = row != nullptr;
+            const __nv_bfloat16* row = row_at(max(pk[r], 0), c * 16 + g + 8 * r);
 #pragma unroll
-            for (int j = 0; j < KEY_CHUNKS; ++j) kf[r][j] = row ? load_16(row + (4 * j + tq) * 8) : make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < KEY_CHUNKS; ++j) kf[r][j] = pk[r] >= 0 ? load_16(row + (4 * j + tq) * 8) : make_uint4(0, 0, 0, 0);
         }
     };
+    look_up(chunk, pk);
+    look_up(chunk + step, next);
     load_keys(chunk);
     for (; chunk < chunk_end; chunk += step) {
         // values of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9: columns 64 c + 8 g .. + 7
         uint4 vf[4][VAL_CHUNKS];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const __nv_bfloat16* row = row_of(chunk * 16 + 2 * tq + (r & 1) + 8 * (r >> 1));
+            const int in = 2 * tq + (r & 1), key = chunk * 16 + in + 8 * (r >> 1);
+            const int page = __shfl_sync(0xffffffffu, pk[r >> 1], in * 4);         // (a lane with g = in has it, if the key is there)
+            const __nv_bfloat16* row = row_at(max(page, 0), key) + plane;
 #pragma unroll
-            for (int c = 0; c < VAL_CHUNKS; ++c) vf[r][c] = row ? load_16(row + plane + 64 * c + 8 * g) : make_uint4(0, 0, 0, 0);
+            for (int c = 0; c < VAL_CHUNKS; ++c) vf[r][c] = page >= 0 ? load_16(row + 64 * c + 8 * g) : make_uint4(0, 0, 0, 0);
         }
         float s[NB][4];
 #pragma unroll
@@ -519,8 +576,10 @@ own_attention_kernel(const OwnParams p) {
                 mma_16816(s[n], a1, qf[n][j].z, qf[n][j].w);
             }
         }
-        const bool see[2] = {seen[0], seen[1]};
+        const bool see[2] = {pk[0] >= 0, pk[1] >= 0};
+        pk[0] = next[0]; pk[1] = next[1];
         load_keys(chunk + step);
+        look_up(chunk + 2 * step, next);
         uint32_t pt[NB][2];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
@@ -582,105 +641,87 @@ own_attention_kernel(const OwnParams p) {
                 *reinterpret_cast<float2*>(&part_o[warp][row][64 * (i >> 2) + 8 * g + 2 * (i & 3)]) = make_float2(o[n][i][h], o[n][i][h + 2]);
         }
     __syncthreads();
-    const bool together = ctas > 1;
-    if (together) cluster_sync();
-    rv_pdl_wait();                                   // the prefixes' sums are there
-
-    // ---- the merge: every CTA of the cluster takes its share of the (head, four columns)
+    const size_t rows_all = (size_t)p.num_seqs * p.nh, row0 = (size_t)seq * p.nh + kvh * G + head0;
+    if (pieces > 1) {
+        // this piece's sums, for the CTA that arrives last
+        for (int i = tid; i < heads * (HD / 4); i += OWN_THREADS) {
+            const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
+            Merged v = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+            for (int w = 0; w < OWN_WARPS; ++w) v.take(part_ml[w][row][0], part_ml[w][row][1], *reinterpret_cast<const float4*>(&part_o[w][row][d]));
+            const size_t at = (size_t)rank * rows_all + row0 + row;
+            *reinterpret_cast<float4*>(p.own_o + at * HD + d) = v.o;
+            if (d == 0) *reinterpret_cast<float2*>(p.own_ml + at * 2) = make_float2(v.m, v.l);
+        }
+        __threadfence();
+        __syncthreads();
+    }
+    rv_pdl_wait();                                   // the prefixes' sums are there, the counters are zero
+    if (pieces > 1) {
+        if (tid == 0) {
+            last_one = atomicAdd(p.arrivals + ((size_t)seq * p.nkv * p.row_blocks + blockIdx.y), 1) == pieces - 1;
+            __threadfence();
+        }
+        __syncthreads();
+        if (!last_one) return;
+    }
     const int place = p.plan.place(seq);
     int2 parts = make_int2(0, 0);
     if (place >= 0) parts = p.plan.parts(place / SP_ROWS);
-    const size_t pre_step = (size_t)p.nkv * SP_ROWS;
-    for (int i = rank * OWN_THREADS + tid; i < heads * (HD / 4); i += ctas * OWN_THREADS) {
+    for (int i = tid; i < heads * (HD / 4); i += OWN_THREADS) {
         const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
         const int head = kvh * G + head0 + row;
-        float m = -INFINITY, l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto take = [&](float pm, float pl, const float4& po) {            // one more part; one without keys may hold any sum
-            if (pm == -INFINITY) return;
-            const float m_new = fmaxf(m, pm);
-            const float keep = fast_exp2(m - m_new), f = fast_exp2(pm - m_new);
-            m = m_new;
-            l = l * keep + pl * f;
-            acc.x = acc.x * keep + po.x * f; acc.y = acc.y * keep + po.y * f;
-            acc.z = acc.z * keep + po.z * f; acc.w = acc.w * keep + po.w * f;
-        };
-        if (place >= 0) {
-            const size_t at = ((size_t)parts.x * p.nkv + kvh) * SP_ROWS + place % SP_ROWS + head0 + row;
-            for (int s0 = 0; s0 < parts.y; s0 += 8) {                      // eight parts' loads in flight at a time
-                float2 ml[8];
-                float4 v[8];
+        Merged v = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+        if (place >= 0)
+            v.take_rows(p.pre_o, p.pre_ml, ((size_t)parts.x * p.nkv + kvh) * SP_ROWS + place % SP_ROWS + head0 + row, (size_t)p.nkv * SP_ROWS, parts.y, d);
+        if (pieces > 1) {
+            v.take_rows(p.own_o, p.own_ml, row0 + row, rows_all, pieces, d);
+        } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const size_t r = at + (size_t)min(s0 + k, parts.y - 1) * pre_step;
-                    ml[k] = __ldcg(reinterpret_cast<const float2*>(p.pre_ml) + r);
-                    v[k] = __ldcg(reinterpret_cast<const float4*>(p.pre_o + r * HD + d));
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (s0 + k < parts.y) take(ml[k].x, ml[k].y, v[k]);
-            }
+            for (int w = 0; w < OWN_WARPS; ++w) v.take(part_ml[w][row][0], part_ml[w][row][1], *reinterpret_cast<const float4*>(&part_o[w][row][d]));
         }
-        for (int c = 0; c < ctas; ++c) {
-#pragma unroll
-            for (int w = 0; w < OWN_WARPS; ++w) {
-                if (together) {
-                    const float2 ml = load_cluster2(cluster_smem(smem_u32(&part_ml[w][row][0]), c));
-                    take(ml.x, ml.y, load_cluster4(cluster_smem(smem_u32(&part_o[w][row][d]), c)));
-                } else {
-                    take(part_ml[w][row][0], part_ml[w][row][1], *reinterpret_cast<const float4*>(&part_o[w][row][d]));
-                }
-            }
-        }
-        float num = 1.f, den = l;
+        float num = 1.f, den = v.l;
         if (p.sinks) {                               // exp(sink) joins the denominator; it has no value
             const float sk = p.sinks[head] * 1.4426950408889634f;
-            const float m_new = fmaxf(m, sk);
-            num = m == -INFINITY ? 0.f : fast_exp2(m - m_new);
-            den = l * num + fast_exp2(sk - m_new);
+            const float m_new = fmaxf(v.m, sk);
+            num = v.m == -INFINITY ? 0.f : fast_exp2(v.m - m_new);
+            den = v.l * num + fast_exp2(sk - m_new);
         }
         float inv = den > 0.f ? num / den : 0.f;
-        const size_t row_out = (size_t)seq * p.nh + head;
-        if (p.gate) inv *= p.gate[row_out];
-        rv_store4(p.out, RV_DTYPE_BF16, row_out * HD + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        if (p.gate) inv *= p.gate[row0 + row];
+        rv_store4(p.out, RV_DTYPE_BF16, (row0 + row) * HD + d, make_float4(v.o.x * inv, v.o.y * inv, v.o.z * inv, v.o.w * inv));
     }
-    if (together) cluster_sync();                    // nobody leaves while its sums are being read
 }
 
 // ---------------------------------------------------------------- host side
 // The arguments, packed by the caller in this order (a step makes this call once a layer).
 struct SharedArgs {
     const void* q; const void* cache; const int* block_tables; const int* ctx_lens; const int* plan;
-    float* pre_o; float* pre_ml; void* out; const float* sinks; const float* gate; int* status; cudaStream_t stream; long long num_pages;
-    int num_seqs, cap_tiles, cap_items, nh, nkv, hd, page_size, max_blocks, ctas;
+    float* pre_o; float* pre_ml; float* own_o; float* own_ml; int* arrivals; void* out; const float* sinks; const float* gate; int* status;
+    cudaStream_t stream; long long num_pages;
+    int num_seqs, cap_tiles, cap_items, nh, nkv, hd, page_size, max_blocks, piece, pieces;
     float scale, softcap;
 };
 
-template <int NB>
-static int launch_own(const OwnParams& p, int num_seqs, int ctas, cudaStream_t stream) {
-    const dim3 grid(ctas, p.nkv * p.row_blocks, num_seqs);
-    if (ctas == 1) RV_LAUNCH_ST = rv_launch(own_attention_kernel<NB>, grid, dim3(OWN_THREADS), 0, stream, p);
-    else RV_LAUNCH_ST = rv_launch_cluster(own_attention_kernel<NB>, grid, dim3(OWN_THREADS), 0, stream, (unsigned)ctas, p);
-    return rv_launch_status();
-}
-
-// part_o [cap_items, nkv, SP_ROWS, HEAD_DIM] and part_ml [.., 2] receive the prefixes' sums; `ctas`: 1, 2, 4 or 8 CTAs share the own
-// keys of a (sequence, kv head).
+// pre_o [cap_items, nkv, SP_ROWS, HEAD_DIM] and pre_ml [.., 2] receive the prefixes' sums.  `piece`: own keys of a (sequence, kv head) that a CTA
+// takes, `pieces`: the most CTAs that share a sequence; with more than one, own_o [pieces, num_seqs, nh, HEAD_DIM], own_ml [.., 2] and
+// arrivals [num_seqs, nkv, ceil(group / 16)] are theirs.
 RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     if (a->hd != HEAD_DIM) return RV_ERR_UNSUPPORTED;
     const int nh = a->nh, nkv = a->nkv, page_size = a->page_size;
     if (a->num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size <= 0 || a->max_blocks <= 0 || a->num_pages <= 0 || a->cap_tiles < 0 ||
         a->cap_items <= 0 || !a->plan || !a->pre_o || !a->pre_ml || a->num_pages > 0x7fffffffLL)
         return RV_ERR_BAD_SIZE;
-    if (a->ctas != 1 && a->ctas != 2 && a->ctas != 4 && a->ctas != 8) return RV_ERR_BAD_SIZE;
+    if (a->piece < 1 || a->pieces < 1 || (a->pieces > 1 && (!a->own_o || !a->own_ml || !a->arrivals))) return RV_ERR_BAD_SIZE;
     const int G = nh / nkv;
     if (G > SP_ROWS || (page_size & (page_size - 1)) || page_size < 8) return RV_ERR_UNSUPPORTED;
     // a row of the tensor map is an int in the kernel
     if (a->num_pages * 2 * nkv * page_size > 0x7fffffffLL) return RV_ERR_UNSUPPORTED;
     const int row_blocks = G <= 8 ? 1 : (G + 15) / 16;
-    if ((long long)nkv * row_blocks > 65535 || a->cap_items > 65535 || a->num_seqs > 65535) return RV_ERR_UNSUPPORTED;
+    if ((long long)nkv * row_blocks > 65535 || (long long)a->num_seqs * nkv * row_blocks > 0x7fffffffLL || a->cap_items > 65535 || a->num_seqs > 65535) return RV_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->cache) | reinterpret_cast<uintptr_t>(a->pre_o) |
-         reinterpret_cast<uintptr_t>(a->plan) | reinterpret_cast<uintptr_t>(a->out)) % 16 || reinterpret_cast<uintptr_t>(a->pre_ml) % 8)
+         reinterpret_cast<uintptr_t>(a->plan) | reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(a->own_o)) % 16 ||
+        (reinterpret_cast<uintptr_t>(a->pre_ml) | reinterpret_cast<uintptr_t>(a->own_ml)) % 8)
         return RV_ERR_ALIGNMENT;
     if (a->num_seqs == 0) return RV_OK;
     alignas(64) CUtensorMap map_kv;
@@ -690,6 +731,7 @@ RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     p.plan = shared_plan(a->plan, a->num_seqs, a->cap_tiles, a->cap_items);
     p.q = (const __nv_bfloat16*)a->q; p.block_tables = a->block_tables; p.ctx_lens = a->ctx_lens;
     p.part_o = a->pre_o; p.part_ml = a->pre_ml; p.status = a->status;
+    p.arrivals = a->arrivals; p.num_arrivals = a->pieces > 1 ? a->num_seqs * nkv * row_blocks : 0;
     p.nh = nh; p.nkv = nkv; p.page_size = page_size; p.max_blocks = a->max_blocks; p.num_pages = (int)a->num_pages;
     p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
@@ -705,6 +747,10 @@ RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     o.plan = p.plan; o.q = p.q; o.cache = (const __nv_bfloat16*)a->cache; o.block_tables = p.block_tables; o.ctx_lens = p.ctx_lens;
     o.pre_o = p.part_o; o.pre_ml = p.part_ml; o.sinks = a->sinks; o.gate = a->gate; o.out = (__nv_bfloat16*)a->out;
     o.nh = nh; o.nkv = nkv; o.page_shift = p.page_shift; o.page_size = page_size; o.max_blocks = a->max_blocks; o.num_pages = p.num_pages;
-    o.row_blocks = row_blocks; o.scale_log2e = p.scale_log2e; o.cap_log2e = p.cap_log2e; o.scale_over_cap = p.scale_over_cap;
-    return G <= 8 ? launch_own<1>(o, a->num_seqs, a->ctas, a->stream) : launch_own<2>(o, a->num_seqs, a->ctas, a->stream);
+    o.own_o = a->own_o; o.own_ml = a->own_ml; o.arrivals = a->arrivals; o.num_seqs = a->num_seqs;
+    o.row_blocks = row_blocks; o.piece = a->piece; o.scale_log2e = p.scale_log2e; o.cap_log2e = p.cap_log2e; o.scale_over_cap = p.scale_over_cap;
+    const dim3 grid(a->pieces, nkv * row_blocks, a->num_seqs);
+    if (G <= 8) RV_LAUNCH_ST = rv_launch(own_attention_kernel<1>, grid, dim3(OWN_THREADS), 0, a->stream, o);
+    else RV_LAUNCH_ST = rv_launch(own_attention_kernel<2>, grid, dim3(OWN_THREADS), 0, a->stream, o);
+    return rv_launch_status();
 }

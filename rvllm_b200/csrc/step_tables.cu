@@ -12,9 +12,10 @@
 //
 // One launch, no order between its CTAs: where a sequence's pages begin in the list, and its tokens in the step, are sums over
 // the sequences before it, which every CTA forms for itself (integers: any order gives the same), and an entry that is new in
-// this step is read from the list, never from the row that another CTA may be writing.  A CTA takes one sequence of
-// one group; the lengths are read once per CTA (a few KB from L2), the entries once in the whole grid.  Every index that
-// comes from device memory is checked against its bound; an entry that would lie outside counts as absent (-1).
+// this step is read from the list, never from the row that another CTA may be writing.  A CTA takes 1, 2, 4 or 8 neighbouring
+// sequences of one group, with 256, 128, 64 or 32 threads each: one while the CTAs find room at once, more where the sums, which
+// a CTA forms once, would be what it spends its time on.  Every index that comes from device memory is checked against its bound;
+// an entry that would lie outside counts as absent (-1).
 #include "common.cuh"
 
 #define TABLE_THREADS 256
@@ -38,64 +39,65 @@ struct TableParams {
 
 __device__ __forceinline__ int blocks_in_use(const TableParams& p, int b) {
     const int row = p.rows[b];
+    const unsigned end = (unsigned)max(p.starts[b], 0) + (unsigned)max(p.q_lens[b], 0);
     if (row < 0 || row >= p.table_rows) return 0;
-    const long long end = (long long)max(p.starts[b], 0) + max(p.q_lens[b], 0);
-    const long long u = (end + p.page_size - 1) / p.page_size;
-    return (int)(u < p.table_width ? u : p.table_width);
+    return (int)min((end + (unsigned)p.page_size - 1u) / (unsigned)p.page_size, (unsigned)p.table_width);
 }
 
-// Sum over the block of a pair of integers; every thread gets both.  `scratch` holds 2 * 8 integers.
-__device__ __forceinline__ void block_sum2(int& a, int& b, int* scratch) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
-    if (lane == 0) { scratch[warp] = a; scratch[8 + warp] = b; }
-    __syncthreads();
-    a = b = 0;
-#pragma unroll
-    for (int w = 0; w < TABLE_THREADS / 32; ++w) { a += scratch[w]; b += scratch[8 + w]; }
-    __syncthreads();
-}
-
+template <int PER>
 __global__ void __launch_bounds__(TABLE_THREADS)
 step_tables_kernel(const TableParams p) {
-    __shared__ int scratch[16];
+    constexpr int THREADS = TABLE_THREADS / PER;             // of a sequence
+    __shared__ int sums[2][TABLE_THREADS / 32];
+    __shared__ int own[2][PER];                              // new pages and tokens of this CTA's sequences
     rv_pdl_wait();
-    const int tid = threadIdx.x;
-    const int b = blockIdx.x, g = blockIdx.y;
-    // pages taken before this sequence (all groups before g, then the sequences before b), tokens before it
+    const int tid = threadIdx.x, g = blockIdx.y, b0 = blockIdx.x * PER;
+    // pages taken before this CTA's first sequence (all groups before g, then the sequences before b0), tokens before it
     int pages = 0, tokens = 0;
-    for (long long i = tid; i < (long long)g * p.num_seqs + b; i += TABLE_THREADS) {
-        const int s = (int)(i % p.num_seqs);
-        pages += max(0, blocks_in_use(p, s) - max(p.held[i], 0));
+    for (int s = tid; s < p.num_seqs; s += TABLE_THREADS) {
+        const int used = blocks_in_use(p, s);
+        const int until = s < b0 ? g + 1 : g;                // groups in which s comes before
+        for (int i = 0; i < until; ++i) pages += max(0, used - max(p.held[(size_t)i * p.num_seqs + s], 0));
+        if (s < b0) tokens += max(p.q_lens[s], 0);
     }
-    for (int s = tid; s < b; s += TABLE_THREADS) tokens += max(p.q_lens[s], 0);
-    block_sum2(pages, tokens, scratch);
-
-    const int row = p.rows[b];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        pages += __shfl_xor_sync(0xffffffffu, pages, o);
+        tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
+    }
+    if ((tid & 31) == 0) { sums[0][tid >> 5] = pages; sums[1][tid >> 5] = tokens; }
+    const int sub = tid / THREADS, at = tid - sub * THREADS, b = b0 + sub;
+    const bool here = b < p.num_seqs;
+    const int row = here ? p.rows[b] : -1;
     const bool real = row >= 0 && row < p.table_rows;
-    const int start = max(p.starts[b], 0), q = max(p.q_lens[b], 0);
-    const int used = blocks_in_use(p, b);
-    const int held = max(p.held[(size_t)g * p.num_seqs + b], 0);
+    const int start = here ? max(p.starts[b], 0) : 0, q = here ? max(p.q_lens[b], 0) : 0;
+    const int used = here ? blocks_in_use(p, b) : 0;
+    const int held = here ? max(p.held[(size_t)g * p.num_seqs + b], 0) : 0;
+    if (PER > 1 && at == 0) { own[0][sub] = max(0, used - held); own[1][sub] = q; }
+    __syncthreads();
+    pages = tokens = 0;
+#pragma unroll
+    for (int w = 0; w < TABLE_THREADS / 32; ++w) { pages += sums[0][w]; tokens += sums[1][w]; }
+    if (PER > 1)
+        for (int i = 0; i < sub; ++i) { pages += own[0][i]; tokens += own[1][i]; }
+    if (!here) return;
+
     int* mine = p.page_table + ((size_t)g * p.table_rows + (real ? row : 0)) * p.table_width;
-    auto entry = [&](int j) -> int {                 // j < used
+    auto entry = [&](int j) -> int {                         // j < used
         if (j < held) return mine[j];
-        const int at = pages + (j - held);
-        return at < p.num_new ? p.new_pages[at] : -1;
+        const int i = pages + (j - held);
+        return i < p.num_new ? p.new_pages[i] : -1;
     };
-    for (int j = held + tid; j < used; j += TABLE_THREADS) mine[j] = entry(j);
+    for (int j = held + at; j < used; j += THREADS) mine[j] = entry(j);
     const int window = p.spans[2 * g], chunk = p.spans[2 * g + 1];
     int first = window > 0 ? max(0, start - window + 1) : 0;
     if (chunk > 0) first = max(first, start / chunk * chunk);
     const int live = first / p.page_size;
     int* out = p.block_tables + ((size_t)g * p.num_seqs + b) * p.max_blocks;
-    for (int j = tid; j < p.max_blocks; j += TABLE_THREADS) out[j] = (j >= live && j < used) ? entry(j) : -1;
-    for (int i = tid; i < q; i += TABLE_THREADS) {
+#pragma unroll 4
+    for (int j = at; j < p.max_blocks; j += THREADS) out[j] = (j >= live && j < used) ? entry(j) : -1;
+    for (int i = at; i < q && tokens + i < p.num_tokens; i += THREADS) {
         const int t = tokens + i;
-        if (t >= p.num_tokens) break;
         const int pos = real ? start + i : 0;
         const int block = pos / p.page_size;
         int slot = -1;
@@ -106,12 +108,12 @@ step_tables_kernel(const TableParams p) {
         p.slot_mapping[(size_t)g * p.num_tokens + t] = slot;
         if (g == 0) { p.positions[t] = pos; p.token_seq[t] = b; }
     }
-    if (b == p.num_seqs - 1)                         // places behind the last sequence's tokens belong to none
-        for (int t = tokens + q + tid; t < p.num_tokens; t += TABLE_THREADS) {
+    if (b == p.num_seqs - 1)                                 // places behind the last sequence's tokens belong to none
+        for (int t = tokens + q + at; t < p.num_tokens; t += THREADS) {
             p.slot_mapping[(size_t)g * p.num_tokens + t] = -1;
             if (g == 0) { p.positions[t] = 0; p.token_seq[t] = -1; }
         }
-    if (g == 0 && tid == 0) {
+    if (g == 0 && at == 0) {
         p.cu_seqlens[b] = tokens;
         if (b == p.num_seqs - 1) p.cu_seqlens[p.num_seqs] = tokens + q;
         p.ctx_lens[b] = real ? start + q : 0;
@@ -133,6 +135,12 @@ RV_EXPORT int rv_step_tables(const TableArgs* a) {
         p.page_size < 1)
         return RV_ERR_BAD_SIZE;
     if (p.groups > 65535) return RV_ERR_UNSUPPORTED;
-    RV_LAUNCH_ST = rv_launch(step_tables_kernel, dim3(p.num_seqs, p.groups), dim3(TABLE_THREADS), 0, a->stream, p);
+    const long long pairs = (long long)p.num_seqs * p.groups, room = 4LL * rv_sm_count();
+    const int per = pairs <= room ? 1 : pairs <= 2 * room ? 2 : pairs <= 4 * room ? 4 : 8;
+    const dim3 grid((p.num_seqs + per - 1) / per, p.groups);
+    if (per == 1) RV_LAUNCH_ST = rv_launch(step_tables_kernel<1>, grid, dim3(TABLE_THREADS), 0, a->stream, p);
+    else if (per == 2) RV_LAUNCH_ST = rv_launch(step_tables_kernel<2>, grid, dim3(TABLE_THREADS), 0, a->stream, p);
+    else if (per == 4) RV_LAUNCH_ST = rv_launch(step_tables_kernel<4>, grid, dim3(TABLE_THREADS), 0, a->stream, p);
+    else RV_LAUNCH_ST = rv_launch(step_tables_kernel<8>, grid, dim3(TABLE_THREADS), 0, a->stream, p);
     return rv_launch_status();
 }

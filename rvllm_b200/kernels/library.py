@@ -55,7 +55,7 @@ def _need(t: torch.Tensor, name: str, dtype=None, dims=None):
 
 
 # arguments of the entry points that take them as one block (the structures of the same names in csrc/)
-_SHARED_ARGS = struct.Struct("=13q9i2f")       # shared_attention_tcgen05.cu
+_SHARED_ARGS = struct.Struct("=16q10i2f")       # shared_attention_tcgen05.cu
 _PLAIN_ARGS = struct.Struct("=14q10i2f")       # shared_prefix.cu
 _TABLE_ARGS = struct.Struct("=13q8iq")         # step_tables.cu
 
@@ -584,12 +584,20 @@ class CudaKernels:
         sinks_at, gate_at = 0 if sinks is None else sinks.data_ptr(), 0 if gate is None else gate.data_ptr()
         stream, cap = torch._C._cuda_getCurrentRawStream(here), softcap or 0.0
         if fast:
-            scratch = torch.empty((pre_rows * (head_dim + 2),), dtype=torch.float32, device=q.device)
+            # one buffer: the prefixes' sums and their maxima and denominators; for sequences that several CTAs share, those of the
+            # pieces, and the counters of arrivals
+            piece, pieces = self._own_pieces(B * num_kv_heads, max_own)
+            own_rows = pieces * B * num_heads if pieces > 1 else 0
+            pairs = B * num_kv_heads * (1 if group <= 8 else -(-group // 16)) if pieces > 1 else 0
+            scratch = torch.empty(((pre_rows + own_rows) * (head_dim + 2) + pairs,), dtype=torch.float32, device=q.device)
             pre = scratch.data_ptr()
+            pre_ml = pre + 4 * pre_rows * head_dim
+            own = pre_ml + 8 * pre_rows
+            own_ml = own + 4 * own_rows * head_dim
             st = self._entry("shared_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",), "rv_shared_attention_tcgen05")(_SHARED_ARGS.pack(
-                q_at, cache_at, tables_at, lens_at, plan_at, pre, pre + 4 * pre_rows * head_dim, out_at, sinks_at, gate_at,
+                q_at, cache_at, tables_at, lens_at, plan_at, pre, pre_ml, own, own_ml, own_ml + 8 * own_rows, out_at, sinks_at, gate_at,
                 self._status.data_ptr(), stream, pages, B, tiles, items, num_heads, num_kv_heads, head_dim, page, tables.shape[1],
-                self._own_ctas(B * num_kv_heads * (1 if group <= 8 else -(-group // 16)), max_own), scale, cap))
+                piece, pieces, scale, cap))
             _check("shared_attention_tcgen05", st)
             COUNTERS['launches'] += 1
             return out
@@ -606,13 +614,10 @@ class CudaKernels:
         COUNTERS['launches'] += 2
         return out
 
-    def _own_ctas(self, pairs: int, max_own: int) -> int:
-        """CTAs that share the keys of a sequence and kv head behind its prefix (a cluster): as many as there is room for, while each
-        still has four chunks of 16 keys for its warps."""
-        ctas = 1
-        while ctas < 8 and pairs * ctas * 2 <= 3 * self.num_sms and max_own > 64 * ctas:
-            ctas *= 2
-        return ctas
+    def _own_pieces(self, pairs: int, max_own: int):
+        """(keys of a piece, most pieces) for the own keys of `pairs` sequences and kv heads."""
+        piece = 128
+        return piece, max(1, min(64, -(-max_own // piece)))
 
     def step_tables(self, page_table: torch.Tensor, rows: torch.Tensor, held: torch.Tensor, starts: torch.Tensor, q_lens: torch.Tensor,
                     new_pages: torch.Tensor, spans: torch.Tensor, num_tokens: int, max_blocks: int, page_size: int,
