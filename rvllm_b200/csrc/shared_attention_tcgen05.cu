@@ -1,21 +1,41 @@
-// Attention of a step's one-token sequences over the cached tokens that groups of them share (bfloat16): the keys of a
-// group's prefix are read once for all of its sequences, on the fifth-generation tensor cores.
+// Attention of a step's one-token sequences, groups of which begin with the same cached tokens (bfloat16): the keys of a group's
+// prefix are read once for all of its sequences, on the fifth-generation tensor cores; the keys behind it sequence by sequence.
 //
 // The queries of a group for one key/value head are n G rows (n sequences, G = nh / nkv heads) against the same P keys:
 //   S = scale Q K^T [n G x P],   m = max_j S,   l = sum_j e^(S - m),   O = e^(S - m) V
-// a matrix product of the size of a prompt's attention, without a triangle.  A CTA owns up to 128 rows (floor(128 / G)
-// whole sequences) of one kv head and one range of the keys and leaves (O, m, l) unnormalised; a second kernel walks the keys behind
-// the prefix, sequence by sequence, takes up what the first has left and writes the result.  Which rows and ranges there are is a list that the
-// host makes once for a set of sequences (they change when a request comes or goes, not from step to step).
+// a matrix product of the size of a prompt's attention, without a triangle.  The keys a sequence has to itself give another
+// (m, l, O) by the same sums, and any number of them, over any ranges of the keys, are put together by
+//   m' = max(m1, m2),   l' = l1 e^(m1 - m') + l2 e^(m2 - m'),   O' likewise,   out = O' / l'.
+// Two kernels: the first has two kinds of CTAs, for ranges of the prefixes and for pieces of the own keys, all of which leave
+// (O, m, l) unnormalised in 32 bits; the second adds them up row by row.
 //
-// Inside a CTA: S = Q K^T of 64 keys into one of two buffers of tensor memory, one thread per row of softmax, P written back
-// over S as bfloat16 pairs and read from there as the A operand of O += P V; two loader warps (keys, values: TMA boxes
-// through the block table) and two warps that issue, as in attention_tcgen05.cu, which has the measurements behind this cut.
-// What differs: rows come from sequences that lie anywhere in the batch (fetched by plain loads and swizzled by hand), keys
-// behind the end of a prefix inside its last page belong to somebody else (their values are set to zero, so that a NaN there
-// does not meet a probability of zero), and warps whose rows are all empty skip the softmax.
-// P is rounded to bfloat16 (2^-9 relative), as both attention kernels of this library do: the tensor core takes no wider A
+// One launch for both kinds, because neither fills the GPU alone: the prefixes' CTAs are few and busy with arithmetic, or many
+// and waiting for memory; the own keys are a latency (lengths, pages, keys, each after the other) repeated for every sequence.  An
+// SM holds two CTAs of either kind, the prefixes' are handed out first.  (As kernels of their own, one after the other, the 64
+// sequences behind 2,048 shared keys with 1 to 700 of their own took 41 to 55 us in several forms; see the table of the kernel.)
+// Which rows and ranges there are is a list that the host makes once for a set of sequences: it changes when a request comes or
+// goes, not from step to step (shared_prefix.cuh).
+//
+// A CTA of the prefixes owns up to 128 rows (floor(128 / G) whole sequences) of one kv head and one range of the keys: S = Q K^T of
+// 64 keys into one of two buffers of tensor memory, one thread per row of softmax, P written back over S as bfloat16 pairs and read
+// from there as the A operand of O += P V; two loader warps (keys, values: TMA boxes through the block table) and two warps that
+// issue, as in attention_tcgen05.cu, which has the measurements behind this cut.  What differs: rows come from sequences that lie
+// anywhere in the batch (fetched by plain loads and swizzled by hand, while the first keys are on their way), keys behind the end of
+// a prefix inside its last page belong to somebody else (their values are set to zero, so that a NaN there does not meet a
+// probability of zero), and warps whose rows are all empty skip the softmax.
+// P is rounded to bfloat16 (2^-9 relative), as in every attention kernel of this library: the tensor core takes no wider A
 // beside a bfloat16 V; sums and maxima are float.
+//
+// The own keys: G rows against each key, so the bytes bound it (hd x 4 bytes a key and kv head) and the tensor cores only save
+// instructions.  A warp works alone, on 16 keys at a time, without shared memory or barriers: keys and values go from global memory
+// straight into the operands of mma.sync.  For that the products are turned over - S^T [16 keys x 8 heads] = K Q^T and
+// O^T [16 dims x 8 heads] += V^T P^T, so that a group of up to eight heads fills the narrow side (a larger group is cut into
+// blocks of eight) - and the order of what is summed over is chosen by what a lane can load in 16 bytes: its eight neighbouring
+// elements of a key serve two steps of the product; of two neighbouring keys' values it takes the same columns, and byte permutes
+// pair them.  P^T gets from the layout of a result to that of an operand by two 8 x 8 transposes (movmatrix).  The loads of a chunk's
+// values and of the next chunk's keys are in flight while its scores are formed, page numbers a chunk ahead of that.  Four warps of a
+// CTA take the chunks of a piece in turn and put their sums together in shared memory.  Keys outside a sequence, and pages that
+// do not exist, are not loaded and count as not there.
 // Cache layer layout: [num_pages, 2 (k, v), nkv, page_size, HEAD_DIM].
 #include "common.cuh"
 #include "shared_prefix.cuh"
@@ -59,22 +79,46 @@ static_assert(SOFTMAX_WARPS * 32 * 36 * 4 <= NK * TILE_BYTES, "the softmax warps
 static_assert(NUM_BARS <= 30, "the barriers, the tensor-memory address and the abort flag share 256 bytes");
 #define RESCALE_LOG2 8.0f
 
-struct PrefixParams {
+struct SharedParams {
     SharedPlan plan;
     const __nv_bfloat16* q;        // [num_seqs, nh, HEAD_DIM]: sequence b brings row b
+    const __nv_bfloat16* cache;
     const int* block_tables;       // [num_seqs, max_blocks]
     const int* ctx_lens;
-    float* part_o;                 // [items, nkv, ROWS, HEAD_DIM]
-    float* part_ml;                // [items, nkv, ROWS, 2]
+    float* pre_o;                  // [items, nkv, ROWS, HEAD_DIM]: the prefixes' sums
+    float* pre_ml;                 // [items, nkv, ROWS, 2]
+    float* own_o;                  // [pieces, num_seqs, nh, HEAD_DIM]: those of the own keys
+    float* own_ml;                 // [pieces, num_seqs, nh, 2]
     int* status;
-    int* arrivals;                 // [num_arrivals]: set to zero here for the kernel behind this one
-    int num_arrivals;
-    int nh, nkv, page_shift, page_size, max_blocks, num_pages;
+    int num_seqs, nh, nkv, page_shift, page_size, max_blocks, num_pages;
+    int prefix_ctas;               // nkv * items; the CTAs behind them are those of the own keys:
+    int head_blocks;               // blocks of eight heads of a group
+    int pieces, piece;             // the most pieces of a sequence, the keys of one
     float scale_log2e, cap_log2e, scale_over_cap;
 };
 
+// The running (maximum, denominator, four columns) of a row, and one more part's taken up into it; one without keys may hold any sum.
+struct Merged {
+    float m = -INFINITY, l = 0.f;
+    float4 o = {0.f, 0.f, 0.f, 0.f};
+    __device__ __forceinline__ void take(float pm, float pl, const float4& po) {
+        if (pm == -INFINITY) return;
+        const float m_new = fmaxf(m, pm);
+        const float keep = fast_exp2(m - m_new), f = fast_exp2(pm - m_new);
+        m = m_new;
+        l = l * keep + pl * f;
+        o.x = o.x * keep + po.x * f; o.y = o.y * keep + po.y * f;
+        o.z = o.z * keep + po.z * f; o.w = o.w * keep + po.w * f;
+    }
+};
+
+// Pieces that the own keys of a sequence are cut into: as many as its own length asks for, at most as many as there is room for.
+__device__ __forceinline__ int pieces_of(int own, int piece, int most) { return max(1, min(most, (own + piece - 1) / piece)); }
+
+__device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* smem, int cta);
+
 __global__ void __launch_bounds__(NUM_THREADS, 2)
-prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const PrefixParams p) {
+shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const SharedParams p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* q_s = smem_raw;                           // [HALVES][128 rows x 128 B]
     unsigned char* k_s = q_s + Q_BYTES;                      // [NK stages][HALVES][KV_TILE keys x 128 B]
@@ -90,10 +134,13 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
     const uint32_t bar_v0 = smem_u32(&bars[B_V]), bar_vfree0 = smem_u32(&bars[B_VFREE]);
     const uint32_t bar_s_full0 = smem_u32(&bars[B_SFULL]), bar_o_full0 = smem_u32(&bars[B_OFULL]), bar_p_full0 = smem_u32(&bars[B_PFULL]);
 
-    const int kvh = blockIdx.x, item = blockIdx.y;
-    const int G = p.nh / p.nkv;
     rv_pdl_wait();
-    for (int i = (item * gridDim.x + kvh) * NUM_THREADS + tid; i < p.num_arrivals; i += gridDim.x * gridDim.y * NUM_THREADS) p.arrivals[i] = 0;
+    if ((int)blockIdx.x >= p.prefix_ctas) {
+        own_keys(p, smem_raw, (int)blockIdx.x - p.prefix_ctas);
+        return;
+    }
+    const int item = blockIdx.x / p.nkv, kvh = blockIdx.x - item * p.nkv;
+    const int G = p.nh / p.nkv;
     if (item >= p.plan.items_used()) return;
     const SharedItem it_ = p.plan.item(item);
     const SharedTile tile = p.plan.tile(it_.tile);
@@ -225,22 +272,30 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
         const int row = warp * 32 + lane;                            // row of the tile = lane of tensor memory
         const bool rows_here = warp * 32 < tile_rows;                // (a warp without rows only hands its buffers on)
         const bool in_range = row < tile_rows;
-        // the rows' queries, 16 bytes at a time, to their places in the 128-byte swizzle; rows without a sequence are zeros
-#pragma unroll 8
-        for (int i = tid; i < ROWS * (HEAD_DIM / 8); i += 32 * SOFTMAX_WARPS) {
-            const int r = i / (HEAD_DIM / 8), chunk = i - r * (HEAD_DIM / 8);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < tile_rows) {
-                const int m = r / G;
-                v = *reinterpret_cast<const uint4*>(p.q + ((size_t)p.plan.member(tile.first + m) * p.nh + kvh * G + (r - m * G)) * HEAD_DIM + chunk * 8);
+        // The rows' queries, 16 bytes a lane, to their places in the 128-byte swizzle; rows without a sequence are zeros.  A warp fetches
+        // its own 32 rows, eight loads at a time (which sequence a row belongs to, the lane of the row has looked up).
+        constexpr int LANES = HEAD_DIM / 8;                          // that bring a row
+        const int my_seq = in_range ? p.plan.member(tile.first + row / G) : -1;
+        const int my_row = in_range ? my_seq * p.nh + kvh * G + row % G : -1;
+#pragma unroll
+        for (int i0 = 0; i0 < LANES; i0 += 8) {
+            uint4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int from = __shfl_sync(0xffffffffu, my_row, (i0 + i) * (32 / LANES) + lane / LANES);
+                v[i] = from >= 0 ? *reinterpret_cast<const uint4*>(p.q + (size_t)from * HEAD_DIM + (lane % LANES) * 8) : make_uint4(0, 0, 0, 0);
             }
-            *reinterpret_cast<uint4*>(q_s + (chunk >> 3) * (ROWS * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = warp * 32 + (i0 + i) * (32 / LANES) + lane / LANES, chunk = lane % LANES;
+                *reinterpret_cast<uint4*>(q_s + (chunk >> 3) * (ROWS * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = v[i];
+            }
         }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_q);
         // a row sees the keys of the range that its sequence has
-        const int limit = in_range ? min(key_hi, p.ctx_lens[p.plan.member(tile.first + row / G)]) : 0;
+        const int limit = in_range ? min(key_hi, p.ctx_lens[my_seq]) : 0;
         const uint32_t t_lane = tmem_base + ((uint32_t)(warp * 32) << 16);
         float m_ref = -INFINITY, l_run = 0.f;
         bool ok = true;
@@ -348,7 +403,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
                 // A thread holds a row, so its stores would be 16 bytes here and there: the warp turns 32 x 32 floats over in shared
                 // memory (its share of the keys' ring, which no product reads any more) and stores whole lines of four rows.
                 const size_t prow0 = ((size_t)item * p.nkv + kvh) * ROWS + warp * 32;
-                if (in_range) *reinterpret_cast<float2*>(p.part_ml + (prow0 + lane) * 2) = make_float2(m_ref, l_run);
+                if (in_range) *reinterpret_cast<float2*>(p.pre_ml + (prow0 + lane) * 2) = make_float2(m_ref, l_run);
                 float* turn = reinterpret_cast<float*>(k_s) + warp * (32 * 36);
                 const int last = min(32, tile_rows - warp * 32);
 #pragma unroll
@@ -364,7 +419,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
                     for (int r0 = 0; r0 < 32; r0 += 4) {
                         const int r = r0 + (lane >> 3);
                         const uint4 v = *reinterpret_cast<const uint4*>(turn + r * 36 + (lane & 7) * 4);
-                        if (r < last) *reinterpret_cast<uint4*>(p.part_o + (prow0 + r) * HEAD_DIM + c + (lane & 7) * 4) = v;
+                        if (r < last) *reinterpret_cast<uint4*>(p.pre_o + (prow0 + r) * HEAD_DIM + c + (lane & 7) * 4) = v;
                     }
                     __syncwarp();
                 }
@@ -392,46 +447,14 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Prefix
 }
 
 // ---------------------------------------------------------------------------------------------
-// The keys behind the prefix, and the merge.  One token per sequence: G rows against each key, so the bytes bound it (hd x 4 bytes
-// a key and kv head) and the tensor cores only save instructions.  A warp works alone, on 16 keys at a time, without shared memory
-// or barriers: keys and values go from global memory straight into the operands of mma.sync.  For that the products are turned
-// over - S^T [16 keys x 8 heads] = K Q^T and O^T [16 dims x 8 heads] += V^T P^T, so that a group of up to eight heads fills the
-// narrow side - and the order of what is summed over is chosen by what a lane can load in 16 bytes: its eight neighbouring elements
-// of a key serve two steps of the product; of two neighbouring keys' values it takes the same columns, and byte permutes pair them.
-// P^T gets from the layout of a result to that of an operand by two 8 x 8 transposes (movmatrix).
-// The loads of a chunk's values and of the next chunk's keys are in flight while its scores are formed.
-// A CTA has four warps of one (sequence, kv head), which take chunks in turn.  Sequences with more than `piece` keys of their own are
-// shared by several CTAs, as many as their own length asks for (the grid is laid out for the longest, the rest leave at once): each
-// leaves its sums, the one that arrives last adds all of them up, in the order of the pieces.  (Clusters that merge through distributed
-// shared memory were measured first: 512 pairs with lengths of 1 to 700 in clusters of 1, 2, 4 took 46, 48 and 68 us.)
-// This kernel does not wait for the one with the prefixes before its last part: it may begin as soon as that one's CTAs have all been
-// placed - each of them only lets it begin after its own wait, so that what both read has been written - and it waits for its end only
-// to take up the partial sums and to count arrivals, in counters that the other kernel has set to zero.
-// Keys outside a sequence, and pages that do not exist, are not loaded and count as not there.
+// A piece of the own keys of a sequence and kv head (see the top of the file).
 #define OWN_WARPS 4
 #define OWN_THREADS (32 * OWN_WARPS)
+#define OWN_STRIDE (HEAD_DIM + 4)              // of a head's sums in shared memory: four floats apart, the columns of a block in turn
 #define KEY_CHUNKS (HEAD_DIM / 32)            // 16-byte loads of a lane per key
 #define VAL_CHUNKS (HEAD_DIM / 64)            // ... per value row
 #define DIM_BLOCKS (HEAD_DIM / 16)
 #define MERGE_BATCH 12
-
-struct OwnParams {
-    SharedPlan plan;
-    const __nv_bfloat16* q;        // [num_seqs, nh, HEAD_DIM]
-    const __nv_bfloat16* cache;
-    const int* block_tables;       // [num_seqs, max_blocks]
-    const int* ctx_lens;
-    const float* pre_o;            // what the prefixes' kernel left
-    const float* pre_ml;
-    const float* sinks;            // [nh] or null
-    const float* gate;             // [num_seqs, nh] or null
-    __nv_bfloat16* out;            // [num_seqs, nh, HEAD_DIM]
-    float* own_o;                  // [pieces, num_seqs, nh, HEAD_DIM]: sums of sequences in several pieces
-    float* own_ml;                 // [pieces, num_seqs, nh, 2]
-    int* arrivals;                 // [num_seqs, nkv, row_blocks]
-    int num_seqs, nh, nkv, page_shift, page_size, max_blocks, num_pages, row_blocks, piece;
-    float scale_log2e, cap_log2e, scale_over_cap;
-};
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -444,82 +467,43 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 }
 // (by way of L2 alone: this kernel reads before it waits, and what is read may have been written on another SM just before)
 __device__ __forceinline__ uint4 load_16(const __nv_bfloat16* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ void own_sync() { asm volatile("bar.sync 1, %0;" ::"n"(OWN_THREADS) : "memory"); }
 
-// The running (maximum, denominator, four columns) of a row, and one more part's taken up into it; one without keys may hold any sum.
-struct Merged {
-    float m, l;
-    float4 o;
-    __device__ __forceinline__ void take(float pm, float pl, const float4& po) {
-        if (pm == -INFINITY) return;
-        const float m_new = fmaxf(m, pm);
-        const float keep = fast_exp2(m - m_new), f = fast_exp2(pm - m_new);
-        m = m_new;
-        l = l * keep + pl * f;
-        o.x = o.x * keep + po.x * f; o.y = o.y * keep + po.y * f;
-        o.z = o.z * keep + po.z * f; o.w = o.w * keep + po.w * f;
-    }
-    // `n` parts, `step` rows apart from row `at` on; MERGE_BATCH parts' loads in flight at a time
-    __device__ __forceinline__ void take_rows(const float* part_o, const float* part_ml, size_t at, size_t step, int n, int d) {
-        for (int s0 = 0; s0 < n; s0 += MERGE_BATCH) {
-            float2 ml[MERGE_BATCH];
-            float4 v[MERGE_BATCH];
-#pragma unroll
-            for (int k = 0; k < MERGE_BATCH; ++k) {
-                const size_t r = at + (size_t)min(s0 + k, n - 1) * step;
-                ml[k] = __ldcg(reinterpret_cast<const float2*>(part_ml) + r);
-                v[k] = __ldcg(reinterpret_cast<const float4*>(part_o + r * HEAD_DIM + d));
-            }
-#pragma unroll
-            for (int k = 0; k < MERGE_BATCH; ++k)
-                if (s0 + k < n) take(ml[k].x, ml[k].y, v[k]);
-        }
-    }
-};
-
-// NB: blocks of eight heads (a group of up to 8 or up to 16)
-template <int NB>
-__global__ void __launch_bounds__(OWN_THREADS, NB == 1 ? 3 : 2)
-own_attention_kernel(const OwnParams p) {
-    rv_pdl_launch_dependents();
+__device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* smem, int cta) {
     constexpr int HD = HEAD_DIM;
-    __shared__ __align__(16) float part_o[OWN_WARPS][8 * NB][HD + 4];      // (rows four floats apart: the columns of a block in turn)
-    __shared__ __align__(8) float part_ml[OWN_WARPS][8 * NB][2];
-    __shared__ int last_one;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int g = lane >> 2, tq = lane & 3;
-    const int kvh = blockIdx.y / p.row_blocks, seq = blockIdx.z;
-    const int G = p.nh / p.nkv;
-    const int head0 = (blockIdx.y - kvh * p.row_blocks) * 8 * NB;          // of the group
-    const int heads = min(8 * NB, G - head0);
-    const int ctx = p.ctx_lens[seq], start = min(p.plan.own_start(seq), max(ctx, 0));
-    // the pieces of this sequence, at most as many as the grid has
-    const int rank = blockIdx.x;
-    const int pieces = max(1, min((int)gridDim.x, (ctx - start + p.piece - 1) / p.piece));
-    if (rank >= pieces) {
-        rv_pdl_wait();
+    rv_pdl_launch_dependents();
+    if (warp >= OWN_WARPS) {                        // the other warpgroup's registers go to the four warps that work
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
         return;
     }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    float* part_o = reinterpret_cast<float*>(smem);                        // [OWN_WARPS][8][OWN_STRIDE]
+    float* part_ml = part_o + OWN_WARPS * 8 * OWN_STRIDE;                  // [OWN_WARPS][8][2]
+    const int g = lane >> 2, tq = lane & 3;
+    const int G = p.nh / p.nkv;
+    // first pieces of all sequences first: the later ones are there for long sequences only
+    const int pairs = p.num_seqs * p.nkv * p.head_blocks;
+    const int rank = cta / pairs, pair = cta - rank * pairs;
+    const int seq = pair / (p.nkv * p.head_blocks), kvh = (pair - seq * p.nkv * p.head_blocks) / p.head_blocks;
+    const int head0 = (pair % p.head_blocks) * 8;                          // of the group
+    const int heads = min(8, G - head0);
+    const int ctx = max(p.ctx_lens[seq], 0), start = min(p.plan.own_start(seq), ctx);
+    const int pieces = pieces_of(ctx - start, p.piece, p.pieces);
+    if (rank >= pieces) return;
     const int* table = p.block_tables + (size_t)seq * p.max_blocks;
 
-    // this lane's queries: head g of a block, elements (4 j + tq) * 8 .. + 7
-    uint4 qf[NB][KEY_CHUNKS];
+    // this lane's queries: head g of the block, elements (4 j + tq) * 8 .. + 7
+    uint4 qf[KEY_CHUNKS];
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int j = 0; j < KEY_CHUNKS; ++j) {
-            qf[n][j] = make_uint4(0, 0, 0, 0);
-            if (8 * n + g < heads)
-                qf[n][j] = load_16(p.q + ((size_t)seq * p.nh + kvh * G + head0 + 8 * n + g) * HD + (4 * j + tq) * 8);
-        }
-    float o[NB][DIM_BLOCKS][4];
-    float m_run[NB][2], l_run[NB][2];                                      // heads 2 tq, 2 tq + 1 of a block
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-#pragma unroll
-        for (int i = 0; i < DIM_BLOCKS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-        m_run[n][0] = m_run[n][1] = -INFINITY;
-        l_run[n][0] = l_run[n][1] = 0.f;
+    for (int j = 0; j < KEY_CHUNKS; ++j) {
+        qf[j] = make_uint4(0, 0, 0, 0);
+        if (g < heads) qf[j] = load_16(p.q + ((size_t)seq * p.nh + kvh * G + head0 + g) * HD + (4 * j + tq) * 8);
     }
+    float o[DIM_BLOCKS][4];
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};        // heads 2 tq, 2 tq + 1
+#pragma unroll
+    for (int i = 0; i < DIM_BLOCKS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     const size_t plane = (size_t)p.nkv * p.page_size * HD;                 // from a key to its value
     // the page of `key`, or -1 where the sequence has no such key
     auto page_of = [&](int key) -> int {
@@ -563,60 +547,48 @@ own_attention_kernel(const OwnParams p) {
 #pragma unroll
             for (int c = 0; c < VAL_CHUNKS; ++c) vf[r][c] = page >= 0 ? load_16(row + 64 * c + 8 * g) : make_uint4(0, 0, 0, 0);
         }
-        float s[NB][4];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < KEY_CHUNKS; ++j) {
             const uint32_t a0[4] = {kf[0][j].x, kf[1][j].x, kf[0][j].y, kf[1][j].y};
             const uint32_t a1[4] = {kf[0][j].z, kf[1][j].z, kf[0][j].w, kf[1][j].w};
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                mma_16816(s[n], a0, qf[n][j].x, qf[n][j].y);
-                mma_16816(s[n], a1, qf[n][j].z, qf[n][j].w);
-            }
+            mma_16816(s, a0, qf[j].x, qf[j].y);
+            mma_16816(s, a1, qf[j].z, qf[j].w);
         }
         const bool see[2] = {pk[0] >= 0, pk[1] >= 0};
         pk[0] = next[0]; pk[1] = next[1];
         load_keys(chunk + step);
         look_up(chunk + 2 * step, next);
-        uint32_t pt[NB][2];
+        float alpha[2];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            float alpha[2];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {                                  // e: key g + 8 (e >> 1), head 2 tq + (e & 1)
-                float v = s[n][e] * p.scale_log2e;
-                if (p.cap_log2e > 0.f) {
-                    const float x = fast_exp2(s[n][e] * p.scale_over_cap * 2.885390081777927f);
-                    v = p.cap_log2e * (1.f - __fdividef(2.f, x + 1.f));
-                }
-                s[n][e] = see[e >> 1] ? v : -INFINITY;
+        for (int e = 0; e < 4; ++e) {                                      // e: key g + 8 (e >> 1), head 2 tq + (e & 1)
+            float v = s[e] * p.scale_log2e;
+            if (p.cap_log2e > 0.f) {
+                const float x = fast_exp2(s[e] * p.scale_over_cap * 2.885390081777927f);
+                v = p.cap_log2e * (1.f - __fdividef(2.f, x + 1.f));
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float mx = fmaxf(s[n][h], s[n][h + 2]);
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                const float m_new = fmaxf(m_run[n][h], mx);
-                const float m_s = m_new == -INFINITY ? 0.f : m_new;
-                alpha[h] = fast_exp2(m_run[n][h] - m_s);                   // 0 while nothing has been seen
-                m_run[n][h] = m_new;
-                s[n][h] = fast_exp2(s[n][h] - m_s);
-                s[n][h + 2] = fast_exp2(s[n][h + 2] - m_s);
-                l_run[n][h] = l_run[n][h] * alpha[h] + s[n][h] + s[n][h + 2];      // this lane's keys; the lanes are added at the end
-            }
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(s[n][0], s[n][1]), hi = __floats2bfloat162_rn(s[n][2], s[n][3]);
-            pt[n][0] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&lo));     // keys 2 tq, 2 tq + 1 of head g
-            pt[n][1] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&hi));     // ... + 8
-#pragma unroll
-            for (int i = 0; i < DIM_BLOCKS; ++i) {
-                o[n][i][0] *= alpha[0]; o[n][i][1] *= alpha[1];
-                o[n][i][2] *= alpha[0]; o[n][i][3] *= alpha[1];
-            }
+            s[e] = see[e >> 1] ? v : -INFINITY;
         }
 #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float mx = fmaxf(s[h], s[h + 2]);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float m_new = fmaxf(m_run[h], mx);
+            const float m_s = m_new == -INFINITY ? 0.f : m_new;
+            alpha[h] = fast_exp2(m_run[h] - m_s);                          // 0 while nothing has been seen
+            m_run[h] = m_new;
+            s[h] = fast_exp2(s[h] - m_s);
+            s[h + 2] = fast_exp2(s[h + 2] - m_s);
+            l_run[h] = l_run[h] * alpha[h] + s[h] + s[h + 2];              // this lane's keys; the lanes are added at the end
+        }
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(s[0], s[1]), hi = __floats2bfloat162_rn(s[2], s[3]);
+        const uint32_t p0 = transpose_8x8(*reinterpret_cast<const uint32_t*>(&lo));      // keys 2 tq, 2 tq + 1 of head g
+        const uint32_t p1 = transpose_8x8(*reinterpret_cast<const uint32_t*>(&hi));      // ... + 8
+#pragma unroll
         for (int i = 0; i < DIM_BLOCKS; ++i) {                             // rows g, g + 8 of a block: columns 64 c + 8 g + 2 w, + 1
+            o[i][0] *= alpha[0]; o[i][1] *= alpha[1];
+            o[i][2] *= alpha[0]; o[i][3] *= alpha[1];
             const int c = i >> 2, w = i & 3;
             auto word = [&](int r) -> uint32_t {
                 const uint4& v = vf[r][c];
@@ -624,133 +596,156 @@ own_attention_kernel(const OwnParams p) {
             };
             const uint32_t a[4] = {__byte_perm(word(0), word(1), 0x5410), __byte_perm(word(0), word(1), 0x7632),
                                    __byte_perm(word(2), word(3), 0x5410), __byte_perm(word(2), word(3), 0x7632)};
-#pragma unroll
-            for (int n = 0; n < NB; ++n) mma_16816(o[n][i], a, pt[n][0], pt[n][1]);
+            mma_16816(o[i], a, p0, p1);
         }
     }
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
+        const int row = warp * 8 + 2 * tq + h;
+        if (g == 0) *reinterpret_cast<float2*>(part_ml + row * 2) = make_float2(m_run[h], l_run[h]);
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) l_run[n][h] += __shfl_xor_sync(0xffffffffu, l_run[n][h], x);
-            const int row = 8 * n + 2 * tq + h;
-            if (g == 0) { part_ml[warp][row][0] = m_run[n][h]; part_ml[warp][row][1] = l_run[n][h]; }
-#pragma unroll
-            for (int i = 0; i < DIM_BLOCKS; ++i)
-                *reinterpret_cast<float2*>(&part_o[warp][row][64 * (i >> 2) + 8 * g + 2 * (i & 3)]) = make_float2(o[n][i][h], o[n][i][h + 2]);
-        }
-    __syncthreads();
-    const size_t rows_all = (size_t)p.num_seqs * p.nh, row0 = (size_t)seq * p.nh + kvh * G + head0;
-    if (pieces > 1) {
-        // this piece's sums, for the CTA that arrives last
-        for (int i = tid; i < heads * (HD / 4); i += OWN_THREADS) {
-            const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
-            Merged v = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll
-            for (int w = 0; w < OWN_WARPS; ++w) v.take(part_ml[w][row][0], part_ml[w][row][1], *reinterpret_cast<const float4*>(&part_o[w][row][d]));
-            const size_t at = (size_t)rank * rows_all + row0 + row;
-            *reinterpret_cast<float4*>(p.own_o + at * HD + d) = v.o;
-            if (d == 0) *reinterpret_cast<float2*>(p.own_ml + at * 2) = make_float2(v.m, v.l);
-        }
-        __threadfence();
-        __syncthreads();
+        for (int i = 0; i < DIM_BLOCKS; ++i)
+            *reinterpret_cast<float2*>(part_o + row * OWN_STRIDE + 64 * (i >> 2) + 8 * g + 2 * (i & 3)) = make_float2(o[i][h], o[i][h + 2]);
     }
-    rv_pdl_wait();                                   // the prefixes' sums are there, the counters are zero
-    if (pieces > 1) {
-        if (tid == 0) {
-            last_one = atomicAdd(p.arrivals + ((size_t)seq * p.nkv * p.row_blocks + blockIdx.y), 1) == pieces - 1;
-            __threadfence();
+    own_sync();
+    for (int i = tid; i < heads * (HD / 4); i += OWN_THREADS) {
+        const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
+        Merged v;
+#pragma unroll
+        for (int w = 0; w < OWN_WARPS; ++w) {
+            const float2 ml = *reinterpret_cast<const float2*>(part_ml + (w * 8 + row) * 2);
+            v.take(ml.x, ml.y, *reinterpret_cast<const float4*>(part_o + (w * 8 + row) * OWN_STRIDE + d));
         }
-        __syncthreads();
-        if (!last_one) return;
+        const size_t at = ((size_t)rank * p.num_seqs + seq) * p.nh + kvh * G + head0 + row;
+        *reinterpret_cast<float4*>(p.own_o + at * HD + d) = v.o;
+        if (d == 0) *reinterpret_cast<float2*>(p.own_ml + at * 2) = make_float2(v.m, v.l);
     }
+}
+
+// ---------------------------------------------------------------------------------------------
+// The sums of a row put together: WARPS warps per (sequence, head), which take its parts in turn, four neighbouring columns a lane
+// and MERGE_BATCH parts' loads in flight.  What it costs is round trips to L2, so a row of many parts gets four warps (one: 45 parts
+// in four trips).
+template <int WARPS>
+__global__ void __launch_bounds__(128)
+shared_merge_kernel(const SharedParams p, const float* __restrict__ sinks, const float* __restrict__ gate, __nv_bfloat16* __restrict__ out) {
+    rv_pdl_launch_dependents();
+    constexpr int LANES = HEAD_DIM / 4;              // that hold a row
+    constexpr int PER_WARP = 32 / LANES;             // rows (or turns of a row) of a warp
+    constexpr int TURNS = WARPS == 1 ? 1 : WARPS * PER_WARP;               // threads groups that share a row
+    __shared__ float4 sh_o[WARPS == 1 ? 1 : TURNS][LANES];
+    __shared__ float2 sh_ml[TURNS];
+    const int tid = threadIdx.x, group = tid / LANES, d = (tid - group * LANES) * 4;
+    const int turn = WARPS == 1 ? 0 : group;
+    const int rows = p.num_seqs * p.nh;
+    const int row = WARPS == 1 ? blockIdx.x * (128 / LANES) + group : blockIdx.x;
+    const bool here = row < rows;
+    const int seq = here ? row / p.nh : 0, head = here ? row - seq * p.nh : 0;
+    const int G = p.nh / p.nkv, kvh = head / G;
+    const int ctx = max(p.ctx_lens[seq], 0);
+    const int pieces = pieces_of(ctx - min(p.plan.own_start(seq), ctx), p.piece, p.pieces);
     const int place = p.plan.place(seq);
     int2 parts = make_int2(0, 0);
     if (place >= 0) parts = p.plan.parts(place / SP_ROWS);
-    for (int i = tid; i < heads * (HD / 4); i += OWN_THREADS) {
-        const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
-        const int head = kvh * G + head0 + row;
-        Merged v = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-        if (place >= 0)
-            v.take_rows(p.pre_o, p.pre_ml, ((size_t)parts.x * p.nkv + kvh) * SP_ROWS + place % SP_ROWS + head0 + row, (size_t)p.nkv * SP_ROWS, parts.y, d);
-        if (pieces > 1) {
-            v.take_rows(p.own_o, p.own_ml, row0 + row, rows_all, pieces, d);
-        } else {
+    rv_pdl_wait();
+    // the parts, prefix first: `turn`, turn + TURNS, ...
+    const int total = here ? parts.y + pieces : 0;
+    const size_t pre_at = ((size_t)parts.x * p.nkv + kvh) * SP_ROWS + (place >= 0 ? place % SP_ROWS + head - kvh * G : 0);
+    Merged v;
+    for (int s0 = turn; s0 < total; s0 += TURNS * MERGE_BATCH) {
+        float2 ml[MERGE_BATCH];
+        float4 o[MERGE_BATCH];
 #pragma unroll
-            for (int w = 0; w < OWN_WARPS; ++w) v.take(part_ml[w][row][0], part_ml[w][row][1], *reinterpret_cast<const float4*>(&part_o[w][row][d]));
+        for (int k = 0; k < MERGE_BATCH; ++k) {
+            const int i = min(s0 + k * TURNS, total - 1);
+            const bool pre = i < parts.y;
+            const size_t at = pre ? pre_at + (size_t)i * p.nkv * SP_ROWS : (size_t)(i - parts.y) * rows + row;
+            ml[k] = __ldcg(reinterpret_cast<const float2*>(pre ? p.pre_ml : p.own_ml) + at);
+            o[k] = __ldcg(reinterpret_cast<const float4*>((pre ? p.pre_o : p.own_o) + at * HEAD_DIM + d));
         }
-        float num = 1.f, den = v.l;
-        if (p.sinks) {                               // exp(sink) joins the denominator; it has no value
-            const float sk = p.sinks[head] * 1.4426950408889634f;
-            const float m_new = fmaxf(v.m, sk);
-            num = v.m == -INFINITY ? 0.f : fast_exp2(v.m - m_new);
-            den = v.l * num + fast_exp2(sk - m_new);
-        }
-        float inv = den > 0.f ? num / den : 0.f;
-        if (p.gate) inv *= p.gate[row0 + row];
-        rv_store4(p.out, RV_DTYPE_BF16, (row0 + row) * HD + d, make_float4(v.o.x * inv, v.o.y * inv, v.o.z * inv, v.o.w * inv));
+#pragma unroll
+        for (int k = 0; k < MERGE_BATCH; ++k)
+            if (s0 + k * TURNS < total) v.take(ml[k].x, ml[k].y, o[k]);
     }
+    if (WARPS > 1) {
+        sh_o[turn][d / 4] = v.o;
+        if (d == 0) sh_ml[turn] = make_float2(v.m, v.l);
+        __syncthreads();
+        if (turn > 0) return;
+#pragma unroll
+        for (int t = 1; t < TURNS; ++t) v.take(sh_ml[t].x, sh_ml[t].y, sh_o[t][d / 4]);
+    }
+    if (!here) return;
+    float num = 1.f, den = v.l;
+    if (sinks) {                                     // exp(sink) joins the denominator; it has no value
+        const float sk = sinks[head] * 1.4426950408889634f;
+        const float m_new = fmaxf(v.m, sk);
+        num = v.m == -INFINITY ? 0.f : fast_exp2(v.m - m_new);
+        den = v.l * num + fast_exp2(sk - m_new);
+    }
+    float inv = den > 0.f ? num / den : 0.f;
+    if (gate) inv *= gate[row];
+    rv_store4(out, RV_DTYPE_BF16, (size_t)row * HEAD_DIM + d, make_float4(v.o.x * inv, v.o.y * inv, v.o.z * inv, v.o.w * inv));
 }
 
 // ---------------------------------------------------------------- host side
 // The arguments, packed by the caller in this order (a step makes this call once a layer).
 struct SharedArgs {
     const void* q; const void* cache; const int* block_tables; const int* ctx_lens; const int* plan;
-    float* pre_o; float* pre_ml; float* own_o; float* own_ml; int* arrivals; void* out; const float* sinks; const float* gate; int* status;
+    float* pre_o; float* pre_ml; float* own_o; float* own_ml; void* out; const float* sinks; const float* gate; int* status;
     cudaStream_t stream; long long num_pages;
-    int num_seqs, cap_tiles, cap_items, nh, nkv, hd, page_size, max_blocks, piece, pieces;
+    int num_seqs, cap_tiles, cap_items, nh, nkv, hd, page_size, max_blocks, piece, pieces, most_parts;
     float scale, softcap;
 };
 
-// pre_o [cap_items, nkv, SP_ROWS, HEAD_DIM] and pre_ml [.., 2] receive the prefixes' sums.  `piece`: own keys of a (sequence, kv head) that a CTA
-// takes, `pieces`: the most CTAs that share a sequence; with more than one, own_o [pieces, num_seqs, nh, HEAD_DIM], own_ml [.., 2] and
-// arrivals [num_seqs, nkv, ceil(group / 16)] are theirs.
+// pre_o [cap_items, nkv, SP_ROWS, HEAD_DIM], pre_ml [.., 2], own_o [pieces, num_seqs, nh, HEAD_DIM] and own_ml [.., 2] receive the parts'
+// sums.  `piece`: own keys of a (sequence, kv head) that a CTA takes, `pieces`: the most CTAs that share a sequence (a longer one has
+// longer pieces); `most_parts`: about as many parts as a row has (it decides how the merge is laid out, nothing else).
 RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     if (a->hd != HEAD_DIM) return RV_ERR_UNSUPPORTED;
     const int nh = a->nh, nkv = a->nkv, page_size = a->page_size;
     if (a->num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size <= 0 || a->max_blocks <= 0 || a->num_pages <= 0 || a->cap_tiles < 0 ||
-        a->cap_items <= 0 || !a->plan || !a->pre_o || !a->pre_ml || a->num_pages > 0x7fffffffLL)
+        a->cap_items < 0 || a->piece < 1 || a->pieces < 1 || !a->plan || !a->pre_o || !a->pre_ml || !a->own_o || !a->own_ml)
         return RV_ERR_BAD_SIZE;
-    if (a->piece < 1 || a->pieces < 1 || (a->pieces > 1 && (!a->own_o || !a->own_ml || !a->arrivals))) return RV_ERR_BAD_SIZE;
     const int G = nh / nkv;
     if (G > SP_ROWS || (page_size & (page_size - 1)) || page_size < 8) return RV_ERR_UNSUPPORTED;
-    // a row of the tensor map is an int in the kernel
-    if (a->num_pages * 2 * nkv * page_size > 0x7fffffffLL) return RV_ERR_UNSUPPORTED;
-    const int row_blocks = G <= 8 ? 1 : (G + 15) / 16;
-    if ((long long)nkv * row_blocks > 65535 || (long long)a->num_seqs * nkv * row_blocks > 0x7fffffffLL || a->cap_items > 65535 || a->num_seqs > 65535) return RV_ERR_UNSUPPORTED;
+    // a row of the tensor map, a CTA and a row of the result are ints in the kernels
+    const int head_blocks = (G + 7) / 8;
+    const long long prefix_ctas = (long long)nkv * a->cap_items, own_ctas = (long long)a->num_seqs * nkv * head_blocks * a->pieces;
+    if (a->num_pages > 0x7fffffffLL / 2 / nkv / page_size || prefix_ctas + own_ctas > 0x7fffffffLL || (long long)a->num_seqs * nh > 0x7fffffffLL)
+        return RV_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->cache) | reinterpret_cast<uintptr_t>(a->pre_o) |
-         reinterpret_cast<uintptr_t>(a->plan) | reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(a->own_o)) % 16 ||
+         reinterpret_cast<uintptr_t>(a->own_o) | reinterpret_cast<uintptr_t>(a->plan) | reinterpret_cast<uintptr_t>(a->out)) % 16 ||
         (reinterpret_cast<uintptr_t>(a->pre_ml) | reinterpret_cast<uintptr_t>(a->own_ml)) % 8)
         return RV_ERR_ALIGNMENT;
     if (a->num_seqs == 0) return RV_OK;
     alignas(64) CUtensorMap map_kv;
     int st = rv_make_bf16_map(&map_kv, a->cache, a->num_pages * 2 * nkv * page_size, HEAD_DIM, page_size < KV_TILE ? page_size : KV_TILE);
     if (st != RV_OK) return st;
-    PrefixParams p;
+    SharedParams p;
     p.plan = shared_plan(a->plan, a->num_seqs, a->cap_tiles, a->cap_items);
-    p.q = (const __nv_bfloat16*)a->q; p.block_tables = a->block_tables; p.ctx_lens = a->ctx_lens;
-    p.part_o = a->pre_o; p.part_ml = a->pre_ml; p.status = a->status;
-    p.arrivals = a->arrivals; p.num_arrivals = a->pieces > 1 ? a->num_seqs * nkv * row_blocks : 0;
-    p.nh = nh; p.nkv = nkv; p.page_size = page_size; p.max_blocks = a->max_blocks; p.num_pages = (int)a->num_pages;
+    p.q = (const __nv_bfloat16*)a->q; p.cache = (const __nv_bfloat16*)a->cache; p.block_tables = a->block_tables; p.ctx_lens = a->ctx_lens;
+    p.pre_o = a->pre_o; p.pre_ml = a->pre_ml; p.own_o = a->own_o; p.own_ml = a->own_ml; p.status = a->status;
+    p.num_seqs = a->num_seqs; p.nh = nh; p.nkv = nkv; p.page_size = page_size; p.max_blocks = a->max_blocks; p.num_pages = (int)a->num_pages;
+    p.prefix_ctas = (int)prefix_ctas; p.head_blocks = head_blocks; p.pieces = a->pieces; p.piece = a->piece;
     p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     p.scale_log2e = a->scale * 1.4426950408889634f;
     p.cap_log2e = a->softcap > 0.f ? a->softcap * 1.4426950408889634f : 0.f;
     p.scale_over_cap = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
     const int smem = Q_BYTES + NK * TILE_BYTES + NV * TILE_BYTES + 256;
+    static_assert((OWN_WARPS * 8 * (OWN_STRIDE + 2)) * 4 <= Q_BYTES, "the own keys' sums lie where the other kind has its queries");
     static RvPerDevice configured;
-    if (int e = rv_configure_smem(configured, prefix_attention_kernel, smem)) return e;
-    RV_LAUNCH_ST = rv_launch(prefix_attention_kernel, dim3(nkv, a->cap_items), dim3(NUM_THREADS), smem, a->stream, map_kv, p);
+    if (int e = rv_configure_smem(configured, shared_attention_kernel, smem)) return e;
+    RV_LAUNCH_ST = rv_launch(shared_attention_kernel, dim3((unsigned)(prefix_ctas + own_ctas)), dim3(NUM_THREADS), smem, a->stream, map_kv, p);
     if ((st = rv_launch_status()) != RV_OK) return st;
-    OwnParams o;
-    o.plan = p.plan; o.q = p.q; o.cache = (const __nv_bfloat16*)a->cache; o.block_tables = p.block_tables; o.ctx_lens = p.ctx_lens;
-    o.pre_o = p.part_o; o.pre_ml = p.part_ml; o.sinks = a->sinks; o.gate = a->gate; o.out = (__nv_bfloat16*)a->out;
-    o.nh = nh; o.nkv = nkv; o.page_shift = p.page_shift; o.page_size = page_size; o.max_blocks = a->max_blocks; o.num_pages = p.num_pages;
-    o.own_o = a->own_o; o.own_ml = a->own_ml; o.arrivals = a->arrivals; o.num_seqs = a->num_seqs;
-    o.row_blocks = row_blocks; o.piece = a->piece; o.scale_log2e = p.scale_log2e; o.cap_log2e = p.cap_log2e; o.scale_over_cap = p.scale_over_cap;
-    const dim3 grid(a->pieces, nkv * row_blocks, a->num_seqs);
-    if (G <= 8) RV_LAUNCH_ST = rv_launch(own_attention_kernel<1>, grid, dim3(OWN_THREADS), 0, a->stream, o);
-    else RV_LAUNCH_ST = rv_launch(own_attention_kernel<2>, grid, dim3(OWN_THREADS), 0, a->stream, o);
+    const int rows = a->num_seqs * nh, per_block = 128 / (HEAD_DIM / 4);
+    if (a->most_parts > MERGE_BATCH)
+        RV_LAUNCH_ST = rv_launch(shared_merge_kernel<4>, dim3(rows), dim3(128), 0, a->stream, p, a->sinks, a->gate, (__nv_bfloat16*)a->out);
+    else
+        RV_LAUNCH_ST = rv_launch(shared_merge_kernel<1>, dim3((rows + per_block - 1) / per_block), dim3(128), 0, a->stream, p, a->sinks, a->gate,
+                                 (__nv_bfloat16*)a->out);
     return rv_launch_status();
 }

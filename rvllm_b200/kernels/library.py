@@ -55,7 +55,7 @@ def _need(t: torch.Tensor, name: str, dtype=None, dims=None):
 
 
 # arguments of the entry points that take them as one block (the structures of the same names in csrc/)
-_SHARED_ARGS = struct.Struct("=16q10i2f")       # shared_attention_tcgen05.cu
+_SHARED_ARGS = struct.Struct("=15q11i2f")       # shared_attention_tcgen05.cu
 _PLAIN_ARGS = struct.Struct("=14q10i2f")       # shared_prefix.cu
 _TABLE_ARGS = struct.Struct("=13q8iq")         # step_tables.cu
 
@@ -584,20 +584,17 @@ class CudaKernels:
         sinks_at, gate_at = 0 if sinks is None else sinks.data_ptr(), 0 if gate is None else gate.data_ptr()
         stream, cap = torch._C._cuda_getCurrentRawStream(here), softcap or 0.0
         if fast:
-            # one buffer: the prefixes' sums and their maxima and denominators; for sequences that several CTAs share, those of the
-            # pieces, and the counters of arrivals
-            piece, pieces = self._own_pieces(B * num_kv_heads, max_own)
-            own_rows = pieces * B * num_heads if pieces > 1 else 0
-            pairs = B * num_kv_heads * (1 if group <= 8 else -(-group // 16)) if pieces > 1 else 0
-            scratch = torch.empty(((pre_rows + own_rows) * (head_dim + 2) + pairs,), dtype=torch.float32, device=q.device)
+            # one buffer: the prefixes' sums, their maxima and denominators, and those of the own keys
+            piece, pieces = self._own_pieces(B * num_kv_heads * -(-group // 8), max_own)
+            own_rows = pieces * B * num_heads
+            scratch = torch.empty(((pre_rows + own_rows) * (head_dim + 2),), dtype=torch.float32, device=q.device)
             pre = scratch.data_ptr()
             pre_ml = pre + 4 * pre_rows * head_dim
             own = pre_ml + 8 * pre_rows
-            own_ml = own + 4 * own_rows * head_dim
             st = self._entry("shared_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",), "rv_shared_attention_tcgen05")(_SHARED_ARGS.pack(
-                q_at, cache_at, tables_at, lens_at, plan_at, pre, pre_ml, own, own_ml, own_ml + 8 * own_rows, out_at, sinks_at, gate_at,
+                q_at, cache_at, tables_at, lens_at, plan_at, pre, pre_ml, own, own + 4 * own_rows * head_dim, out_at, sinks_at, gate_at,
                 self._status.data_ptr(), stream, pages, B, tiles, items, num_heads, num_kv_heads, head_dim, page, tables.shape[1],
-                piece, pieces, scale, cap))
+                piece, pieces, pieces + shared.most_parts, scale, cap))
             _check("shared_attention_tcgen05", st)
             COUNTERS['launches'] += 1
             return out

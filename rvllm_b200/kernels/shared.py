@@ -112,6 +112,7 @@ class SharedPrefixes:
             at += 4 * capacity[0]
             host[at:at + 4 * len(items)] = np.asarray(items, np.int32).ravel()
         self.capacity, self.num_items, self.num_tiles = capacity, len(items), len(tiles)
+        self.most_parts = max((n for _, n in parts), default=0)
         # the fewest keys that any sequence has before its own begin (0: one has no prefix)
         self.shortest = min((t for _, t in kept), default=0) if len(flat) == B else 0
         return host
