@@ -33,9 +33,10 @@
 // blocks of eight) - and the order of what is summed over is chosen by what a lane can load in 16 bytes: its eight neighbouring
 // elements of a key serve two steps of the product; of two neighbouring keys' values it takes the same columns, and byte permutes
 // pair them.  P^T gets from the layout of a result to that of an operand by two 8 x 8 transposes (movmatrix).  The loads of a chunk's
-// values and of the next chunk's keys are in flight while its scores are formed, page numbers a chunk ahead of that.  Four warps of a
-// CTA take the chunks of a piece in turn and put their sums together in shared memory.  Keys outside a sequence, and pages that
-// do not exist, are not loaded and count as not there.
+// values and of the next chunk's keys are in flight while its scores are formed, page numbers a chunk ahead of that.  The own keys of
+// all sequences, cut into pieces, are one list that the warps of a fixed number of CTAs take in turn: a CTA for each sequence and
+// kv head, or several, spent most of its 4 to 10 us on being set up, and lengths of 1 to 700 left most of them idle (41 us and more
+// for 64 sequences of eight kv heads).  Keys outside a sequence, and pages that do not exist, are not loaded and count as not there.
 // Cache layer layout: [num_pages, 2 (k, v), nkv, page_size, HEAD_DIM].
 #include "common.cuh"
 #include "shared_prefix.cuh"
@@ -61,7 +62,8 @@ static_assert(HEAD_DIM == 64 || HEAD_DIM == 128, "this kernel is built for head 
 #define REGS_SOFTMAX 200
 #define REGS_OTHERS 56
 #define TMEM_COLS 256
-#define S_COL 0
+#define S_COL 0                     // one S buffer of 64 columns: free again as soon as the softmax warps have read it
+#define P_COL 64                    // two P buffers (bf16 pairs) of 32 columns
 #define O_COL 128
 #define NK (HEAD_DIM == 128 ? 3 : 4)
 #define NV (HEAD_DIM == 128 ? 2 : 4)
@@ -71,8 +73,9 @@ static_assert(HEAD_DIM == 64 || HEAD_DIM == 128, "this kernel is built for head 
 #define B_KFREE (B_K + NK)
 #define B_V (B_KFREE + NK)
 #define B_VFREE (B_V + NV)
-#define B_SFULL (B_VFREE + NV)     // [2] each from here on
-#define B_OFULL (B_SFULL + 2)
+#define B_SFULL (B_VFREE + NV)
+#define B_SFREE (B_SFULL + 1)
+#define B_OFULL (B_SFREE + 1)      // [2] each from here on
 #define B_PFULL (B_OFULL + 2)
 #define NUM_BARS (B_PFULL + 2)
 static_assert(SOFTMAX_WARPS * 32 * 36 * 4 <= NK * TILE_BYTES, "the softmax warps turn their rows over in the keys' ring");
@@ -132,7 +135,8 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
     const uint32_t bar_q = smem_u32(&bars[B_Q]);
     const uint32_t bar_k0 = smem_u32(&bars[B_K]), bar_kfree0 = smem_u32(&bars[B_KFREE]);
     const uint32_t bar_v0 = smem_u32(&bars[B_V]), bar_vfree0 = smem_u32(&bars[B_VFREE]);
-    const uint32_t bar_s_full0 = smem_u32(&bars[B_SFULL]), bar_o_full0 = smem_u32(&bars[B_OFULL]), bar_p_full0 = smem_u32(&bars[B_PFULL]);
+    const uint32_t bar_s_full = smem_u32(&bars[B_SFULL]), bar_s_free = smem_u32(&bars[B_SFREE]);
+    const uint32_t bar_o_full0 = smem_u32(&bars[B_OFULL]), bar_p_full0 = smem_u32(&bars[B_PFULL]);
 
     rv_pdl_wait();
     if ((int)blockIdx.x >= p.prefix_ctas) {
@@ -155,8 +159,8 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
         mbar_init(bar_q, SOFTMAX_WARPS);
         for (int i = 0; i < NK; ++i) { mbar_init(bar_k0 + 8 * i, 1); mbar_init(bar_kfree0 + 8 * i, 1); }
         for (int i = 0; i < NV; ++i) { mbar_init(bar_v0 + 8 * i, 1); mbar_init(bar_vfree0 + 8 * i, 1); }
+        mbar_init(bar_s_full, 1); mbar_init(bar_s_free, SOFTMAX_WARPS);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar_s_full0 + 8 * i, 1);
             mbar_init(bar_o_full0 + 8 * i, 1);
             mbar_init(bar_p_full0 + 8 * i, SOFTMAX_WARPS);                  // one arrival per warp
         }
@@ -219,7 +223,9 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
             if (++stage == stages) { stage = 0; phase ^= 1; }
         }
     } else if (warp == QK_WARP) {
-        // ------------------------------------------------------------ S = Q K^T, over P(i - 2) once that product has finished
+        // ------------------------------------------------------------ S = Q K^T
+        // S(i) goes where S(i - 1) was, once the four warps have read that.  It is issued after the product with P(i - 2) has
+        // finished, so a softmax warp that has seen S(i) may write P(i) where P(i - 2) was.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
         if (lane == 0) {
             const uint32_t idesc_s = umma_idesc_bf16(ROWS, KV_TILE);
@@ -227,9 +233,9 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
             uint32_t k_phase = 0;
             const bool ready = mbar_wait(bar_q, 0, &abort_flag, 1);
             for (int i = 0; i < n_it && ready; ++i) {
-                const int buf = i & 1;
                 if (!mbar_wait(bar_k0 + 8 * k_stage, k_phase, &abort_flag, 5)) break;
-                if (i >= 2 && !mbar_wait(bar_o_full0 + 8 * buf, ((i - 2) >> 1) & 1, &abort_flag, 6)) break;
+                if (i >= 2 && !mbar_wait(bar_o_full0 + 8 * (i & 1), ((i - 2) >> 1) & 1, &abort_flag, 6)) break;
+                if (i >= 1 && !mbar_wait(bar_s_free, (i - 1) & 1, &abort_flag, 13)) break;
                 tcgen05_fence_after();
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h) {
@@ -237,9 +243,9 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
                     const uint64_t dk = umma_desc(smem_u32(k_s) + k_stage * TILE_BYTES + h * (KV_TILE * 128));
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        tcgen05_mma_bf16(tmem_base + S_COL + buf * KV_TILE, dq + (uint64_t)(2 * j), dk + (uint64_t)(2 * j), idesc_s, (h | j) != 0);
+                        tcgen05_mma_bf16(tmem_base + S_COL, dq + (uint64_t)(2 * j), dk + (uint64_t)(2 * j), idesc_s, (h | j) != 0);
                 }
-                tcgen05_commit(bar_s_full0 + 8 * buf);
+                tcgen05_commit(bar_s_full);
                 tcgen05_commit(bar_kfree0 + 8 * k_stage);
                 if (++k_stage == NK) { k_stage = 0; k_phase ^= 1; }
             }
@@ -256,7 +262,7 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
                 if (!mbar_wait(bar_v0 + 8 * v_stage, v_phase, &abort_flag, 7)) break;
                 if (!mbar_wait(bar_p_full0 + 8 * b, (i >> 1) & 1, &abort_flag, 8)) break;
                 tcgen05_fence_after();
-                const uint32_t tp = tmem_base + S_COL + b * KV_TILE;
+                const uint32_t tp = tmem_base + P_COL + b * (KV_TILE / 2);
                 const uint64_t dv = umma_desc_mn(smem_u32(v_s) + v_stage * TILE_BYTES, KV_TILE * 128);
 #pragma unroll
                 for (int j = 0; j < KV_TILE / 16; ++j)
@@ -300,10 +306,19 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
         float m_ref = -INFINITY, l_run = 0.f;
         bool ok = true;
         for (int it = 0; it < n_it; ++it) {
-            const int sb = it & 1;
+            const int pb = it & 1;
             const int key0 = (t_begin + it) * KV_TILE;
-            if (!mbar_wait(bar_s_full0 + 8 * sb, (it >> 1) & 1, &abort_flag, 9)) { ok = false; break; }
+            if (!mbar_wait(bar_s_full, it & 1, &abort_flag, 9)) { ok = false; break; }
             tcgen05_fence_after();
+            uint32_t s0[32], s1[32];
+            if (rows_here) {
+                tmem_ld_32x32(t_lane + S_COL, s0);
+                tmem_ld_32x32(t_lane + S_COL + 32, s1);
+                tmem_ld_wait();
+            }
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_s_free);
             if (key0 + KV_TILE > key_hi) {
                 // values of keys behind the range's end: zeros, before the product may read them (it waits for P of all four warps)
                 if (!mbar_wait(bar_v0 + 8 * (it % NV), (it / NV) & 1, &abort_flag, 12)) { ok = false; break; }
@@ -316,12 +331,6 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
                 fence_async_smem();
             }
             if (rows_here) {
-                uint32_t s0[32], s1[32];
-                tmem_ld_32x32(t_lane + S_COL + sb * KV_TILE, s0);
-                tmem_ld_32x32(t_lane + S_COL + sb * KV_TILE + 32, s1);
-                tmem_ld_wait();
-                tcgen05_fence_before();
-                __syncwarp();
                 // with a cap the scores become c log2(e) tanh(scale s / c) here (tanh as 1 - 2 / (e^2x + 1)), and the scale below is 1
                 const float eff_scale = p.cap_log2e > 0.f ? 1.f : p.scale_log2e;
                 if (p.cap_log2e > 0.f) {
@@ -349,52 +358,58 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
                     mx[3] = max3(mx[3], __uint_as_float(s1[e + 2]), __uint_as_float(s1[e + 3]));
                 }
                 const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * eff_scale;
-                // the reference maximum is raised only when it is far behind: O then needs a pass
-                const bool first_data = m_ref == -INFINITY && m_tile > -INFINITY;
-                const bool raise = first_data || m_tile > m_ref + RESCALE_LOG2;
-                float factor = 1.f;
-                if (raise) {
-                    factor = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_tile);
-                    m_ref = m_tile;
-                    l_run *= factor;
-                }
-                if (__any_sync(0xffffffffu, raise && it > 0)) {
-                    // the product of the tile before must have finished; the one after waits for this warp's P
-                    if (!mbar_wait(bar_o_full0 + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, &abort_flag, 11)) { ok = false; break; }
-                    tcgen05_fence_after();
-#pragma unroll
-                    for (int c = 0; c < HEAD_DIM; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(t_lane + O_COL + c, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-                        tmem_st_32x32(t_lane + O_COL + c, o);
-                    }
-                    tmem_st_wait();
-                    tcgen05_fence_before();
-                }
-                const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
-                float l_tile = 0.f, l_tile2 = 0.f;
+                // The reference maximum is raised only when it is more than 2^8 behind: O then needs a pass.  The exponentials do not
+                // wait to know: they are formed under the old reference beside the maximum, and once more in the rare tile that raises it.
+                bool raise = m_tile > m_ref + RESCALE_LOG2 || (m_ref == -INFINITY && m_tile > -INFINITY);
                 uint32_t pk[32];
+                float l_tile, l_tile2;
+                for (;;) {
+                    const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
+                    l_tile = l_tile2 = 0.f;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {                   // keys 2j and 2j + 1 of the tile: one column of P
-                    const int e = 2 * j;
-                    float a0, a1;
-                    fma2(a0, a1, __uint_as_float(e < 32 ? s0[e] : s1[e - 32]), __uint_as_float(e + 1 < 32 ? s0[e + 1] : s1[e + 1 - 32]),
-                         eff_scale, neg_m);
-                    const float x0 = fast_exp2(a0), x1 = fast_exp2(a1);
-                    add2(l_tile, l_tile2, x0, x1);
-                    __nv_bfloat162 h2 = __floats2bfloat162_rn(x0, x1);
-                    pk[j] = *reinterpret_cast<uint32_t*>(&h2);
+                    for (int j = 0; j < 32; ++j) {               // keys 2j and 2j + 1 of the tile: one column of P
+                        const int e = 2 * j;
+                        float a0, a1;
+                        fma2(a0, a1, __uint_as_float(e < 32 ? s0[e] : s1[e - 32]), __uint_as_float(e + 1 < 32 ? s0[e + 1] : s1[e + 1 - 32]),
+                             eff_scale, neg_m);
+                        const float x0 = fast_exp2(a0), x1 = fast_exp2(a1);
+                        add2(l_tile, l_tile2, x0, x1);
+                        __nv_bfloat162 h2 = __floats2bfloat162_rn(x0, x1);
+                        pk[j] = *reinterpret_cast<uint32_t*>(&h2);
+                    }
+                    if (!__any_sync(0xffffffffu, raise)) break;
+                    float factor = 1.f;
+                    if (raise) {
+                        factor = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_tile);
+                        m_ref = m_tile;
+                        l_run *= factor;
+                        raise = false;
+                    }
+                    if (it > 0) {
+                        // the product of the tile before must have finished; the one after waits for this warp's P
+                        if (!mbar_wait(bar_o_full0 + 8 * (pb ^ 1), ((it - 1) >> 1) & 1, &abort_flag, 11)) { ok = false; break; }
+                        tcgen05_fence_after();
+#pragma unroll
+                        for (int c = 0; c < HEAD_DIM; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld_32x32(t_lane + O_COL + c, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                            tmem_st_32x32(t_lane + O_COL + c, o);
+                        }
+                        tmem_st_wait();
+                        tcgen05_fence_before();
+                    }
                 }
+                if (!ok) break;
                 l_run += l_tile + l_tile2;
-                tmem_st_32x32(t_lane + S_COL + sb * KV_TILE, pk);
+                tmem_st_32x32(t_lane + P_COL + pb * (KV_TILE / 2), pk);
                 tmem_st_wait();
             }
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_p_full0 + 8 * sb);
+            if (lane == 0) mbar_arrive(bar_p_full0 + 8 * pb);
         }
         if (ok) {
             ok = mbar_wait(bar_o_full0 + 8 * ((n_it - 1) & 1), ((n_it - 1) >> 1) & 1, &abort_flag, 10);
@@ -447,14 +462,14 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
 }
 
 // ---------------------------------------------------------------------------------------------
-// A piece of the own keys of a sequence and kv head (see the top of the file).
+// The own keys (see the top of the file).
 #define OWN_WARPS 4
 #define OWN_THREADS (32 * OWN_WARPS)
-#define OWN_STRIDE (HEAD_DIM + 4)              // of a head's sums in shared memory: four floats apart, the columns of a block in turn
 #define KEY_CHUNKS (HEAD_DIM / 32)            // 16-byte loads of a lane per key
 #define VAL_CHUNKS (HEAD_DIM / 64)            // ... per value row
 #define DIM_BLOCKS (HEAD_DIM / 16)
 #define MERGE_BATCH 12
+#define MAX_SEQS 16384                        // of a step: what the list of pieces has room for
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -467,32 +482,17 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 }
 // (by way of L2 alone: this kernel reads before it waits, and what is read may have been written on another SM just before)
 __device__ __forceinline__ uint4 load_16(const __nv_bfloat16* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); }
-__device__ __forceinline__ void own_sync() { asm volatile("bar.sync 1, %0;" ::"n"(OWN_THREADS) : "memory"); }
-
-__device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* smem, int cta) {
+// Piece `rank` of `pieces` of sequence `seq`: heads head0 .. head0 + 7 of kv head kvh (of a group of G), by one warp.
+__device__ __forceinline__ void own_piece(const SharedParams& p, int seq, int rank, int pieces, int kvh, int head0, int G, int lane) {
     constexpr int HD = HEAD_DIM;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    rv_pdl_launch_dependents();
-    if (warp >= OWN_WARPS) {                        // the other warpgroup's registers go to the four warps that work
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
-        return;
-    }
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
-    float* part_o = reinterpret_cast<float*>(smem);                        // [OWN_WARPS][8][OWN_STRIDE]
-    float* part_ml = part_o + OWN_WARPS * 8 * OWN_STRIDE;                  // [OWN_WARPS][8][2]
     const int g = lane >> 2, tq = lane & 3;
-    const int G = p.nh / p.nkv;
-    // first pieces of all sequences first: the later ones are there for long sequences only
-    const int pairs = p.num_seqs * p.nkv * p.head_blocks;
-    const int rank = cta / pairs, pair = cta - rank * pairs;
-    const int seq = pair / (p.nkv * p.head_blocks), kvh = (pair - seq * p.nkv * p.head_blocks) / p.head_blocks;
-    const int head0 = (pair % p.head_blocks) * 8;                          // of the group
     const int heads = min(8, G - head0);
     const int ctx = max(p.ctx_lens[seq], 0), start = min(p.plan.own_start(seq), ctx);
-    const int pieces = pieces_of(ctx - start, p.piece, p.pieces);
-    if (rank >= pieces) return;
     const int* table = p.block_tables + (size_t)seq * p.max_blocks;
-
+    // its chunks of 16 keys
+    const int first = start / 16, chunks = (ctx + 15) / 16 - first, per = (chunks + pieces - 1) / pieces;
+    int chunk = first + rank * per;
+    const int chunk_end = min(first + chunks, chunk + per);
     // this lane's queries: head g of the block, elements (4 j + tq) * 8 .. + 7
     uint4 qf[KEY_CHUNKS];
 #pragma unroll
@@ -514,16 +514,13 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* s
     auto row_at = [&](int page, int key) -> const __nv_bfloat16* {
         return p.cache + (((size_t)page * 2 * p.nkv + kvh) * p.page_size + (key & (p.page_size - 1))) * HD;
     };
-    const int step = OWN_WARPS * pieces;
-    const int chunk_end = (ctx + 15) / 16;
-    int chunk = start / 16 + rank * OWN_WARPS + warp;
     // Pages of the chunk's keys, looked up a chunk ahead of the keys themselves: of keys g and g + 8 by every lane; with pages of 16
     // keys or more that is the page of all of them, with pages of 8 one for each half.
     int pk[2], next[2];
     uint4 kf[2][KEY_CHUNKS];                                               // keys g and g + 8 of the chunk
     auto look_up = [&](int c, int (&to)[2]) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) to[r] = page_of(c * 16 + g + 8 * r);
+        for (int r = 0; r < 2; ++r) to[r] = c < chunk_end ? page_of(c * 16 + g + 8 * r) : -1;
     };
     auto load_keys = [&](int c) {
 #pragma unroll
@@ -534,9 +531,9 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* s
         }
     };
     look_up(chunk, pk);
-    look_up(chunk + step, next);
+    look_up(chunk + 1, next);
     load_keys(chunk);
-    for (; chunk < chunk_end; chunk += step) {
+    for (; chunk < chunk_end; ++chunk) {
         // values of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9: columns 64 c + 8 g .. + 7
         uint4 vf[4][VAL_CHUNKS];
 #pragma unroll
@@ -557,8 +554,8 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* s
         }
         const bool see[2] = {pk[0] >= 0, pk[1] >= 0};
         pk[0] = next[0]; pk[1] = next[1];
-        load_keys(chunk + step);
-        look_up(chunk + 2 * step, next);
+        load_keys(chunk + 1);
+        look_up(chunk + 2, next);
         float alpha[2];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {                                      // e: key g + 8 (e >> 1), head 2 tq + (e & 1)
@@ -599,28 +596,72 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* s
             mma_16816(o[i], a, p0, p1);
         }
     }
+    // a lane has eight neighbouring columns of its two heads in every 64
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
-        const int row = warp * 8 + 2 * tq + h;
-        if (g == 0) *reinterpret_cast<float2*>(part_ml + row * 2) = make_float2(m_run[h], l_run[h]);
+        const int head = 2 * tq + h;
+        if (head >= heads) continue;
+        const size_t at = ((size_t)rank * p.num_seqs + seq) * p.nh + kvh * G + head0 + head;
+        if (g == 0) *reinterpret_cast<float2*>(p.own_ml + at * 2) = make_float2(m_run[h], l_run[h]);
 #pragma unroll
-        for (int i = 0; i < DIM_BLOCKS; ++i)
-            *reinterpret_cast<float2*>(part_o + row * OWN_STRIDE + 64 * (i >> 2) + 8 * g + 2 * (i & 3)) = make_float2(o[i][h], o[i][h + 2]);
+        for (int c = 0; c < VAL_CHUNKS; ++c)
+#pragma unroll
+            for (int w = 0; w < 4; w += 2) {
+                const int i = 4 * c + w;
+                *reinterpret_cast<float4*>(p.own_o + at * HD + 64 * c + 8 * g + 2 * w) = make_float4(o[i][h], o[i][h + 2], o[i + 1][h], o[i + 1][h + 2]);
+            }
     }
-    own_sync();
-    for (int i = tid; i < heads * (HD / 4); i += OWN_THREADS) {
-        const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
-        Merged v;
+}
+
+__device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* smem, int cta) {
+    constexpr int HD = HEAD_DIM;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    rv_pdl_launch_dependents();
+    if (warp >= OWN_WARPS) {                        // the other warpgroup's registers go to the four warps that work
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
+        return;
+    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    const int G = p.nh / p.nkv, blocks = p.nkv * p.head_blocks;
+    // before[s]: pieces of the sequences before s
+    int* before = reinterpret_cast<int*>(smem);                            // [num_seqs + 1], behind it [OWN_WARPS]
+    int* of_warp = before + p.num_seqs + 1;
+    const int each = (p.num_seqs + OWN_THREADS - 1) / OWN_THREADS, s_lo = min(tid * each, p.num_seqs), s_hi = min(s_lo + each, p.num_seqs);
+    int mine = 0;
+    for (int s = s_lo; s < s_hi; ++s) {
+        const int ctx = max(p.ctx_lens[s], 0);
+        before[s] = mine;
+        mine += pieces_of(ctx - min(p.plan.own_start(s), ctx), p.piece, p.pieces);
+    }
+    int upto = mine;
 #pragma unroll
-        for (int w = 0; w < OWN_WARPS; ++w) {
-            const float2 ml = *reinterpret_cast<const float2*>(part_ml + (w * 8 + row) * 2);
-            v.take(ml.x, ml.y, *reinterpret_cast<const float4*>(part_o + (w * 8 + row) * OWN_STRIDE + d));
+    for (int x = 1; x < 32; x <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += other;
+    }
+    if (lane == 31) of_warp[warp] = upto;
+    asm volatile("bar.sync 1, %0;" ::"n"(OWN_THREADS) : "memory");
+    int base = upto - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < OWN_WARPS; ++w) {
+        base += w < warp ? of_warp[w] : 0;
+        total += of_warp[w];
+    }
+    for (int s = s_lo; s < s_hi; ++s) before[s] += base;
+    if (tid == 0) before[p.num_seqs] = total;
+    asm volatile("bar.sync 1, %0;" ::"n"(OWN_THREADS) : "memory");
+    const int warps = ((int)gridDim.x - p.prefix_ctas) * OWN_WARPS;
+    for (long long at = cta * OWN_WARPS + warp; at < (long long)total * blocks; at += warps) {
+        // piece `at / blocks` of all, block of heads `at mod blocks`
+        const int piece = (int)(at / blocks), block = (int)(at - (long long)piece * blocks);
+        int seq = 0;
+        for (int hi = p.num_seqs - 1; seq < hi;) {                         // the last sequence that begins at or before it
+            const int mid = (seq + hi + 1) >> 1;
+            if (before[mid] <= piece) seq = mid; else hi = mid - 1;
         }
-        const size_t at = ((size_t)rank * p.num_seqs + seq) * p.nh + kvh * G + head0 + row;
-        *reinterpret_cast<float4*>(p.own_o + at * HD + d) = v.o;
-        if (d == 0) *reinterpret_cast<float2*>(p.own_ml + at * 2) = make_float2(v.m, v.l);
+        own_piece(p, seq, piece - before[seq], before[seq + 1] - before[seq], block / p.head_blocks, (block % p.head_blocks) * 8, G, lane);
     }
 }
 
@@ -696,25 +737,26 @@ struct SharedArgs {
     const void* q; const void* cache; const int* block_tables; const int* ctx_lens; const int* plan;
     float* pre_o; float* pre_ml; float* own_o; float* own_ml; void* out; const float* sinks; const float* gate; int* status;
     cudaStream_t stream; long long num_pages;
-    int num_seqs, cap_tiles, cap_items, nh, nkv, hd, page_size, max_blocks, piece, pieces, most_parts;
+    int num_seqs, cap_tiles, cap_items, nh, nkv, hd, page_size, max_blocks, piece, pieces, own_ctas, most_parts;
     float scale, softcap;
 };
 
 // pre_o [cap_items, nkv, SP_ROWS, HEAD_DIM], pre_ml [.., 2], own_o [pieces, num_seqs, nh, HEAD_DIM] and own_ml [.., 2] receive the parts'
-// sums.  `piece`: own keys of a (sequence, kv head) that a CTA takes, `pieces`: the most CTAs that share a sequence (a longer one has
-// longer pieces); `most_parts`: about as many parts as a row has (it decides how the merge is laid out, nothing else).
+// sums.  `piece`: own keys of a (sequence, kv head) that a warp takes at a time, `pieces`: the most pieces of a sequence (a longer one has
+// longer ones), `own_ctas`: CTAs that take them in turn; `most_parts`: about as many parts as a row has (it decides how the merge is laid out, nothing else).
 RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     if (a->hd != HEAD_DIM) return RV_ERR_UNSUPPORTED;
     const int nh = a->nh, nkv = a->nkv, page_size = a->page_size;
     if (a->num_seqs < 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size <= 0 || a->max_blocks <= 0 || a->num_pages <= 0 || a->cap_tiles < 0 ||
-        a->cap_items < 0 || a->piece < 1 || a->pieces < 1 || !a->plan || !a->pre_o || !a->pre_ml || !a->own_o || !a->own_ml)
+        a->cap_items < 0 || a->piece < 1 || a->pieces < 1 || a->own_ctas < 1 || !a->plan || !a->pre_o || !a->pre_ml || !a->own_o || !a->own_ml)
         return RV_ERR_BAD_SIZE;
     const int G = nh / nkv;
     if (G > SP_ROWS || (page_size & (page_size - 1)) || page_size < 8) return RV_ERR_UNSUPPORTED;
     // a row of the tensor map, a CTA and a row of the result are ints in the kernels
     const int head_blocks = (G + 7) / 8;
-    const long long prefix_ctas = (long long)nkv * a->cap_items, own_ctas = (long long)a->num_seqs * nkv * head_blocks * a->pieces;
-    if (a->num_pages > 0x7fffffffLL / 2 / nkv / page_size || prefix_ctas + own_ctas > 0x7fffffffLL || (long long)a->num_seqs * nh > 0x7fffffffLL)
+    const long long prefix_ctas = (long long)nkv * a->cap_items;
+    if (a->num_pages > 0x7fffffffLL / 2 / nkv / page_size || prefix_ctas + a->own_ctas > 0x7fffffffLL || (long long)a->num_seqs * nh > 0x7fffffffLL ||
+        (long long)a->num_seqs * a->pieces > 0x7fffffffLL || a->num_seqs > MAX_SEQS)
         return RV_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->cache) | reinterpret_cast<uintptr_t>(a->pre_o) |
          reinterpret_cast<uintptr_t>(a->own_o) | reinterpret_cast<uintptr_t>(a->plan) | reinterpret_cast<uintptr_t>(a->out)) % 16 ||
@@ -736,10 +778,10 @@ RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     p.cap_log2e = a->softcap > 0.f ? a->softcap * 1.4426950408889634f : 0.f;
     p.scale_over_cap = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
     const int smem = Q_BYTES + NK * TILE_BYTES + NV * TILE_BYTES + 256;
-    static_assert((OWN_WARPS * 8 * (OWN_STRIDE + 2)) * 4 <= Q_BYTES, "the own keys' sums lie where the other kind has its queries");
+    static_assert((MAX_SEQS + 1 + OWN_WARPS) * 4 <= Q_BYTES + NK * TILE_BYTES + NV * TILE_BYTES, "the list of pieces lies in the same shared memory");
     static RvPerDevice configured;
     if (int e = rv_configure_smem(configured, shared_attention_kernel, smem)) return e;
-    RV_LAUNCH_ST = rv_launch(shared_attention_kernel, dim3((unsigned)(prefix_ctas + own_ctas)), dim3(NUM_THREADS), smem, a->stream, map_kv, p);
+    RV_LAUNCH_ST = rv_launch(shared_attention_kernel, dim3((unsigned)(prefix_ctas + a->own_ctas)), dim3(NUM_THREADS), smem, a->stream, map_kv, p);
     if ((st = rv_launch_status()) != RV_OK) return st;
     const int rows = a->num_seqs * nh, per_block = 128 / (HEAD_DIM / 4);
     if (a->most_parts > MERGE_BATCH)

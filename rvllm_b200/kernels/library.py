@@ -55,7 +55,7 @@ def _need(t: torch.Tensor, name: str, dtype=None, dims=None):
 
 
 # arguments of the entry points that take them as one block (the structures of the same names in csrc/)
-_SHARED_ARGS = struct.Struct("=15q11i2f")       # shared_attention_tcgen05.cu
+_SHARED_ARGS = struct.Struct("=15q12i2f")       # shared_attention_tcgen05.cu
 _PLAIN_ARGS = struct.Struct("=14q10i2f")       # shared_prefix.cu
 _TABLE_ARGS = struct.Struct("=13q8iq")         # step_tables.cu
 
@@ -571,7 +571,8 @@ class CudaKernels:
             self._check_attention_extras(q, num_heads, sinks, gate)
             _same_device(here, tuple((t, name) for t, name in ((sinks, "sinks"), (gate, "gate")) if t is not None))
         group = num_heads // num_kv_heads
-        fast = dt == 1 and head_dim in (64, 128) and page & (page - 1) == 0 and page >= 8 and pages * 2 * num_kv_heads * page < 2 ** 31
+        fast = dt == 1 and head_dim in (64, 128) and page & (page - 1) == 0 and page >= 8 and pages * 2 * num_kv_heads * page < 2 ** 31 \
+            and B <= 16384
         tiles, items = shared.capacity
         if items == 0 or B == 0 or group > TILE_ROWS or not (fast or (head_dim % 4 == 0 and head_dim <= 256)):
             return self.paged_attention(q, cache_layer, meta, num_heads, num_kv_heads, head_dim, scale, None, softcap, sinks, gate)
@@ -585,7 +586,7 @@ class CudaKernels:
         stream, cap = torch._C._cuda_getCurrentRawStream(here), softcap or 0.0
         if fast:
             # one buffer: the prefixes' sums, their maxima and denominators, and those of the own keys
-            piece, pieces = self._own_pieces(B * num_kv_heads * -(-group // 8), max_own)
+            piece, pieces, own_ctas = self._own_pieces(B * num_kv_heads * -(-group // 8), max_own, items * num_kv_heads)
             own_rows = pieces * B * num_heads
             scratch = torch.empty(((pre_rows + own_rows) * (head_dim + 2),), dtype=torch.float32, device=q.device)
             pre = scratch.data_ptr()
@@ -594,7 +595,7 @@ class CudaKernels:
             st = self._entry("shared_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",), "rv_shared_attention_tcgen05")(_SHARED_ARGS.pack(
                 q_at, cache_at, tables_at, lens_at, plan_at, pre, pre_ml, own, own + 4 * own_rows * head_dim, out_at, sinks_at, gate_at,
                 self._status.data_ptr(), stream, pages, B, tiles, items, num_heads, num_kv_heads, head_dim, page, tables.shape[1],
-                piece, pieces, pieces + shared.most_parts, scale, cap))
+                piece, pieces, own_ctas, pieces + shared.most_parts, scale, cap))
             _check("shared_attention_tcgen05", st)
             COUNTERS['launches'] += 1
             return out
@@ -611,10 +612,15 @@ class CudaKernels:
         COUNTERS['launches'] += 2
         return out
 
-    def _own_pieces(self, pairs: int, max_own: int):
-        """(keys of a piece, most pieces) for the own keys of `pairs` sequences and kv heads."""
-        piece = 128
-        return piece, max(1, min(64, -(-max_own // piece)))
+    def _own_pieces(self, pairs: int, max_own: int, prefix_ctas: int):
+        """(keys of a piece, most pieces of a sequence, CTAs) for the own keys of `pairs` sequences and blocks of heads."""
+        places = 2 * self.num_sms
+        ctas = places - prefix_ctas if prefix_ctas <= self.num_sms else places
+        piece = 64
+        while piece < 256 and pairs * -(-max_own // piece) > 8 * places:
+            piece *= 2
+        pieces = max(1, min(64, -(-max_own // piece)))
+        return piece, pieces, max(1, min(ctas, -(-pairs * pieces // 4)))
 
     def step_tables(self, page_table: torch.Tensor, rows: torch.Tensor, held: torch.Tensor, starts: torch.Tensor, q_lens: torch.Tensor,
                     new_pages: torch.Tensor, spans: torch.Tensor, num_tokens: int, max_blocks: int, page_size: int,
