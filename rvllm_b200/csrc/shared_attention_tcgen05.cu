@@ -26,17 +26,16 @@
 // P is rounded to bfloat16 (2^-9 relative), as in every attention kernel of this library: the tensor core takes no wider A
 // beside a bfloat16 V; sums and maxima are float.
 //
-// The own keys: G rows against each key, so the bytes bound it (hd x 4 bytes a key and kv head) and the tensor cores only save
-// instructions.  A warp works alone, on 16 keys at a time, without shared memory or barriers: keys and values go from global memory
-// straight into the operands of mma.sync.  For that the products are turned over - S^T [16 keys x 8 heads] = K Q^T and
-// O^T [16 dims x 8 heads] += V^T P^T, so that a group of up to eight heads fills the narrow side (a larger group is cut into
-// blocks of eight) - and the order of what is summed over is chosen by what a lane can load in 16 bytes: its eight neighbouring
-// elements of a key serve two steps of the product; of two neighbouring keys' values it takes the same columns, and byte permutes
-// pair them.  P^T gets from the layout of a result to that of an operand by two 8 x 8 transposes (movmatrix).  The loads of a chunk's
-// values and of the next chunk's keys are in flight while its scores are formed, page numbers a chunk ahead of that.  The own keys of
-// all sequences, cut into pieces, are one list that the warps of a fixed number of CTAs take in turn: a CTA for each sequence and
-// kv head, or several, spent most of its 4 to 10 us on being set up, and lengths of 1 to 700 left most of them idle (41 us and more
-// for 64 sequences of eight kv heads).  Keys outside a sequence, and pages that do not exist, are not loaded and count as not there.
+// The own keys: G rows against each key, so the bytes bound it (hd x 4 bytes a key and kv head) and what has to be won is latency: the
+// lengths, the pages and the keys of a sequence follow from one another, and most sequences have few keys of their own.  All of
+// them, cut into pieces, are one list, which the warps of a fixed number of CTAs take in turn; a warp works alone, on 16 keys at a time,
+// and asks for the next chunks (TMA, into stages of its own) across the ends of pieces, so that their memory latencies overlap.  The
+// products are turned over - S^T [16 keys x 8 heads] = K Q^T and O^T [16 dims x 8 heads] += V^T P^T on mma.sync, keys and values by
+// ldmatrix - so that a group of up to eight heads fills the narrow side (a larger group is cut into blocks of eight); P^T gets from
+// the layout of a result to that of an operand by two 8 x 8 transposes (movmatrix).  (Before, for 64 sequences with 1 to 700 own keys
+// of eight kv heads behind 2,048 shared ones, the whole step: a CTA per sequence and kv head, or several in a cluster, 41 to 70 us,
+// most of it set-up; a list of pieces whose keys went from global memory straight into registers 50 us, 8 to 13 us a piece of 64.)
+// Keys outside a sequence, and pages that do not exist, count as not there.
 // Cache layer layout: [num_pages, 2 (k, v), nkv, page_size, HEAD_DIM].
 #include "common.cuh"
 #include "shared_prefix.cuh"
@@ -118,10 +117,10 @@ struct Merged {
 // Pieces that the own keys of a sequence are cut into: as many as its own length asks for, at most as many as there is room for.
 __device__ __forceinline__ int pieces_of(int own, int piece, int most) { return max(1, min(most, (own + piece - 1) / piece)); }
 
-__device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* smem, int cta);
+__device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMap& map, unsigned char* smem, int cta);
 
 __global__ void __launch_bounds__(NUM_THREADS, 2)
-shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const SharedParams p) {
+shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ CUtensorMap map_own, const SharedParams p) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* q_s = smem_raw;                           // [HALVES][128 rows x 128 B]
     unsigned char* k_s = q_s + Q_BYTES;                      // [NK stages][HALVES][KV_TILE keys x 128 B]
@@ -140,15 +139,13 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
 
     rv_pdl_wait();
     if ((int)blockIdx.x >= p.prefix_ctas) {
-        own_keys(p, smem_raw, (int)blockIdx.x - p.prefix_ctas);
+        own_keys(p, map_own, smem_raw, (int)blockIdx.x - p.prefix_ctas);
         return;
     }
     const int item = blockIdx.x / p.nkv, kvh = blockIdx.x - item * p.nkv;
     const int G = p.nh / p.nkv;
-    if (item >= p.plan.items_used()) return;
-    const SharedItem it_ = p.plan.item(item);
-    const SharedTile tile = p.plan.tile(it_.tile);
-    const int key_lo = it_.key_begin, key_hi = it_.key_end;                 // a multiple of KV_TILE; the end may lie inside a page
+    const SharedItem tile = p.plan.item(item);
+    const int key_lo = tile.key_begin, key_hi = tile.key_end;               // a multiple of KV_TILE; the end may lie inside a page
     const int tile_rows = min(tile.count, ROWS / G) * G;
     if (key_hi <= key_lo || tile_rows <= 0) return;
     const int t_begin = key_lo / KV_TILE, n_it = (key_hi + KV_TILE - 1) / KV_TILE - t_begin;
@@ -360,6 +357,8 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
                 const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * eff_scale;
                 // The reference maximum is raised only when it is more than 2^8 behind: O then needs a pass.  The exponentials do not
                 // wait to know: they are formed under the old reference beside the maximum, and once more in the rare tile that raises it.
+                // (The first tile has its maximum to begin with.)
+                if (it == 0) m_ref = m_tile;
                 bool raise = m_tile > m_ref + RESCALE_LOG2 || (m_ref == -INFINITY && m_tile > -INFINITY);
                 uint32_t pk[32];
                 float l_tile, l_tile2;
@@ -385,22 +384,20 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
                         l_run *= factor;
                         raise = false;
                     }
-                    if (it > 0) {
-                        // the product of the tile before must have finished; the one after waits for this warp's P
-                        if (!mbar_wait(bar_o_full0 + 8 * (pb ^ 1), ((it - 1) >> 1) & 1, &abort_flag, 11)) { ok = false; break; }
-                        tcgen05_fence_after();
+                    // the product of the tile before must have finished; the one after waits for this warp's P
+                    if (!mbar_wait(bar_o_full0 + 8 * (pb ^ 1), ((it - 1) >> 1) & 1, &abort_flag, 11)) { ok = false; break; }
+                    tcgen05_fence_after();
 #pragma unroll
-                        for (int c = 0; c < HEAD_DIM; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld_32x32(t_lane + O_COL + c, o);
-                            tmem_ld_wait();
+                    for (int c = 0; c < HEAD_DIM; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(t_lane + O_COL + c, o);
+                        tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-                            tmem_st_32x32(t_lane + O_COL + c, o);
-                        }
-                        tmem_st_wait();
-                        tcgen05_fence_before();
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                        tmem_st_32x32(t_lane + O_COL + c, o);
                     }
+                    tmem_st_wait();
+                    tcgen05_fence_before();
                 }
                 if (!ok) break;
                 l_run += l_tile + l_tile2;
@@ -465,169 +462,63 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const Shared
 // The own keys (see the top of the file).
 #define OWN_WARPS 4
 #define OWN_THREADS (32 * OWN_WARPS)
-#define KEY_CHUNKS (HEAD_DIM / 32)            // 16-byte loads of a lane per key
-#define VAL_CHUNKS (HEAD_DIM / 64)            // ... per value row
+#define OWN_CHUNK 16                           // keys
+#define OWN_STAGES 2                           // of a warp; two CTAs an SM have 8 warps x 2 x 8 KB on their way (head size 128)
 #define DIM_BLOCKS (HEAD_DIM / 16)
+#define SLAB_BYTES (OWN_CHUNK * 128)           // 64 columns of a chunk
+#define CHUNK_BYTES (HALVES * SLAB_BYTES)
+#define QUERY_BYTES (8 * HEAD_DIM * 2)
+#define STAGE_BYTES (2 * CHUNK_BYTES + QUERY_BYTES)                        // keys, values, the piece's queries (with its first chunk)
 #define MERGE_BATCH 12
-#define MAX_SEQS 16384                        // of a step: what the list of pieces has room for
+#define MAX_SEQS 4096                          // of a step: what the list of pieces has room for
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
     return d;
 }
-// (by way of L2 alone: this kernel reads before it waits, and what is read may have been written on another SM just before)
-__device__ __forceinline__ uint4 load_16(const __nv_bfloat16* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); }
-// Piece `rank` of `pieces` of sequence `seq`: heads head0 .. head0 + 7 of kv head kvh (of a group of G), by one warp.
-__device__ __forceinline__ void own_piece(const SharedParams& p, int seq, int rank, int pieces, int kvh, int head0, int G, int lane) {
-    constexpr int HD = HEAD_DIM;
-    const int g = lane >> 2, tq = lane & 3;
-    const int heads = min(8, G - head0);
-    const int ctx = max(p.ctx_lens[seq], 0), start = min(p.plan.own_start(seq), ctx);
-    const int* table = p.block_tables + (size_t)seq * p.max_blocks;
-    // its chunks of 16 keys
-    const int first = start / 16, chunks = (ctx + 15) / 16 - first, per = (chunks + pieces - 1) / pieces;
-    int chunk = first + rank * per;
-    const int chunk_end = min(first + chunks, chunk + per);
-    // this lane's queries: head g of the block, elements (4 j + tq) * 8 .. + 7
-    uint4 qf[KEY_CHUNKS];
-#pragma unroll
-    for (int j = 0; j < KEY_CHUNKS; ++j) {
-        qf[j] = make_uint4(0, 0, 0, 0);
-        if (g < heads) qf[j] = load_16(p.q + ((size_t)seq * p.nh + kvh * G + head0 + g) * HD + (4 * j + tq) * 8);
-    }
-    float o[DIM_BLOCKS][4];
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};        // heads 2 tq, 2 tq + 1
-#pragma unroll
-    for (int i = 0; i < DIM_BLOCKS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    const size_t plane = (size_t)p.nkv * p.page_size * HD;                 // from a key to its value
-    // the page of `key`, or -1 where the sequence has no such key
-    auto page_of = [&](int key) -> int {
-        if (key < start || key >= ctx || (key >> p.page_shift) >= p.max_blocks) return -1;
-        const int page = __ldg(table + (key >> p.page_shift));
-        return page < p.num_pages ? page : -1;
-    };
-    auto row_at = [&](int page, int key) -> const __nv_bfloat16* {
-        return p.cache + (((size_t)page * 2 * p.nkv + kvh) * p.page_size + (key & (p.page_size - 1))) * HD;
-    };
-    // Pages of the chunk's keys, looked up a chunk ahead of the keys themselves: of keys g and g + 8 by every lane; with pages of 16
-    // keys or more that is the page of all of them, with pages of 8 one for each half.
-    int pk[2], next[2];
-    uint4 kf[2][KEY_CHUNKS];                                               // keys g and g + 8 of the chunk
-    auto look_up = [&](int c, int (&to)[2]) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) to[r] = c < chunk_end ? page_of(c * 16 + g + 8 * r) : -1;
-    };
-    auto load_keys = [&](int c) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const __nv_bfloat16* row = row_at(max(pk[r], 0), c * 16 + g + 8 * r);
-#pragma unroll
-            for (int j = 0; j < KEY_CHUNKS; ++j) kf[r][j] = pk[r] >= 0 ? load_16(row + (4 * j + tq) * 8) : make_uint4(0, 0, 0, 0);
-        }
-    };
-    look_up(chunk, pk);
-    look_up(chunk + 1, next);
-    load_keys(chunk);
-    for (; chunk < chunk_end; ++chunk) {
-        // values of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9: columns 64 c + 8 g .. + 7
-        uint4 vf[4][VAL_CHUNKS];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int in = 2 * tq + (r & 1), key = chunk * 16 + in + 8 * (r >> 1);
-            const int page = __shfl_sync(0xffffffffu, pk[r >> 1], in * 4);         // (a lane with g = in has it, if the key is there)
-            const __nv_bfloat16* row = row_at(max(page, 0), key) + plane;
-#pragma unroll
-            for (int c = 0; c < VAL_CHUNKS; ++c) vf[r][c] = page >= 0 ? load_16(row + 64 * c + 8 * g) : make_uint4(0, 0, 0, 0);
-        }
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < KEY_CHUNKS; ++j) {
-            const uint32_t a0[4] = {kf[0][j].x, kf[1][j].x, kf[0][j].y, kf[1][j].y};
-            const uint32_t a1[4] = {kf[0][j].z, kf[1][j].z, kf[0][j].w, kf[1][j].w};
-            mma_16816(s, a0, qf[j].x, qf[j].y);
-            mma_16816(s, a1, qf[j].z, qf[j].w);
-        }
-        const bool see[2] = {pk[0] >= 0, pk[1] >= 0};
-        pk[0] = next[0]; pk[1] = next[1];
-        load_keys(chunk + 1);
-        look_up(chunk + 2, next);
-        float alpha[2];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {                                      // e: key g + 8 (e >> 1), head 2 tq + (e & 1)
-            float v = s[e] * p.scale_log2e;
-            if (p.cap_log2e > 0.f) {
-                const float x = fast_exp2(s[e] * p.scale_over_cap * 2.885390081777927f);
-                v = p.cap_log2e * (1.f - __fdividef(2.f, x + 1.f));
-            }
-            s[e] = see[e >> 1] ? v : -INFINITY;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float mx = fmaxf(s[h], s[h + 2]);
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            const float m_new = fmaxf(m_run[h], mx);
-            const float m_s = m_new == -INFINITY ? 0.f : m_new;
-            alpha[h] = fast_exp2(m_run[h] - m_s);                          // 0 while nothing has been seen
-            m_run[h] = m_new;
-            s[h] = fast_exp2(s[h] - m_s);
-            s[h + 2] = fast_exp2(s[h + 2] - m_s);
-            l_run[h] = l_run[h] * alpha[h] + s[h] + s[h + 2];              // this lane's keys; the lanes are added at the end
-        }
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(s[0], s[1]), hi = __floats2bfloat162_rn(s[2], s[3]);
-        const uint32_t p0 = transpose_8x8(*reinterpret_cast<const uint32_t*>(&lo));      // keys 2 tq, 2 tq + 1 of head g
-        const uint32_t p1 = transpose_8x8(*reinterpret_cast<const uint32_t*>(&hi));      // ... + 8
-#pragma unroll
-        for (int i = 0; i < DIM_BLOCKS; ++i) {                             // rows g, g + 8 of a block: columns 64 c + 8 g + 2 w, + 1
-            o[i][0] *= alpha[0]; o[i][1] *= alpha[1];
-            o[i][2] *= alpha[0]; o[i][3] *= alpha[1];
-            const int c = i >> 2, w = i & 3;
-            auto word = [&](int r) -> uint32_t {
-                const uint4& v = vf[r][c];
-                return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w;
-            };
-            const uint32_t a[4] = {__byte_perm(word(0), word(1), 0x5410), __byte_perm(word(0), word(1), 0x7632),
-                                   __byte_perm(word(2), word(3), 0x5410), __byte_perm(word(2), word(3), 0x7632)};
-            mma_16816(o[i], a, p0, p1);
-        }
-    }
-    // a lane has eight neighbouring columns of its two heads in every 64
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
-        const int head = 2 * tq + h;
-        if (head >= heads) continue;
-        const size_t at = ((size_t)rank * p.num_seqs + seq) * p.nh + kvh * G + head0 + head;
-        if (g == 0) *reinterpret_cast<float2*>(p.own_ml + at * 2) = make_float2(m_run[h], l_run[h]);
-#pragma unroll
-        for (int c = 0; c < VAL_CHUNKS; ++c)
-#pragma unroll
-            for (int w = 0; w < 4; w += 2) {
-                const int i = 4 * c + w;
-                *reinterpret_cast<float4*>(p.own_o + at * HD + 64 * c + 8 * g + 2 * w) = make_float4(o[i][h], o[i][h + 2], o[i + 1][h], o[i + 1][h + 2]);
-            }
-    }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* smem, int cta) {
+// A warp's place in the list of pieces: which piece, and which chunk of it comes next.
+struct OwnCursor {
+    long long at;                  // piece x block of heads, in the whole list
+    int seq, rank, kvh, head0;
+    int chunk, chunk_end, ctx, start;
+    bool first;                    // no chunk of the piece has been asked for yet
+    int page;                      // of this lane's box of the chunk, -1 without one
+};
+
+__device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMap& map, unsigned char* smem, int cta) {
     constexpr int HD = HEAD_DIM;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     rv_pdl_launch_dependents();
-    if (warp >= OWN_WARPS) {                        // the other warpgroup's registers go to the four warps that work
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
-        return;
-    }
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    if (warp >= OWN_WARPS) return;
     const int G = p.nh / p.nkv, blocks = p.nkv * p.head_blocks;
-    // before[s]: pieces of the sequences before s
-    int* before = reinterpret_cast<int*>(smem);                            // [num_seqs + 1], behind it [OWN_WARPS]
-    int* of_warp = before + p.num_seqs + 1;
+    unsigned char* ring = smem + warp * (OWN_STAGES * STAGE_BYTES);        // (stages start on 1,024-byte boundaries: see the swizzle)
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OWN_WARPS * OWN_STAGES * STAGE_BYTES);
+    int* of_warp = reinterpret_cast<int*>(bars + OWN_WARPS * OWN_STAGES);
+    volatile int& abort_flag = *reinterpret_cast<volatile int*>(of_warp + OWN_WARPS);
+    int* before = of_warp + OWN_WARPS + 1;                                 // [num_seqs + 1]: pieces of the sequences before one
+    const uint32_t bar0 = smem_u32(bars + warp * OWN_STAGES);
+    if (tid == 0) abort_flag = 0;
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < OWN_STAGES; ++i) mbar_init(bar0 + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     const int each = (p.num_seqs + OWN_THREADS - 1) / OWN_THREADS, s_lo = min(tid * each, p.num_seqs), s_hi = min(s_lo + each, p.num_seqs);
     int mine = 0;
     for (int s = s_lo; s < s_hi; ++s) {
@@ -652,16 +543,188 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, unsigned char* s
     for (int s = s_lo; s < s_hi; ++s) before[s] += base;
     if (tid == 0) before[p.num_seqs] = total;
     asm volatile("bar.sync 1, %0;" ::"n"(OWN_THREADS) : "memory");
+
     const int warps = ((int)gridDim.x - p.prefix_ctas) * OWN_WARPS;
-    for (long long at = cta * OWN_WARPS + warp; at < (long long)total * blocks; at += warps) {
-        // piece `at / blocks` of all, block of heads `at mod blocks`
-        const int piece = (int)(at / blocks), block = (int)(at - (long long)piece * blocks);
+    const long long all = (long long)total * blocks;
+    auto enter = [&](OwnCursor& c) {                 // the piece at c.at
+        if (c.at >= all) return;
+        const int piece = (int)(c.at / blocks), block = (int)(c.at - (long long)piece * blocks);
         int seq = 0;
         for (int hi = p.num_seqs - 1; seq < hi;) {                         // the last sequence that begins at or before it
             const int mid = (seq + hi + 1) >> 1;
             if (before[mid] <= piece) seq = mid; else hi = mid - 1;
         }
-        own_piece(p, seq, piece - before[seq], before[seq + 1] - before[seq], block / p.head_blocks, (block % p.head_blocks) * 8, G, lane);
+        c.seq = seq;
+        c.rank = piece - before[seq];
+        c.kvh = block / p.head_blocks;
+        c.head0 = (block - c.kvh * p.head_blocks) * 8;
+        c.ctx = max(p.ctx_lens[seq], 0);
+        c.start = min(p.plan.own_start(seq), c.ctx);
+        const int pieces = before[seq + 1] - before[seq];
+        const int lo = c.start / OWN_CHUNK, chunks = (c.ctx + OWN_CHUNK - 1) / OWN_CHUNK - lo, per = (chunks + pieces - 1) / pieces;
+        c.chunk = min(lo + c.rank * per, lo + chunks);
+        c.chunk_end = min(lo + chunks, c.chunk + per);
+        c.first = true;
+    };
+    auto next = [&](OwnCursor& c) {                  // the chunk behind c's, of the next piece if need be (an empty piece counts as one)
+        c.first = false;
+        if (++c.chunk >= c.chunk_end) { c.at += warps; enter(c); }
+    };
+    const int box_keys = p.page_size < OWN_CHUNK ? p.page_size : OWN_CHUNK, boxes = OWN_CHUNK / box_keys;
+    // Lane i < boxes has the i-th box of a chunk's keys, lane 16 + i that of its values.  Its page is looked up when the chunk before has
+    // been asked for, and looked at when the copy is.
+    auto look_up = [&](OwnCursor& c) {
+        const int key = c.chunk * OWN_CHUNK + (lane & 15) * box_keys;
+        c.page = -1;
+        if (c.at < all && (lane & 15) < boxes && c.chunk < c.chunk_end && key < c.ctx && key + box_keys > c.start && (key >> p.page_shift) < p.max_blocks)
+            c.page = __ldg(p.block_tables + (size_t)c.seq * p.max_blocks + (key >> p.page_shift));
+    };
+    auto ask = [&](const OwnCursor& c, int stage) {
+        const int which = lane >> 4, key = c.chunk * OWN_CHUNK + (lane & 15) * box_keys;
+        const int page = c.page < p.num_pages ? c.page : -1;
+        const unsigned mask = __ballot_sync(0xffffffffu, page >= 0);
+        const uint32_t bar = bar0 + 8 * stage, to = smem_u32(ring) + stage * STAGE_BYTES;
+        const int heads = min(8, G - c.head0);
+        if (lane == 0) {
+            mbar_expect_tx(bar, (uint32_t)__popc(mask) * HALVES * (uint32_t)box_keys * 128u + (c.first ? (uint32_t)heads * HD * 2u : 0u));
+            if (c.first) bulk_load(to + 2 * CHUNK_BYTES, p.q + ((size_t)c.seq * p.nh + c.kvh * G + c.head0) * HD, (uint32_t)heads * HD * 2u, bar);
+        }
+        __syncwarp();
+        if (page >= 0) {
+            const int row = ((page * 2 + which) * p.nkv + c.kvh) * p.page_size + (key & (p.page_size - 1));
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+                tma_load_2d(to + which * CHUNK_BYTES + h * SLAB_BYTES + (lane & 15) * box_keys * 128, &map, h * 64, row, bar);
+        }
+        return mask & 0xffffu;                       // the boxes of keys that come
+    };
+
+    OwnCursor ahead, now;
+    ahead.at = now.at = cta * OWN_WARPS + warp;
+    enter(ahead);
+    now = ahead;
+    look_up(ahead);
+    unsigned here[OWN_STAGES];                       // which boxes of a stage have keys
+    int asked = 0, taken = 0;
+#pragma unroll
+    for (int i = 0; i < OWN_STAGES; ++i)
+        if (ahead.at < all) { here[i] = ask(ahead, i); ++asked; next(ahead); look_up(ahead); }
+    const int g = lane >> 2, tq = lane & 3;
+    uint32_t qf[DIM_BLOCKS][2];
+    float o[DIM_BLOCKS][4], m_run[2], l_run[2];      // heads 2 tq, 2 tq + 1
+    bool ok = true;
+    while (now.at < all && ok) {
+#pragma unroll
+        for (int stage = 0; stage < OWN_STAGES; ++stage) {
+            if (now.at >= all) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, (taken / OWN_STAGES) & 1, &abort_flag, 14))) { ok = false; break; }
+            ++taken;
+            const uint32_t ks = smem_u32(ring) + stage * STAGE_BYTES, vs = ks + CHUNK_BYTES;
+            if (now.first) {
+                // Q as the B operand: elements 2 tq, 2 tq + 1 (and 8 on) of head g in every 16; heads beyond the block are zeros
+                const uint32_t* q = reinterpret_cast<const uint32_t*>(ring + stage * STAGE_BYTES + 2 * CHUNK_BYTES) + g * (HD / 2) + tq;
+                const bool have = g < G - now.head0;
+#pragma unroll
+                for (int i = 0; i < DIM_BLOCKS; ++i) {
+                    qf[i][0] = have ? q[8 * i] : 0u;
+                    qf[i][1] = have ? q[8 * i + 4] : 0u;
+                    o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+                }
+                m_run[0] = m_run[1] = -INFINITY;
+                l_run[0] = l_run[1] = 0.f;
+            }
+            // which of the chunk's keys there are, a bit each
+            const int key0 = now.chunk * OWN_CHUNK;
+            unsigned see = 0;
+            if (now.chunk < now.chunk_end) {
+                const int lo = max(now.start - key0, 0), hi = min(now.ctx - key0, OWN_CHUNK);
+                see = hi > lo ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
+                if (here[stage] != (1u << boxes) - 1u)
+                    for (int i = 0; i < boxes; ++i)
+                        if (!(here[stage] >> i & 1u)) see &= ~(((1u << box_keys) - 1u) << (i * box_keys));
+            }
+            if (see != 0xffffu) {
+                // values of keys that are not there: zeros, so that what an earlier request left, a NaN for instance, does not meet a
+                // probability of zero
+                if (!(see >> (lane >> 1) & 1u)) {
+                    unsigned char* row = ring + stage * STAGE_BYTES + CHUNK_BYTES + (lane >> 1) * 128 + (lane & 1) * 64;
+#pragma unroll
+                    for (int i = 0; i < 4 * HALVES; ++i)
+                        *reinterpret_cast<uint4*>(row + (i >> 2) * SLAB_BYTES + (i & 3) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();                  // (the next copy into the stage comes behind these writes)
+                __syncwarp();
+            }
+            if (see) {
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
+                const int r = (lane & 7) + ((lane >> 3) & 1) * 8, half = lane >> 4;
+#pragma unroll
+                for (int i = 0; i < DIM_BLOCKS; ++i) {                     // keys r, 8 columns at 16 i + 8 half
+                    uint32_t a[4];
+                    ldmatrix_4(a, ks + (i >> 2) * SLAB_BYTES + r * 128 + (((2 * (i & 3) + half) ^ (r & 7)) << 4));
+                    mma_16816(s, a, qf[i][0], qf[i][1]);
+                }
+                float alpha[2];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {                              // e: key g + 8 (e >> 1), head 2 tq + (e & 1)
+                    float v = s[e] * p.scale_log2e;
+                    if (p.cap_log2e > 0.f) {
+                        const float x = fast_exp2(s[e] * p.scale_over_cap * 2.885390081777927f);
+                        v = p.cap_log2e * (1.f - __fdividef(2.f, x + 1.f));
+                    }
+                    s[e] = see >> (g + 8 * (e >> 1)) & 1u ? v : -INFINITY;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float mx = fmaxf(s[h], s[h + 2]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                    const float m_new = fmaxf(m_run[h], mx);
+                    const float m_s = m_new == -INFINITY ? 0.f : m_new;
+                    alpha[h] = fast_exp2(m_run[h] - m_s);                  // 0 while nothing has been seen
+                    m_run[h] = m_new;
+                    s[h] = fast_exp2(s[h] - m_s);
+                    s[h + 2] = fast_exp2(s[h + 2] - m_s);
+                    l_run[h] = l_run[h] * alpha[h] + s[h] + s[h + 2];      // this lane's keys; the lanes are added at the end
+                }
+                const __nv_bfloat162 lo2 = __floats2bfloat162_rn(s[0], s[1]), hi2 = __floats2bfloat162_rn(s[2], s[3]);
+                const uint32_t p0 = transpose_8x8(*reinterpret_cast<const uint32_t*>(&lo2));     // keys 2 tq, 2 tq + 1 of head g
+                const uint32_t p1 = transpose_8x8(*reinterpret_cast<const uint32_t*>(&hi2));     // ... + 8
+                const int vr = (lane & 7) + (lane >> 4) * 8, vhalf = (lane >> 3) & 1;
+#pragma unroll
+                for (int i = 0; i < DIM_BLOCKS; ++i) {                     // columns 16 i + g and 8 on
+                    o[i][0] *= alpha[0]; o[i][1] *= alpha[1];
+                    o[i][2] *= alpha[0]; o[i][3] *= alpha[1];
+                    uint32_t a[4];
+                    ldmatrix_4t(a, vs + (i >> 2) * SLAB_BYTES + vr * 128 + (((2 * (i & 3) + vhalf) ^ (vr & 7)) << 4));
+                    mma_16816(o[i], a, p0, p1);
+                }
+            }
+            __syncwarp();                            // the stage has been read
+            if (ahead.at < all) { here[stage] = ask(ahead, stage); ++asked; next(ahead); look_up(ahead); }
+            if (now.chunk + 1 >= now.chunk_end) {    // the piece's last chunk
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float l = l_run[h];
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+                    const int head = now.head0 + 2 * tq + h;
+                    if (head >= G) continue;
+                    const size_t row = ((size_t)now.rank * p.num_seqs + now.seq) * p.nh + now.kvh * G + head;
+                    if (g == 0) *reinterpret_cast<float2*>(p.own_ml + row * 2) = make_float2(m_run[h], l);
+                    float* to = p.own_o + row * HD + g;
+#pragma unroll
+                    for (int i = 0; i < DIM_BLOCKS; ++i) { to[16 * i] = o[i][h]; to[16 * i + 8] = o[i][h + 2]; }
+                }
+            }
+            next(now);
+        }
+    }
+    // A wait gave up: copies may still be on their way into this CTA's shared memory.  Waited for (bounded) before it is given up.
+    if (!ok && lane == 0) {
+        volatile int ignore = 0;
+        for (int i = taken; i < asked; ++i) mbar_wait(bar0 + 8 * (i % OWN_STAGES), (i / OWN_STAGES) & 1, &ignore, 0);
+        if (p.status) atomicCAS(p.status, 0, abort_flag);
     }
 }
 
@@ -763,11 +826,12 @@ RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
         (reinterpret_cast<uintptr_t>(a->pre_ml) | reinterpret_cast<uintptr_t>(a->own_ml)) % 8)
         return RV_ERR_ALIGNMENT;
     if (a->num_seqs == 0) return RV_OK;
-    alignas(64) CUtensorMap map_kv;
+    alignas(64) CUtensorMap map_kv, map_own;
     int st = rv_make_bf16_map(&map_kv, a->cache, a->num_pages * 2 * nkv * page_size, HEAD_DIM, page_size < KV_TILE ? page_size : KV_TILE);
+    if (st == RV_OK) st = rv_make_bf16_map(&map_own, a->cache, a->num_pages * 2 * nkv * page_size, HEAD_DIM, page_size < OWN_CHUNK ? page_size : OWN_CHUNK);
     if (st != RV_OK) return st;
     SharedParams p;
-    p.plan = shared_plan(a->plan, a->num_seqs, a->cap_tiles, a->cap_items);
+    p.plan = shared_plan(a->plan, a->num_seqs, a->cap_tiles);
     p.q = (const __nv_bfloat16*)a->q; p.cache = (const __nv_bfloat16*)a->cache; p.block_tables = a->block_tables; p.ctx_lens = a->ctx_lens;
     p.pre_o = a->pre_o; p.pre_ml = a->pre_ml; p.own_o = a->own_o; p.own_ml = a->own_ml; p.status = a->status;
     p.num_seqs = a->num_seqs; p.nh = nh; p.nkv = nkv; p.page_size = page_size; p.max_blocks = a->max_blocks; p.num_pages = (int)a->num_pages;
@@ -778,10 +842,12 @@ RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     p.cap_log2e = a->softcap > 0.f ? a->softcap * 1.4426950408889634f : 0.f;
     p.scale_over_cap = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
     const int smem = Q_BYTES + NK * TILE_BYTES + NV * TILE_BYTES + 256;
-    static_assert((MAX_SEQS + 1 + OWN_WARPS) * 4 <= Q_BYTES + NK * TILE_BYTES + NV * TILE_BYTES, "the list of pieces lies in the same shared memory");
+    static_assert(OWN_WARPS * OWN_STAGES * (STAGE_BYTES + 8) + (OWN_WARPS + 1 + MAX_SEQS + 1) * 4 <= Q_BYTES + (NK + NV) * TILE_BYTES,
+                  "the own keys' stages and their list lie in the same shared memory");
+    static_assert(STAGE_BYTES % 1024 == 0, "the swizzle goes by address bits 7 to 9");
     static RvPerDevice configured;
     if (int e = rv_configure_smem(configured, shared_attention_kernel, smem)) return e;
-    RV_LAUNCH_ST = rv_launch(shared_attention_kernel, dim3((unsigned)(prefix_ctas + a->own_ctas)), dim3(NUM_THREADS), smem, a->stream, map_kv, p);
+    RV_LAUNCH_ST = rv_launch(shared_attention_kernel, dim3((unsigned)(prefix_ctas + a->own_ctas)), dim3(NUM_THREADS), smem, a->stream, map_kv, map_own, p);
     if ((st = rv_launch_status()) != RV_OK) return st;
     const int rows = a->num_seqs * nh, per_block = 128 / (HEAD_DIM / 4);
     if (a->most_parts > MERGE_BATCH)

@@ -60,12 +60,11 @@ shared_plain_kernel(const PlainParams p) {
         key_hi = min(ctx, key_lo + per * PLAIN_TILE);
     } else {
         item = blockIdx.y;
-        if (item >= p.plan.items_used()) return;
-        const SharedItem it = p.plan.item(item);
-        const SharedTile tile = p.plan.tile(it.tile);
+        const SharedItem tile = p.plan.item(item);
         table_seq = tile.table_seq; first = tile.first;
         rows = min(tile.count, SP_ROWS / G) * G;
-        key_lo = it.key_begin; key_hi = it.key_end;
+        key_lo = tile.key_begin; key_hi = tile.key_end;
+        if (key_hi <= key_lo) return;
     }
     if (row0 >= rows) return;
     if (tid < R) {
@@ -302,7 +301,7 @@ RV_EXPORT int rv_shared_attention_plain(const PlainArgs* a) {
         return RV_ERR_ALIGNMENT;
     if (a->num_seqs == 0) return RV_OK;
     PlainParams p;
-    p.plan = shared_plan(a->plan, a->num_seqs, a->cap_tiles, a->cap_items);
+    p.plan = shared_plan(a->plan, a->num_seqs, a->cap_tiles);
     p.q = a->q; p.cache = a->cache; p.block_tables = a->block_tables; p.ctx_lens = a->ctx_lens;
     p.num_pages = a->num_pages; p.num_seqs = a->num_seqs;
     p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = a->page_size; p.max_blocks = a->max_blocks; p.splits = a->splits;

@@ -572,7 +572,7 @@ class CudaKernels:
             _same_device(here, tuple((t, name) for t, name in ((sinks, "sinks"), (gate, "gate")) if t is not None))
         group = num_heads // num_kv_heads
         fast = dt == 1 and head_dim in (64, 128) and page & (page - 1) == 0 and page >= 8 and pages * 2 * num_kv_heads * page < 2 ** 31 \
-            and B <= 16384
+            and B <= 4096
         tiles, items = shared.capacity
         if items == 0 or B == 0 or group > TILE_ROWS or not (fast or (head_dim % 4 == 0 and head_dim <= 256)):
             return self.paged_attention(q, cache_layer, meta, num_heads, num_kv_heads, head_dim, scale, None, softcap, sinks, gate)
@@ -617,9 +617,9 @@ class CudaKernels:
         places = 2 * self.num_sms
         ctas = places - prefix_ctas if prefix_ctas <= self.num_sms else places
         piece = 64
-        while piece < 256 and pairs * -(-max_own // piece) > 8 * places:
+        while -(-max_own // piece) > 64:
             piece *= 2
-        pieces = max(1, min(64, -(-max_own // piece)))
+        pieces = max(1, -(-max_own // piece))
         return piece, pieces, max(1, min(ctas, -(-pairs * pieces // 4)))
 
     def step_tables(self, page_table: torch.Tensor, rows: torch.Tensor, held: torch.Tensor, starts: torch.Tensor, q_lens: torch.Tensor,

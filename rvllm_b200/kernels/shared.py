@@ -52,7 +52,7 @@ class SharedPrefixes:
     def ints(num_seqs: int, capacity: Tuple[int, int]) -> int:
         """32-bit integers of the array."""
         tiles, items = capacity
-        return (4 + 3 * num_seqs + 2 * tiles + 3) // 4 * 4 + 4 * tiles + 4 * items
+        return (4 + 3 * num_seqs + 2 * tiles + 3) // 4 * 4 + 8 * items
 
     @property
     def own_start(self) -> torch.Tensor:
@@ -96,7 +96,8 @@ class SharedPrefixes:
                 k = -(-n // step)
                 edges = [n * j // k for j in range(k + 1)]
                 parts.append((len(items), k))
-                items += [(i, a * KEY_TILE, min(b * KEY_TILE, tiles[i][3]), 0) for a, b in zip(edges, edges[1:])]
+                seq, first, count, tokens = tiles[i]
+                items += [(a * KEY_TILE, min(b * KEY_TILE, tokens), seq, first, count, i, 0, 0) for a, b in zip(edges, edges[1:])]
         capacity = capacity or (len(tiles), len(items))
         if len(tiles) > capacity[0] or len(items) > capacity[1]:
             raise KernelError(f"shared prefixes: {len(tiles)} row tiles and {len(items)} ranges of keys do not fit a capacity of {capacity}")
@@ -108,9 +109,7 @@ class SharedPrefixes:
         if tiles:
             host[4 + 3 * B:4 + 3 * B + 2 * len(tiles)] = np.asarray(parts, np.int32).ravel()
             at = (4 + 3 * B + 2 * capacity[0] + 3) // 4 * 4
-            host[at:at + 4 * len(tiles)] = np.asarray(tiles, np.int32).ravel()
-            at += 4 * capacity[0]
-            host[at:at + 4 * len(items)] = np.asarray(items, np.int32).ravel()
+            host[at:at + 8 * len(items)] = np.asarray(items, np.int32).ravel()
         self.capacity, self.num_items, self.num_tiles = capacity, len(items), len(tiles)
         self.most_parts = max((n for _, n in parts), default=0)
         # the fewest keys that any sequence has before its own begin (0: one has no prefix)

@@ -13,9 +13,10 @@ def unpack(s):
     v, B = s.device_ints.tolist(), s.num_seqs
     tiles, items = s.capacity
     at = (4 + 3 * B + 2 * tiles + 3) // 4 * 4
+    ranges = [v[at + 8 * i:at + 8 * i + 8] for i in range(items)]
+    rows = {r[5]: r[2:5] for r in ranges[:v[0]]}
     return dict(items_used=v[0], tiles_used=v[1], own_start=v[4:4 + B], place=v[4 + B:4 + 2 * B], members=v[4 + 2 * B:4 + 3 * B],
-                parts=[v[4 + 3 * B + 2 * i:4 + 3 * B + 2 * i + 2] for i in range(tiles)], tiles=[v[at + 4 * i:at + 4 * i + 4] for i in range(tiles)],
-                items=[v[at + 4 * tiles + 4 * i:at + 4 * tiles + 4 * i + 4] for i in range(items)], size=len(v))
+                parts=[v[4 + 3 * B + 2 * i:4 + 3 * B + 2 * i + 2] for i in range(tiles)], tiles=rows, items=ranges, size=len(v))
 
 
 @pytest.mark.parametrize("seed", range(12))
@@ -41,18 +42,18 @@ def test_every_row_and_key_once(seed):
             assert u["own_start"][b] == 0 and u["place"][b] == -1
             continue
         tile, row = divmod(u["place"][b], 128)
-        seq, first, count, tokens = u["tiles"][tile]
-        assert tokens == of[b][1] == u["own_start"][b] and seq in groups[of[b][0]][0]
+        seq, first, count = u["tiles"][tile]
+        assert of[b][1] == u["own_start"][b] and seq in groups[of[b][0]][0]
         assert row % per == 0 and row + per <= 128 and u["members"][first + row // per] == b and row // per < count
         rows.add((tile, row))
     assert len(rows) == len(of)
     for t in range(u["tiles_used"]):
         first, n = u["parts"][t]
         at = 0
-        for tile, lo, hi, _ in u["items"][first:first + n]:
+        for lo, hi, seq, _, _, tile, _, _ in u["items"][first:first + n]:
             assert tile == t and lo == at and lo % 64 == 0 and lo < hi
             at = hi
-        assert at == u["tiles"][t][3]
+        assert at == u["own_start"][u["tiles"][t][0]]
     assert u["items_used"] == sum(n for _, n in u["parts"][:u["tiles_used"]])
 
 
