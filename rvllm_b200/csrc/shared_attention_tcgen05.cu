@@ -505,6 +505,9 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
     constexpr int HD = HEAD_DIM;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     rv_pdl_launch_dependents();
+    // No second CTA of a kernel with tensor memory is placed on an SM while the first may still ask for some, so a CTA that needs
+    // none says so (without this line the own keys' CTAs ran one an SM).
+    if (warp == OWN_WARPS) asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     if (warp >= OWN_WARPS) return;
     const int G = p.nh / p.nkv, blocks = p.nkv * p.head_blocks;
     unsigned char* ring = smem + warp * (OWN_STAGES * STAGE_BYTES);        // (stages start on 1,024-byte boundaries: see the swizzle)
@@ -730,21 +733,20 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
 
 // ---------------------------------------------------------------------------------------------
 // The sums of a row put together: WARPS warps per (sequence, head), which take its parts in turn, four neighbouring columns a lane
-// and MERGE_BATCH parts' loads in flight.  What it costs is round trips to L2, so a row of many parts gets four warps (one: 45 parts
-// in four trips).
+// and MERGE_BATCH parts' loads in flight.  What it costs is round trips to L2 - a row of 45 parts takes one warp four - and waves of
+// blocks, five of which fit an SM: so as many warps a row as still leave one wave.
 template <int WARPS>
 __global__ void __launch_bounds__(128)
 shared_merge_kernel(const SharedParams p, const float* __restrict__ sinks, const float* __restrict__ gate, __nv_bfloat16* __restrict__ out) {
     rv_pdl_launch_dependents();
     constexpr int LANES = HEAD_DIM / 4;              // that hold a row
-    constexpr int PER_WARP = 32 / LANES;             // rows (or turns of a row) of a warp
-    constexpr int TURNS = WARPS == 1 ? 1 : WARPS * PER_WARP;               // threads groups that share a row
-    __shared__ float4 sh_o[WARPS == 1 ? 1 : TURNS][LANES];
-    __shared__ float2 sh_ml[TURNS];
+    constexpr int TURNS = WARPS == 1 ? 1 : WARPS * 32 / LANES;             // groups of lanes that share one
+    constexpr int ROWS_HERE = 128 / LANES / TURNS;   // rows of a block
+    __shared__ float4 sh_o[TURNS == 1 ? 1 : 128 / LANES][LANES];
+    __shared__ float2 sh_ml[128 / LANES];
     const int tid = threadIdx.x, group = tid / LANES, d = (tid - group * LANES) * 4;
-    const int turn = WARPS == 1 ? 0 : group;
-    const int rows = p.num_seqs * p.nh;
-    const int row = WARPS == 1 ? blockIdx.x * (128 / LANES) + group : blockIdx.x;
+    const int turn = group % TURNS;
+    const int rows = p.num_seqs * p.nh, row = blockIdx.x * ROWS_HERE + group / TURNS;
     const bool here = row < rows;
     const int seq = here ? row / p.nh : 0, head = here ? row - seq * p.nh : 0;
     const int G = p.nh / p.nkv, kvh = head / G;
@@ -773,13 +775,13 @@ shared_merge_kernel(const SharedParams p, const float* __restrict__ sinks, const
         for (int k = 0; k < MERGE_BATCH; ++k)
             if (s0 + k * TURNS < total) v.take(ml[k].x, ml[k].y, o[k]);
     }
-    if (WARPS > 1) {
-        sh_o[turn][d / 4] = v.o;
-        if (d == 0) sh_ml[turn] = make_float2(v.m, v.l);
+    if (TURNS > 1) {
+        sh_o[group][d / 4] = v.o;
+        if (d == 0) sh_ml[group] = make_float2(v.m, v.l);
         __syncthreads();
         if (turn > 0) return;
 #pragma unroll
-        for (int t = 1; t < TURNS; ++t) v.take(sh_ml[t].x, sh_ml[t].y, sh_o[t][d / 4]);
+        for (int t = 1; t < TURNS; ++t) v.take(sh_ml[group + t].x, sh_ml[group + t].y, sh_o[group + t][d / 4]);
     }
     if (!here) return;
     float num = 1.f, den = v.l;
@@ -849,11 +851,12 @@ RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     if (int e = rv_configure_smem(configured, shared_attention_kernel, smem)) return e;
     RV_LAUNCH_ST = rv_launch(shared_attention_kernel, dim3((unsigned)(prefix_ctas + a->own_ctas)), dim3(NUM_THREADS), smem, a->stream, map_kv, map_own, p);
     if ((st = rv_launch_status()) != RV_OK) return st;
-    const int rows = a->num_seqs * nh, per_block = 128 / (HEAD_DIM / 4);
-    if (a->most_parts > MERGE_BATCH)
-        RV_LAUNCH_ST = rv_launch(shared_merge_kernel<4>, dim3(rows), dim3(128), 0, a->stream, p, a->sinks, a->gate, (__nv_bfloat16*)a->out);
-    else
-        RV_LAUNCH_ST = rv_launch(shared_merge_kernel<1>, dim3((rows + per_block - 1) / per_block), dim3(128), 0, a->stream, p, a->sinks, a->gate,
-                                 (__nv_bfloat16*)a->out);
+    const int rows = a->num_seqs * nh, wave = 5 * rv_sm_count();
+    const auto merge = [&](auto kernel, int per_block) {
+        return rv_launch(kernel, dim3((rows + per_block - 1) / per_block), dim3(128), 0, a->stream, p, a->sinks, a->gate, (__nv_bfloat16*)a->out);
+    };
+    if (a->most_parts <= MERGE_BATCH || rows > 2 * wave) RV_LAUNCH_ST = merge(shared_merge_kernel<1>, 128 / (HEAD_DIM / 4));
+    else if (rows > wave) RV_LAUNCH_ST = merge(shared_merge_kernel<2>, 2);
+    else RV_LAUNCH_ST = merge(shared_merge_kernel<4>, 1);
     return rv_launch_status();
 }
