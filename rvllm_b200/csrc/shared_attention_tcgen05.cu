@@ -830,7 +830,8 @@ RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     if (a->num_seqs == 0) return RV_OK;
     alignas(64) CUtensorMap map_kv, map_own;
     int st = rv_make_bf16_map(&map_kv, a->cache, a->num_pages * 2 * nkv * page_size, HEAD_DIM, page_size < KV_TILE ? page_size : KV_TILE);
-    if (st == RV_OK) st = rv_make_bf16_map(&map_own, a->cache, a->num_pages * 2 * nkv * page_size, HEAD_DIM, page_size < OWN_CHUNK ? page_size : OWN_CHUNK);
+    if (page_size <= OWN_CHUNK) map_own = map_kv;        // (boxes of a page)
+    else if (st == RV_OK) st = rv_make_bf16_map(&map_own, a->cache, a->num_pages * 2 * nkv * page_size, HEAD_DIM, OWN_CHUNK);
     if (st != RV_OK) return st;
     SharedParams p;
     p.plan = shared_plan(a->plan, a->num_seqs, a->cap_tiles);

@@ -8,10 +8,11 @@
 
 // ---------------------------------------------------------------------------------------------
 // The plain kernel of both parts: 32-bit products and sums, one CTA per (row block, kv head, range of keys).  The rows of a CTA share
-// the keys, so a tile of 32 keys and values goes to shared memory once and meets 4 * RPW rows: a warp owns RPW rows, its lanes the
+// the keys, so a tile of 32 keys and values goes to shared memory once and meets 8 * RPW rows: a warp owns RPW rows, its lanes the
 // 32 keys of the tile for the scores and hd / 32 columns for the sums.  In float32 the arithmetic bounds it (no tensor core takes
-// 32 bits); RPW = 8 reads a shared word per four multiply-adds, RPW = 2 serves the few rows of one sequence.
-#define PLAIN_THREADS 128
+// 32 bits); RPW = 4 reads five shared words per four multiply-adds each, RPW = 1 serves the few rows of one sequence.  Both parts are
+// one launch, the prefixes' CTAs first.
+#define PLAIN_THREADS 256
 #define PLAIN_TILE 32
 #define PLAIN_MAX_DIM 256
 
@@ -21,20 +22,20 @@ struct PlainParams {
     const void* cache;             // [num_pages, 2, nkv, page_size, hd]
     const int* block_tables;       // [num_seqs, max_blocks]
     const int* ctx_lens;
-    float* part_o;                 // prefixes: [items, nkv, SP_ROWS, hd]; own keys: [splits, num_seqs, nh, hd]
-    float* part_ml;                // ... and the same with 2 in place of hd
+    float* pre_o;                  // [items, nkv, SP_ROWS, hd]: the prefixes' sums
+    float* pre_ml;                 // ... and the same with 2 in place of hd
+    float* own_o;                  // [splits, num_seqs, nh, hd]: those of the own keys
+    float* own_ml;
+    int prefix_ctas;               // kv heads x row blocks x items; behind them kv heads x blocks of eight heads x splits x sequences
     long long num_pages;
     int num_seqs, nh, nkv, hd, page_size, max_blocks, splits;
     float scale, softcap;          // softcap 0: none
 };
 
-// OWN: the keys behind the prefix, one sequence a CTA (blockIdx: kv head x row block, split, sequence);
-// else a range of a group's prefix (kv head x row block, item)
+// OWN: the keys behind the prefix of one sequence; else a range of a group's prefix
 template <typename T, int RPW, int DPL, bool OWN>
-__global__ void __launch_bounds__(PLAIN_THREADS)
-shared_plain_kernel(const PlainParams p) {
-    extern __shared__ __align__(16) float sh[];
-    constexpr int R = 4 * RPW;
+__device__ __forceinline__ void plain_part(const PlainParams& p, float* sh, int cta) {
+    constexpr int R = PLAIN_THREADS / 32 * RPW;
     const int stride = p.hd + 4;                            // (a multiple of four that is odd in units of 16 bytes for hd a multiple of 8)
     float* q_s = sh;                                        // [R][hd]
     float* k_s = q_s + R * p.hd;                            // [PLAIN_TILE][stride]
@@ -44,23 +45,21 @@ shared_plain_kernel(const PlainParams p) {
     int* lim_s = tok_s + R;                                 // [R] keys that a row sees end here
     int* there_s = lim_s + R;                               // [PLAIN_TILE] whether a key's page exists
 
-    rv_pdl_launch_dependents();
-    rv_pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int kvh = blockIdx.x % p.nkv, row0 = blockIdx.x / p.nkv * R;
     const int G = p.nh / p.nkv;
-    int key_lo, key_hi, table_seq, rows, first = 0, item = 0;
+    const int row_blocks = ((OWN ? G : SP_ROWS / G * G) + R - 1) / R;
+    const int kvh = cta % p.nkv, row0 = cta / p.nkv % row_blocks * R, which = cta / (p.nkv * row_blocks);
+    int key_lo, key_hi, table_seq, rows, first = 0;
     if (OWN) {
-        table_seq = blockIdx.z;
+        table_seq = which % p.num_seqs;
         rows = G;
         const int ctx = p.ctx_lens[table_seq], start = p.plan.own_start(table_seq);
         const int tiles = ctx > start ? (ctx - start + PLAIN_TILE - 1) / PLAIN_TILE : 0;
         const int per = (tiles + p.splits - 1) / p.splits;
-        key_lo = start + (int)blockIdx.y * per * PLAIN_TILE;
+        key_lo = start + which / p.num_seqs * per * PLAIN_TILE;
         key_hi = min(ctx, key_lo + per * PLAIN_TILE);
     } else {
-        item = blockIdx.y;
-        const SharedItem tile = p.plan.item(item);
+        const SharedItem tile = p.plan.item(which);
         table_seq = tile.table_seq; first = tile.first;
         rows = min(tile.count, SP_ROWS / G) * G;
         key_lo = tile.key_begin; key_hi = tile.key_end;
@@ -77,14 +76,15 @@ shared_plain_kernel(const PlainParams p) {
         tok_s[tid] = tok; lim_s[tid] = lim;
     }
     __syncthreads();
-    // a quarter of the columns of key tid / 4 (of row tid / 4) per thread
+    // an eighth of the columns of key tid / 8 (of row tid / 8) per thread
     constexpr int dt = sizeof(T) == 4 ? RV_DTYPE_F32 : RV_DTYPE_BF16;
-    const int mine = tid >> 2, quarter = (tid & 3) * 4;
+    constexpr int SHARE = PLAIN_THREADS / PLAIN_TILE;
+    const int mine = tid / SHARE, from = tid % SHARE * 4;
     if (mine < R) {
         const int tok = tok_s[mine];
         const size_t at = ((size_t)max(tok, 0) * p.nh + kvh * G + (row0 + mine) % G) * p.hd;
 #pragma unroll 4
-        for (int d = quarter; d < p.hd; d += 16) {
+        for (int d = from; d < p.hd; d += 4 * SHARE) {
             const float4 v = rv_load4(p.q, dt, at + d);
             *reinterpret_cast<float4*>(q_s + mine * p.hd + d) =
                 tok >= 0 ? make_float4(v.x * p.scale, v.y * p.scale, v.z * p.scale, v.w * p.scale) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -102,24 +102,39 @@ shared_plain_kernel(const PlainParams p) {
         for (int d = 0; d < DPL; ++d) acc[i][d] = 0.f;
     }
     const size_t plane = (size_t)p.nkv * p.page_size * p.hd;
-    int page = page_of(key_lo + mine);
+    // the next tile's words wait in registers while this one is worked on
+    float4 next_k[DPL], next_v[DPL];
+    bool there = false;
+    auto fetch = [&](int key0, int page) {
+        there = page >= 0 && page < p.num_pages;
+        const size_t at = (((size_t)max(page, 0) * 2 * p.nkv + kvh) * p.page_size + (key0 + mine) % p.page_size) * p.hd;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) {
+            const int d = from + 4 * SHARE * i;
+            next_k[i] = next_v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (there && d < p.hd) { next_k[i] = rv_load4(p.cache, dt, at + d); next_v[i] = rv_load4(p.cache, dt, at + plane + d); }
+        }
+    };
+    fetch(key_lo, page_of(key_lo + mine));
+    int page = page_of(key_lo + PLAIN_TILE + mine);
     for (int key0 = key_lo; key0 < key_hi; key0 += PLAIN_TILE) {
         __syncthreads();                                    // the tile before has been read
-        const bool there = page >= 0 && page < p.num_pages;
-        const size_t at = (((size_t)max(page, 0) * 2 * p.nkv + kvh) * p.page_size + (key0 + mine) % p.page_size) * p.hd;
-#pragma unroll 4
-        for (int d = quarter; d < p.hd; d += 16) {
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-            if (there) { x = rv_load4(p.cache, dt, at + d); y = rv_load4(p.cache, dt, at + plane + d); }
-            *reinterpret_cast<float4*>(k_s + mine * stride + d) = x;
-            *reinterpret_cast<float4*>(v_s + mine * stride + d) = y;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) {
+            const int d = from + 4 * SHARE * i;
+            if (d < p.hd) {
+                *reinterpret_cast<float4*>(k_s + mine * stride + d) = next_k[i];
+                *reinterpret_cast<float4*>(v_s + mine * stride + d) = next_v[i];
+            }
         }
-        if (quarter == 0) there_s[mine] = there;
-        page = page_of(key0 + PLAIN_TILE + mine);
+        if (from == 0) there_s[mine] = there;
         __syncthreads();
+        fetch(key0 + PLAIN_TILE, page);
+        page = page_of(key0 + 2 * PLAIN_TILE + mine);
         float s[RPW];
 #pragma unroll
         for (int i = 0; i < RPW; ++i) s[i] = 0.f;
+#pragma unroll 4
         for (int d = 0; d < p.hd; d += 4) {
             const float4 a = *reinterpret_cast<const float4*>(k_s + lane * stride + d);
 #pragma unroll
@@ -164,31 +179,36 @@ shared_plain_kernel(const PlainParams p) {
     for (int i = 0; i < RPW; ++i) {
         const int r = warp * RPW + i;
         if (row0 + r >= rows || tok_s[r] < 0) continue;
-        const size_t prow = OWN ? ((size_t)blockIdx.y * p.num_seqs + tok_s[r]) * p.nh + kvh * G + row0 + r
-                                : ((size_t)item * p.nkv + kvh) * SP_ROWS + row0 + r;
+        const size_t prow = OWN ? ((size_t)(which / p.num_seqs) * p.num_seqs + tok_s[r]) * p.nh + kvh * G + row0 + r
+                                : ((size_t)which * p.nkv + kvh) * SP_ROWS + row0 + r;
+        float* sums = (OWN ? p.own_o : p.pre_o) + prow * p.hd;
 #pragma unroll
         for (int c = 0; c < DPL; c += 4) {
             const int d = c * 32 + lane * 4;
-            if (d < p.hd) *reinterpret_cast<float4*>(p.part_o + prow * p.hd + d) = make_float4(acc[i][c], acc[i][c + 1], acc[i][c + 2], acc[i][c + 3]);
+            if (d < p.hd) *reinterpret_cast<float4*>(sums + d) = make_float4(acc[i][c], acc[i][c + 1], acc[i][c + 2], acc[i][c + 3]);
         }
-        if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m[i], l[i]);
+        if (lane == 0) *reinterpret_cast<float2*>((OWN ? p.own_ml : p.pre_ml) + prow * 2) = make_float2(m[i], l[i]);
     }
 }
 
-template <typename T, int RPW, int DPL, bool OWN>
-static int launch_plain(const PlainParams& p, dim3 grid, cudaStream_t stream) {
-    const int R = 4 * RPW;
-    const int smem = (R * p.hd + 2 * PLAIN_TILE * (p.hd + 4) + R * PLAIN_TILE + 2 * R + PLAIN_TILE) * 4;
-    const int most = (R * PLAIN_MAX_DIM + 2 * PLAIN_TILE * (PLAIN_MAX_DIM + 4) + R * PLAIN_TILE + 2 * R + PLAIN_TILE) * 4;
-    static RvPerDevice configured;
-    if (int e = rv_configure_smem(configured, shared_plain_kernel<T, RPW, DPL, OWN>, most)) return e;
-    RV_LAUNCH_ST = rv_launch(shared_plain_kernel<T, RPW, DPL, OWN>, grid, dim3(PLAIN_THREADS), smem, stream, p);
-    return rv_launch_status();
+template <typename T, int DPL>
+__global__ void __launch_bounds__(PLAIN_THREADS)
+shared_plain_kernel(const PlainParams p) {
+    extern __shared__ __align__(16) float sh[];
+    rv_pdl_launch_dependents();
+    rv_pdl_wait();
+    if ((int)blockIdx.x < p.prefix_ctas) plain_part<T, 4, DPL, false>(p, sh, blockIdx.x);
+    else plain_part<T, 1, DPL, true>(p, sh, (int)blockIdx.x - p.prefix_ctas);
 }
 
-template <typename T, int RPW, bool OWN>
-static int launch_plain_dim(const PlainParams& p, dim3 grid, cudaStream_t stream) {
-    return p.hd <= 128 ? launch_plain<T, RPW, 4, OWN>(p, grid, stream) : launch_plain<T, RPW, 8, OWN>(p, grid, stream);
+template <typename T, int DPL>
+static int launch_plain(const PlainParams& p, unsigned ctas, cudaStream_t stream) {
+    constexpr int R = PLAIN_THREADS / 32 * 4;
+    const auto bytes = [](int hd) { return (R * hd + 2 * PLAIN_TILE * (hd + 4) + R * PLAIN_TILE + 2 * R + PLAIN_TILE) * 4; };
+    static RvPerDevice configured;
+    if (int e = rv_configure_smem(configured, shared_plain_kernel<T, DPL>, bytes(PLAIN_MAX_DIM))) return e;
+    RV_LAUNCH_ST = rv_launch(shared_plain_kernel<T, DPL>, dim3(ctas), dim3(PLAIN_THREADS), bytes(p.hd), stream, p);
+    return rv_launch_status();
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -294,7 +314,10 @@ RV_EXPORT int rv_shared_attention_plain(const PlainArgs* a) {
         return RV_ERR_BAD_SIZE;
     if (a->dtype != RV_DTYPE_F32 && a->dtype != RV_DTYPE_BF16) return RV_ERR_BAD_DTYPE;
     if (hd % 4 || hd > PLAIN_MAX_DIM || nh / nkv > SP_ROWS) return RV_ERR_UNSUPPORTED;
-    if (a->num_seqs > 65535 || a->splits > 65535 || a->cap_items > 65535) return RV_ERR_UNSUPPORTED;
+    const int G = nh / nkv;
+    const long long prefix_ctas = (long long)a->cap_items * nkv * ((SP_ROWS / G * G + 31) / 32);
+    const long long own_ctas = (long long)a->num_seqs * a->splits * nkv * ((G + 7) / 8);
+    if (prefix_ctas + own_ctas > 0x7fffffffLL) return RV_ERR_UNSUPPORTED;       // (blocks of the launch)
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->cache) | reinterpret_cast<uintptr_t>(a->pre_o) |
          reinterpret_cast<uintptr_t>(a->own_o) | reinterpret_cast<uintptr_t>(a->plan) | reinterpret_cast<uintptr_t>(a->out)) % 16 ||
         (reinterpret_cast<uintptr_t>(a->pre_ml) | reinterpret_cast<uintptr_t>(a->own_ml)) % 8)
@@ -306,14 +329,11 @@ RV_EXPORT int rv_shared_attention_plain(const PlainArgs* a) {
     p.num_pages = a->num_pages; p.num_seqs = a->num_seqs;
     p.nh = nh; p.nkv = nkv; p.hd = hd; p.page_size = a->page_size; p.max_blocks = a->max_blocks; p.splits = a->splits;
     p.scale = a->scale; p.softcap = a->softcap;
-    const int G = nh / nkv;
     const bool wide = a->dtype == RV_DTYPE_F32;
-    const dim3 grid(nkv * ((SP_ROWS / G * G + 31) / 32), a->cap_items), own_grid(nkv * ((G + 7) / 8), a->splits, a->num_seqs);
-    p.part_o = a->pre_o; p.part_ml = a->pre_ml;
-    int st = wide ? launch_plain_dim<float, 8, false>(p, grid, a->stream) : launch_plain_dim<__nv_bfloat16, 8, false>(p, grid, a->stream);
-    if (st != RV_OK) return st;
-    p.part_o = a->own_o; p.part_ml = a->own_ml;
-    st = wide ? launch_plain_dim<float, 2, true>(p, own_grid, a->stream) : launch_plain_dim<__nv_bfloat16, 2, true>(p, own_grid, a->stream);
+    p.pre_o = a->pre_o; p.pre_ml = a->pre_ml; p.own_o = a->own_o; p.own_ml = a->own_ml; p.prefix_ctas = (int)prefix_ctas;
+    const unsigned ctas = (unsigned)(prefix_ctas + own_ctas);
+    int st = hd <= 128 ? (wide ? launch_plain<float, 4>(p, ctas, a->stream) : launch_plain<__nv_bfloat16, 4>(p, ctas, a->stream))
+                       : (wide ? launch_plain<float, 8>(p, ctas, a->stream) : launch_plain<__nv_bfloat16, 8>(p, ctas, a->stream));
     if (st != RV_OK) return st;
     MergeParams m;
     m.plan = p.plan; m.pre_o = a->pre_o; m.pre_ml = a->pre_ml; m.own_o = a->own_o; m.own_ml = a->own_ml;

@@ -60,15 +60,6 @@ _PLAIN_ARGS = struct.Struct("=14q10i2f")       # shared_prefix.cu
 _TABLE_ARGS = struct.Struct("=13q8iq")         # step_tables.cu
 
 
-def _same_device(here: int, named) -> None:
-    """Every tensor is contiguous and lies on the current CUDA device, on whose stream the kernels are launched."""
-    for t, name in named:
-        if t.get_device() != here:
-            raise KernelError(f"{name} must be a CUDA tensor on the current device, cuda:{here}; it lies on {t.device}")
-        if not t.is_contiguous():
-            raise KernelError(f"{name} must be contiguous, got strides {t.stride()} for shape {tuple(t.shape)}")
-
-
 class AttentionMeta:
     """Per-step, per-cache-group arguments of the attention kernels (device int32 tensors) and
     the few host-side numbers that size their launches."""
@@ -544,32 +535,35 @@ class CudaKernels:
         the TMA-fed decode kernels.  float32, and other sizes whose head is a multiple of 4 up to 256: the plain kernels.  What
         neither takes (more than 128 query heads on a key/value head among it), and steps without a group, go to
         `paged_attention`, to which every table is whole."""
-        tables, lens = meta.block_tables, meta.ctx_lens
+        tables, lens, ints = meta.block_tables, meta.ctx_lens, shared.device_ints
         here = torch._C._cuda_getDevice()
-        _same_device(here, ((q, "q"), (cache_layer, "cache_layer"), (tables, "block_tables"), (lens, "ctx_lens"), (shared.device_ints, "shared")))
+        for t in (q, cache_layer, tables, lens, ints):
+            if t.get_device() != here or not t.is_contiguous():
+                raise KernelError(f"shared_prefix_attention: contiguous tensors on the current device, cuda:{here}; one of shape {tuple(t.shape)} "
+                                  f"has strides {t.stride()} on {t.device}")
+        dtype, B = q.dtype, meta.num_seqs
         dt = self._dt(q, "q")
-        if q.dim() != 2 or cache_layer.dim() != 5 or cache_layer.dtype != q.dtype or tables.dim() != 2 or tables.dtype != torch.int32 \
-                or lens.dim() != 1 or lens.dtype != torch.int32:
-            raise KernelError(f"shared_prefix_attention: q {tuple(q.shape)} of {q.dtype}, a cache layer {tuple(cache_layer.shape)} of "
+        if cache_layer.dtype != dtype or tables.dtype is not torch.int32 or lens.dtype is not torch.int32 or q.dim() != 2 \
+                or cache_layer.dim() != 5 or tables.dim() != 2 or lens.dim() != 1:
+            raise KernelError(f"shared_prefix_attention: q {tuple(q.shape)} of {dtype}, a cache layer {tuple(cache_layer.shape)} of "
                               f"{cache_layer.dtype}, block tables {tuple(tables.shape)} of {tables.dtype}, lengths {tuple(lens.shape)} of {lens.dtype}")
-        B = meta.num_seqs
-        tokens, width = q.shape
         pages, planes, kv_heads, page, size = cache_layer.shape
-        if meta.max_q_len > 1 or tokens != B:
-            raise KernelError(f"shared_prefix_attention: {tokens} tokens of {B} sequences, the longest of {meta.max_q_len}: every sequence "
-                              "brings one")
-        if num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or width != num_heads * head_dim:
-            raise KernelError(f"shared_prefix_attention: rows of {width} for {num_heads} heads of {head_dim} on {num_kv_heads}")
+        table_rows, max_blocks = tables.shape
+        if meta.max_q_len > 1 or num_heads < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or q.shape != (B, num_heads * head_dim):
+            raise KernelError(f"shared_prefix_attention: q {tuple(q.shape)} for {B} sequences, the longest of {meta.max_q_len} tokens, and {num_heads} "
+                              f"heads of {head_dim} on {num_kv_heads}: every sequence brings one token")
         if planes != 2 or kv_heads != num_kv_heads or size != head_dim:
             raise KernelError(f"shared_prefix_attention: a cache layer of shape {tuple(cache_layer.shape)} for {num_kv_heads} key/value heads of {head_dim}")
-        if (shared.num_seqs, shared.num_heads, shared.num_kv_heads) != (B, num_heads, num_kv_heads):
+        if shared.num_seqs != B or shared.num_heads != num_heads or shared.num_kv_heads != num_kv_heads:
             raise KernelError(f"shared_prefix_attention: prefixes laid out for {shared.num_seqs} sequences of {shared.num_heads} heads on "
                               f"{shared.num_kv_heads}, a step of {B} of {num_heads} on {num_kv_heads}")
-        if tables.shape[0] < B or lens.shape[0] < B:
-            raise KernelError(f"shared_prefix_attention: tables of {tables.shape[0]} and lengths of {lens.shape[0]} sequences for {B}")
+        if table_rows < B or lens.shape[0] < B:
+            raise KernelError(f"shared_prefix_attention: tables of {table_rows} and lengths of {lens.shape[0]} sequences for {B}")
         if sinks is not None or gate is not None:
             self._check_attention_extras(q, num_heads, sinks, gate)
-            _same_device(here, tuple((t, name) for t, name in ((sinks, "sinks"), (gate, "gate")) if t is not None))
+            for t in (sinks, gate):
+                if t is not None and t.get_device() != here:
+                    raise KernelError(f"shared_prefix_attention: sinks or gate on {t.device}, the current device is cuda:{here}")
         group = num_heads // num_kv_heads
         fast = dt == 1 and head_dim in (64, 128) and page & (page - 1) == 0 and page >= 8 and pages * 2 * num_kv_heads * page < 2 ** 31 \
             and B <= 4096
@@ -578,23 +572,23 @@ class CudaKernels:
             return self.paged_attention(q, cache_layer, meta, num_heads, num_kv_heads, head_dim, scale, None, softcap, sinks, gate)
         if max_own is None:
             max_own = meta.max_ctx_len - shared.shortest
+        max_own = max(1, min(max_own, meta.max_ctx_len))
         pre_rows = items * num_kv_heads * TILE_ROWS
         out = torch.empty_like(q)
-        plan_at, q_at, cache_at, tables_at, lens_at, out_at = (shared.device_ints.data_ptr(), q.data_ptr(), cache_layer.data_ptr(), tables.data_ptr(),
-                                                               lens.data_ptr(), out.data_ptr())
         sinks_at, gate_at = 0 if sinks is None else sinks.data_ptr(), 0 if gate is None else gate.data_ptr()
         stream, cap = torch._C._cuda_getCurrentRawStream(here), softcap or 0.0
         if fast:
             # one buffer: the prefixes' sums, their maxima and denominators, and those of the own keys
-            piece, pieces, own_ctas = self._own_pieces(B * num_kv_heads * -(-group // 8), max_own, items * num_kv_heads)
+            piece, pieces, own_ctas = self._own_pieces(B * num_kv_heads * -(-group // 8), max_own)
             own_rows = pieces * B * num_heads
             scratch = torch.empty(((pre_rows + own_rows) * (head_dim + 2),), dtype=torch.float32, device=q.device)
             pre = scratch.data_ptr()
             pre_ml = pre + 4 * pre_rows * head_dim
             own = pre_ml + 8 * pre_rows
             st = self._entry("shared_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",), "rv_shared_attention_tcgen05")(_SHARED_ARGS.pack(
-                q_at, cache_at, tables_at, lens_at, plan_at, pre, pre_ml, own, own + 4 * own_rows * head_dim, out_at, sinks_at, gate_at,
-                self._status.data_ptr(), stream, pages, B, tiles, items, num_heads, num_kv_heads, head_dim, page, tables.shape[1],
+                q.data_ptr(), cache_layer.data_ptr(), tables.data_ptr(), lens.data_ptr(), ints.data_ptr(), pre, pre_ml, own,
+                own + 4 * own_rows * head_dim, out.data_ptr(), sinks_at, gate_at, self._status.data_ptr(), stream, pages, B, tiles, items,
+                num_heads, num_kv_heads, head_dim, page, max_blocks,
                 piece, pieces, own_ctas, pieces + shared.most_parts, scale, cap))
             _check("shared_attention_tcgen05", st)
             COUNTERS['launches'] += 1
@@ -606,20 +600,19 @@ class CudaKernels:
         pre_ml = pre + 4 * pre_rows * head_dim
         own = pre_ml + 8 * pre_rows
         st = self._entry("shared_prefix.cu", (), "rv_shared_attention_plain")(_PLAIN_ARGS.pack(
-            q_at, cache_at, tables_at, lens_at, plan_at, pre, pre_ml, own, own + 4 * own_rows * head_dim, out_at, sinks_at, gate_at, stream, pages,
-            B, tiles, items, num_heads, num_kv_heads, head_dim, page, tables.shape[1], splits, dt, scale, cap))
+            q.data_ptr(), cache_layer.data_ptr(), tables.data_ptr(), lens.data_ptr(), ints.data_ptr(), pre, pre_ml, own, own + 4 * own_rows * head_dim,
+            out.data_ptr(), sinks_at, gate_at, stream, pages, B, tiles, items, num_heads, num_kv_heads, head_dim, page, max_blocks, splits, dt, scale, cap))
         _check("shared_attention_plain", st)
-        COUNTERS['launches'] += 2
+        COUNTERS['launches'] += 1
         return out
 
-    def _own_pieces(self, pairs: int, max_own: int, prefix_ctas: int):
+    def _own_pieces(self, pairs: int, max_own: int):
         """(keys of a piece, most pieces of a sequence, CTAs) for the own keys of `pairs` sequences and blocks of heads."""
-        places = 2 * self.num_sms
-        ctas = places - prefix_ctas if prefix_ctas <= self.num_sms else places
-        piece = 64
-        while -(-max_own // piece) > 64:
+        ctas = 2 * self.num_sms
+        piece = 16                       # few sequences: a warp each for as little as a chunk; many: 64 keys (a warp's set-up is worth two chunks)
+        while (piece < 64 and pairs * -(-max_own // piece) > 4 * ctas) or max_own > 64 * piece:
             piece *= 2
-        pieces = max(1, -(-max_own // piece))
+        pieces = -(-max_own // piece)
         return piece, pieces, max(1, min(ctas, -(-pairs * pieces // 4)))
 
     def step_tables(self, page_table: torch.Tensor, rows: torch.Tensor, held: torch.Tensor, starts: torch.Tensor, q_lens: torch.Tensor,

@@ -13,17 +13,20 @@ TILE_ROWS = 128            # rows of a row tile (SP_ROWS of csrc/shared_prefix.c
 KEY_TILE = 64              # keys of a tile: ranges of keys begin at multiples of it
 
 
-def _cut(tiles_of: Sequence[int], kv_heads: int, places: int) -> int:
-    """Key tiles of a range so that the ranges of all row tiles and kv heads come closest to filling `places` CTAs once (at
-    least two: a CTA costs about as much as three tiles to set up and to merge)."""
-    lo, hi = 2, max(max(tiles_of), 2)
-    while lo < hi:
-        mid = (lo + hi) // 2
-        if sum(-(-n // mid) for n in tiles_of) * kv_heads <= places:
-            hi = mid
-        else:
-            lo = mid + 1
-    return lo
+def _cut(tiles_of: Sequence[int], kv_heads: int, num_sms: int) -> int:
+    """Key tiles of a range: such that the ranges of all row tiles and kv heads are at most one CTA an SM, and no fewer than two
+    (a CTA costs about as much as three to set up and to merge); where that makes them longer than eight, two CTAs an SM."""
+    def least(places: int) -> int:
+        lo, hi = 2, max(max(tiles_of), 2)
+        while lo < hi:
+            mid = (lo + hi) // 2
+            if sum(-(-n // mid) for n in tiles_of) * kv_heads <= places:
+                hi = mid
+            else:
+                lo = mid + 1
+        return lo
+    one = least(num_sms)
+    return one if one <= 8 else least(2 * num_sms)
 
 
 class SharedPrefixes:
@@ -91,7 +94,7 @@ class SharedPrefixes:
         key_tiles = [-(-t[3] // KEY_TILE) for t in tiles]
         items, parts = [], []
         if tiles:
-            step = _cut(key_tiles, self.num_kv_heads, 2 * self.num_sms)
+            step = _cut(key_tiles, self.num_kv_heads, self.num_sms)
             for i, n in enumerate(key_tiles):
                 k = -(-n // step)
                 edges = [n * j // k for j in range(k + 1)]
