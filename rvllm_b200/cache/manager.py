@@ -15,6 +15,10 @@ A group whose values are not as wide as its keys (`KvCacheNeed.value_dim`) keeps
 value rows.  A chunk group (`KvCacheNeed.chunk`) gives a page back once the block of positions that the next
 query lies in starts above it.  A cache slot whose mixer is made of several mixers (`CompositeNeed`) has one
 sub-view per member, each handled as a cache slot of its own.
+
+Requests that begin with the same tokens can hold the same pages (`share`), where every group keeps all keys and no layer
+has state of fixed size: a page whose tokens are all known to be the same and computed is taken over, what follows is the
+request's own.
 """
 from __future__ import annotations
 
@@ -51,6 +55,7 @@ class _Request:
     num_tokens: int = 0
     tables: List[List[int]] = field(default_factory=list)   # per group: page of each logical block, -1 if freed
     first_live: List[int] = field(default_factory=list)     # per group: first logical block still held
+    on_device: List[int] = field(default_factory=list)      # per group: blocks that the step function's table on the device has
 
 
 def flat_needs(needs: Dict[int, object]) -> Dict[object, object]:
@@ -160,10 +165,60 @@ class CacheManager:
         if req in self.requests:
             raise SchedulerError(f"request {req!r} is already in the cache")
         slot = self.slots.allocate(req)
-        self.requests[req] = _Request(slot, 0, [[] for _ in self.groups], [0 for _ in self.groups])
+        self.requests[req] = _Request(slot, 0, [[] for _ in self.groups], [0 for _ in self.groups], [0 for _ in self.groups])
         for t in self._state.values():
             t[slot].zero_()
         return slot
+
+    @property
+    def can_share(self) -> bool:
+        """True where a request's first pages say all there is to know about its first tokens."""
+        return bool(self.groups) and not self._has_window and not self._state_needs
+
+    def share(self, req: Hashable, donor: Hashable, num_tokens: int) -> None:
+        """The pages of `donor`'s first `num_tokens` tokens (a multiple of the page size) become the first pages of `req`, which has
+        none yet.  The caller knows that both begin with these tokens and that the donor's are in the cache."""
+        r, d = self.requests[req], self.requests[donor]
+        if not self.can_share:
+            raise SchedulerError("pages cannot be shared: a layer has a window, a chunk or state of its own")
+        if r.num_tokens or any(r.tables):
+            raise SchedulerError(f"request {req!r} has tokens already")
+        if num_tokens < 1 or num_tokens % self.page_size or num_tokens > d.num_tokens:
+            raise SchedulerError(f"request {req!r}: {num_tokens} tokens of {donor!r} cannot be shared: it has {d.num_tokens}, in pages of {self.page_size}")
+        n = num_tokens // self.page_size
+        for g, mine, theirs in zip(self.groups, r.tables, d.tables):
+            g.pool.share(theirs[:n], req)
+            mine.extend(theirs[:n])
+        r.num_tokens = num_tokens
+
+    def shared_groups(self, reqs) -> List[Tuple[List[int], int]]:
+        """Which of the requests `reqs` begin with the same pages: (places in `reqs`, tokens) per group, each request in one group at
+        most.  Where a few of those that share a beginning share more among themselves, the grouping that saves the most keys is taken."""
+        if not self.can_share:
+            return []
+        tables = [self.requests[r].tables[0] for r in reqs]
+
+        def grouped(members: List[int], depth: int):
+            """(keys saved, groups) of requests whose first `depth` pages are the same"""
+            if len(members) < 2:
+                return 0, []
+            first = tables[members[0]]
+            common = min(len(tables[m]) for m in members)
+            for m in members[1:]:
+                t, n = tables[m], depth
+                while n < common and t[n] == first[n]:
+                    n += 1
+                common = n
+            parts: Dict[int, List[int]] = {}
+            for m in members:
+                if len(tables[m]) > common:
+                    parts.setdefault(tables[m][common], []).append(m)
+            saved, groups = (len(members) - 1) * common * self.page_size, [(members, common * self.page_size)] if common else []
+            deeper = [grouped(ms, common) for ms in parts.values() if len(ms) > 1]
+            if sum(d[0] for d in deeper) > saved:
+                return sum(d[0] for d in deeper), [g for d in deeper for g in d[1]]
+            return saved, groups
+        return grouped(list(range(len(tables))), 0)[1]
 
     def num_tokens(self, req: Hashable) -> int:
         return self.requests[req].num_tokens
@@ -263,10 +318,10 @@ class CacheManager:
                 for p in r.tables[gi]:
                     if p < 0:
                         continue
-                    if p in held:
+                    if p in held and not (g.pool.holds(p, held[p]) and g.pool.holds(p, req)):
                         raise SchedulerError(f"page {p} of group {gi} is in the tables of {held[p]!r} and {req!r}")
                     held[p] = req
-                    if g.pool.owner(p) != req:
+                    if not g.pool.holds(p, req):
                         raise SchedulerError(f"page {p} of group {gi}: table of {req!r}, pool says {g.pool.owner(p)!r}")
             if len(held) + g.pool.num_free != g.pool.num_pages:
                 raise SchedulerError(f"group {gi}: {len(held)} held + {g.pool.num_free} free != {g.pool.num_pages}")

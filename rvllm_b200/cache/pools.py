@@ -3,11 +3,12 @@
 The reference has the page layout only (v3/crates/rvllm-mem/src/kv_layout.rs:10-47) and
 static identity block tables (v3/crates/rvllm-runtime/src/bring_up.rs:420-435); its scheduler
 spec names an allocator (v3/specs/07-scheduler.md:76,97) that was never written.  The free
-list is a stack, so a page given back is the next one handed out.
+list is a stack, so a page given back is the next one handed out.  A page may get further holders (requests that begin
+with the same tokens); it is free again when the last of them gives it back.
 """
 from __future__ import annotations
 
-from typing import Hashable, List, Optional
+from typing import Dict, Hashable, List, Optional, Set
 
 from ..errors import KvExhausted, SchedulerError
 
@@ -19,10 +20,24 @@ class PagePool:
         self.num_pages = num_pages
         self._free: List[int] = list(range(num_pages - 1, -1, -1))   # page 0 on top
         self._owner: List[Optional[Hashable]] = [None] * num_pages
+        self._others: Dict[int, Set[Hashable]] = {}      # holders beside the owner, of pages that have any
 
     @property
     def num_free(self) -> int:
         return len(self._free)
+
+    def share(self, pages, owner: Hashable) -> None:
+        """One more holder for pages that are held."""
+        for p in pages:
+            if not 0 <= p < self.num_pages or self._owner[p] is None:
+                raise SchedulerError(f"page {p} is not held by anybody: it cannot be shared")
+            if self.holds(p, owner):
+                raise SchedulerError(f"page {p} is held by {owner!r} already")
+        for p in pages:
+            self._others.setdefault(p, set()).add(owner)
+
+    def holds(self, page: int, owner: Hashable) -> bool:
+        return self._owner[page] == owner or owner in self._others.get(page, ())
 
     def allocate(self, n: int, owner: Hashable) -> List[int]:
         if n > len(self._free):
@@ -40,8 +55,17 @@ class PagePool:
                 raise SchedulerError(f"page {p} does not exist")
             if self._owner[p] is None:
                 raise SchedulerError(f"page {p} is freed twice")
-            if self._owner[p] != owner:
+            if not self.holds(p, owner):
                 raise SchedulerError(f"page {p} is held by {self._owner[p]!r}, not by {owner!r}")
+            others = self._others.get(p)
+            if others is not None:                       # it stays with the others
+                if self._owner[p] == owner:
+                    self._owner[p] = others.pop()
+                else:
+                    others.remove(owner)
+                if not others:
+                    del self._others[p]
+                continue
             self._owner[p] = None
             self._free.append(p)
 

@@ -47,6 +47,8 @@ def _engine_options(ap: argparse.ArgumentParser) -> None:
                     help="no CUDA graphs for decode steps (also RVLLM_NO_GRAPH=1)")
     ap.add_argument("--no-async-scheduling", action="store_true", default=os.environ.get("RVLLM_NO_ASYNC") == "1",
                     help="wait for every step's tokens before the next step is launched (also RVLLM_NO_ASYNC=1)")
+    ap.add_argument("--share-prefixes", action="store_true",
+                    help="requests that begin with the same tokens hold the same pages of the cache, and decode steps read these once")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--capture-graphs", action="store_true",
                     help="capture the decode CUDA graphs of every batch and context bucket before the first request")
@@ -66,7 +68,7 @@ def _llm(args, **over):
               gpu_memory_utilization=args.gpu_memory_utilization, max_model_len=args.max_model_len,
               max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens,
               max_prefill_chunk=args.max_prefill_chunk, enforce_eager=args.enforce_eager, seed=args.seed,
-              async_scheduling=not args.no_async_scheduling)
+              async_scheduling=not args.no_async_scheduling, share_prefixes=args.share_prefixes)
     kw.update(over)
     if args.config:
         with open(args.config) as f:
@@ -94,18 +96,20 @@ def cmd_generate(args) -> int:
     stops = tuple(_ids(args.eos)) if args.eos else ()
     sp = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                         seed=args.sampling_seed, max_tokens=args.max_tokens, stop_token_ids=stops,
-                        ignore_eos=args.ignore_eos)
+                        ignore_eos=args.ignore_eos, n=args.n)
     t0 = time.perf_counter()
     outs = llm.generate(prompts, sp)
     dt = time.perf_counter() - t0
     for o in outs:
-        c = o.outputs[0]
-        rec = {"request_id": o.request_id, "prompt_tokens": len(o.prompt_token_ids), "token_ids": c.token_ids,
-               "finish_reason": c.finish_reason}
-        if c.text is not None:
-            rec["text"] = c.text
-        print(json.dumps(rec))
-    n = sum(len(o.outputs[0].token_ids) for o in outs)
+        for i, c in enumerate(o.outputs):
+            rec = {"request_id": o.request_id, "prompt_tokens": len(o.prompt_token_ids), "token_ids": c.token_ids,
+                   "finish_reason": c.finish_reason}
+            if len(o.outputs) > 1:
+                rec["sample"] = i
+            if c.text is not None:
+                rec["text"] = c.text
+            print(json.dumps(rec))
+    n = sum(len(c.token_ids) for o in outs for c in o.outputs)
     print(f"generated {n} tokens in {dt:.3f} s ({n / dt:.1f} tok/s)", file=sys.stderr)
     return 0
 
@@ -200,6 +204,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     g.add_argument("--temperature", type=float, default=0.0)
     g.add_argument("--top-k", type=int, default=0)
     g.add_argument("--top-p", type=float, default=1.0)
+    g.add_argument("--n", type=int, default=1, help="samples of every prompt")
     g.add_argument("--sampling-seed", type=int, default=None)
     g.add_argument("--eos", default=os.environ.get("RVLLM_EOS"), help="extra stop token ids, e.g. 2,151645 (also $RVLLM_EOS)")
     g.add_argument("--ignore-eos", action="store_true")

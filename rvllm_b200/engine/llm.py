@@ -9,7 +9,7 @@ bench_harness.py:21-30).
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Dict, Hashable, List, Optional, Sequence, Union
 
 import torch
@@ -61,12 +61,12 @@ class LLM:
                  num_blocks: Optional[int] = None, gpu_memory_utilization: float = 0.9,
                  max_model_len: Optional[int] = None, max_num_seqs: int = 64, max_num_batched_tokens: int = 2048,
                  max_prefill_chunk: Optional[int] = None, enable_chunked_prefill: bool = True,
-                 enforce_eager: bool = False, async_scheduling: bool = True):
+                 enforce_eager: bool = False, async_scheduling: bool = True, share_prefixes: bool = False):
         ec = EngineConfig(dtype=dtype, block_size=block_size, num_blocks=num_blocks,
                           gpu_memory_utilization=gpu_memory_utilization, max_model_len=max_model_len,
                           max_num_seqs=max_num_seqs, max_num_batched_tokens=max_num_batched_tokens,
                           max_prefill_chunk=max_prefill_chunk, enable_chunked_prefill=enable_chunked_prefill,
-                          enforce_eager=enforce_eager, seed=seed, device=device)
+                          enforce_eager=enforce_eager, share_prefixes=share_prefixes, seed=seed, device=device)
         self.engine = Engine(model, config=config, engine_config=ec, random_weights=random_weights, seed=seed)
         self.config = self.engine.config
         self.sampler = Sampler(self.engine.kernels)
@@ -89,7 +89,7 @@ class LLM:
     def _new_scheduler(self) -> Scheduler:
         ec = self.config
         return Scheduler(self.engine.cache, ec.max_num_seqs, ec.max_num_batched_tokens, ec.max_model_len,
-                         ec.max_prefill_chunk, ec.enable_chunked_prefill, self.engine.spec.eos_token_ids)
+                         ec.max_prefill_chunk, ec.enable_chunked_prefill, self.engine.spec.eos_token_ids, ec.share_prefixes)
 
     # ---- requests ----------------------------------------------------------------------------
     def add_request(self, prompt_token_ids: Sequence[int], params: SamplingParams,
@@ -175,7 +175,9 @@ class LLM:
     def generate(self, prompts: Union[Sequence[Sequence[int]], Sequence[str]],
                  sampling_params: Union[SamplingParams, Sequence[SamplingParams], None] = None) -> List[RequestOutput]:
         """Generate for every prompt (lists of token ids, or strings when the model folder has a
-        tokenizer); outputs come back in the order of the prompts."""
+        tokenizer); outputs come back in the order of the prompts, with `n` samples each.  With `share_prefixes` the
+        samples of a prompt, and prompts that begin alike, hold the same pages of the cache, and a decode step reads the
+        keys of a shared beginning once for all of them."""
         if sampling_params is None:
             sampling_params = SamplingParams()
         if isinstance(sampling_params, SamplingParams):
@@ -188,12 +190,13 @@ class LLM:
                 if self.tokenizer is None:
                     raise ConfigError("string prompts need a tokenizer.json in the model folder; pass token ids instead")
                 p = self.tokenizer.encode(p)
-            reqs.append(self.add_request(p, sp))
+            samples = [sp] if sp.n == 1 else [replace(sp, n=1, seed=None if sp.seed is None else (sp.seed + i) % 2 ** 63) for i in range(sp.n)]
+            reqs.append([self.add_request(p, one) for one in samples])
         while self.scheduler.has_unfinished():
             self.step()
         outs = []
-        for r in reqs:
-            text = self.tokenizer.decode(r.output) if self.tokenizer is not None else None
-            outs.append(RequestOutput(r.req_id, list(r.prompt), [CompletionOutput(list(r.output), r.finish_reason, text)],
-                                      r.num_preemptions))
+        for samples in reqs:
+            done = [CompletionOutput(list(r.output), r.finish_reason, self.tokenizer.decode(r.output) if self.tokenizer is not None else None)
+                    for r in samples]
+            outs.append(RequestOutput(samples[0].req_id, list(samples[0].prompt), done, sum(r.num_preemptions for r in samples)))
         return outs

@@ -20,6 +20,12 @@ This scheduler does what the spec sketches:
 * a request finishes when it has produced `max_tokens` ("length"), a stop or EOS token
   ("stop"), or has reached `max_model_len` ("length"); its pages and slot are freed at once.
 
+With `share_prefixes`, a request that is admitted takes over the pages of the running request that it has the longest beginning
+in common with, as far as that has been computed, and starts behind them (at least its last token is its own); a request whose
+beginning is still being computed for another one waits for it when that saves `SHARE_WAIT_PAGES` pages or more, and lets those
+behind it pass.  A pre-empted request takes over pages again when it comes back.  Off by default: the tokens are the same in exact
+arithmetic, but which portions a prompt is computed in shows in the last bits.
+
 Same arrivals and seeds give the same sequence of batches.
 
 Accounting a step has two halves, so that the next step can be decided while the device still
@@ -42,6 +48,7 @@ from ..errors import KvExhausted, SchedulerError
 from ..sampling.params import SamplingParams
 
 WAITING, RUNNING, FINISHED = "waiting", "running", "finished"
+SHARE_WAIT_PAGES = 4    # a request waits for a beginning that another one is computing when it is this many pages longer
 PENDING = -1        # stands in `Request.output` for a token that is being sampled
 
 
@@ -58,6 +65,8 @@ class Request:
     arrival: int = 0
     num_preemptions: int = 0
     unresolved: int = 0            # stand-ins at the end of `output`
+    shared_tokens: int = 0         # tokens at the beginning that were taken over when it was last admitted
+    common: dict = field(default_factory=dict, repr=False)     # while it waits: tokens in common with the prompts of running requests
 
     @property
     def all_tokens(self) -> List[int]:
@@ -103,8 +112,9 @@ class ScheduledBatch:
 class Scheduler:
     def __init__(self, cache: CacheManager, max_num_seqs: int, max_num_batched_tokens: int,
                  max_model_len: int, max_prefill_chunk: Optional[int] = None,
-                 enable_chunked_prefill: bool = True, eos_token_ids: Sequence[int] = ()):
+                 enable_chunked_prefill: bool = True, eos_token_ids: Sequence[int] = (), share_prefixes: bool = False):
         self.cache = cache
+        self.share_prefixes = share_prefixes and cache.can_share
         self.max_num_seqs = max_num_seqs
         self.max_num_batched_tokens = max_num_batched_tokens
         self.max_model_len = max_model_len
@@ -150,6 +160,31 @@ class Scheduler:
             n = min(n, self.max_prefill_chunk)
         return n
 
+    def _donor(self, req: Request):
+        """(running request, tokens of it that `req` can take over, whether to wait for more).  Only what has been computed can be taken
+        over, in whole pages, and the last token stays to be computed."""
+        page = self.cache.page_size
+        tokens = None
+        best, have, coming = None, 0, 0
+        live = {id(r) for r in self.running}
+        for gone in [k for k in req.common if k not in live]:
+            del req.common[gone]
+        for other in self.running:
+            common = req.common.get(id(other))
+            if common is None:
+                # whole pages of the two prompts (and what `req` has produced before it was pre-empted) that are the same
+                if tokens is None:
+                    tokens = req.all_tokens
+                theirs, common, most = other.prompt, 0, min(len(tokens) - 1, len(other.prompt))
+                while common + page <= most and tokens[common:common + page] == theirs[common:common + page]:
+                    common += page
+                req.common[id(other)] = common
+            ready = min(common, other.num_computed // page * page)
+            if ready > have:
+                best, have = other, ready
+            coming = max(coming, common)
+        return best, have, coming - have >= SHARE_WAIT_PAGES * page
+
     def _preempt(self, req: Request, preempted: List[Request]) -> None:
         self.cache.free(req.req_id)
         self.running.remove(req)
@@ -191,22 +226,35 @@ class Scheduler:
             budget -= n
 
         # admissions, in arrival order (pre-empted requests wait at the front)
-        while self.waiting and budget > 0 and len(self.running) < self.max_num_seqs:
-            req = self.waiting[0]
+        at = 0
+        while at < len(self.waiting) and budget > 0 and len(self.running) < self.max_num_seqs:
+            req = self.waiting[at]
             if req in preempted:
                 break                       # do not re-admit in the step that evicted it
-            n = self._portion(req, budget)
-            if not self.enable_chunked_prefill and n < req.remaining:
+            donor, shared = None, 0
+            if self.share_prefixes:
+                donor, shared, wait = self._donor(req)
+                if wait:
+                    at += 1                 # its beginning is being computed for another request
+                    continue
+            n = min(req.remaining - shared, budget)
+            if req.remaining - shared > 1 and self.max_prefill_chunk is not None:
+                n = min(n, self.max_prefill_chunk)
+            if not self.enable_chunked_prefill and n < req.remaining - shared:
                 break
-            if not self.cache.can_append(None, n, reserved):
+            need = self.cache.pages_needed(None, n, shared)
+            if any(a + b > free for a, b, free in zip(need, reserved, self.cache.num_free_pages())):
                 break
-            self.waiting.popleft()
+            del self.waiting[at]
             self.cache.admit(req.req_id)
+            if shared:
+                self.cache.share(req.req_id, donor.req_id, shared)
+            req.num_computed = req.shared_tokens = shared
+            req.common.clear()
             req.state = RUNNING
             self.running.append(req)
-            need = self.cache.pages_needed(req.req_id, n)
             reserved = [a + b for a, b in zip(reserved, need)]
-            entries.append(ScheduledEntry(req, 0, n, n == req.remaining))
+            entries.append(ScheduledEntry(req, shared, n, n == req.remaining))
             scheduled_ids.add(req.req_id)
             budget -= n
 

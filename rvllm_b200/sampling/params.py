@@ -32,6 +32,7 @@ class SamplingParams:
     max_tokens: int = 16
     stop_token_ids: Tuple[int, ...] = ()
     ignore_eos: bool = False
+    n: int = 1                     # samples of the prompt (`LLM.generate`); sample i > 0 of a seed draws from seed + i
 
     def __post_init__(self):
         problems = []
@@ -45,6 +46,8 @@ class SamplingParams:
             problems.append(f"max_tokens must be >= 1, got {self.max_tokens}")
         if self.seed is not None and not (0 <= self.seed < 2 ** 63):
             problems.append(f"seed must be in [0, 2^63), got {self.seed}")
+        if self.n < 1:
+            problems.append(f"n must be >= 1, got {self.n}")
         if problems:
             raise SamplingError("; ".join(problems))
         object.__setattr__(self, "stop_token_ids", tuple(self.stop_token_ids))
