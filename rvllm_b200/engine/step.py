@@ -12,6 +12,10 @@ metadata with separate synchronous copies (bring_up.rs:698-708); its packed layo
 (v3/crates/rvllm-metadata/src/layout.rs:19-55: token ids, positions, context lengths, block
 tables, slot mapping, sequence starts; padding rows have slot -1, pack.rs:79-86) is what the
 buffer here follows, extended per cache group.
+
+Where the kernel library offers `step_tables`, the buffer holds the requests' lengths and the pages handed out since the last
+step, and the block tables, slot maps, positions and sequence starts are built on the device, in front of a table of all
+requests' pages that stays there; otherwise the host writes them out.
 """
 from __future__ import annotations
 
@@ -24,6 +28,11 @@ import torch
 from ..cache import CacheManager
 from ..errors import KvExhausted, SchedulerError
 from ..kernels.library import COUNTERS, AttentionMeta
+from ..kernels.shared import StepPrefixes, StepTables
+
+# A decode step reads shared beginnings once (instead of as many times as requests hold them) when that saves at least this many keys.
+SHARED_MIN_KEYS = 1024
+SHARED_MOST_GROUPS = 8         # of a captured step: those that save the most
 
 
 @dataclass
@@ -62,6 +71,12 @@ class ModelRunner:
         self._ring_events: List[Optional[object]] = [None, None, None]
         self._ring_next = 0
         self._dev: Optional[torch.Tensor] = None
+        self._groups_of = ((), [])       # the requests of the last decode step, and which of them share beginnings
+        self._page_table = None
+        if cache.groups and self.device.type == "cuda" and hasattr(kernels, "step_tables"):
+            G = len(cache.groups)
+            self._page_table = torch.full((G, cache.max_seqs, self.max_blocks), -1, dtype=torch.int32, device=self.device)
+            self._spans = torch.tensor([[g.need.window or 0, g.need.chunk or 0] for g in cache.groups], dtype=torch.int32, device=self.device)
         self.steps_run = 0
         self.last_h2d_bytes = 0
 
@@ -142,6 +157,8 @@ class ModelRunner:
         `late` = (sampled ids on the device, one index per entry): an entry with index j >= 0 is a
         one-token sequence whose token is sampled[j], which the host has not read; its token is
         put in place on the device after the copy."""
+        if self._page_table is not None:
+            return self._pack_lengths(entries, starts, pad_to, buffers, late, ctx_limit)
         cache = self.cache
         n_real = len(entries)
         B = pad_to if pad_to is not None else n_real
@@ -246,6 +263,118 @@ class ModelRunner:
                 num_decode=sum(1 for n in q_lens if n == 1)))
         return ctx
 
+    def _new_pages(self, entries) -> int:
+        """Pages of the entries that the table on the device does not have yet."""
+        return sum(len(t) - n for e in entries for r in (self.cache.requests[e.req_id],) for t, n in zip(r.tables, r.on_device))
+
+    def _pack_lengths(self, entries, starts, pad_to, buffers, late, ctx_limit) -> StepContext:
+        """`pack` where the device builds the tables: the buffer holds, in this order, state slots, starts and token counts of the
+        sequences, the blocks that each has on the device by group, tokens, wanted rows, sources of late tokens, new pages; behind
+        them (on the device only) lie the tables that are built."""
+        cache = self.cache
+        n_real, G = len(entries), len(cache.groups)
+        B = pad_to if pad_to is not None else n_real
+        pads = B - n_real
+        q_lens = [len(e.tokens) for e in entries] + [1] * pads
+        T = sum(q_lens)
+        ctx_lens = [s + n for s, n in zip(starts, q_lens)] + [0] * pads
+        held = [cache.requests[e.req_id] for e in entries]
+        if pad_to is not None:
+            rows = np.arange(B, dtype=np.int32)
+            MB, room = self.max_blocks, G * B                      # (a decoded token takes one page of a group at most)
+        else:
+            ends = np.cumsum([0] + q_lens)
+            rows = np.asarray([ends[i] + w for i, e in enumerate(entries) for w in e.want], dtype=np.int32)
+            MB, room = max(1, cache.blocks_for(max(ctx_lens))), self._new_pages(entries)
+        R = len(rows)
+        sent = 3 * B + G * B + T + R + B + max(room, 1)
+        built = (G * B * MB, G * T, T, T, B + 1, B)
+        if buffers is None:
+            ring_i, host, dev = self._buffers(sent + sum(built))
+        else:
+            ring_i, (host, dev) = None, buffers
+        h = host.numpy()
+        o_start, o_q, o_held = B, 2 * B, 3 * B
+        o_tok = o_held + G * B
+        o_rows, o_late, o_new = o_tok + T, o_tok + T + R, o_tok + T + R + B
+        h[:n_real] = [r.state_slot for r in held]
+        h[n_real:B] = -1
+        h[o_start:o_start + n_real] = starts
+        h[o_start + n_real:o_start + B] = 0
+        h[o_q:o_q + B] = q_lens
+        h[o_rows:o_rows + R] = rows
+        if T == B:
+            h[o_tok:o_tok + n_real] = [e.tokens[0] for e in entries]
+            h[o_tok + n_real:o_tok + T] = 0
+        else:
+            at = o_tok
+            for e, n in zip(entries, q_lens):
+                h[at:at + n] = e.tokens
+                at += n
+        at = o_new
+        for g in range(G):
+            h[o_held + g * B:o_held + g * B + n_real] = [r.on_device[g] for r in held]
+            h[o_held + g * B + n_real:o_held + (g + 1) * B] = 0
+            for r in held:
+                new = r.tables[g][r.on_device[g]:]
+                if new:
+                    h[at:at + len(new)] = new
+                    at += len(new)
+                    r.on_device[g] += len(new)
+        h[o_late:o_late + n_real] = late[1] if late is not None else -1
+        h[o_late + n_real:o_late + B] = -1
+        dev[:at].copy_(host[:at], non_blocking=True)
+        self.last_h2d_bytes = at * 4
+        if ring_i is not None:
+            ev = self._ring_events[ring_i] or torch.cuda.Event()
+            ev.record()
+            self._ring_events[ring_i] = ev
+
+        tables, slots, positions, token_seq, cu, ctx_dev = dev[sent:sent + sum(built)].split_with_sizes(built)
+        made = StepTables(tables.view(G, B, MB), slots.view(G, T), positions, token_seq, cu, ctx_dev)
+        self.kernels.step_tables(self._page_table, dev[:B], dev[o_held:o_tok].view(G, B), dev[o_start:o_q], dev[o_q:o_held], dev[o_new:max(at, o_new + 1)],
+                                 self._spans, T, MB, cache.page_size, out=made)
+        ctx = StepContext()
+        ctx.kernels = self.kernels
+        ctx.num_tokens, ctx.num_seqs = T, B
+        ctx.token_ids = dev[o_tok:o_tok + T]
+        ctx.positions, ctx.token_seq, ctx.cu_seqlens = positions, token_seq, cu
+        if late is not None:
+            self.kernels.late_tokens(ctx.token_ids, cu, dev[o_late:o_late + B], late[0])
+        ctx.state_slots = dev[:B]
+        ctx.logit_rows = dev[o_rows:o_rows + R]
+        ctx.q_lens, ctx.ctx_lens = q_lens, ctx_lens
+        ctx.req_ids = [e.req_id for e in entries]
+        longest = (ctx_limit or self.max_model_len) if pad_to is not None else max(ctx_lens)
+        ctx.attention = [AttentionMeta(block_tables=made.block_tables[g], cu_seqlens=cu, ctx_lens=ctx_dev, token_seq=token_seq,
+                                       slot_mapping=made.slot_mapping[g], num_seqs=B, max_q_len=max(q_lens), max_ctx_len=longest,
+                                       page_size=cache.page_size, num_decode=q_lens.count(1)) for g in range(G)]
+        return ctx
+
+    # ---- beginnings that requests share ----------------------------------------------------------
+    def _shared_groups(self, entries):
+        """(places, tokens) per group of entries that begin with the same cached tokens, for a step of decoded tokens; none where it
+        would not save enough.  Pages that are shared stay as they are while their requests live, so the answer holds until the set
+        of requests changes."""
+        if not self.cache.can_share or self._page_table is None or any(len(e.tokens) != 1 for e in entries):
+            return []
+        reqs = tuple(e.req_id for e in entries)
+        if reqs != self._groups_of[0]:
+            groups = sorted(self.cache.shared_groups(reqs), key=lambda g: -(len(g[0]) - 1) * g[1])[:SHARED_MOST_GROUPS]
+            if sum((len(m) - 1) * t for m, t in groups) < SHARED_MIN_KEYS:
+                groups = []
+            self._groups_of = (reqs, groups)
+        return self._groups_of[1]
+
+    @staticmethod
+    def _longest_own(starts, groups) -> int:
+        """The most keys that an entry has behind its group's beginning, this step's token included."""
+        own = [s + 1 for s in starts]
+        for members, tokens in groups:
+            for m in members:
+                own[m] -= tokens
+        return max(own)
+
     def _pack_decode(self, entries, starts, B, MB, h, host, dev, offs, take, late=None, ctx_limit=None) -> StepContext:
         """`pack` for a padded batch of one-token sequences (T = R = B): whole-array writes."""
         cache = self.cache
@@ -337,6 +466,11 @@ class ModelRunner:
             logits = self._step_graph(entries, starts, bucket, late_tokens)
         else:
             ctx = self.pack(entries, starts, late=late_tokens)
+            groups = self._shared_groups(entries)
+            if groups:
+                shared = StepPrefixes(groups, len(entries), self.device, num_sms=self.kernels.num_sms)
+                for m in ctx.attention:
+                    m.shared, m.max_own_len = shared, self._longest_own(starts, groups)
             hidden = self.model.forward(ctx, self.cache)
             logits = self.model.compute_logits(hidden, ctx) if ctx.logit_rows.numel() else None
         for e in entries:
@@ -370,30 +504,50 @@ class ModelRunner:
 
     def _step_graph(self, entries, starts, bucket: int, late=None) -> torch.Tensor:
         ctx_limit = self._ctx_bucket(max(starts) + 1)
-        bucket = (bucket, ctx_limit)
+        groups = self._shared_groups(entries)
+        # a step that reads shared beginnings once is another graph, laid out for the keys behind them
+        own_limit = self._ctx_bucket(self._longest_own(starts, groups)) if groups else 0
+        bucket = (bucket, ctx_limit, own_limit)
         state = self._graphs.get(bucket)
-        if state is None:
+        if state is None or (self._page_table is not None and self._new_pages(entries) > len(self.cache.groups) * len(entries)):
             # the first step of a bucket runs eagerly: it loads every kernel library and lets the
             # GEMM library set itself up; the graph is captured right after it for later steps
+            # (so does one whose requests have just taken over pages that the device's table lacks)
             ctx = self.pack(entries, starts, late=late)
+            if groups:
+                shared = StepPrefixes(groups, len(entries), self.device, num_sms=self.kernels.num_sms)
+                for m in ctx.attention:
+                    m.shared, m.max_own_len = shared, own_limit
             hidden = self.model.forward(ctx, self.cache)
             logits = self.model.compute_logits(hidden, ctx)
-            self._graphs[bucket] = self._capture(*bucket)
+            if state is None:
+                self._graphs[bucket] = self._capture(*bucket)
             return logits
-        host, dev, graph, out, launches = state
+        host, dev, graph, out, launches, shared = state
         self._graph_event.synchronize()
         self.pack(entries, starts, pad_to=bucket[0], buffers=(host, dev), late=late, ctx_limit=ctx_limit)
+        if shared is not None:
+            shared.set_groups(groups)
         self._graph_event.record()
         graph.replay()
         COUNTERS["launches"] += launches       # the kernels of this project inside the replayed graph
         return out[:len(entries)]
 
-    def _capture(self, bucket: int, ctx_limit: int):
+    def _graph_buffers(self, bucket: int):
+        """Staging and device buffer of a captured step of `bucket` sequences, in either form of `pack`."""
         G = len(self.cache.groups)
-        n_ints = 3 * bucket + (bucket + 1) + 2 * bucket + bucket + G * (bucket + bucket * self.max_blocks) + bucket + 16
-        host = torch.empty((n_ints,), dtype=torch.int32, pin_memory=True)
-        dev = torch.empty((n_ints,), dtype=torch.int32, device=self.device)
+        n_ints = 8 * bucket + 2 + 2 * G * bucket + G * (bucket + bucket * self.max_blocks) + 5 * bucket + 16
+        return torch.empty((n_ints,), dtype=torch.int32, pin_memory=True), torch.empty((n_ints,), dtype=torch.int32, device=self.device)
+
+    def _capture(self, bucket: int, ctx_limit: int, own_limit: int = 0):
+        host, dev = self._graph_buffers(bucket)
         ctx = self.pack([], [], pad_to=bucket, buffers=(host, dev), ctx_limit=ctx_limit)   # all rows padded: writes nothing
+        shared = None
+        if own_limit:
+            shared = StepPrefixes([], bucket, self.device, SHARED_MOST_GROUPS, self.kernels.num_sms)
+            for m in ctx.attention:
+                m.shared, m.max_own_len = shared, own_limit
+            self.model.compute_logits(self.model.forward(ctx, self.cache), ctx)     # (makes the layouts, which no capture may)
         torch.cuda.synchronize(self.device)
         graph = torch.cuda.CUDAGraph()
         before = COUNTERS["launches"]
@@ -407,7 +561,7 @@ class ModelRunner:
         if self._graph_event is None:
             self._graph_event = torch.cuda.Event()
             self._graph_event.record()
-        return host, dev, graph, out, launches
+        return host, dev, graph, out, launches, shared
 
     def capture_decode_graphs(self, max_context: Optional[int] = None, batch_sizes: Optional[Sequence[int]] = None) -> int:
         """Capture the decode graphs ahead of time, for every batch bucket (or the given ones) and
@@ -429,16 +583,12 @@ class ModelRunner:
             if bucket not in self.graph_batch_sizes:
                 raise SchedulerError(f"{bucket} is not one of the graph batch sizes {self.graph_batch_sizes}")
             for ctx_limit in ctx_buckets:
-                if (bucket, ctx_limit) not in self._graphs:
+                if (bucket, ctx_limit, 0) not in self._graphs:
                     # a first, uncaptured run of the padded batch: it loads the kernel libraries
                     # and lets the GEMM library choose its algorithms outside the capture
-                    G = len(self.cache.groups)
-                    n_ints = 3 * bucket + (bucket + 1) + 2 * bucket + bucket + G * (bucket + bucket * self.max_blocks) + bucket + 16
-                    host = torch.empty((n_ints,), dtype=torch.int32, pin_memory=True)
-                    dev = torch.empty((n_ints,), dtype=torch.int32, device=self.device)
-                    ctx = self.pack([], [], pad_to=bucket, buffers=(host, dev), ctx_limit=ctx_limit)
+                    ctx = self.pack([], [], pad_to=bucket, buffers=self._graph_buffers(bucket), ctx_limit=ctx_limit)
                     self.model.compute_logits(self.model.forward(ctx, self.cache), ctx)
-                    self._graphs[(bucket, ctx_limit)] = self._capture(bucket, ctx_limit)
+                    self._graphs[(bucket, ctx_limit, 0)] = self._capture(bucket, ctx_limit)
                     made += 1
         return made
 

@@ -5,7 +5,7 @@ from typing import Optional
 
 from ..errors import KernelError
 from .library import CudaKernels, AttentionMeta
-from .shared import SharedPrefixes, StepTables
+from .shared import SharedPrefixes, StepPrefixes, StepTables
 
 _library = None
 

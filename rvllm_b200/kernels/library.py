@@ -11,6 +11,7 @@ built, construction raises `KernelError`.
 """
 from __future__ import annotations
 
+import copy
 import ctypes
 import os
 import struct
@@ -21,7 +22,7 @@ import torch
 
 from ..errors import KernelError
 from . import build
-from .shared import SharedPrefixes, StepTables, TILE_ROWS
+from .shared import SharedPrefixes, StepPrefixes, StepTables, TILE_ROWS
 
 _DT = {torch.float32: 0, torch.bfloat16: 1}
 _GATED_PREFILL, _GATED_DECODE = {"silu": 2, "gelu_tanh": 4, "swiglu_clamp": 5}, {"silu": 1, "gelu_tanh": 2, "swiglu_clamp": 3}
@@ -64,7 +65,7 @@ class AttentionMeta:
     """Per-step, per-cache-group arguments of the attention kernels (device int32 tensors) and
     the few host-side numbers that size their launches."""
     __slots__ = ("block_tables", "cu_seqlens", "ctx_lens", "token_seq", "slot_mapping", "num_seqs",
-                 "max_q_len", "max_ctx_len", "max_blocks", "page_size", "num_decode")
+                 "max_q_len", "max_ctx_len", "max_blocks", "page_size", "num_decode", "shared", "max_own_len")
 
     def __init__(self, block_tables, cu_seqlens, ctx_lens, token_seq, slot_mapping, num_seqs,
                  max_q_len, max_ctx_len, page_size, num_decode=0):
@@ -74,6 +75,9 @@ class AttentionMeta:
         self.num_seqs, self.max_q_len, self.max_ctx_len = num_seqs, max_q_len, max_ctx_len
         self.max_blocks = block_tables.shape[1]
         self.page_size = page_size
+        # which sequences begin with the same cached tokens (`StepPrefixes`; None: none do, or nothing is made of it), and the most
+        # keys that any of them has behind that
+        self.shared, self.max_own_len = None, None
 
 
 class CudaKernels:
@@ -321,10 +325,14 @@ class CudaKernels:
         softmax denominator; `gate` (float [tokens, heads]): multiplies each head's output; `distance_bias` (a
         `parts.distance.DistanceBias`): added to a score by the distance between query and key, after the cap.
 
+        A step whose sequences share beginnings (`meta.shared`) goes to `shared_prefix_attention`.
         bfloat16 with a head size that is a multiple of 16 and pages of a power of two go to the
         tensor-core flash kernel (one token per sequence: the decode tiling, keys split over CTAs
         when the batch alone cannot fill the GPU); everything else goes to the plain kernel."""
         page = cache_layer.shape[3]
+        if meta.shared is not None and meta.max_q_len == 1 and window is None and distance_bias is None and num_heads // num_kv_heads <= TILE_ROWS:
+            return self.shared_prefix_attention(q, cache_layer, meta, meta.shared.layout(num_heads, num_kv_heads), num_heads, num_kv_heads,
+                                                head_dim, scale, softcap, sinks, gate, meta.max_own_len)
         extras = softcap is not None or sinks is not None or gate is not None or distance_bias is not None
         if q.dtype != torch.bfloat16 or head_dim % 16 or head_dim > 256 or (page & (page - 1)):
             return self.paged_attention_plain(q, cache_layer, meta, num_heads, num_kv_heads, head_dim, scale, window,
@@ -569,7 +577,11 @@ class CudaKernels:
             and B <= 4096
         tiles, items = shared.capacity
         if items == 0 or B == 0 or group > TILE_ROWS or not (fast or (head_dim % 4 == 0 and head_dim <= 256)):
-            return self.paged_attention(q, cache_layer, meta, num_heads, num_kv_heads, head_dim, scale, None, softcap, sinks, gate)
+            whole = meta
+            if meta.shared is not None:
+                whole = copy.copy(meta)
+                whole.shared = None
+            return self.paged_attention(q, cache_layer, whole, num_heads, num_kv_heads, head_dim, scale, None, softcap, sinks, gate)
         if max_own is None:
             max_own = meta.max_ctx_len - shared.shortest
         max_own = max(1, min(max_own, meta.max_ctx_len))

@@ -47,9 +47,18 @@ class SharedPrefixes:
             raise KernelError(f"shared prefixes: {num_seqs} sequences of {num_heads} heads on {num_kv_heads} key/value heads")
         self.num_seqs, self.num_heads, self.num_kv_heads = num_seqs, num_heads, num_kv_heads
         self.num_sms = num_sms
-        self.capacity = None
         host = self._lay_out(groups, capacity)
+        # with a capacity the launches are sized for any groups that fit it
+        self.capacity = capacity or (self.num_tiles, self.num_items)
+        if capacity is not None:
+            self.most_parts, self.shortest = capacity[1], 0
         self.device_ints = torch.from_numpy(host).to(device)
+
+    def refill(self, groups) -> None:
+        """Other groups of the same step size, into the same array (on the current stream)."""
+        most_parts, shortest = self.most_parts, self.shortest
+        self.device_ints.copy_(torch.from_numpy(self._lay_out(groups, self.capacity)))
+        self.most_parts, self.shortest = most_parts, shortest
 
     @staticmethod
     def ints(num_seqs: int, capacity: Tuple[int, int]) -> int:
@@ -113,11 +122,43 @@ class SharedPrefixes:
             host[4 + 3 * B:4 + 3 * B + 2 * len(tiles)] = np.asarray(parts, np.int32).ravel()
             at = (4 + 3 * B + 2 * capacity[0] + 3) // 4 * 4
             host[at:at + 8 * len(items)] = np.asarray(items, np.int32).ravel()
-        self.capacity, self.num_items, self.num_tiles = capacity, len(items), len(tiles)
+        self.num_items, self.num_tiles = len(items), len(tiles)
         self.most_parts = max((n for _, n in parts), default=0)
         # the fewest keys that any sequence has before its own begin (0: one has no prefix)
         self.shortest = min((t for _, t in kept), default=0) if len(flat) == B else 0
         return host
+
+
+class StepPrefixes:
+    """The groups of a step for every layout of heads that its layers have (one `SharedPrefixes` each, made when a layer first asks).
+
+    `most_groups`: fixes the arrays' capacities for up to so many groups; `set_groups` then fills them anew, wherever a captured
+    graph holds them."""
+
+    def __init__(self, groups, num_seqs: int, device, most_groups: Optional[int] = None, num_sms: int = 148):
+        self.groups, self.num_seqs, self.device, self.most_groups, self.num_sms = groups, num_seqs, device, most_groups, num_sms
+        self._layouts = {}
+
+    def layout(self, num_heads: int, num_kv_heads: int) -> SharedPrefixes:
+        made = self._layouts.get((num_heads, num_kv_heads))
+        if made is None:
+            capacity = None
+            if self.most_groups is not None:
+                members = max(1, TILE_ROWS // (num_heads // num_kv_heads))
+                tiles = -(-self.num_seqs // members) + self.most_groups
+                capacity = (tiles, tiles + -(-2 * self.num_sms // num_kv_heads))
+            made = SharedPrefixes(self.groups, self.num_seqs, num_heads, num_kv_heads, self.device, capacity, self.num_sms)
+            self._layouts[(num_heads, num_kv_heads)] = made
+        return made
+
+    def set_groups(self, groups) -> None:
+        if groups == self.groups:
+            return
+        if self.most_groups is None or len(groups) > self.most_groups:
+            raise KernelError(f"shared prefixes: {len(groups)} groups where {self.most_groups} fit")
+        self.groups = groups
+        for made in self._layouts.values():
+            made.refill(groups)
 
 
 @dataclass

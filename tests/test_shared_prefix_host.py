@@ -85,3 +85,183 @@ def test_refused_heads():
             SharedPrefixes([], 4, *heads, "cpu")
     with pytest.raises(KernelError):
         SharedPrefixes([([0, 1], 5)], 4, 256, 1, "cpu")
+
+
+# ------------------------------------------------------------------------------------------------- pages with several holders
+def manager(num_pages=16, page=4, max_seqs=8, needs=None):
+    from rvllm_b200.cache import CacheManager
+    from rvllm_b200.parts import KvCacheNeed
+    return CacheManager(needs or {0: KvCacheNeed(2, 16, None), 1: KvCacheNeed(1, 16, None)}, num_pages, page, max_seqs, torch.float32, "cpu", allocate=False)
+
+
+def test_a_shared_page_is_free_when_its_last_holder_gives_it_back():
+    from rvllm_b200 import SchedulerError
+    m = manager()
+    m.admit("a"); m.append("a", 10)
+    m.admit("b"); m.share("b", "a", 8)
+    assert m.num_tokens("b") == 8 and m.append("b", 3) == 8
+    assert m.block_table("b", 0)[:2] == m.block_table("a", 0)[:2] and m.block_table("b", 1)[2] != m.block_table("a", 1)[2]
+    assert m.num_free_pages() == [12, 12]
+    m.check()
+    m.admit("c"); m.share("c", "b", 8)
+    m.free("a")
+    m.check()
+    assert m.num_free_pages() == [13, 13]
+    m.free("c"); m.check()
+    assert m.num_free_pages() == [13, 13]
+    with pytest.raises(SchedulerError, match="held by"):
+        m.groups[0].pool.release([m.block_table("b", 0)[0]], "a")
+    m.free("b"); m.check()
+    assert m.num_free_pages() == [16, 16]
+
+
+def test_what_cannot_be_shared_is_refused():
+    from rvllm_b200 import SchedulerError
+    from rvllm_b200.parts import KvCacheNeed, StateNeed
+    m = manager()
+    m.admit("a"); m.append("a", 10); m.admit("b")
+    for n in (0, 3, 12, -4):
+        with pytest.raises(SchedulerError):
+            m.share("b", "a", n)
+    m.append("b", 1)
+    with pytest.raises(SchedulerError, match="has tokens"):
+        m.share("b", "a", 4)
+    m.check()
+    pool = m.groups[0].pool
+    with pytest.raises(SchedulerError, match="not held"):
+        pool.share([15], "b")
+    with pytest.raises(SchedulerError, match="already"):
+        pool.share([m.block_table("a", 0)[0]], "a")
+    for needs in ({0: KvCacheNeed(2, 16, 20)}, {0: KvCacheNeed(2, 16, None), 1: StateNeed((4,))}, {0: KvCacheNeed(2, 16, None, chunk=8)}, {0: StateNeed((4,))}):
+        w = manager(needs=needs)
+        w.admit("a"); w.append("a", 8); w.admit("b")
+        assert not w.can_share and w.shared_groups(["a", "b"]) == []
+        with pytest.raises(SchedulerError):
+            w.share("b", "a", 4)
+
+
+def test_groups_that_save_the_most():
+    m = manager(num_pages=400, page=4, max_seqs=20)
+    m.admit("root"); m.append("root", 8)
+    # two sets of four that share 100 tokens each, all of them 8; and two that share nothing
+    for s in "xy":
+        m.admit(s + "0"); m.share(s + "0", "root", 8); m.append(s + "0", 92 + 3)
+        for i in (1, 2, 3):
+            m.admit(s + str(i)); m.share(s + str(i), s + "0", 100); m.append(s + str(i), i)
+    m.admit("p"); m.append("p", 9); m.admit("q"); m.append("q", 9)
+    names = ["p", "x1", "y3", "x0", "q", "y0", "x3", "y2", "x2", "y1"]
+    groups = {tuple(sorted(names[i] for i in ms)): t for ms, t in m.shared_groups(names)}
+    assert groups == {("x0", "x1", "x2", "x3"): 100, ("y0", "y1", "y2", "y3"): 100}
+    # of six that share 8 tokens, two share 8 more: the six are worth more
+    m2 = manager(num_pages=100)
+    m2.admit("a"); m2.append("a", 20)
+    for i in range(4):
+        m2.admit(i); m2.share(i, "a", 8); m2.append(i, 2)
+    m2.admit("b"); m2.share("b", "a", 16); m2.append("b", 1)
+    assert [(sorted(map(str, (["a", 0, 1, 2, 3, "b"][i] for i in ms))), t) for ms, t in m2.shared_groups(["a", 0, 1, 2, 3, "b"])] == \
+        [(["0", "1", "2", "3", "a", "b"], 8)]
+    assert m2.shared_groups(["a"]) == [] and m2.shared_groups([]) == []
+
+
+# ------------------------------------------------------------------------------------------------------------- scheduling
+def scheduler(num_pages=64, page=4, max_seqs=8, budget=64, chunk=None, chunked=True, share=True, max_len=256):
+    from rvllm_b200.cache import CacheManager
+    from rvllm_b200.engine import Scheduler
+    from rvllm_b200.parts import KvCacheNeed
+    cache = CacheManager({0: KvCacheNeed(1, 16, None)}, num_pages, page, max_seqs, allocate=False)
+    return cache, Scheduler(cache, max_seqs, budget, max_len, chunk, chunked, (), share_prefixes=share)
+
+
+def run_step(cache, sched):
+    batch = sched.schedule()
+    for e in batch.entries:
+        cache.append(e.request.req_id, e.num_tokens)
+        assert cache.num_tokens(e.request.req_id) == e.start + e.num_tokens
+    done = sched.update(batch, {e.request.req_id: 1000 + 7 * hash(e.request.req_id) % 50 + len(e.request.output) for e in batch.entries if e.samples})
+    cache.check()
+    return batch, done
+
+
+def request(rid, prompt, max_tokens=4):
+    from rvllm_b200 import SamplingParams
+    from rvllm_b200.engine import Request
+    return Request(rid, list(prompt), SamplingParams(max_tokens=max_tokens))
+
+
+def shape(batch):
+    return [(e.request.req_id, e.start, e.num_tokens, e.samples) for e in batch.entries]
+
+
+def test_a_request_starts_behind_what_another_has_computed():
+    cache, s = scheduler()
+    s.add_request(request("a", range(30)))
+    run_step(cache, s)
+    s.add_request(request("b", list(range(22)) + [99] * 5))
+    s.add_request(request("c", range(30)))                     # the same prompt: its last token is its own
+    s.add_request(request("d", [7] * 10))
+    b, _ = run_step(cache, s)
+    assert shape(b) == [("a", 30, 1, True), ("b", 20, 7, True), ("c", 28, 2, True), ("d", 0, 10, True)]
+    assert cache.block_table("b", 0)[:5] == cache.block_table("a", 0)[:5] and cache.block_table("c", 0)[:7] == cache.block_table("a", 0)[:7]
+    while s.has_unfinished():
+        run_step(cache, s)
+    assert cache.num_free_pages() == [64]
+
+
+def test_samples_of_one_prompt_wait_for_the_first_and_others_pass():
+    cache, s = scheduler(budget=16, chunk=16)
+    for i in range(3):
+        s.add_request(request(i, range(40)))
+    s.add_request(request("x", [5] * 6))
+    got = [shape(run_step(cache, s)[0]) for _ in range(4)]
+    # the first is computed in portions; the others are admitted when all but 4 pages of what they share is there
+    assert got[0] == [(0, 0, 16, False)] and got[1][0] == (0, 16, 16, False)
+    assert any(e[0] == "x" for g in got[:4] for e in g) or any(e[0] == "x" for e in shape(run_step(cache, s)[0]))
+    seen = {}
+    while s.has_unfinished():
+        b, _ = run_step(cache, s)
+        for e in b.entries:
+            seen.setdefault(e.request.req_id, e.start)
+    for g in got:
+        for rid, start, _, _ in g:
+            seen[rid] = min(seen.get(rid, start), start)
+    assert seen[1] >= 24 and seen[2] >= 24
+    assert cache.num_free_pages() == [64]
+
+
+def test_without_the_option_nothing_is_shared():
+    cache, s = scheduler(share=False)
+    for i in range(3):
+        s.add_request(request(i, range(20)))
+    b, _ = run_step(cache, s)
+    assert shape(b) == [(0, 0, 20, True), (1, 0, 20, True), (2, 0, 20, True)]
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_no_page_is_lost_under_random_arrivals_and_preemption(seed):
+    rng = random.Random(seed)
+    cache, s = scheduler(num_pages=rng.randint(22, 40), max_seqs=6, budget=rng.choice((8, 16, 40)), chunk=rng.choice((None, 7)), max_len=80)
+    stems = [[rng.randint(0, 9) for _ in range(rng.randint(4, 40))] for _ in range(3)]
+    todo = [request(i, rng.choice(stems)[:rng.randint(1, 40)] + [rng.randint(0, 9) for _ in range(rng.randint(1, 6))], rng.randint(1, 30)) for i in range(20)]
+    reqs, steps, shared = list(todo), 0, 0
+    while todo or s.has_unfinished():
+        while todo and rng.random() < 0.5:
+            s.add_request(todo.pop())
+        if not s.has_unfinished():
+            continue
+        run_step(cache, s)
+        shared += sum(r.shared_tokens for r in s.running)
+        steps += 1
+        if rng.random() < 0.03 and s.running:
+            s.abort(rng.choice(s.running).req_id)
+            cache.check()
+        assert steps < 3000
+    assert cache.num_free_pages() == [cache.num_pages] and shared > 0
+    for r in reqs:
+        assert r.finish_reason == "abort" or len(r.output) == r.params.max_tokens
+
+
+def test_samples_per_prompt():
+    from rvllm_b200 import SamplingError, SamplingParams
+    assert SamplingParams().n == 1
+    with pytest.raises(SamplingError):
+        SamplingParams(n=0)
