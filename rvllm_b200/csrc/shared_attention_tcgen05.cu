@@ -151,6 +151,10 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
     const int t_begin = key_lo / KV_TILE, n_it = (key_hi + KV_TILE - 1) / KV_TILE - t_begin;
     const int* table = p.block_tables + (size_t)tile.table_seq * p.max_blocks;
 
+    // a softmax thread's row (its lane of tensor memory), and the sequence that it belongs to
+    const int row = warp * 32 + lane;
+    const bool in_range = warp < SOFTMAX_WARPS && row < tile_rows;
+    const int my_seq = in_range ? p.plan.member(tile.first + row / G) : -1;
     if (tid == 0) {
         abort_flag = 0;
         mbar_init(bar_q, SOFTMAX_WARPS);
@@ -272,27 +276,21 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
     } else {
         // ------------------------------------------------------------ softmax warps: one thread per row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
-        const int row = warp * 32 + lane;                            // row of the tile = lane of tensor memory
         const bool rows_here = warp * 32 < tile_rows;                // (a warp without rows only hands its buffers on)
-        const bool in_range = row < tile_rows;
         // The rows' queries, 16 bytes a lane, to their places in the 128-byte swizzle; rows without a sequence are zeros.  A warp fetches
-        // its own 32 rows, eight loads at a time (which sequence a row belongs to, the lane of the row has looked up).
+        // its own 32 rows, all loads at a time.
         constexpr int LANES = HEAD_DIM / 8;                          // that bring a row
-        const int my_seq = in_range ? p.plan.member(tile.first + row / G) : -1;
         const int my_row = in_range ? my_seq * p.nh + kvh * G + row % G : -1;
+        uint4 qv[LANES];
 #pragma unroll
-        for (int i0 = 0; i0 < LANES; i0 += 8) {
-            uint4 v[8];
+        for (int i = 0; i < LANES; ++i) {
+            const int from = __shfl_sync(0xffffffffu, my_row, i * (32 / LANES) + lane / LANES);
+            qv[i] = from >= 0 ? *reinterpret_cast<const uint4*>(p.q + (size_t)from * HEAD_DIM + (lane % LANES) * 8) : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int from = __shfl_sync(0xffffffffu, my_row, (i0 + i) * (32 / LANES) + lane / LANES);
-                v[i] = from >= 0 ? *reinterpret_cast<const uint4*>(p.q + (size_t)from * HEAD_DIM + (lane % LANES) * 8) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = warp * 32 + (i0 + i) * (32 / LANES) + lane / LANES, chunk = lane % LANES;
-                *reinterpret_cast<uint4*>(q_s + (chunk >> 3) * (ROWS * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = v[i];
-            }
+        for (int i = 0; i < LANES; ++i) {
+            const int r = warp * 32 + i * (32 / LANES) + lane / LANES, chunk = lane % LANES;
+            *reinterpret_cast<uint4*>(q_s + (chunk >> 3) * (ROWS * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = qv[i];
         }
         fence_async_smem();
         __syncwarp();
@@ -463,14 +461,15 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
 #define OWN_WARPS 4
 #define OWN_THREADS (32 * OWN_WARPS)
 #define OWN_CHUNK 16                           // keys
-#define OWN_STAGES 2                           // of a warp; two CTAs an SM have 8 warps x 2 x 8 KB on their way (head size 128)
+#define OWN_STAGES 2                           // of a warp; two CTAs an SM have 8 warps x 2 x 8 KB on their way (head size 128; three: no faster)
 #define DIM_BLOCKS (HEAD_DIM / 16)
-#define SLAB_BYTES (OWN_CHUNK * 128)           // 64 columns of a chunk
-#define CHUNK_BYTES (HALVES * SLAB_BYTES)
+#define KEY_BYTES (HEAD_DIM * 2)               // a key, or a value, in shared memory: HALVES rows of 128 bytes
 #define QUERY_BYTES (8 * HEAD_DIM * 2)
-#define STAGE_BYTES (2 * CHUNK_BYTES + QUERY_BYTES)                        // keys, values, the piece's queries (with its first chunk)
-#define MERGE_BATCH 12
-#define MAX_SEQS 4096                          // of a step: what the list of pieces has room for
+#define STAGE_BYTES (2 * OWN_CHUNK * KEY_BYTES)                            // of a box (a page, or the 16 keys of it): its keys, then its values
+#define RING_BYTES (OWN_STAGES * STAGE_BYTES + QUERY_BYTES)                // of a warp; the queries come with a piece's first chunk
+#define MERGE_BATCH 8
+#define MERGE_BLOCKS 7                         // of an SM
+#define MAX_SEQS 2048                          // of a step: what the list of pieces has room for
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -492,9 +491,14 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
+}
+
 // A warp's place in the list of pieces: which piece, and which chunk of it comes next.
 struct OwnCursor {
-    long long at;                  // piece x block of heads, in the whole list
+    unsigned at;                   // piece x block of heads, in the whole list
     int seq, rank, kvh, head0;
     int chunk, chunk_end, ctx, start;
     bool first;                    // no chunk of the piece has been asked for yet
@@ -510,11 +514,13 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
     if (warp == OWN_WARPS) asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     if (warp >= OWN_WARPS) return;
     const int G = p.nh / p.nkv, blocks = p.nkv * p.head_blocks;
-    unsigned char* ring = smem + warp * (OWN_STAGES * STAGE_BYTES);        // (stages start on 1,024-byte boundaries: see the swizzle)
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OWN_WARPS * OWN_STAGES * STAGE_BYTES);
+    unsigned char* ring = smem + warp * RING_BYTES;                        // (stages start on 1,024-byte boundaries: see the swizzle)
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OWN_WARPS * RING_BYTES);
     int* of_warp = reinterpret_cast<int*>(bars + OWN_WARPS * OWN_STAGES);
     volatile int& abort_flag = *reinterpret_cast<volatile int*>(of_warp + OWN_WARPS);
     int* before = of_warp + OWN_WARPS + 1;                                 // [num_seqs + 1]: pieces of the sequences before one
+    int* ends = before + p.num_seqs + 1;                                   // [num_seqs]: context lengths
+    int* begins = ends + p.num_seqs;                                       // [num_seqs]: first own keys
     const uint32_t bar0 = smem_u32(bars + warp * OWN_STAGES);
     if (tid == 0) abort_flag = 0;
     if (lane == 0) {
@@ -525,9 +531,9 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
     const int each = (p.num_seqs + OWN_THREADS - 1) / OWN_THREADS, s_lo = min(tid * each, p.num_seqs), s_hi = min(s_lo + each, p.num_seqs);
     int mine = 0;
     for (int s = s_lo; s < s_hi; ++s) {
-        const int ctx = max(p.ctx_lens[s], 0);
-        before[s] = mine;
-        mine += pieces_of(ctx - min(p.plan.own_start(s), ctx), p.piece, p.pieces);
+        const int ctx = max(p.ctx_lens[s], 0), start = min(p.plan.own_start(s), ctx);
+        before[s] = mine; ends[s] = ctx; begins[s] = start;
+        mine += pieces_of(ctx - start, p.piece, p.pieces);
     }
     int upto = mine;
 #pragma unroll
@@ -548,10 +554,10 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
     asm volatile("bar.sync 1, %0;" ::"n"(OWN_THREADS) : "memory");
 
     const int warps = ((int)gridDim.x - p.prefix_ctas) * OWN_WARPS;
-    const long long all = (long long)total * blocks;
+    const unsigned all = (unsigned)total * blocks;
     auto enter = [&](OwnCursor& c) {                 // the piece at c.at
         if (c.at >= all) return;
-        const int piece = (int)(c.at / blocks), block = (int)(c.at - (long long)piece * blocks);
+        const int piece = (int)(c.at / (unsigned)blocks), block = (int)c.at - piece * blocks;
         int seq = 0;
         for (int hi = p.num_seqs - 1; seq < hi;) {                         // the last sequence that begins at or before it
             const int mid = (seq + hi + 1) >> 1;
@@ -561,8 +567,8 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
         c.rank = piece - before[seq];
         c.kvh = block / p.head_blocks;
         c.head0 = (block - c.kvh * p.head_blocks) * 8;
-        c.ctx = max(p.ctx_lens[seq], 0);
-        c.start = min(p.plan.own_start(seq), c.ctx);
+        c.ctx = ends[seq];
+        c.start = begins[seq];
         const int pieces = before[seq + 1] - before[seq];
         const int lo = c.start / OWN_CHUNK, chunks = (c.ctx + OWN_CHUNK - 1) / OWN_CHUNK - lo, per = (chunks + pieces - 1) / pieces;
         c.chunk = min(lo + c.rank * per, lo + chunks);
@@ -574,153 +580,167 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
         if (++c.chunk >= c.chunk_end) { c.at += warps; enter(c); }
     };
     const int box_keys = p.page_size < OWN_CHUNK ? p.page_size : OWN_CHUNK, boxes = OWN_CHUNK / box_keys;
-    // Lane i < boxes has the i-th box of a chunk's keys, lane 16 + i that of its values.  Its page is looked up when the chunk before has
-    // been asked for, and looked at when the copy is.
+    const int box_bytes = 2 * box_keys * KEY_BYTES;
+    // Lane i < boxes has the i-th box of a chunk, keys and values in one copy.  Its page is looked up when the chunk before has been
+    // asked for, and looked at when the copy is.
     auto look_up = [&](OwnCursor& c) {
-        const int key = c.chunk * OWN_CHUNK + (lane & 15) * box_keys;
+        const int key = c.chunk * OWN_CHUNK + lane * box_keys;
         c.page = -1;
-        if (c.at < all && (lane & 15) < boxes && c.chunk < c.chunk_end && key < c.ctx && key + box_keys > c.start && (key >> p.page_shift) < p.max_blocks)
+        if (c.at < all && lane < boxes && c.chunk < c.chunk_end && key < c.ctx && key + box_keys > c.start && (key >> p.page_shift) < p.max_blocks)
             c.page = __ldg(p.block_tables + (size_t)c.seq * p.max_blocks + (key >> p.page_shift));
     };
-    auto ask = [&](const OwnCursor& c, int stage) {
-        const int which = lane >> 4, key = c.chunk * OWN_CHUNK + (lane & 15) * box_keys;
+    auto ask = [&](const OwnCursor& c, int stage) -> unsigned {
         const int page = c.page < p.num_pages ? c.page : -1;
         const unsigned mask = __ballot_sync(0xffffffffu, page >= 0);
-        const uint32_t bar = bar0 + 8 * stage, to = smem_u32(ring) + stage * STAGE_BYTES;
-        const int heads = min(8, G - c.head0);
+        const uint32_t bar = bar0 + 8 * stage;
+        const uint32_t query_bytes = c.first ? (uint32_t)min(8, G - c.head0) * HD * 2u : 0u;
         if (lane == 0) {
-            mbar_expect_tx(bar, (uint32_t)__popc(mask) * HALVES * (uint32_t)box_keys * 128u + (c.first ? (uint32_t)heads * HD * 2u : 0u));
-            if (c.first) bulk_load(to + 2 * CHUNK_BYTES, p.q + ((size_t)c.seq * p.nh + c.kvh * G + c.head0) * HD, (uint32_t)heads * HD * 2u, bar);
+            mbar_expect_tx(bar, (uint32_t)__popc(mask) * (uint32_t)box_bytes + query_bytes);
+            if (c.first) bulk_load(smem_u32(ring) + OWN_STAGES * STAGE_BYTES, p.q + ((size_t)c.seq * p.nh + c.kvh * G + c.head0) * HD, query_bytes, bar);
         }
         __syncwarp();
-        if (page >= 0) {
-            const int row = ((page * 2 + which) * p.nkv + c.kvh) * p.page_size + (key & (p.page_size - 1));
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h)
-                tma_load_2d(to + which * CHUNK_BYTES + h * SLAB_BYTES + (lane & 15) * box_keys * 128, &map, h * 64, row, bar);
-        }
-        return mask & 0xffffu;                       // the boxes of keys that come
+        if (page >= 0)
+            tma_load_4d(smem_u32(ring) + stage * STAGE_BYTES + lane * box_bytes, &map, 0, 0,
+                        c.kvh * p.page_size + ((c.chunk * OWN_CHUNK + lane * box_keys) & (p.page_size - 1)), 2 * page, bar);
+        return mask;                                 // the boxes that come
     };
+    // where key r of a chunk is in its stage (its value lies box_bytes / 2 further)
+    auto key_at = [&](int r) { return (r / box_keys) * box_bytes + (r % box_keys) * KEY_BYTES; };
 
-    OwnCursor ahead, now;
+    OwnCursor ahead, now, pending;
     ahead.at = now.at = cta * OWN_WARPS + warp;
     enter(ahead);
-    now = ahead;
+    now = pending = ahead;
     look_up(ahead);
-    unsigned here[OWN_STAGES];                       // which boxes of a stage have keys
+    unsigned here = 0;                               // which boxes of a stage have keys, two bits a stage
     int asked = 0, taken = 0;
-#pragma unroll
-    for (int i = 0; i < OWN_STAGES; ++i)
-        if (ahead.at < all) { here[i] = ask(ahead, i); ++asked; next(ahead); look_up(ahead); }
+    bool queries = false;                            // those of a piece are on their way, or lie there unread: one piece's at a time
+    auto ask_ahead = [&]() {
+        while (ahead.at < all && asked - taken < OWN_STAGES && !(ahead.first && queries)) {
+            const int stage = asked % OWN_STAGES;
+            here = (here & ~(3u << (2 * stage))) | ask(ahead, stage) << (2 * stage);
+            if (ahead.first) { queries = true; pending = ahead; }
+            ++asked;
+            next(ahead);
+            look_up(ahead);
+        }
+    };
+    ask_ahead();
     const int g = lane >> 2, tq = lane & 3;
     uint32_t qf[DIM_BLOCKS][2];
     float o[DIM_BLOCKS][4], m_run[2], l_run[2];      // heads 2 tq, 2 tq + 1
     bool ok = true;
-    while (now.at < all && ok) {
+    // a lane's row of the keys and of the values as ldmatrix takes them: its place in a stage, the eight columns it names
+    const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_half = lane >> 4, v_row = (lane & 7) + (lane >> 4) * 8, v_half = (lane >> 3) & 1;
+    const uint32_t k_at = key_at(k_row), v_at = key_at(v_row) + box_bytes / 2;
+    auto column = [](uint32_t row, int i, int half) {                      // of 16 i + 8 half, in the 128-byte swizzle
+        const uint32_t line = row + (i >> 2) * 128;
+        return line + (((2 * (i & 3) + half) ^ ((line >> 7) & 7)) << 4);
+    };
+    bool fresh = true;                               // the next chunk is the first of a piece
+    while (taken < asked) {
+        const int stage = taken % OWN_STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, (taken / OWN_STAGES) & 1, &abort_flag, 14))) { ok = false; break; }
+        const uint32_t at = smem_u32(ring) + stage * STAGE_BYTES;
+        if (fresh) {
+            now = pending;
+            // Q as the B operand: elements 2 tq, 2 tq + 1 (and 8 on) of head g in every 16; heads beyond the block are zeros
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(ring + OWN_STAGES * STAGE_BYTES) + g * (HD / 2) + tq;
+            const bool have = g < G - now.head0;
 #pragma unroll
-        for (int stage = 0; stage < OWN_STAGES; ++stage) {
-            if (now.at >= all) break;
-            if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, (taken / OWN_STAGES) & 1, &abort_flag, 14))) { ok = false; break; }
-            ++taken;
-            const uint32_t ks = smem_u32(ring) + stage * STAGE_BYTES, vs = ks + CHUNK_BYTES;
-            if (now.first) {
-                // Q as the B operand: elements 2 tq, 2 tq + 1 (and 8 on) of head g in every 16; heads beyond the block are zeros
-                const uint32_t* q = reinterpret_cast<const uint32_t*>(ring + stage * STAGE_BYTES + 2 * CHUNK_BYTES) + g * (HD / 2) + tq;
-                const bool have = g < G - now.head0;
-#pragma unroll
-                for (int i = 0; i < DIM_BLOCKS; ++i) {
-                    qf[i][0] = have ? q[8 * i] : 0u;
-                    qf[i][1] = have ? q[8 * i + 4] : 0u;
-                    o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-                }
-                m_run[0] = m_run[1] = -INFINITY;
-                l_run[0] = l_run[1] = 0.f;
+            for (int i = 0; i < DIM_BLOCKS; ++i) {
+                qf[i][0] = have ? q[8 * i] : 0u;
+                qf[i][1] = have ? q[8 * i + 4] : 0u;
+                o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
             }
-            // which of the chunk's keys there are, a bit each
-            const int key0 = now.chunk * OWN_CHUNK;
-            unsigned see = 0;
-            if (now.chunk < now.chunk_end) {
-                const int lo = max(now.start - key0, 0), hi = min(now.ctx - key0, OWN_CHUNK);
-                see = hi > lo ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
-                if (here[stage] != (1u << boxes) - 1u)
-                    for (int i = 0; i < boxes; ++i)
-                        if (!(here[stage] >> i & 1u)) see &= ~(((1u << box_keys) - 1u) << (i * box_keys));
+            m_run[0] = m_run[1] = -INFINITY;
+            l_run[0] = l_run[1] = 0.f;
+            queries = false;
+        }
+        // which of the chunk's keys there are, a bit each
+        const int key0 = now.chunk * OWN_CHUNK;
+        unsigned see = 0;
+        if (now.chunk < now.chunk_end) {
+            const int lo = max(now.start - key0, 0), hi = min(now.ctx - key0, OWN_CHUNK);
+            see = hi > lo ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
+            const unsigned got = here >> (2 * stage) & 3u;
+            if (got != (1u << boxes) - 1u)
+                for (int i = 0; i < boxes; ++i)
+                    if (!(got >> i & 1u)) see &= ~(((1u << box_keys) - 1u) << (i * box_keys));
+        }
+        if (see != 0xffffu) {
+            // values of keys that are not there: zeros, so that what an earlier request left, a NaN for instance, does not meet a
+            // probability of zero
+            if (!(see >> (lane >> 1) & 1u)) {
+                unsigned char* to = ring + stage * STAGE_BYTES + key_at(lane >> 1) + box_bytes / 2 + (lane & 1) * (KEY_BYTES / 2);
+#pragma unroll
+                for (int i = 0; i < KEY_BYTES / 32; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(0, 0, 0, 0);
             }
-            if (see != 0xffffu) {
-                // values of keys that are not there: zeros, so that what an earlier request left, a NaN for instance, does not meet a
-                // probability of zero
-                if (!(see >> (lane >> 1) & 1u)) {
-                    unsigned char* row = ring + stage * STAGE_BYTES + CHUNK_BYTES + (lane >> 1) * 128 + (lane & 1) * 64;
+            fence_async_smem();                      // (the next copy into the stage comes behind these writes)
+            __syncwarp();
+        }
+        if (see) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < 4 * HALVES; ++i)
-                        *reinterpret_cast<uint4*>(row + (i >> 2) * SLAB_BYTES + (i & 3) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_async_smem();                  // (the next copy into the stage comes behind these writes)
-                __syncwarp();
+            for (int i = 0; i < DIM_BLOCKS; ++i) {
+                uint32_t a[4];
+                ldmatrix_4(a, at + column(k_at, i, k_half));
+                mma_16816(s, a, qf[i][0], qf[i][1]);
             }
-            if (see) {
-                float s[4] = {0.f, 0.f, 0.f, 0.f};
-                const int r = (lane & 7) + ((lane >> 3) & 1) * 8, half = lane >> 4;
+            float alpha[2];
 #pragma unroll
-                for (int i = 0; i < DIM_BLOCKS; ++i) {                     // keys r, 8 columns at 16 i + 8 half
-                    uint32_t a[4];
-                    ldmatrix_4(a, ks + (i >> 2) * SLAB_BYTES + r * 128 + (((2 * (i & 3) + half) ^ (r & 7)) << 4));
-                    mma_16816(s, a, qf[i][0], qf[i][1]);
+            for (int e = 0; e < 4; ++e) {                                  // e: key g + 8 (e >> 1), head 2 tq + (e & 1)
+                float v = s[e] * p.scale_log2e;
+                if (p.cap_log2e > 0.f) {
+                    const float x = fast_exp2(s[e] * p.scale_over_cap * 2.885390081777927f);
+                    v = p.cap_log2e * (1.f - __fdividef(2.f, x + 1.f));
                 }
-                float alpha[2];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {                              // e: key g + 8 (e >> 1), head 2 tq + (e & 1)
-                    float v = s[e] * p.scale_log2e;
-                    if (p.cap_log2e > 0.f) {
-                        const float x = fast_exp2(s[e] * p.scale_over_cap * 2.885390081777927f);
-                        v = p.cap_log2e * (1.f - __fdividef(2.f, x + 1.f));
-                    }
-                    s[e] = see >> (g + 8 * (e >> 1)) & 1u ? v : -INFINITY;
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float mx = fmaxf(s[h], s[h + 2]);
-#pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                    const float m_new = fmaxf(m_run[h], mx);
-                    const float m_s = m_new == -INFINITY ? 0.f : m_new;
-                    alpha[h] = fast_exp2(m_run[h] - m_s);                  // 0 while nothing has been seen
-                    m_run[h] = m_new;
-                    s[h] = fast_exp2(s[h] - m_s);
-                    s[h + 2] = fast_exp2(s[h + 2] - m_s);
-                    l_run[h] = l_run[h] * alpha[h] + s[h] + s[h + 2];      // this lane's keys; the lanes are added at the end
-                }
-                const __nv_bfloat162 lo2 = __floats2bfloat162_rn(s[0], s[1]), hi2 = __floats2bfloat162_rn(s[2], s[3]);
-                const uint32_t p0 = transpose_8x8(*reinterpret_cast<const uint32_t*>(&lo2));     // keys 2 tq, 2 tq + 1 of head g
-                const uint32_t p1 = transpose_8x8(*reinterpret_cast<const uint32_t*>(&hi2));     // ... + 8
-                const int vr = (lane & 7) + (lane >> 4) * 8, vhalf = (lane >> 3) & 1;
-#pragma unroll
-                for (int i = 0; i < DIM_BLOCKS; ++i) {                     // columns 16 i + g and 8 on
-                    o[i][0] *= alpha[0]; o[i][1] *= alpha[1];
-                    o[i][2] *= alpha[0]; o[i][3] *= alpha[1];
-                    uint32_t a[4];
-                    ldmatrix_4t(a, vs + (i >> 2) * SLAB_BYTES + vr * 128 + (((2 * (i & 3) + vhalf) ^ (vr & 7)) << 4));
-                    mma_16816(o[i], a, p0, p1);
-                }
+                s[e] = see >> (g + 8 * (e >> 1)) & 1u ? v : -INFINITY;
             }
-            __syncwarp();                            // the stage has been read
-            if (ahead.at < all) { here[stage] = ask(ahead, stage); ++asked; next(ahead); look_up(ahead); }
-            if (now.chunk + 1 >= now.chunk_end) {    // the piece's last chunk
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float l = l_run[h];
+            for (int h = 0; h < 2; ++h) {
+                float mx = fmaxf(s[h], s[h + 2]);
 #pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-                    const int head = now.head0 + 2 * tq + h;
-                    if (head >= G) continue;
-                    const size_t row = ((size_t)now.rank * p.num_seqs + now.seq) * p.nh + now.kvh * G + head;
-                    if (g == 0) *reinterpret_cast<float2*>(p.own_ml + row * 2) = make_float2(m_run[h], l);
-                    float* to = p.own_o + row * HD + g;
-#pragma unroll
-                    for (int i = 0; i < DIM_BLOCKS; ++i) { to[16 * i] = o[i][h]; to[16 * i + 8] = o[i][h + 2]; }
-                }
+                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                const float m_new = fmaxf(m_run[h], mx);
+                const float m_s = m_new == -INFINITY ? 0.f : m_new;
+                alpha[h] = fast_exp2(m_run[h] - m_s);                      // 0 while nothing has been seen
+                m_run[h] = m_new;
+                s[h] = fast_exp2(s[h] - m_s);
+                s[h + 2] = fast_exp2(s[h + 2] - m_s);
+                l_run[h] = l_run[h] * alpha[h] + s[h] + s[h + 2];          // this lane's keys; the lanes are added at the end
             }
-            next(now);
+            const __nv_bfloat162 lo2 = __floats2bfloat162_rn(s[0], s[1]), hi2 = __floats2bfloat162_rn(s[2], s[3]);
+            const uint32_t p0 = transpose_8x8(*reinterpret_cast<const uint32_t*>(&lo2));         // keys 2 tq, 2 tq + 1 of head g
+            const uint32_t p1 = transpose_8x8(*reinterpret_cast<const uint32_t*>(&hi2));         // ... + 8
+#pragma unroll
+            for (int i = 0; i < DIM_BLOCKS; ++i) {                         // columns 16 i + g and 8 on
+                o[i][0] *= alpha[0]; o[i][1] *= alpha[1];
+                o[i][2] *= alpha[0]; o[i][3] *= alpha[1];
+                uint32_t a[4];
+                ldmatrix_4t(a, at + column(v_at, i, v_half));
+                mma_16816(o[i], a, p0, p1);
+            }
+        }
+        __syncwarp();                                // the stage has been read, and so have a first chunk's queries
+        ++taken;
+        ask_ahead();
+        fresh = now.chunk + 1 >= now.chunk_end;
+        ++now.chunk;
+        if (fresh) {                                 // that was the piece's last chunk
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float l = l_run[h];
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+                const int head = now.head0 + 2 * tq + h;
+                if (head >= G) continue;
+                const size_t to_row = ((size_t)now.rank * p.num_seqs + now.seq) * p.nh + now.kvh * G + head;
+                if (g == 0) *reinterpret_cast<float2*>(p.own_ml + to_row * 2) = make_float2(m_run[h], l);
+                float* to = p.own_o + to_row * HD + g;
+#pragma unroll
+                for (int i = 0; i < DIM_BLOCKS; ++i) { to[16 * i] = o[i][h]; to[16 * i + 8] = o[i][h + 2]; }
+            }
         }
     }
     // A wait gave up: copies may still be on their way into this CTA's shared memory.  Waited for (bounded) before it is given up.
@@ -733,10 +753,10 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
 
 // ---------------------------------------------------------------------------------------------
 // The sums of a row put together: WARPS warps per (sequence, head), which take its parts in turn, four neighbouring columns a lane
-// and MERGE_BATCH parts' loads in flight.  What it costs is round trips to L2 - a row of 45 parts takes one warp four - and waves of
-// blocks, five of which fit an SM: so as many warps a row as still leave one wave.
+// and MERGE_BATCH parts' loads in flight.  What it costs is round trips to L2 - a row of 45 parts takes one warp six - and waves of
+// blocks: so as many warps a row as still leave one wave.
 template <int WARPS>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, MERGE_BLOCKS)
 shared_merge_kernel(const SharedParams p, const float* __restrict__ sinks, const float* __restrict__ gate, __nv_bfloat16* __restrict__ out) {
     rv_pdl_launch_dependents();
     constexpr int LANES = HEAD_DIM / 4;              // that hold a row
@@ -797,6 +817,20 @@ shared_merge_kernel(const SharedParams p, const float* __restrict__ sinks, const
 }
 
 // ---------------------------------------------------------------- host side
+// A cache layer as [planes of all pages][rows of a plane][64-element parts of a row][64]: a box brings some keys of a page and head
+// and their values, in 128-byte rows with 128-byte swizzle.
+static int make_own_map(CUtensorMap* map, const void* cache, long long num_pages, int nkv, int page_size) {
+    RvEncodeTiledFn fn = rv_encode_fn();
+    if (!fn) return RV_ERR_UNSUPPORTED;
+    const cuuint64_t dims[4] = {64, HALVES, (cuuint64_t)nkv * page_size, (cuuint64_t)num_pages * 2};
+    const cuuint64_t strides[3] = {128, KEY_BYTES, (cuuint64_t)nkv * page_size * KEY_BYTES};
+    const cuuint32_t box[4] = {64, HALVES, (cuuint32_t)(page_size < OWN_CHUNK ? page_size : OWN_CHUNK), 2};
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(cache), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? RV_OK : RV_ERR_BAD_SIZE;
+}
+
 // The arguments, packed by the caller in this order (a step makes this call once a layer).
 struct SharedArgs {
     const void* q; const void* cache; const int* block_tables; const int* ctx_lens; const int* plan;
@@ -821,7 +855,7 @@ RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     const int head_blocks = (G + 7) / 8;
     const long long prefix_ctas = (long long)nkv * a->cap_items;
     if (a->num_pages > 0x7fffffffLL / 2 / nkv / page_size || prefix_ctas + a->own_ctas > 0x7fffffffLL || (long long)a->num_seqs * nh > 0x7fffffffLL ||
-        (long long)a->num_seqs * a->pieces > 0x7fffffffLL || a->num_seqs > MAX_SEQS)
+        (long long)a->num_seqs * a->pieces > 0x7fffffffLL / (nkv * head_blocks) || a->num_seqs > MAX_SEQS)
         return RV_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->cache) | reinterpret_cast<uintptr_t>(a->pre_o) |
          reinterpret_cast<uintptr_t>(a->own_o) | reinterpret_cast<uintptr_t>(a->plan) | reinterpret_cast<uintptr_t>(a->out)) % 16 ||
@@ -830,8 +864,7 @@ RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     if (a->num_seqs == 0) return RV_OK;
     alignas(64) CUtensorMap map_kv, map_own;
     int st = rv_make_bf16_map(&map_kv, a->cache, a->num_pages * 2 * nkv * page_size, HEAD_DIM, page_size < KV_TILE ? page_size : KV_TILE);
-    if (page_size <= OWN_CHUNK) map_own = map_kv;        // (boxes of a page)
-    else if (st == RV_OK) st = rv_make_bf16_map(&map_own, a->cache, a->num_pages * 2 * nkv * page_size, HEAD_DIM, OWN_CHUNK);
+    if (st == RV_OK) st = make_own_map(&map_own, a->cache, a->num_pages, nkv, page_size);
     if (st != RV_OK) return st;
     SharedParams p;
     p.plan = shared_plan(a->plan, a->num_seqs, a->cap_tiles);
@@ -845,14 +878,14 @@ RV_EXPORT int rv_shared_attention_tcgen05(const SharedArgs* a) {
     p.cap_log2e = a->softcap > 0.f ? a->softcap * 1.4426950408889634f : 0.f;
     p.scale_over_cap = a->softcap > 0.f ? a->scale / a->softcap : 0.f;
     const int smem = Q_BYTES + NK * TILE_BYTES + NV * TILE_BYTES + 256;
-    static_assert(OWN_WARPS * OWN_STAGES * (STAGE_BYTES + 8) + (OWN_WARPS + 1 + MAX_SEQS + 1) * 4 <= Q_BYTES + (NK + NV) * TILE_BYTES,
+    static_assert(OWN_WARPS * (RING_BYTES + 8 * OWN_STAGES) + (OWN_WARPS + 1 + 3 * MAX_SEQS + 1) * 4 <= Q_BYTES + (NK + NV) * TILE_BYTES + 256,
                   "the own keys' stages and their list lie in the same shared memory");
-    static_assert(STAGE_BYTES % 1024 == 0, "the swizzle goes by address bits 7 to 9");
+    static_assert(STAGE_BYTES % 1024 == 0 && RING_BYTES % 1024 == 0, "the swizzle goes by address bits 7 to 9");
     static RvPerDevice configured;
     if (int e = rv_configure_smem(configured, shared_attention_kernel, smem)) return e;
     RV_LAUNCH_ST = rv_launch(shared_attention_kernel, dim3((unsigned)(prefix_ctas + a->own_ctas)), dim3(NUM_THREADS), smem, a->stream, map_kv, map_own, p);
     if ((st = rv_launch_status()) != RV_OK) return st;
-    const int rows = a->num_seqs * nh, wave = 5 * rv_sm_count();
+    const int rows = a->num_seqs * nh, wave = MERGE_BLOCKS * rv_sm_count();
     const auto merge = [&](auto kernel, int per_block) {
         return rv_launch(kernel, dim3((rows + per_block - 1) / per_block), dim3(128), 0, a->stream, p, a->sinks, a->gate, (__nv_bfloat16*)a->out);
     };

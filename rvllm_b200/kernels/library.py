@@ -574,7 +574,7 @@ class CudaKernels:
                     raise KernelError(f"shared_prefix_attention: sinks or gate on {t.device}, the current device is cuda:{here}")
         group = num_heads // num_kv_heads
         fast = dt == 1 and head_dim in (64, 128) and page & (page - 1) == 0 and page >= 8 and pages * 2 * num_kv_heads * page < 2 ** 31 \
-            and B <= 4096
+            and B <= 2048
         tiles, items = shared.capacity
         if items == 0 or B == 0 or group > TILE_ROWS or not (fast or (head_dim % 4 == 0 and head_dim <= 256)):
             whole = meta
