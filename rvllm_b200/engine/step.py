@@ -30,9 +30,16 @@ from ..errors import KvExhausted, SchedulerError
 from ..kernels.library import COUNTERS, AttentionMeta
 from ..kernels.shared import StepPrefixes, StepTables
 
-# A decode step reads shared beginnings once (instead of as many times as requests hold them) when that saves at least this many keys.
-SHARED_MIN_KEYS = 1024
-SHARED_MOST_GROUPS = 8         # of a captured step: those that save the most
+SHARED_MOST_GROUPS = 8         # groups of a captured step: those that save the most
+# A decode step reads shared beginnings once, instead of as many times as requests hold them, where that is the faster way:
+# * bfloat16: the keys and values it saves a layer are this many bytes and half of those that it reads sequence by sequence.  32 heads of
+#   128 on 8, shared against each for itself: 16 requests with 16 keys of their own behind 256 (15.7 MB saved) 8.7 and 8.5 us, behind
+#   512 8.8 and 10.0, 8 behind 2,048 (59 MB) 10.7 and 12.7, 64 with 1,024 of their own (268 MB) behind 512 (132 MB) 62 and 55,
+#   behind 2,048 65 and 93, with 16 behind 8,192 25 and 225;
+SHARED_MIN_BYTES = 24 << 20
+# * float32: some beginning is this long (28 heads of 128 on 4: 2 requests behind 256 25 and 14 us, behind 1,024 32 and 45, 16 behind
+#   1,024 31 and 104), or the bytes saved are two thirds of the above (64 behind 256: 37 and 103).
+SHARED_MIN_TOKENS_F32 = 512
 
 
 @dataclass
@@ -72,6 +79,8 @@ class ModelRunner:
         self._ring_next = 0
         self._dev: Optional[torch.Tensor] = None
         self._groups_of = ((), [])       # the requests of the last decode step, and which of them share beginnings
+        needs = [g.need for g in cache.groups]
+        self._key_bytes = max((n.num_kv_heads * n.row_elements for n in needs), default=0) * torch.empty((), dtype=cache.dtype).element_size()
         self._page_table = None
         if cache.groups and self.device.type == "cuda" and hasattr(kernels, "step_tables"):
             G = len(cache.groups)
@@ -352,19 +361,26 @@ class ModelRunner:
         return ctx
 
     # ---- beginnings that requests share ----------------------------------------------------------
-    def _shared_groups(self, entries):
+    def _shared_groups(self, entries, starts):
         """(places, tokens) per group of entries that begin with the same cached tokens, for a step of decoded tokens; none where it
-        would not save enough.  Pages that are shared stay as they are while their requests live, so the answer holds until the set
-        of requests changes."""
+        would not pay.  Pages that are shared stay as they are while their requests live, so the groups hold until the set of
+        requests changes."""
         if not self.cache.can_share or self._page_table is None or any(len(e.tokens) != 1 for e in entries):
             return []
         reqs = tuple(e.req_id for e in entries)
         if reqs != self._groups_of[0]:
             groups = sorted(self.cache.shared_groups(reqs), key=lambda g: -(len(g[0]) - 1) * g[1])[:SHARED_MOST_GROUPS]
-            if sum((len(m) - 1) * t for m, t in groups) < SHARED_MIN_KEYS:
-                groups = []
             self._groups_of = (reqs, groups)
-        return self._groups_of[1]
+        groups = self._groups_of[1]
+        return groups if groups and self._worth_sharing(groups, sum(starts) + len(starts)) else []
+
+    def _worth_sharing(self, groups, keys: int) -> bool:
+        """Whether a step of `keys` keys in all takes less time with the groups' beginnings read once (the figures are at the top)."""
+        saved = sum((len(m) - 1) * t for m, t in groups)
+        own = keys - sum(len(m) * t for m, t in groups)
+        if self.cache.dtype == torch.float32:
+            return max(t for _, t in groups) >= SHARED_MIN_TOKENS_F32 or saved * self._key_bytes >= SHARED_MIN_BYTES * 2 // 3
+        return saved * self._key_bytes >= SHARED_MIN_BYTES + own * self._key_bytes // 2
 
     @staticmethod
     def _longest_own(starts, groups) -> int:
@@ -466,7 +482,7 @@ class ModelRunner:
             logits = self._step_graph(entries, starts, bucket, late_tokens)
         else:
             ctx = self.pack(entries, starts, late=late_tokens)
-            groups = self._shared_groups(entries)
+            groups = self._shared_groups(entries, starts)
             if groups:
                 shared = StepPrefixes(groups, len(entries), self.device, num_sms=self.kernels.num_sms)
                 for m in ctx.attention:
@@ -504,7 +520,7 @@ class ModelRunner:
 
     def _step_graph(self, entries, starts, bucket: int, late=None) -> torch.Tensor:
         ctx_limit = self._ctx_bucket(max(starts) + 1)
-        groups = self._shared_groups(entries)
+        groups = self._shared_groups(entries, starts)
         # a step that reads shared beginnings once is another graph, laid out for the keys behind them
         own_limit = self._ctx_bucket(self._longest_own(starts, groups)) if groups else 0
         bucket = (bucket, ctx_limit, own_limit)

@@ -17,8 +17,8 @@ SHAPED = {"architectures": ["LlamaForCausalLM"], "hidden_size": 256, "num_hidden
 
 @pytest.fixture(autouse=True)
 def share_little(monkeypatch):
-    from rvllm_b200.engine import step
-    monkeypatch.setattr(step, "SHARED_MIN_KEYS", 1)
+    from rvllm_b200.engine.step import ModelRunner
+    monkeypatch.setattr(ModelRunner, "_worth_sharing", lambda self, groups, keys: True)
 
 
 def make(folder, dtype, **kw):

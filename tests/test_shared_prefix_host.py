@@ -265,3 +265,15 @@ def test_samples_per_prompt():
     assert SamplingParams().n == 1
     with pytest.raises(SamplingError):
         SamplingParams(n=0)
+
+
+def test_when_a_step_reads_shared_beginnings_once():
+    """The rule, at the sizes of a layer of 8 key/value heads of 128 in bfloat16 (4 KB a key) and of 4 in float32."""
+    from types import SimpleNamespace
+    from rvllm_b200.engine.step import ModelRunner
+    half = SimpleNamespace(cache=SimpleNamespace(dtype=torch.bfloat16), _key_bytes=4096)
+    worth = lambda r, n, shared, own: ModelRunner._worth_sharing(r, [(list(range(n)), shared)], n * (shared + own))  # noqa: E731
+    assert not worth(half, 2, 64, 5) and not worth(half, 16, 256, 16) and worth(half, 16, 512, 16) and worth(half, 64, 2048, 1024)
+    assert not worth(half, 64, 512, 1024) and worth(half, 4, 8192, 100)
+    full = SimpleNamespace(cache=SimpleNamespace(dtype=torch.float32), _key_bytes=4096)
+    assert not worth(full, 2, 256, 5) and worth(full, 2, 1024, 5) and worth(full, 64, 256, 5)
