@@ -355,8 +355,9 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
                 const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * eff_scale;
                 // The reference maximum is raised only when it is more than 2^8 behind: O then needs a pass.  The exponentials do not
                 // wait to know: they are formed under the old reference beside the maximum, and once more in the rare tile that raises it.
-                // (The first tile has its maximum to begin with.)
-                if (it == 0) m_ref = m_tile;
+                // (The first tile has its maximum to begin with; the empty statement keeps this a branch, a selection would make every
+                // tile's exponentials wait.)
+                if (it == 0) { m_ref = m_tile; asm volatile("" : "+f"(m_ref)); }
                 bool raise = m_tile > m_ref + RESCALE_LOG2 || (m_ref == -INFINITY && m_tile > -INFINITY);
                 uint32_t pk[32];
                 float l_tile, l_tile2;
@@ -371,8 +372,8 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
                              eff_scale, neg_m);
                         const float x0 = fast_exp2(a0), x1 = fast_exp2(a1);
                         add2(l_tile, l_tile2, x0, x1);
-                        __nv_bfloat162 h2 = __floats2bfloat162_rn(x0, x1);
-                        pk[j] = *reinterpret_cast<uint32_t*>(&h2);
+                        const __nv_bfloat162 h2 = __floats2bfloat162_rn(x0, x1);
+                        pk[j] = *reinterpret_cast<const uint32_t*>(&h2);
                     }
                     if (!__any_sync(0xffffffffu, raise)) break;
                     float factor = 1.f;
