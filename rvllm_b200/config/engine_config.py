@@ -33,11 +33,11 @@ class EngineConfig:
     max_num_batched_tokens: int = 2048
     max_prefill_chunk: Optional[int] = None  # None: limited by the token budget only
     enable_chunked_prefill: bool = True
-    share_prefixes: bool = False            # requests that begin with the same tokens hold the same pages of the cache
     enforce_eager: bool = False             # never replay decode steps from CUDA graphs
     cuda_graph_batch_sizes: Tuple[int, ...] = (1, 2, 4, 8, 16, 32, 64)
     seed: int = 0
     device: str = "cuda:0"
+    share_prefixes: bool = False            # requests that begin with the same tokens hold the same pages of the cache
 
     def validated(self, max_position_embeddings: int) -> "EngineConfig":
         """Return a copy with defaults filled in, or raise one error naming every problem."""
