@@ -539,10 +539,11 @@ class CudaKernels:
         lengths see different parts of a prefix.  `max_own`: no sequence has more keys behind its prefix (sizes the launch
         only; without it the longest context less the shortest prefix is taken).
 
-        bfloat16 with heads of 64 or 128 and pages of a power of two from 8 on: the prefixes on the tcgen05 kernel, the rest on
-        the TMA-fed decode kernels.  float32, and other sizes whose head is a multiple of 4 up to 256: the plain kernels.  What
-        neither takes (more than 128 query heads on a key/value head among it), and steps without a group, go to
-        `paged_attention`, to which every table is whole."""
+        bfloat16 with heads of 64 or 128, pages of a power of two from 8 on and up to 2,048 sequences: the tcgen05 kernel.
+        float32, and other sizes whose head is a multiple of 4 up to 256: the plain kernel.  What neither takes (more than 128
+        query heads on a key/value head among it), and steps without a group, go to `paged_attention`, to which every table is
+        whole.  An entry of a block table that names no page inside what a sequence sees is not followed; what it gives is not
+        defined."""
         tables, lens, ints = meta.block_tables, meta.ctx_lens, shared.device_ints
         here = torch._C._cuda_getDevice()
         for t in (q, cache_layer, tables, lens, ints):
@@ -567,6 +568,10 @@ class CudaKernels:
                               f"{shared.num_kv_heads}, a step of {B} of {num_heads} on {num_kv_heads}")
         if table_rows < B or lens.shape[0] < B:
             raise KernelError(f"shared_prefix_attention: tables of {table_rows} and lengths of {lens.shape[0]} sequences for {B}")
+        if not scale > 0:
+            raise KernelError(f"shared_prefix_attention: scale must be positive, got {scale}")
+        if self._status.get_device() != here:
+            raise KernelError(f"shared_prefix_attention: this library is that of {self._status.device}, the current device is cuda:{here}")
         if sinks is not None or gate is not None:
             self._check_attention_extras(q, num_heads, sinks, gate)
             for t in (sinks, gate):

@@ -205,6 +205,11 @@ def test_long_prefix_in_many_ranges():
     check(make([(3, 9001)], 1, 8, 2, 64, 16, torch.bfloat16, seed=6, own=(1, 40)))
 
 
+def test_more_sequences_than_the_list_of_pieces_has_room_for():
+    check(make([(2100, 33)], 2, 2, 1, 64, 16, torch.bfloat16, seed=8, own=(1, 20)))
+    check(make([(2040, 33)], 2, 2, 1, 64, 16, torch.bfloat16, seed=8, own=(1, 20)))
+
+
 def test_without_groups_it_is_the_paged_attention():
     s = make([], 5, 32, 8, 128, 16, torch.bfloat16, own=(1, 300), stale="0")
     nh, nkv, hd = s["dims"]
@@ -284,7 +289,7 @@ def test_refusals():
     s = make([(4, 50)], 1, 8, 2, 64, 16, torch.bfloat16, own=(1, 20))
     nh, nkv, hd = s["dims"]
     shared = SharedPrefixes(s["plan"], 5, nh, nkv, "cuda")
-    call = lambda q=s["q"], c=s["cache"], m=s["meta"], p=shared, h=(nh, nkv, hd), **kw: lib().shared_prefix_attention(q, c, m, p, *h, 0.125, **kw)  # noqa: E731
+    call = lambda q=s["q"], c=s["cache"], m=s["meta"], p=shared, h=(nh, nkv, hd), scale=0.125, **kw: lib().shared_prefix_attention(q, c, m, p, *h, scale, **kw)  # noqa: E731
     call()
     m = s["meta"]
     two = AttentionMeta(m.block_tables, m.cu_seqlens, m.ctx_lens, m.token_seq, None, 5, 2, 100, 16, 4)
@@ -292,7 +297,7 @@ def test_refusals():
            dict(c=s["cache"][:, :1].contiguous()), dict(c=s["cache"].transpose(2, 3)), dict(m=two), dict(h=(8, 4, 64)), dict(h=(8, 2, 32)),
            dict(p=SharedPrefixes(s["plan"], 6, nh, nkv, "cuda")), dict(p=SharedPrefixes(s["plan"], 5, 2, 2, "cuda")),
            dict(p=SharedPrefixes(s["plan"], 5, nh, nkv, "cpu")), dict(sinks=torch.zeros(3, device="cuda")), dict(sinks=torch.zeros(8)),
-           dict(gate=torch.zeros(5, 7, device="cuda")), dict(gate=torch.zeros(5, 8, device="cuda", dtype=torch.bfloat16))]
+           dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")), dict(gate=torch.zeros(5, 7, device="cuda")), dict(gate=torch.zeros(5, 8, device="cuda", dtype=torch.bfloat16))]
     for kw in bad:
         with pytest.raises(KernelError):
             call(**kw)
