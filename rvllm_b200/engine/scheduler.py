@@ -66,7 +66,7 @@ class Request:
     num_preemptions: int = 0
     unresolved: int = 0            # stand-ins at the end of `output`
     shared_tokens: int = 0         # tokens at the beginning that were taken over when it was last admitted
-    common: dict = field(default_factory=dict, repr=False)     # while it waits: tokens in common with the prompts of running requests
+    common: dict = field(default_factory=dict, repr=False)     # while it waits: tokens in common with the prompts of running requests, by their arrival
 
     @property
     def all_tokens(self) -> List[int]:
@@ -166,11 +166,11 @@ class Scheduler:
         page = self.cache.page_size
         tokens = None
         best, have, coming = None, 0, 0
-        live = {id(r) for r in self.running}
+        live = {r.arrival for r in self.running}
         for gone in [k for k in req.common if k not in live]:
             del req.common[gone]
         for other in self.running:
-            common = req.common.get(id(other))
+            common = req.common.get(other.arrival)
             if common is None:
                 # whole pages of the two prompts (and what `req` has produced before it was pre-empted) that are the same
                 if tokens is None:
@@ -178,7 +178,7 @@ class Scheduler:
                 theirs, common, most = other.prompt, 0, min(len(tokens) - 1, len(other.prompt))
                 while common + page <= most and tokens[common:common + page] == theirs[common:common + page]:
                     common += page
-                req.common[id(other)] = common
+                req.common[other.arrival] = common
             ready = min(common, other.num_computed // page * page)
             if ready > have:
                 best, have = other, ready

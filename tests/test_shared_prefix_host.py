@@ -236,6 +236,20 @@ def test_without_the_option_nothing_is_shared():
     assert shape(b) == [(0, 0, 20, True), (1, 0, 20, True), (2, 0, 20, True)]
 
 
+def test_what_two_have_in_common_is_not_kept_by_address(monkeypatch):
+    """Objects of requests that ended leave their addresses to others."""
+    monkeypatch.setattr("rvllm_b200.engine.scheduler.id", lambda _: 1, raising=False)
+    cache, s = scheduler()
+    s.add_request(request("a", range(30), max_tokens=2))
+    s.add_request(request("b", range(50, 80), max_tokens=20))
+    run_step(cache, s)
+    w = request("w", list(range(50, 74)) + [1], max_tokens=9)
+    s.add_request(w)
+    for _ in range(4):
+        run_step(cache, s)
+    assert w.shared_tokens == 24
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_no_page_is_lost_under_random_arrivals_and_preemption(seed):
     rng = random.Random(seed)
