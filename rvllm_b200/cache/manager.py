@@ -100,6 +100,7 @@ class CacheManager:
         self.slots = SlotPool(max_seqs)
         self._has_window = any(g.need.window is not None or g.need.chunk is not None for g in self.groups)
         self.requests: Dict[Hashable, _Request] = {}
+        self.changes = 0               # how often a request came, went or took over pages
         if allocate:
             for g in self.groups:
                 if g.need.flat_pages:
@@ -165,6 +166,7 @@ class CacheManager:
         if req in self.requests:
             raise SchedulerError(f"request {req!r} is already in the cache")
         slot = self.slots.allocate(req)
+        self.changes += 1
         self.requests[req] = _Request(slot, 0, [[] for _ in self.groups], [0 for _ in self.groups], [0 for _ in self.groups])
         for t in self._state.values():
             t[slot].zero_()
@@ -185,6 +187,7 @@ class CacheManager:
             raise SchedulerError(f"request {req!r} has tokens already")
         if num_tokens < 1 or num_tokens % self.page_size or num_tokens > d.num_tokens:
             raise SchedulerError(f"request {req!r}: {num_tokens} tokens of {donor!r} cannot be shared: it has {d.num_tokens}, in pages of {self.page_size}")
+        self.changes += 1
         n = num_tokens // self.page_size
         for g, mine, theirs in zip(self.groups, r.tables, d.tables):
             g.pool.share(theirs[:n], req)
@@ -302,6 +305,7 @@ class CacheManager:
 
     def free(self, req: Hashable) -> None:
         r = self.requests.pop(req)
+        self.changes += 1
         for g, table in zip(self.groups, r.tables):
             g.pool.release([p for p in table if p >= 0], req)
         self.slots.release(r.state_slot, req)

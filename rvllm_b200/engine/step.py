@@ -78,7 +78,10 @@ class ModelRunner:
         self._ring_events: List[Optional[object]] = [None, None, None]
         self._ring_next = 0
         self._dev: Optional[torch.Tensor] = None
-        self._groups_of = ((), [])       # the requests of the last decode step, and which of them share beginnings
+        # the requests of the last decode step (and how often the cache's had changed), which of them share beginnings, and the layout
+        # that eager steps have for these groups
+        self._groups_of = (None, [])
+        self._eager_prefixes: Optional[StepPrefixes] = None
         needs = [g.need for g in cache.groups]
         self._key_bytes = max((n.num_kv_heads * n.row_elements for n in needs), default=0) * torch.empty((), dtype=cache.dtype).element_size()
         self._page_table = None
@@ -329,7 +332,6 @@ class ModelRunner:
                 if new:
                     h[at:at + len(new)] = new
                     at += len(new)
-                    r.on_device[g] += len(new)
         h[o_late:o_late + n_real] = late[1] if late is not None else -1
         h[o_late + n_real:o_late + B] = -1
         dev[:at].copy_(host[:at], non_blocking=True)
@@ -343,6 +345,8 @@ class ModelRunner:
         made = StepTables(tables.view(G, B, MB), slots.view(G, T), positions, token_seq, cu, ctx_dev)
         self.kernels.step_tables(self._page_table, dev[:B], dev[o_held:o_tok].view(G, B), dev[o_start:o_q], dev[o_q:o_held], dev[o_new:max(at, o_new + 1)],
                                  self._spans, T, MB, cache.page_size, out=made)
+        for r in held:
+            r.on_device = [len(t) for t in r.tables]
         ctx = StepContext()
         ctx.kernels = self.kernels
         ctx.num_tokens, ctx.num_seqs = T, B
@@ -367,9 +371,9 @@ class ModelRunner:
         requests changes."""
         if not self.cache.can_share or self._page_table is None or any(len(e.tokens) != 1 for e in entries):
             return []
-        reqs = tuple(e.req_id for e in entries)
+        reqs = (self.cache.changes, tuple(e.req_id for e in entries))
         if reqs != self._groups_of[0]:
-            groups = sorted(self.cache.shared_groups(reqs), key=lambda g: -(len(g[0]) - 1) * g[1])[:SHARED_MOST_GROUPS]
+            groups = sorted(self.cache.shared_groups(reqs[1]), key=lambda g: -(len(g[0]) - 1) * g[1])[:SHARED_MOST_GROUPS]
             self._groups_of = (reqs, groups)
         groups = self._groups_of[1]
         return groups if groups and self._worth_sharing(groups, sum(starts) + len(starts)) else []
@@ -381,6 +385,12 @@ class ModelRunner:
         if self.cache.dtype == torch.float32:
             return max(t for _, t in groups) >= SHARED_MIN_TOKENS_F32 or saved * self._key_bytes >= SHARED_MIN_BYTES * 2 // 3
         return saved * self._key_bytes >= SHARED_MIN_BYTES + own * self._key_bytes // 2
+
+    def _eager_shared(self, groups, num_seqs: int) -> StepPrefixes:
+        last = self._eager_prefixes
+        if last is None or last.num_seqs != num_seqs or last.groups != groups:
+            last = self._eager_prefixes = StepPrefixes(groups, num_seqs, self.device, num_sms=self.kernels.num_sms)
+        return last
 
     @staticmethod
     def _longest_own(starts, groups) -> int:
@@ -484,7 +494,7 @@ class ModelRunner:
             ctx = self.pack(entries, starts, late=late_tokens)
             groups = self._shared_groups(entries, starts)
             if groups:
-                shared = StepPrefixes(groups, len(entries), self.device, num_sms=self.kernels.num_sms)
+                shared = self._eager_shared(groups, len(entries))
                 for m in ctx.attention:
                     m.shared, m.max_own_len = shared, self._longest_own(starts, groups)
             hidden = self.model.forward(ctx, self.cache)
@@ -531,7 +541,7 @@ class ModelRunner:
             # (so does one whose requests have just taken over pages that the device's table lacks)
             ctx = self.pack(entries, starts, late=late)
             if groups:
-                shared = StepPrefixes(groups, len(entries), self.device, num_sms=self.kernels.num_sms)
+                shared = self._eager_shared(groups, len(entries))
                 for m in ctx.attention:
                     m.shared, m.max_own_len = shared, own_limit
             hidden = self.model.forward(ctx, self.cache)

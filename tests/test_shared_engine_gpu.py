@@ -127,6 +127,32 @@ def test_bfloat16_logits_with_a_shared_beginning(eager, monkeypatch):
     assert float((x - y).abs().max()) <= 2e-2 * float(y.abs().max())
 
 
+def test_an_identifier_that_is_used_again(monkeypatch):
+    """Requests that share, end, and come back under the same identifiers with other beginnings: nothing of the first is kept."""
+    from rvllm_b200.engine import StepEntry
+    folder = folder_for(SHAPED)
+    a, b = stems(515, seed=9)
+    logits = []
+    for share in (True, False):
+        eng = make(folder, "float32", share_prefixes=share).engine
+        got = []
+        for stem in (a[:64], (b + a)[:64]):
+            eng.runner.step([StepEntry(0, stem + [1], ())])
+            for i in (1, 2):
+                if share and stem == a[:64]:
+                    eng.cache.admit(i); eng.cache.share(i, 0, 64)
+                    eng.runner.step([StepEntry(i, [i + 5], ())])
+                else:
+                    eng.runner.step([StepEntry(i, (stem if i == 1 or stem == a[:64] else stem[::-1]) + [i + 5], ())])
+            for t in range(3):
+                got.append(eng.runner.step([StepEntry(i, [t + i], (0,)) for i in range(3)]).cpu())
+            for i in range(3):
+                eng.runner.finish(i)
+        logits.append(torch.cat(got))
+    # float32 sums in another order: a few hundred roundings of 2^-24 of values the size of the logits
+    assert float((logits[0] - logits[1]).abs().max()) <= 2e-4 * float(logits[1].abs().max())
+
+
 # ------------------------------------------------------------------------------------------------------------ step tables
 def windowed():
     return dict(plain_windows={"architectures": ["Qwen2ForCausalLM"], "hidden_size": 64, "num_hidden_layers": 4, "num_attention_heads": 4,
