@@ -48,12 +48,13 @@ template <int PER>
 __global__ void __launch_bounds__(TABLE_THREADS)
 step_tables_kernel(const TableParams p) {
     constexpr int THREADS = TABLE_THREADS / PER;             // of a sequence
-    __shared__ int sums[2][TABLE_THREADS / 32];
-    __shared__ int own[2][PER];                              // new pages and tokens of this CTA's sequences
+    __shared__ unsigned sums[2][TABLE_THREADS / 32];
+    __shared__ unsigned own[2][PER];                              // new pages and tokens of this CTA's sequences
     rv_pdl_wait();
     const int tid = threadIdx.x, g = blockIdx.y, b0 = blockIdx.x * PER;
-    // pages taken before this CTA's first sequence (all groups before g, then the sequences before b0), tokens before it
-    int pages = 0, tokens = 0;
+    // pages taken before this CTA's first sequence (all groups before g, then the sequences before b0), tokens before it (unsigned, as
+    // every place that follows from them: lengths whose sums pass 31 bits give places that are out of range, or others' in it)
+    unsigned pages = 0, tokens = 0;
     for (int s = tid; s < p.num_seqs; s += TABLE_THREADS) {
         const int used = blocks_in_use(p, s);
         const int until = s < b0 ? g + 1 : g;                // groups in which s comes before
@@ -72,7 +73,7 @@ step_tables_kernel(const TableParams p) {
     const bool real = row >= 0 && row < p.table_rows;
     const int start = here ? max(p.starts[b], 0) : 0, q = here ? max(p.q_lens[b], 0) : 0;
     const int used = here ? blocks_in_use(p, b) : 0;
-    const int held = here ? max(p.held[(size_t)g * p.num_seqs + b], 0) : 0;
+    const int held = here ? min(max(p.held[(size_t)g * p.num_seqs + b], 0), p.table_width) : 0;
     if (PER > 1 && at == 0) { own[0][sub] = max(0, used - held); own[1][sub] = q; }
     __syncthreads();
     pages = tokens = 0;
@@ -85,8 +86,8 @@ step_tables_kernel(const TableParams p) {
     int* mine = p.page_table + ((size_t)g * p.table_rows + (real ? row : 0)) * p.table_width;
     auto entry = [&](int j) -> int {                         // j < used
         if (j < held) return mine[j];
-        const int i = pages + (j - held);
-        return i < p.num_new ? p.new_pages[i] : -1;
+        const unsigned i = pages + (unsigned)(j - held);
+        return i < (unsigned)p.num_new ? p.new_pages[i] : -1;
     };
     for (int j = held + at; j < used; j += THREADS) mine[j] = entry(j);
     const int window = p.spans[2 * g], chunk = p.spans[2 * g + 1];
@@ -96,27 +97,28 @@ step_tables_kernel(const TableParams p) {
     int* out = p.block_tables + ((size_t)g * p.num_seqs + b) * p.max_blocks;
 #pragma unroll 4
     for (int j = at; j < p.max_blocks; j += THREADS) out[j] = (j >= live && j < used) ? entry(j) : -1;
-    for (int i = at; i < q && tokens + i < p.num_tokens; i += THREADS) {
-        const int t = tokens + i;
-        const int pos = real ? start + i : 0;
-        const int block = pos / p.page_size;
+    for (int i = at; i < q; i += THREADS) {
+        const unsigned t = tokens + (unsigned)i;
+        if (t >= (unsigned)p.num_tokens) break;
+        const unsigned pos = real ? (unsigned)start + (unsigned)i : 0u;
+        const unsigned block = pos / (unsigned)p.page_size;
         int slot = -1;
-        if (real && block < used) {
-            const int page = entry(block);
-            if (page >= 0) slot = page * p.page_size + (pos - block * p.page_size);
+        if (real && block < (unsigned)used) {
+            const int page = entry((int)block);
+            if (page >= 0) slot = page * p.page_size + (int)(pos - block * (unsigned)p.page_size);
         }
         p.slot_mapping[(size_t)g * p.num_tokens + t] = slot;
-        if (g == 0) { p.positions[t] = pos; p.token_seq[t] = b; }
+        if (g == 0) { p.positions[t] = (int)pos; p.token_seq[t] = b; }
     }
     if (b == p.num_seqs - 1)                                 // places behind the last sequence's tokens belong to none
-        for (int t = tokens + q + at; t < p.num_tokens; t += THREADS) {
+        for (unsigned t = tokens + (unsigned)q + (unsigned)at; t < (unsigned)p.num_tokens; t += THREADS) {
             p.slot_mapping[(size_t)g * p.num_tokens + t] = -1;
             if (g == 0) { p.positions[t] = 0; p.token_seq[t] = -1; }
         }
     if (g == 0 && at == 0) {
-        p.cu_seqlens[b] = tokens;
-        if (b == p.num_seqs - 1) p.cu_seqlens[p.num_seqs] = tokens + q;
-        p.ctx_lens[b] = real ? start + q : 0;
+        p.cu_seqlens[b] = (int)tokens;
+        if (b == p.num_seqs - 1) p.cu_seqlens[p.num_seqs] = (int)(tokens + (unsigned)q);
+        p.ctx_lens[b] = real ? (int)((unsigned)start + (unsigned)q) : 0;
     }
     // The step's other kernels may read this metadata before they wait for their predecessor, so nothing behind this kernel may
     // start before all of it is written: it gives no early signal, and what it wrote is out when a CTA ends.

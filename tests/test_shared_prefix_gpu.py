@@ -123,7 +123,7 @@ CASES = [
     ([(2, 300)], 0, 128, 1, 128, 16, (1, 20)),                    # 128 heads on one
     ([(3, 90)], 1, 16, 16, 128, 128, (1, 20)),                    # pages larger than a tile
     ([(64, 1000)], 3, 16, 4, 128, 16, (1, 64)),
-    ([(300, 77)], 0, 4, 2, 64, 16, (1, 5)),                       # more sequences than the evenly cut kernel takes
+    ([(300, 77)], 0, 4, 2, 64, 16, (1, 5)),                       # hundreds of sequences, few keys each
 ]
 
 
@@ -395,6 +395,28 @@ def test_step_tables_check_what_the_device_holds():
     assert table[0, 2].tolist() == [5, -1, -1] and table[0, [0, 1, 3]].abs().sum() == 0
     assert got.block_tables.tolist() == [[[5, -1, -1, -1, -1], [-1] * 5]] and got.ctx_lens.tolist() == [70, 0]
     assert got.slot_mapping.tolist() == [[-1] * 20] and guard.eq(9).all()
+
+
+def test_step_tables_with_lengths_past_31_bits():
+    """Sums that leave 32-bit integers: every tensor lies between guards, and these stay as they are."""
+    from rvllm_b200.kernels import StepTables
+    top = 2 ** 31 - 1
+    many = 600                                       # (more than a CTA takes by itself)
+    for starts, q, held in (([top] * 5, [top] * 5, [top] * 5), ([top - 3, 0, top, 7, 1], [9, top, top, 3, 1], [0, top, -top, 3, 1]),
+                            ([1] * many, [top // 2] * many, [top] * many)):
+        B, T, MB, W = len(starts), 40, 6, 4
+        shapes = [(1, B, W), (1, B, MB), (1, T), (T,), (T,), (B + 1,), (B,)]
+        room = torch.full((sum(math.prod(s) + 64 for s in shapes) + 64,), 123456789, dtype=torch.int32, device="cuda")
+        views, at = [], 64
+        for s in shapes:
+            views.append(room[at:at + math.prod(s)].view(s))
+            at += math.prod(s) + 64
+        lib().step_tables(views[0], i32(list(range(B))), i32([held]), i32(starts), i32(q), i32([3, 4]), i32([[0, 0]]), T, MB, 16, out=StepTables(*views[1:]))
+        at = 0
+        for s in shapes:
+            assert room[at:at + 64].eq(123456789).all()
+            at += math.prod(s) + 64
+        assert room[at:].eq(123456789).all()
 
 
 def test_step_tables_captured():
