@@ -99,12 +99,13 @@ struct SharedParams {
     float scale_log2e, cap_log2e, scale_over_cap;
 };
 
-// The running (maximum, denominator, four columns) of a row, and one more part's taken up into it; one without keys may hold any sum.
+// The running (maximum, denominator, four columns) of a row, and one more part's taken up into it.  One without keys (l = 0) may hold any sum; one whose
+// scores are no numbers has a maximum of -inf and an l that is none either, and passes that on.
 struct Merged {
     float m = -INFINITY, l = 0.f;
     float4 o = {0.f, 0.f, 0.f, 0.f};
     __device__ __forceinline__ void take(float pm, float pl, const float4& po) {
-        if (pm == -INFINITY) return;
+        if (pl == 0.f) return;
         const float m_new = fmaxf(m, pm);
         const float keep = fast_exp2(m - m_new), f = fast_exp2(pm - m_new);
         m = m_new;
@@ -812,7 +813,7 @@ shared_merge_kernel(const SharedParams p, const float* __restrict__ sinks, const
         num = v.m == -INFINITY ? 0.f : fast_exp2(v.m - m_new);
         den = v.l * num + fast_exp2(sk - m_new);
     }
-    float inv = den > 0.f ? num / den : 0.f;
+    float inv = den == 0.f ? 0.f : num / den;        // (what is no number stays so)
     if (gate) inv *= gate[row];
     rv_store4(out, RV_DTYPE_BF16, (size_t)row * HEAD_DIM + d, make_float4(v.o.x * inv, v.o.y * inv, v.o.z * inv, v.o.w * inv));
 }

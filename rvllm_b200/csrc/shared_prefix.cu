@@ -291,7 +291,7 @@ shared_merge_kernel(const MergeParams p) {
         num = exp2f(v.m - m_new);
         den = v.l * num + exp2f(sk - m_new);
     }
-    float inv = den > 0.f ? num / den : 0.f;
+    float inv = den == 0.f ? 0.f : num / den;            // (what is no number stays so)
     if (p.gate) inv *= p.gate[out_row];
     constexpr int dt = sizeof(T) == 4 ? RV_DTYPE_F32 : RV_DTYPE_BF16;
     rv_store4(p.out, dt, out_row * p.hd + d, make_float4(v.o.x * inv, v.o.y * inv, v.o.z * inv, v.o.w * inv));

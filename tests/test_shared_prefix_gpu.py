@@ -199,6 +199,23 @@ def test_max_own_sizes_the_launch_only():
     check(s, max_own=1)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_what_is_not_a_number_stays_so(dtype):
+    """A query of NaN, and keys of NaN or infinity that a sequence sees, give NaN to that sequence (or its heads) and to no other."""
+    s = make([(5, 70)], 2, 8, 2, 64, 16, dtype, seed=3, own=[9, 20, 33, 4, 18, 40, 7])
+    nh, nkv, hd = s["dims"]
+    s["q"][1] = float("nan")
+    for b, value in ((3, float("nan")), (4, float("inf"))):
+        at = s["ctx"][b] - 1                         # its own last key, of one kv head
+        s["cache"][s["meta"].block_tables[b, at // 16], 0, 1, at % 16] = value
+    got = run(s).view(7, nkv, nh // nkv, hd).cpu()
+    lib().raise_on_abort()
+    want = torch.zeros(7, nkv, dtype=torch.bool)
+    want[1] = True
+    want[3, 1] = want[4, 1] = True
+    assert torch.equal(got.isnan().all(-1).all(-1), want) and torch.equal(got.isnan().any(-1).any(-1), want)
+
+
 def test_long_prefix_in_many_ranges():
     s = make([(3, 9001)], 1, 8, 2, 128, 16, torch.bfloat16, seed=6, own=(1, 40))
     check(s)
