@@ -118,6 +118,11 @@ struct Merged {
 // Pieces that the own keys of a sequence are cut into: as many as its own length asks for, at most as many as there is room for.
 __device__ __forceinline__ int pieces_of(int own, int piece, int most) { return max(1, min(most, (own + piece - 1) / piece)); }
 
+// A wait of a whole warp, whose lanes all give up when one does.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code));
+}
+
 __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMap& map, unsigned char* smem, int cta);
 
 __global__ void __launch_bounds__(NUM_THREADS, 2)
@@ -304,7 +309,7 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
         for (int it = 0; it < n_it; ++it) {
             const int pb = it & 1;
             const int key0 = (t_begin + it) * KV_TILE;
-            if (!mbar_wait(bar_s_full, it & 1, &abort_flag, 9)) { ok = false; break; }
+            if (!warp_wait(bar_s_full, it & 1, &abort_flag, 9)) { ok = false; break; }
             tcgen05_fence_after();
             uint32_t s0[32], s1[32];
             if (rows_here) {
@@ -317,7 +322,7 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
             if (lane == 0) mbar_arrive(bar_s_free);
             if (key0 + KV_TILE > key_hi) {
                 // values of keys behind the range's end: zeros, before the product may read them (it waits for P of all four warps)
-                if (!mbar_wait(bar_v0 + 8 * (it % NV), (it / NV) & 1, &abort_flag, 12)) { ok = false; break; }
+                if (!warp_wait(bar_v0 + 8 * (it % NV), (it / NV) & 1, &abort_flag, 12)) { ok = false; break; }
                 const int from = key_hi - key0, n = (KV_TILE - from) * 8;
                 unsigned char* vt = v_s + (it % NV) * TILE_BYTES;
                 for (int i = tid; i < HALVES * n; i += 32 * SOFTMAX_WARPS) {
@@ -385,7 +390,7 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
                         raise = false;
                     }
                     // the product of the tile before must have finished; the one after waits for this warp's P
-                    if (!mbar_wait(bar_o_full0 + 8 * (pb ^ 1), ((it - 1) >> 1) & 1, &abort_flag, 11)) { ok = false; break; }
+                    if (!warp_wait(bar_o_full0 + 8 * (pb ^ 1), ((it - 1) >> 1) & 1, &abort_flag, 11)) { ok = false; break; }
                     tcgen05_fence_after();
 #pragma unroll
                     for (int c = 0; c < HEAD_DIM; c += 32) {
@@ -409,7 +414,7 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid
             if (lane == 0) mbar_arrive(bar_p_full0 + 8 * pb);
         }
         if (ok) {
-            ok = mbar_wait(bar_o_full0 + 8 * ((n_it - 1) & 1), ((n_it - 1) >> 1) & 1, &abort_flag, 10);
+            ok = warp_wait(bar_o_full0 + 8 * ((n_it - 1) & 1), ((n_it - 1) >> 1) & 1, &abort_flag, 10);
             tcgen05_fence_after();
             if (ok && rows_here) {
                 // A thread holds a row, so its stores would be 16 bytes here and there: the warp turns 32 x 32 floats over in shared
@@ -642,7 +647,7 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
     bool fresh = true;                               // the next chunk is the first of a piece
     while (taken < asked) {
         const int stage = taken % OWN_STAGES;
-        if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, (taken / OWN_STAGES) & 1, &abort_flag, 14))) { ok = false; break; }
+        if (!warp_wait(bar0 + 8 * stage, (taken / OWN_STAGES) & 1, &abort_flag, 14)) { ok = false; break; }
         const uint32_t at = smem_u32(ring) + stage * STAGE_BYTES;
         if (fresh) {
             now = pending;
