@@ -624,13 +624,22 @@ class CudaKernels:
         return out
 
     def _own_pieces(self, pairs: int, max_own: int):
-        """(keys of a piece, most pieces of a sequence, CTAs) for the own keys of `pairs` sequences and blocks of heads."""
+        """(keys of a piece, most pieces of a sequence, CTAs) for the own keys of `pairs` sequences and blocks of heads.
+
+        A piece costs a warp its set-up and the merge another part, and too few leave warps idle at the end.  So: pieces of a chunk
+        (16) while there are warps for them; up to 64, and then 128, while more than one, and four, wait for each warp; from there on
+        only for sequences of more than eight pieces, eight of which wait.  Measured in us with 64 / 128 / 256 / 512 keys, head
+        size 128, 8 kv heads, own lengths from 1 to the last figure: 64 sequences to 700: 34 / 31 / 36 / 44; 64 to 4,000:
+        121 / 114 / 110 / 122; 256 to 2,000: 216 / 205 / 196 / 201; 512 to 1,000: 214 / 203 / 203 / 219; 1,024 to 500:
+        234 / 229 / 238 / 251; and 57 sequences to 399, where three wait for a warp: 27.7 / 29.4."""
         ctas = 2 * self.num_sms
-        piece = 16                       # few sequences: a warp each for as little as a chunk; many: 64 keys (a warp's set-up is worth two chunks)
-        while (piece < 64 and pairs * -(-max_own // piece) > 4 * ctas) or max_own > 64 * piece:
+        warps, piece = 4 * ctas, 16
+        while True:
+            pieces = -(-max_own // piece)
+            waiting = pairs * pieces
+            if not (waiting > warps if piece < 64 else waiting > 4 * warps if piece < 128 else pieces > 8 and waiting > 8 * warps) and pieces <= 64:
+                return piece, pieces, max(1, min(ctas, -(-waiting // 4)))
             piece *= 2
-        pieces = -(-max_own // piece)
-        return piece, pieces, max(1, min(ctas, -(-pairs * pieces // 4)))
 
     def step_tables(self, page_table: torch.Tensor, rows: torch.Tensor, held: torch.Tensor, starts: torch.Tensor, q_lens: torch.Tensor,
                     new_pages: torch.Tensor, spans: torch.Tensor, num_tokens: int, max_blocks: int, page_size: int,

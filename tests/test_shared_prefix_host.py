@@ -291,3 +291,17 @@ def test_when_a_step_reads_shared_beginnings_once():
     assert not worth(half, 64, 512, 1024) and worth(half, 4, 8192, 100)
     full = SimpleNamespace(cache=SimpleNamespace(dtype=torch.float32), _key_bytes=4096)
     assert not worth(full, 2, 256, 5) and worth(full, 2, 1024, 5) and worth(full, 64, 256, 5)
+
+
+def test_pieces_of_the_own_keys():
+    """The parts' sums stay small however many sequences there are and however long they are; a few sequences have a warp a chunk."""
+    from rvllm_b200.kernels.library import CudaKernels
+    k = CudaKernels.__new__(CudaKernels)
+    k.num_sms = 148
+    assert k._own_pieces(4, 7) == (16, 1, 1) and k._own_pieces(32, 157) == (16, 10, 80)
+    assert k._own_pieces(456, 399)[:2] == (64, 7) and k._own_pieces(512, 692)[:2] == (128, 6) and k._own_pieces(2048, 2000)[:2] == (256, 8)
+    for pairs in (1, 30, 500, 2048, 16384, 65536):
+        for most in (1, 15, 16, 17, 300, 4000, 70000, 2 ** 20, 2 ** 31 - 1):
+            piece, pieces, ctas = k._own_pieces(pairs, most)
+            assert (pieces - 1) * piece < most <= pieces * piece and 1 <= ctas <= 296 and 4 * (ctas - 1) < pairs * pieces
+            assert pieces <= 64 and (pieces <= 8 or pairs * pieces <= 8 * 4 * 296)
