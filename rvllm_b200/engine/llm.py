@@ -15,7 +15,7 @@ from typing import Dict, Hashable, List, Optional, Sequence, Union
 import torch
 
 from ..config import EngineConfig
-from ..errors import ConfigError
+from ..errors import ConfigError, SamplingError
 from ..sampling import Sampler, SamplingParams, request_seed
 from .core import Engine
 from .scheduler import PENDING, Request, ScheduledBatch, Scheduler
@@ -94,6 +94,8 @@ class LLM:
     # ---- requests ----------------------------------------------------------------------------
     def add_request(self, prompt_token_ids: Sequence[int], params: SamplingParams,
                     request_id: Optional[Hashable] = None) -> Request:
+        if params.n != 1:
+            raise SamplingError(f"n = {params.n}: a request is one sample; `generate` makes n of a prompt")
         rid = request_id if request_id is not None else self._next_id
         number = self._next_id
         self._next_id += 1
