@@ -196,12 +196,13 @@ class CacheManager:
 
     def shared_groups(self, reqs) -> List[Tuple[List[int], int]]:
         """Which of the requests `reqs` begin with the same pages: (places in `reqs`, tokens) per group, each request in one group at
-        most.  Where a few of those that share a beginning share more among themselves, the grouping that saves the most keys is taken."""
+        most.  Where a few of those that share a beginning share more among themselves, the grouping that saves the most keys is taken
+        (looked for up to 64 beginnings within one another)."""
         if not self.can_share:
             return []
         tables = [self.requests[r].tables[0] for r in reqs]
 
-        def grouped(members: List[int], depth: int):
+        def grouped(members: List[int], depth: int, inside: int = 0):
             """(keys saved, groups) of requests whose first `depth` pages are the same"""
             if len(members) < 2:
                 return 0, []
@@ -217,7 +218,7 @@ class CacheManager:
                 if len(tables[m]) > common:
                     parts.setdefault(tables[m][common], []).append(m)
             saved, groups = (len(members) - 1) * common * self.page_size, [(members, common * self.page_size)] if common else []
-            deeper = [grouped(ms, common) for ms in parts.values() if len(ms) > 1]
+            deeper = [grouped(ms, common, inside + 1) for ms in parts.values() if len(ms) > 1 and inside < 64]
             if sum(d[0] for d in deeper) > saved:
                 return sum(d[0] for d in deeper), [g for d in deeper for g in d[1]]
             return saved, groups

@@ -163,6 +163,19 @@ def test_groups_that_save_the_most():
     assert m2.shared_groups(["a"]) == [] and m2.shared_groups([]) == []
 
 
+def test_beginnings_within_one_another():
+    """1,500 requests, each of which goes on from the one before: a chain as deep as the step is wide."""
+    n = 1500
+    m = manager(num_pages=3 * n + 10, page=1, max_seqs=n + 1)
+    m.admit(0); m.append(0, 2)
+    for i in range(1, n):
+        m.admit(i); m.share(i, i - 1, i); m.append(i, 2)
+    groups = m.shared_groups(list(range(n)))
+    assert groups and all(len(ms) > 1 for ms, _ in groups) and sorted(x for ms, _ in groups for x in ms) == sorted({x for ms, _ in groups for x in ms})
+    for ms, t in groups:
+        assert len({tuple(m.block_table(i, 0)[:t]) for i in ms}) == 1
+
+
 # ------------------------------------------------------------------------------------------------------------- scheduling
 def scheduler(num_pages=64, page=4, max_seqs=8, budget=64, chunk=None, chunked=True, share=True, max_len=256):
     from rvllm_b200.cache import CacheManager
@@ -279,6 +292,26 @@ def test_samples_per_prompt():
     assert SamplingParams().n == 1
     with pytest.raises(SamplingError):
         SamplingParams(n=0)
+
+
+@pytest.fixture
+def emulated():
+    import rvllm_b200.kernels as kernel_pkg
+    from emulated_kernels import EmulatedKernels
+    kernel_pkg.set_library(EmulatedKernels())
+    yield
+    kernel_pkg.set_library(None)
+
+
+def test_a_request_is_one_sample(emulated):
+    from rvllm_b200 import LLM, SamplingError, SamplingParams
+    from model_tools import model_folder
+    llm = LLM(model_folder("tiny_llama"), dtype="float32", device="cpu", block_size=8, num_blocks=32, max_model_len=64, max_num_seqs=3)
+    with pytest.raises(SamplingError, match="one sample"):
+        llm.add_request([1, 2, 3], SamplingParams(n=2))
+    assert not llm.scheduler.has_unfinished()
+    out, = llm.generate([[1, 2, 3]], SamplingParams(n=2, max_tokens=4, ignore_eos=True))
+    assert [len(o.token_ids) for o in out.outputs] == [4, 4] and out.outputs[0].token_ids == out.outputs[1].token_ids
 
 
 def test_when_a_step_reads_shared_beginnings_once():
