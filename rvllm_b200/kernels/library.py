@@ -517,15 +517,12 @@ class CudaKernels:
         return out
 
     # ------------------------------------------------------------------ tokens that requests share
-    def _entry(self, source: str, defines, name: str):
-        """An exported function that takes its arguments packed into one block of bytes, looked up once (twenty arguments as ctypes
-        objects were half of what such a call cost the host)."""
-        key = (source, defines, name)
-        fn = self._entries.get(key)
-        if fn is None:
-            fn = getattr(self._lib(source, defines), name)
-            fn.argtypes = [ctypes.c_char_p]
-            self._entries[key] = fn
+    def _entry(self, key, source: str, name: str, *defines: str):
+        """An exported function that takes its arguments packed into one block of bytes, looked up once and kept under `key` (twenty
+        arguments as ctypes objects were half of what such a call cost the host)."""
+        fn = getattr(self._lib(source, defines), name)
+        fn.argtypes = [ctypes.c_char_p]
+        self._entries[key] = fn
         return fn
 
     def shared_prefix_attention(self, q, cache_layer, meta: AttentionMeta, shared: SharedPrefixes, num_heads, num_kv_heads, head_dim,
@@ -598,11 +595,12 @@ class CudaKernels:
             # one buffer: the prefixes' sums, their maxima and denominators, and those of the own keys
             piece, pieces, own_ctas = self._own_pieces(B * num_kv_heads * -(-group // 8), max_own)
             own_rows = pieces * B * num_heads
-            scratch = torch.empty(((pre_rows + own_rows) * (head_dim + 2),), dtype=torch.float32, device=q.device)
+            scratch = q.new_empty((pre_rows + own_rows) * (head_dim + 2), dtype=torch.float32)
             pre = scratch.data_ptr()
             pre_ml = pre + 4 * pre_rows * head_dim
             own = pre_ml + 8 * pre_rows
-            st = self._entry("shared_attention_tcgen05.cu", (f"-DHEAD_DIM={head_dim}",), "rv_shared_attention_tcgen05")(_SHARED_ARGS.pack(
+            entry = self._entries.get(head_dim) or self._entry(head_dim, "shared_attention_tcgen05.cu", "rv_shared_attention_tcgen05", f"-DHEAD_DIM={head_dim}")
+            st = entry(_SHARED_ARGS.pack(
                 q.data_ptr(), cache_layer.data_ptr(), tables.data_ptr(), lens.data_ptr(), ints.data_ptr(), pre, pre_ml, own,
                 own + 4 * own_rows * head_dim, out.data_ptr(), sinks_at, gate_at, self._status.data_ptr(), stream, pages, B, tiles, items,
                 num_heads, num_kv_heads, head_dim, page, max_blocks,
@@ -612,11 +610,12 @@ class CudaKernels:
             return out
         splits = max(1, min(64, -(-max_own // 64), 4 * self.num_sms // (B * num_kv_heads)))
         own_rows = splits * B * num_heads
-        scratch = torch.empty(((pre_rows + own_rows) * (head_dim + 2),), dtype=torch.float32, device=q.device)
+        scratch = q.new_empty((pre_rows + own_rows) * (head_dim + 2), dtype=torch.float32)
         pre = scratch.data_ptr()
         pre_ml = pre + 4 * pre_rows * head_dim
         own = pre_ml + 8 * pre_rows
-        st = self._entry("shared_prefix.cu", (), "rv_shared_attention_plain")(_PLAIN_ARGS.pack(
+        entry = self._entries.get("plain") or self._entry("plain", "shared_prefix.cu", "rv_shared_attention_plain")
+        st = entry(_PLAIN_ARGS.pack(
             q.data_ptr(), cache_layer.data_ptr(), tables.data_ptr(), lens.data_ptr(), ints.data_ptr(), pre, pre_ml, own, own + 4 * own_rows * head_dim,
             out.data_ptr(), sinks_at, gate_at, stream, pages, B, tiles, items, num_heads, num_kv_heads, head_dim, page, max_blocks, splits, dt, scale, cap))
         _check("shared_attention_plain", st)
@@ -671,17 +670,21 @@ class CudaKernels:
         if num_tokens < 0 or max_blocks < 1 or page_size < 1 or G < 1 or B < 1 or R < 1 or width < 1:
             raise KernelError(f"step_tables: {num_tokens} tokens of {B} sequences, {max_blocks} blocks of {page_size}, a page table of {(G, R, width)}")
         if out is None:
-            # one allocation: block tables, slots, positions, sequences of the tokens, their starts, context lengths
-            parts = torch.empty((G * (B * max_blocks + num_tokens) + 2 * num_tokens + 2 * B + 1,), dtype=torch.int32, device=page_table.device
-                                ).split_with_sizes((G * B * max_blocks, G * num_tokens, num_tokens, num_tokens, B + 1, B))
-            out = StepTables(parts[0].view(G, B, max_blocks), parts[1].view(G, num_tokens), parts[2], parts[3], parts[4], parts[5])
+            # one allocation: block tables, slots, positions, sequences of the tokens, their starts, context lengths (the first two cut out
+            # by strides: a split and two views of its parts cost the host 1.3 us more)
+            entries = G * B * max_blocks
+            parts = page_table.new_empty(entries + (G + 2) * num_tokens + 2 * B + 1)
+            out = StepTables(parts.as_strided((G, B, max_blocks), (B * max_blocks, max_blocks, 1)),
+                             parts.as_strided((G, num_tokens), (num_tokens, 1), entries),
+                             *parts.split_with_sizes((entries + G * num_tokens, num_tokens, num_tokens, B + 1, B))[1:])
         else:
             for t, shape in ((out.block_tables, (G, B, max_blocks)), (out.slot_mapping, (G, num_tokens)), (out.positions, (num_tokens,)),
                              (out.token_seq, (num_tokens,)), (out.cu_seqlens, (B + 1,)), (out.ctx_lens, (B,))):
                 if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != here or not t.is_contiguous():
                     raise KernelError(f"step_tables: an output of shape {tuple(t.shape)} and {t.dtype} on {t.device} where contiguous int32 {shape} "
                                       f"on cuda:{here} is written")
-        st = self._entry("step_tables.cu", (), "rv_step_tables")(_TABLE_ARGS.pack(
+        entry = self._entries.get("tables") or self._entry("tables", "step_tables.cu", "rv_step_tables")
+        st = entry(_TABLE_ARGS.pack(
             page_table.data_ptr(), rows.data_ptr(), held.data_ptr(), starts.data_ptr(), q_lens.data_ptr(), new_pages.data_ptr(), spans.data_ptr(),
             out.block_tables.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.token_seq.data_ptr(),
             out.cu_seqlens.data_ptr(), out.ctx_lens.data_ptr(), G, B, R, width, new_pages.shape[0], num_tokens, max_blocks, page_size,

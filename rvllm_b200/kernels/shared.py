@@ -39,7 +39,7 @@ class SharedPrefixes:
     its set of sequences stays.  It takes part in no computation but `CudaKernels.shared_prefix_attention`.
 
     `capacity` = (row tiles, ranges of keys): fixes the size of the arrays, so that a captured graph serves other groups of
-    the same number of sequences ."""
+    the same number of sequences."""
 
     def __init__(self, groups, num_seqs: int, num_heads: int, num_kv_heads: int, device, capacity: Optional[Tuple[int, int]] = None,
                  num_sms: int = 148):
@@ -161,7 +161,7 @@ class StepPrefixes:
             made.refill(groups)
 
 
-@dataclass
+@dataclass(slots=True)
 class StepTables:
     """What `CudaKernels.step_tables` writes (int32, on the device)."""
     block_tables: torch.Tensor         # [groups, sequences, max_blocks]
