@@ -57,7 +57,7 @@ def _need(t: torch.Tensor, name: str, dtype=None, dims=None):
 
 # arguments of the entry points that take them as one block (the structures of the same names in csrc/)
 _SHARED_ARGS = struct.Struct("=15q12i2f")       # shared_attention_tcgen05.cu
-_PLAIN_ARGS = struct.Struct("=14q10i2f")       # shared_prefix.cu
+_PLAIN_ARGS = struct.Struct("=14q12i2f")       # shared_prefix.cu
 _TABLE_ARGS = struct.Struct("=13q8iq")         # step_tables.cu
 
 
@@ -608,8 +608,13 @@ class CudaKernels:
             _check("shared_attention_tcgen05", st)
             COUNTERS['launches'] += 1
             return out
+        # own keys in pieces of 64 or more; the ranges of the prefixes, cut for the tensor cores, in as many parts of 64 keys as two CTAs
+        # an SM take (a tile of 64 keys takes a CTA 5 us; 16 sequences behind 777 keys, 28 heads on 4: 25.9 us in ranges of two, 21.1 of one)
         splits = max(1, min(64, -(-max_own // 64), 4 * self.num_sms // (B * num_kv_heads)))
         own_rows = splits * B * num_heads
+        row_blocks = -(-shared.widest * group // 32)
+        cuts = max(1, min(shared.longest, (2 * self.num_sms - B * splits * num_kv_heads * -(-group // 8)) // (items * num_kv_heads * row_blocks)))
+        pre_rows *= cuts
         scratch = q.new_empty((pre_rows + own_rows) * (head_dim + 2), dtype=torch.float32)
         pre = scratch.data_ptr()
         pre_ml = pre + 4 * pre_rows * head_dim
@@ -617,7 +622,8 @@ class CudaKernels:
         entry = self._entries.get("plain") or self._entry("plain", "shared_prefix.cu", "rv_shared_attention_plain")
         st = entry(_PLAIN_ARGS.pack(
             q.data_ptr(), cache_layer.data_ptr(), tables.data_ptr(), lens.data_ptr(), ints.data_ptr(), pre, pre_ml, own, own + 4 * own_rows * head_dim,
-            out.data_ptr(), sinks_at, gate_at, stream, pages, B, tiles, items, num_heads, num_kv_heads, head_dim, page, max_blocks, splits, dt, scale, cap))
+            out.data_ptr(), sinks_at, gate_at, stream, pages, B, tiles, items, num_heads, num_kv_heads, head_dim, page, max_blocks,
+            row_blocks, cuts, splits, dt, scale, cap))
         _check("shared_attention_plain", st)
         COUNTERS['launches'] += 1
         return out

@@ -14,10 +14,14 @@ KEY_TILE = 64              # keys of a tile: ranges of keys begin at multiples o
 
 
 def _cut(tiles_of: Sequence[int], kv_heads: int, num_sms: int) -> int:
-    """Key tiles of a range: such that the ranges of all row tiles and kv heads are at most one CTA an SM, and no fewer than two
-    (a CTA costs about as much as three to set up and to merge); where that makes them longer than eight, two CTAs an SM."""
+    """Key tiles of a range: such that the ranges of all row tiles and kv heads are at most one CTA an SM, and no fewer than two where
+    that leaves more than six parts to merge (a CTA costs about as much as three tiles to set up and to merge; 3 sequences behind 324
+    tokens, 32 heads on 8: 10.7 us in ranges of two tiles, 9.2 of one; 82 behind up to 634, 28 heads on 4: 13.1 and 15.5); where one
+    CTA an SM makes them longer than eight, two CTAs an SM (2 to 5 % for prefixes of 8,000 and more; 64 sequences behind 2,048 tokens,
+    which have their own keys to read beside, 26.7 us with one and 29.4 with two)."""
     def least(places: int) -> int:
-        lo, hi = 2, max(max(tiles_of), 2)
+        lo = 1 if max(tiles_of) <= 6 else 2
+        hi = max(max(tiles_of), lo)
         while lo < hi:
             mid = (lo + hi) // 2
             if sum(-(-n // mid) for n in tiles_of) * kv_heads <= places:
@@ -51,14 +55,14 @@ class SharedPrefixes:
         # with a capacity the launches are sized for any groups that fit it
         self.capacity = capacity or (self.num_tiles, self.num_items)
         if capacity is not None:
-            self.most_parts, self.shortest = capacity[1], 0
+            self.most_parts, self.shortest, self.longest, self.widest = capacity[1], 0, 1, max(1, TILE_ROWS // (num_heads // num_kv_heads))
         self.device_ints = torch.from_numpy(host).to(device)
 
     def refill(self, groups) -> None:
         """Other groups of the same step size, into the same array (on the current stream)."""
-        most_parts, shortest = self.most_parts, self.shortest
+        kept = self.most_parts, self.shortest, self.longest, self.widest
         self.device_ints.copy_(torch.from_numpy(self._lay_out(groups, self.capacity)))
-        self.most_parts, self.shortest = most_parts, shortest
+        self.most_parts, self.shortest, self.longest, self.widest = kept
 
     @staticmethod
     def ints(num_seqs: int, capacity: Tuple[int, int]) -> int:
@@ -124,6 +128,8 @@ class SharedPrefixes:
             host[at:at + 8 * len(items)] = np.asarray(items, np.int32).ravel()
         self.num_items, self.num_tiles = len(items), len(tiles)
         self.most_parts = max((n for _, n in parts), default=0)
+        self.longest = step if tiles else 0          # key tiles of a range
+        self.widest = max((t[2] for t in tiles), default=0)               # sequences of a row tile
         # the fewest keys that any sequence has before its own begin (0: one has no prefix)
         self.shortest = min((t for _, t in kept), default=0) if len(flat) == B else 0
         return host
