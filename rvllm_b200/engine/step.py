@@ -33,13 +33,13 @@ from ..kernels.shared import StepPrefixes, StepTables
 SHARED_MOST_GROUPS = 8         # groups of a captured step: those that save the most
 # A decode step reads shared beginnings once, instead of as many times as requests hold them, where that is the faster way:
 # * bfloat16: the keys and values it saves a layer are this many bytes and half of those that it reads sequence by sequence.  32 heads of
-#   128 on 8, shared against each for itself: 16 requests with 16 keys of their own behind 256 (15.7 MB saved) 8.7 and 8.5 us, behind
-#   512 8.8 and 10.0, 8 behind 2,048 (59 MB) 10.7 and 12.7, 64 with 1,024 of their own (268 MB) behind 512 (132 MB) 62 and 55,
-#   behind 2,048 65 and 93, with 16 behind 8,192 25 and 225;
+#   128 on 8, shared against each for itself: 16 requests with 16 keys of their own behind 256 (15.7 MB saved) 8.3 and 8.5 us, behind
+#   512 9.0 and 10.0, 8 behind 2,048 (59 MB) 10.7 and 12.8, 64 with 1,024 of their own (268 MB) behind 512 (132 MB) 53 and 55,
+#   behind 2,048 58 and 94, with 16 behind 8,192 25 and 225;
 SHARED_MIN_BYTES = 24 << 20
-# * float32: some beginning is this long (28 heads of 128 on 4: 2 requests behind 256 25 and 14 us, behind 1,024 32 and 45, 16 behind
-#   1,024 31 and 104), or the bytes saved are two thirds of the above (64 behind 256: 37 and 103).
-SHARED_MIN_TOKENS_F32 = 512
+# * float32: some beginning is this long (28 heads of 128 on 4: 4 requests with 16 keys of their own behind 64 12.3 and 8.0 us, behind
+#   256 12.6 and 17.2, 16 behind 1,024 32 and 104), or the bytes saved are two thirds of the above (64 behind 64: 15.5 and 46).
+SHARED_MIN_TOKENS_F32 = 256
 
 
 @dataclass

@@ -323,7 +323,7 @@ def test_when_a_step_reads_shared_beginnings_once():
     assert not worth(half, 2, 64, 5) and not worth(half, 16, 256, 16) and worth(half, 16, 512, 16) and worth(half, 64, 2048, 1024)
     assert not worth(half, 64, 512, 1024) and worth(half, 4, 8192, 100)
     full = SimpleNamespace(cache=SimpleNamespace(dtype=torch.float32), _key_bytes=4096)
-    assert not worth(full, 2, 256, 5) and worth(full, 2, 1024, 5) and worth(full, 64, 256, 5)
+    assert not worth(full, 2, 128, 5) and worth(full, 2, 256, 5) and worth(full, 64, 64, 5)
 
 
 def test_pieces_of_the_own_keys():
