@@ -38,7 +38,7 @@ SHARED_MOST_GROUPS = 8         # groups of a captured step: those that save the 
 #   behind 2,048 58 and 94, with 16 behind 8,192 25 and 225;
 SHARED_MIN_BYTES = 24 << 20
 # * float32: some beginning is this long (28 heads of 128 on 4: 4 requests with 16 keys of their own behind 64 12.3 and 8.0 us, behind
-#   256 12.6 and 17.2, 16 behind 1,024 32 and 104), or the bytes saved are two thirds of the above (64 behind 64: 15.5 and 46).
+#   256 12.6 and 17.2, 16 behind 1,024 32 and 104), or the bytes saved are half of the above (64 behind 64: 15.5 and 46).
 SHARED_MIN_TOKENS_F32 = 256
 
 
@@ -383,7 +383,7 @@ class ModelRunner:
         saved = sum((len(m) - 1) * t for m, t in groups)
         own = keys - sum(len(m) * t for m, t in groups)
         if self.cache.dtype == torch.float32:
-            return max(t for _, t in groups) >= SHARED_MIN_TOKENS_F32 or saved * self._key_bytes >= SHARED_MIN_BYTES * 2 // 3
+            return max(t for _, t in groups) >= SHARED_MIN_TOKENS_F32 or saved * self._key_bytes >= SHARED_MIN_BYTES // 2
         return saved * self._key_bytes >= SHARED_MIN_BYTES + own * self._key_bytes // 2
 
     def _eager_shared(self, groups, num_seqs: int) -> StepPrefixes:
