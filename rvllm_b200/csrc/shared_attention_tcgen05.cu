@@ -12,18 +12,18 @@
 // One launch for both kinds, because neither fills the GPU alone: the prefixes' CTAs are few and busy with arithmetic, or many
 // and waiting for memory; the own keys are a latency (lengths, pages, keys, each after the other) repeated for every sequence.  An
 // SM holds two CTAs of either kind, the prefixes' are handed out first.  (As kernels of their own, one after the other, the 64
-// sequences behind 2,048 shared keys with 1 to 700 of their own took 41 to 55 us in several forms; see the table of the kernel.)
+// sequences behind 2,048 shared keys with 1 to 700 of their own took 41 to 55 us in several forms; together they take 26.7.)
 // Which rows and ranges there are is a list that the host makes once for a set of sequences: it changes when a request comes or
 // goes, not from step to step (shared_prefix.cuh).
 //
 // A CTA of the prefixes owns up to 128 rows (floor(128 / G) whole sequences) of one kv head and one range of the keys: S = Q K^T of
-// 64 keys into one of two buffers of tensor memory, one thread per row of softmax, P written back over S as bfloat16 pairs and read
-// from there as the A operand of O += P V; two loader warps (keys, values: TMA boxes through the block table) and two warps that
-// issue, as in attention_tcgen05.cu, which has the measurements behind this cut.  What differs: rows come from sequences that lie
-// anywhere in the batch (fetched by plain loads and swizzled by hand, while the first keys are on their way), keys behind the end of
-// a prefix inside its last page belong to somebody else (their values are set to zero, so that a NaN there does not meet a
-// probability of zero), and warps whose rows are all empty skip the softmax.
-// P is rounded to bfloat16 (2^-9 relative), as in every attention kernel of this library: the tensor core takes no wider A
+// 64 keys into tensor memory, which is free again as soon as the softmax warps have read it, one thread per row of softmax, P into one of
+// two buffers of tensor memory as bfloat16 pairs, read from there as the A operand of O += P V; two loader warps (keys, values: TMA
+// boxes through the block table) and two warps that issue, as in attention_tcgen05.cu, which has the measurements behind this cut.
+// What differs: rows come from sequences that lie anywhere in the batch (fetched by plain loads and swizzled by hand, while the first
+// keys are on their way), keys behind the end of a prefix inside its last page belong to somebody else (their values are set to
+// zero, so that a NaN there does not meet a probability of zero), and warps whose rows are all empty skip the softmax.
+// P is rounded to bfloat16 (2^-8 relative at most), as in every attention kernel of this library: the tensor core takes no wider A
 // beside a bfloat16 V; sums and maxima are float.
 //
 // The own keys: G rows against each key, so the bytes bound it (hd x 4 bytes a key and kv head) and what has to be won is latency: the
@@ -32,10 +32,18 @@
 // and asks for the next chunks (TMA, into stages of its own) across the ends of pieces, so that their memory latencies overlap.  The
 // products are turned over - S^T [16 keys x 8 heads] = K Q^T and O^T [16 dims x 8 heads] += V^T P^T on mma.sync, keys and values by
 // ldmatrix - so that a group of up to eight heads fills the narrow side (a larger group is cut into blocks of eight); P^T gets from
-// the layout of a result to that of an operand by two 8 x 8 transposes (movmatrix).  (Before, for 64 sequences with 1 to 700 own keys
-// of eight kv heads behind 2,048 shared ones, the whole step: a CTA per sequence and kv head, or several in a cluster, 41 to 70 us,
-// most of it set-up; a list of pieces whose keys went from global memory straight into registers 50 us, 8 to 13 us a piece of 64.)
+// the layout of a result to that of an operand by two 8 x 8 transposes (movmatrix).  (The legacy matrix instruction, because its tile
+// has a side of eight: a decoded token's G rows would leave most of tcgen05's 128 empty, and the time is the bytes'.  Before, the whole
+// step of the example: a CTA per sequence and kv head, or several in a cluster, 41 to 70 us, most of it set-up; a list of pieces whose
+// keys went from global memory straight into registers 50 us, 8 to 13 us a piece of 64.)
 // Keys outside a sequence, and pages that do not exist, count as not there.
+//
+// What it takes (one B200, heads of 128; time of both kernels in a graph, bytes or products that it cannot do without):
+//   4 sequences behind 32,768 keys, 32 heads on 8      33.2 us   136 MB, 4.1 TB/s (7 during the prefixes; the merge is 3 us)
+//   64 behind 2,048 with 1 to 700 of their own         26.7 us    49 MB, 1.8 TB/s: filling, the own keys' second half, the merge
+//   256 behind 16,384                                  93.7 us   69 GFLOP, 0.74 PFLOP/s (0.44 of measured): the softmax warps' chain, some
+//                                                               1,900 cycles a tile of 64 keys with two CTAs an SM (tensor pipe busy 40 %)
+//   8 behind 1,003, 28 heads on 4                      10.1 us   two launches and the latencies of one range
 // Cache layer layout: [num_pages, 2 (k, v), nkv, page_size, HEAD_DIM].
 #include "common.cuh"
 #include "shared_prefix.cuh"
@@ -761,7 +769,8 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
 // ---------------------------------------------------------------------------------------------
 // The sums of a row put together: WARPS warps per (sequence, head), which take its parts in turn, four neighbouring columns a lane
 // and MERGE_BATCH parts' loads in flight.  What it costs is round trips to L2 - a row of 45 parts takes one warp six - and waves of
-// blocks: so as many warps a row as still leave one wave.
+// blocks: so as many warps a row as still leave one wave (both kernels with 1 / 2 / 4 warps a row, us: 8 sequences of 28 heads, 18 parts
+// 11.8 / 10.7 / 10.1; 4 of 32, 57 parts 38.5 / 35.0 / 33.2; 64 of 32, 22 parts 28.9 / 26.7 / 29.8; 256 of 32, 34 parts 93.7 / 99 / 110).
 template <int WARPS>
 __global__ void __launch_bounds__(128, MERGE_BLOCKS)
 shared_merge_kernel(const SharedParams p, const float* __restrict__ sinks, const float* __restrict__ gate, __nv_bfloat16* __restrict__ out) {

@@ -7,11 +7,12 @@
 #include "shared_prefix.cuh"
 
 // ---------------------------------------------------------------------------------------------
-// The plain kernel of both parts: 32-bit products and sums, one CTA per (row block, kv head, range of keys).  The rows of a CTA share
-// the keys, so a tile of 32 keys and values goes to shared memory once and meets 8 * RPW rows: a warp owns RPW rows, its lanes the
-// 32 keys of the tile for the scores and hd / 32 columns for the sums.  In float32 the arithmetic bounds it (no tensor core takes
-// 32 bits); RPW = 4 reads five shared words per four multiply-adds each, RPW = 1 serves the few rows of one sequence.  Both parts are
-// one launch, the prefixes' CTAs first.
+// The plain kernel of both parts: 32-bit products and sums (no tensor core takes 32 bits), both parts in one launch, the prefixes' CTAs
+// first.  Arithmetic bounds it, or rather how often a word has to be read from shared memory for it: a CTA of the prefixes takes 32
+// rows and 64 keys at a time, in register tiles (2.2 us a tile at the rate of the multiply-adds of an SM; a tile more a CTA takes 5); the
+// rows of a sequence's own keys are few, a warp has one.  16 sequences behind 777 shared keys, 28 heads of 128 on 4: 21.3 us in a
+// graph, 15.7 of them in this kernel, for 181 MFLOP (2.4 us of the GPU's multiply-adds, 4.5 MB): launches and the latencies of one tile
+// per CTA.  (Before, a lane per key and a warp per four rows, both operands read once per four multiply-adds: 31.2.)
 #define PLAIN_THREADS 256
 #define PLAIN_TILE 32
 #define PLAIN_MAX_DIM 256

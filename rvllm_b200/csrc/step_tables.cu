@@ -13,9 +13,13 @@
 // One launch, no order between its CTAs: where a sequence's pages begin in the list, and its tokens in the step, are sums over
 // the sequences before it, which every CTA forms for itself (integers: any order gives the same), and an entry that is new in
 // this step is read from the list, never from the row that another CTA may be writing.  A CTA takes 1, 2, 4 or 8 neighbouring
-// sequences of one group, with 256, 128, 64 or 32 threads each: one while the CTAs find room at once, more where the sums, which
-// a CTA forms once, would be what it spends its time on.  Every index that comes from device memory is checked against its bound;
-// an entry that would lie outside counts as absent (-1).
+// sequences of one group, with 256, 128, 64 or 32 threads each: one while the CTAs find room at once (four an SM), more where the
+// sums, which a CTA forms once, would be what it spends its time on.  Every index that comes from device memory is checked against its
+// bound; an entry that would lie outside counts as absent (-1).
+// What bounds it is latency - a launch, the lengths, the sums, the entries, each behind the other - and from a few hundred sequences on
+// the sums, not the bytes.  GPU time in graphs with 1 / 2 / 4 / 8 sequences a CTA, us: 64 decoded tokens in contexts up to 32,767 (0.6 MB)
+// 4.5 / 6.5 / 8.7 / 14; 800 in contexts up to 8,000 7.2 / 5.7 / 6.7 / 8.7; 2,000 21 / 15.9 / 9.7 / 11.2; 1,024 in two groups with
+// portions (18 MB) 16.9 / 13.5 / 12.3 / 18.7, which is 1.5 TB/s.
 #include "common.cuh"
 
 #define TABLE_THREADS 256
@@ -49,7 +53,7 @@ __global__ void __launch_bounds__(TABLE_THREADS)
 step_tables_kernel(const TableParams p) {
     constexpr int THREADS = TABLE_THREADS / PER;             // of a sequence
     __shared__ unsigned sums[2][TABLE_THREADS / 32];
-    __shared__ unsigned own[2][PER];                              // new pages and tokens of this CTA's sequences
+    __shared__ unsigned own[2][PER];                         // new pages and tokens of this CTA's sequences
     rv_pdl_wait();
     const int tid = threadIdx.x, g = blockIdx.y, b0 = blockIdx.x * PER;
     // pages taken before this CTA's first sequence (all groups before g, then the sequences before b0), tokens before it (unsigned, as
