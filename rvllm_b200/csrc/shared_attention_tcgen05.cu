@@ -770,7 +770,7 @@ __device__ __forceinline__ void own_keys(const SharedParams& p, const CUtensorMa
 // The sums of a row put together: WARPS warps per (sequence, head), which take its parts in turn, four neighbouring columns a lane
 // and MERGE_BATCH parts' loads in flight.  What it costs is round trips to L2 - a row of 45 parts takes one warp six - and waves of
 // blocks: so as many warps a row as still leave one wave (both kernels with 1 / 2 / 4 warps a row, us: 8 sequences of 28 heads, 18 parts
-// 11.8 / 10.7 / 10.1; 4 of 32, 57 parts 38.5 / 35.0 / 33.2; 64 of 32, 22 parts 28.9 / 26.7 / 29.8; 256 of 32, 34 parts 93.7 / 99 / 110).
+// 11.8 / 10.7 / 10.1; 4 of 32, 57 parts 38.5 / 35.0 / 33.2; 64 of 32, 14 parts 28.9 / 26.7 / 29.8; 256 of 32, 6 parts 93.7 / 99 / 110).
 template <int WARPS>
 __global__ void __launch_bounds__(128, MERGE_BLOCKS)
 shared_merge_kernel(const SharedParams p, const float* __restrict__ sinks, const float* __restrict__ gate, __nv_bfloat16* __restrict__ out) {
