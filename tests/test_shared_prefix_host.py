@@ -314,6 +314,18 @@ def test_a_request_is_one_sample(emulated):
     assert [len(o.token_ids) for o in out.outputs] == [4, 4] and out.outputs[0].token_ids == out.outputs[1].token_ids
 
 
+def test_samples_on_the_command_line(emulated, monkeypatch, capsys):
+    import json
+    from model_tools import model_folder
+    from rvllm_b200 import LLM, cli
+    made = []
+    monkeypatch.setattr(cli, "_llm", lambda args, **kw: made.append(args) or LLM(
+        args.model, dtype="float32", device="cpu", block_size=8, num_blocks=32, max_model_len=64, max_num_seqs=3, share_prefixes=args.share_prefixes))
+    assert cli.main(["generate", "--model", model_folder("tiny_llama"), "--prompt-ids", "1,2,3", "--max-tokens", "4", "--n", "2", "--share-prefixes"]) == 0
+    lines = [json.loads(x) for x in capsys.readouterr().out.splitlines()]
+    assert made[0].share_prefixes and [x["sample"] for x in lines] == [0, 1] and lines[0]["token_ids"] == lines[1]["token_ids"]
+
+
 def test_when_a_step_reads_shared_beginnings_once():
     """The rule, at the sizes of a layer of 8 key/value heads of 128 in bfloat16 (4 KB a key) and of 4 in float32."""
     from types import SimpleNamespace
