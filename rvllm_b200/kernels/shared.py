@@ -43,7 +43,7 @@ class SharedPrefixes:
     its set of sequences stays.  It takes part in no computation but `CudaKernels.shared_prefix_attention`.
 
     `capacity` = (row tiles, ranges of keys): fixes the size of the arrays, so that a captured graph serves other groups of
-    the same number of sequences."""
+    the same number of sequences (`refill`).  Without one the launches are sized for the groups given here, and these stay."""
 
     def __init__(self, groups, num_seqs: int, num_heads: int, num_kv_heads: int, device, capacity: Optional[Tuple[int, int]] = None,
                  num_sms: int = 148):
@@ -53,13 +53,17 @@ class SharedPrefixes:
         self.num_sms = num_sms
         host = self._lay_out(groups, capacity)
         # with a capacity the launches are sized for any groups that fit it
+        self.refillable = capacity is not None
         self.capacity = capacity or (self.num_tiles, self.num_items)
         if capacity is not None:
             self.most_parts, self.shortest, self.longest, self.widest = capacity[1], 0, 1, max(1, TILE_ROWS // (num_heads // num_kv_heads))
         self.device_ints = torch.from_numpy(host).to(device)
 
     def refill(self, groups) -> None:
-        """Other groups of the same step size, into the same array (on the current stream)."""
+        """Other groups of the same step size, into the same array (on the current stream).  It takes a capacity given when the object
+        was made: otherwise a launch is sized for the first groups (their widest row tile decides how many rows are computed at all)."""
+        if not self.refillable:
+            raise KernelError("shared prefixes: laid out for the groups they were made with; other groups need a capacity or a new object")
         kept = self.most_parts, self.shortest, self.longest, self.widest
         self.device_ints.copy_(torch.from_numpy(self._lay_out(groups, self.capacity)))
         self.most_parts, self.shortest, self.longest, self.widest = kept

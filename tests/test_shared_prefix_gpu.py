@@ -285,6 +285,18 @@ def test_captured_and_replayed_with_other_groups():
     assert float(((out.cpu().to(F64) - want).abs() / tol).max()) <= 1.0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_refilled_with_wider_groups(dtype):
+    """A layout with a capacity, made for two sequences behind a short prefix, serves sixteen: every row of their tile is computed."""
+    s = make([(16, 64)], 0, 16, 4, 128, 16, dtype, seed=21, own=(1, 30))
+    shared = SharedPrefixes([([0, 1], 64)], 16, 16, 4, "cuda", capacity=(3, 12))
+    check(s, shared=shared)
+    shared.refill(s["plan"])
+    check(s, shared=shared)
+    shared.refill([])
+    check(s, shared=shared)
+
+
 def test_on_another_stream_and_twice_at_once():
     a = make([(30, 600)], 2, 32, 8, 128, 16, torch.bfloat16, seed=11, own=(1, 100))
     b = make([(30, 333)], 2, 32, 8, 128, 16, torch.bfloat16, seed=12, own=(1, 100))

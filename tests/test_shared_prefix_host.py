@@ -176,6 +176,23 @@ def test_beginnings_within_one_another():
         assert len({tuple(m.block_table(i, 0)[:t]) for i in ms}) == 1
 
 
+def test_other_groups_need_a_capacity():
+    """Without one a launch is sized for the first groups: sixteen members where two were would leave rows of a tile uncomputed."""
+    wide = [(list(range(16)), 64)]
+    exact = SharedPrefixes([([0, 1], 64)], 16, 16, 4, "cpu")
+    before = exact.device_ints.clone()
+    with pytest.raises(KernelError):
+        exact.refill(wide)
+    assert torch.equal(exact.device_ints, before) and exact.widest == 2
+    roomy = SharedPrefixes([([0, 1], 64)], 16, 16, 4, "cpu", capacity=(2, 8))
+    assert roomy.widest == 32                        # whatever the groups, every row of a tile is computed
+    roomy.refill(wide)
+    again = SharedPrefixes(wide, 16, 16, 4, "cpu", capacity=(2, 8))
+    assert torch.equal(roomy.device_ints, again.device_ints)
+    sizes = lambda p: (p.capacity, p.most_parts, p.shortest, p.longest, p.widest)  # noqa: E731
+    assert sizes(roomy) == sizes(again)
+
+
 # ------------------------------------------------------------------------------------------------------------- scheduling
 def scheduler(num_pages=64, page=4, max_seqs=8, budget=64, chunk=None, chunked=True, share=True, max_len=256):
     from rvllm_b200.cache import CacheManager
