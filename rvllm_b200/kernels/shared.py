@@ -51,22 +51,31 @@ class SharedPrefixes:
             raise KernelError(f"shared prefixes: {num_seqs} sequences of {num_heads} heads on {num_kv_heads} key/value heads")
         self.num_seqs, self.num_heads, self.num_kv_heads = num_seqs, num_heads, num_kv_heads
         self.num_sms = num_sms
-        host = self._lay_out(groups, capacity)
-        # with a capacity the launches are sized for any groups that fit it
         self.refillable = capacity is not None
+        host, (self.num_tiles, self.num_items), sizes = self._lay_out(groups, capacity)
+        # with a capacity the launches are sized for any groups that fit it
         self.capacity = capacity or (self.num_tiles, self.num_items)
         if capacity is not None:
-            self.most_parts, self.shortest, self.longest, self.widest = capacity[1], 0, 1, max(1, TILE_ROWS // (num_heads // num_kv_heads))
+            sizes = capacity[1], 0, 1, max(1, TILE_ROWS // (num_heads // num_kv_heads))
+        # the most ranges of a row tile, the fewest keys that any sequence has before its own begin (0: one has no prefix), key tiles of
+        # a range, sequences of a row tile
+        self.most_parts, self.shortest, self.longest, self.widest = sizes
         self.device_ints = torch.from_numpy(host).to(device)
 
     def refill(self, groups) -> None:
         """Other groups of the same step size, into the same array (on the current stream).  It takes a capacity given when the object
         was made: otherwise a launch is sized for the first groups (their widest row tile decides how many rows are computed at all)."""
+        self.write(self.other(groups))
+
+    def other(self, groups):
+        """The array of other groups, as `write` takes it; nothing here changes."""
         if not self.refillable:
             raise KernelError("shared prefixes: laid out for the groups they were made with; other groups need a capacity or a new object")
-        kept = self.most_parts, self.shortest, self.longest, self.widest
-        self.device_ints.copy_(torch.from_numpy(self._lay_out(groups, self.capacity)))
-        self.most_parts, self.shortest, self.longest, self.widest = kept
+        return self._lay_out(groups, self.capacity)[:2]
+
+    def write(self, laid_out) -> None:
+        host, (self.num_tiles, self.num_items) = laid_out
+        self.device_ints.copy_(torch.from_numpy(host))
 
     @staticmethod
     def ints(num_seqs: int, capacity: Tuple[int, int]) -> int:
@@ -79,7 +88,8 @@ class SharedPrefixes:
         """int32 [num_seqs] on the device: the first token of each sequence that lies behind its prefix."""
         return self.device_ints[4:4 + self.num_seqs]
 
-    def _lay_out(self, groups, capacity) -> np.ndarray:
+    def _lay_out(self, groups, capacity):
+        """(the array, its row tiles and ranges in use, the sizes that a launch for these groups alone goes by)"""
         B, per = self.num_seqs, self.num_heads // self.num_kv_heads
         seen = set()
         kept = []
@@ -130,13 +140,9 @@ class SharedPrefixes:
             host[4 + 3 * B:4 + 3 * B + 2 * len(tiles)] = np.asarray(parts, np.int32).ravel()
             at = (4 + 3 * B + 2 * capacity[0] + 3) // 4 * 4
             host[at:at + 8 * len(items)] = np.asarray(items, np.int32).ravel()
-        self.num_items, self.num_tiles = len(items), len(tiles)
-        self.most_parts = max((n for _, n in parts), default=0)
-        self.longest = step if tiles else 0          # key tiles of a range
-        self.widest = max((t[2] for t in tiles), default=0)               # sequences of a row tile
-        # the fewest keys that any sequence has before its own begin (0: one has no prefix)
-        self.shortest = min((t for _, t in kept), default=0) if len(flat) == B else 0
-        return host
+        sizes = (max((n for _, n in parts), default=0), min((t for _, t in kept), default=0) if len(flat) == B else 0,
+                 step if tiles else 0, max((t[2] for t in tiles), default=0))
+        return host, (len(tiles), len(items)), sizes
 
 
 class StepPrefixes:
@@ -166,9 +172,11 @@ class StepPrefixes:
             return
         if self.most_groups is None or len(groups) > self.most_groups:
             raise KernelError(f"shared prefixes: {len(groups)} groups where {self.most_groups} fit")
+        # all layouts first: groups that one of them refuses leave the arrays, and what this object takes them to hold, as they were
+        laid_out = [(made, made.other(groups)) for made in self._layouts.values()]
+        for made, host in laid_out:
+            made.write(host)
         self.groups = groups
-        for made in self._layouts.values():
-            made.refill(groups)
 
 
 @dataclass(slots=True)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from rvllm_b200.errors import KernelError
-from rvllm_b200.kernels import SharedPrefixes
+from rvllm_b200.kernels import SharedPrefixes, StepPrefixes
 
 
 def unpack(s):
@@ -191,6 +191,20 @@ def test_other_groups_need_a_capacity():
     assert torch.equal(roomy.device_ints, again.device_ints)
     sizes = lambda p: (p.capacity, p.most_parts, p.shortest, p.longest, p.widest)  # noqa: E731
     assert sizes(roomy) == sizes(again)
+
+
+def test_refused_groups_leave_a_step_as_it_was():
+    """Groups that a layout refuses are refused again, and all arrays still hold the groups before."""
+    step = StepPrefixes([([0, 1], 64)], 4, "cpu", 2)
+    made = [step.layout(4, 2), step.layout(6, 1)]
+    before = [m.device_ints.clone() for m in made]
+    for bad in ([([0, 9], 64)], [([0, 1], 64), ([1, 2], 64)], [([0, 1], 8), ([2], 4), ([3], 4)], [([0, 1], -1)]):
+        for _ in range(2):
+            with pytest.raises(KernelError):
+                step.set_groups(bad)
+        assert step.groups == [([0, 1], 64)] and all(torch.equal(m.device_ints, b) for m, b in zip(made, before))
+    step.set_groups([([2, 3], 128)])
+    assert step.groups == [([2, 3], 128)] and made[0].own_start.tolist() == made[1].own_start.tolist() == [0, 0, 128, 128]
 
 
 # ------------------------------------------------------------------------------------------------------------- scheduling
