@@ -152,8 +152,14 @@ class StepPrefixes:
     graph holds them."""
 
     def __init__(self, groups, num_seqs: int, device, most_groups: Optional[int] = None, num_sms: int = 148):
-        self.groups, self.num_seqs, self.device, self.most_groups, self.num_sms = groups, num_seqs, device, most_groups, num_sms
+        self.groups = self._own(groups)
+        self.num_seqs, self.device, self.most_groups, self.num_sms = num_seqs, device, most_groups, num_sms
         self._layouts = {}
+
+    @staticmethod
+    def _own(groups):
+        """A copy: the caller may go on with its lists."""
+        return [(list(members), tokens) for members, tokens in groups]
 
     def layout(self, num_heads: int, num_kv_heads: int) -> SharedPrefixes:
         made = self._layouts.get((num_heads, num_kv_heads))
@@ -168,6 +174,7 @@ class StepPrefixes:
         return made
 
     def set_groups(self, groups) -> None:
+        groups = self._own(groups)
         if groups == self.groups:
             return
         if self.most_groups is None or len(groups) > self.most_groups:

@@ -207,6 +207,21 @@ def test_refused_groups_leave_a_step_as_it_was():
     assert step.groups == [([2, 3], 128)] and made[0].own_start.tolist() == made[1].own_start.tolist() == [0, 0, 128, 128]
 
 
+def test_a_step_keeps_groups_of_its_own():
+    """A caller that goes on with its lists finds what it then sets in the arrays."""
+    members = [0, 1]
+    groups = [(members, 64)]
+    step = StepPrefixes(groups, 4, "cpu", 2)
+    made = step.layout(4, 2)
+    members.append(2)
+    step.set_groups(groups)
+    assert made.own_start.tolist() == [64, 64, 64, 0]
+    groups.append(([2], 8))
+    groups[0] = ([3, 1], 128)
+    step.set_groups(groups)
+    assert made.own_start.tolist() == [0, 128, 0, 128]
+
+
 # ------------------------------------------------------------------------------------------------------------- scheduling
 def scheduler(num_pages=64, page=4, max_seqs=8, budget=64, chunk=None, chunked=True, share=True, max_len=256):
     from rvllm_b200.cache import CacheManager
