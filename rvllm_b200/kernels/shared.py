@@ -33,6 +33,13 @@ def _cut(tiles_of: Sequence[int], kv_heads: int, num_sms: int) -> int:
     return one if one <= 8 else least(2 * num_sms)
 
 
+def _staged(host: np.ndarray, device) -> torch.Tensor:
+    """The array in memory that a copy to `device` reads without making the host wait for the stream (which as a rule is at work on the
+    step before).  Pinned memory from torch's host allocator, which does not hand it out again before the copy has been done."""
+    t = torch.from_numpy(host)
+    return t.pin_memory() if torch.device(device).type == "cuda" else t
+
+
 class SharedPrefixes:
     """The groups of a step's sequences whose first tokens are the same cached ones, laid out for the kernels.
 
@@ -60,7 +67,7 @@ class SharedPrefixes:
         # the most ranges of a row tile, the fewest keys that any sequence has before its own begin (0: one has no prefix), key tiles of
         # a range, sequences of a row tile
         self.most_parts, self.shortest, self.longest, self.widest = sizes
-        self.device_ints = torch.from_numpy(host).to(device)
+        self.device_ints = _staged(host, device).to(device, non_blocking=True)
 
     def refill(self, groups) -> None:
         """Other groups of the same step size, into the same array (on the current stream).  It takes a capacity given when the object
@@ -75,7 +82,7 @@ class SharedPrefixes:
 
     def write(self, laid_out) -> None:
         host, (self.num_tiles, self.num_items) = laid_out
-        self.device_ints.copy_(torch.from_numpy(host))
+        self.device_ints.copy_(_staged(host, self.device_ints.device), non_blocking=True)
 
     @staticmethod
     def ints(num_seqs: int, capacity: Tuple[int, int]) -> int:

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from rvllm_b200.errors import KernelError
-from rvllm_b200.kernels import AttentionMeta, SharedPrefixes, get_library
+from rvllm_b200.kernels import AttentionMeta, SharedPrefixes, StepPrefixes, get_library
 
 pytestmark = pytest.mark.gpu
 
@@ -295,6 +295,30 @@ def test_refilled_with_wider_groups(dtype):
     check(s, shared=shared)
     shared.refill([])
     check(s, shared=shared)
+
+
+def test_groups_are_sent_while_the_device_is_busy():
+    """New groups and new layouts travel on the stream: the host does not wait for what was launched before them, and one after the
+    other arrive as they were."""
+    plans = [[(list(range(n)), 64 * n), (list(range(n, 60)), 100)] for n in (3, 20, 41)]
+    make_one = lambda plan: SharedPrefixes(plan, 64, 32, 8, "cuda", capacity=(20, 80))  # noqa: E731
+    want = [make_one(p).device_ints.cpu() for p in plans]
+    shared, step = make_one([]), StepPrefixes([], 64, "cuda", 4)
+    layout = step.layout(32, 8)
+    torch.cuda.synchronize()
+    copies = []
+    torch.cuda._sleep(200_000_000)                   # about a tenth of a second
+    busy = torch.cuda.Event()
+    busy.record()
+    for p in plans:
+        shared.refill(p)
+        copies.append(shared.device_ints.clone())
+    step.set_groups(plans[0])
+    late = make_one(plans[2])
+    assert not busy.query(), "the host waited for the device"
+    torch.cuda.synchronize()
+    assert all(torch.equal(c.cpu(), w) for c, w in zip(copies, want)) and torch.equal(late.device_ints.cpu(), want[2])
+    assert layout.own_start.tolist() == want[0][4:68].tolist()
 
 
 def test_on_another_stream_and_twice_at_once():
