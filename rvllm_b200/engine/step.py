@@ -82,7 +82,8 @@ class ModelRunner:
         # that eager steps have for these groups
         self._groups_of = (None, [])
         self._eager_prefixes: Optional[StepPrefixes] = None
-        needs = [g.need for g in cache.groups]
+        # bytes of a key and its value in the largest of the groups whose shared beginnings are read once (0: there is no such group)
+        needs = [g.need for g in cache.groups if self._reads_once(g.need)]
         self._key_bytes = max((n.num_kv_heads * n.row_elements for n in needs), default=0) * torch.empty((), dtype=cache.dtype).element_size()
         self._page_table = None
         if cache.groups and self.device.type == "cuda" and hasattr(kernels, "step_tables"):
@@ -365,11 +366,16 @@ class ModelRunner:
         return ctx
 
     # ---- beginnings that requests share ----------------------------------------------------------
+    def _reads_once(self, need) -> bool:
+        """Whether the attention of a cache group reads beginnings that sequences share once."""
+        rule = getattr(self.kernels, "reads_prefixes_once", None)
+        return rule is not None and rule(self.cache.dtype, need.num_kv_heads, need.head_dim, self.cache.page_size, self.cache.num_pages, self.cache.max_seqs)
+
     def _shared_groups(self, entries, starts):
         """(places, tokens) per group of entries that begin with the same cached tokens, for a step of decoded tokens; none where it
         would not pay.  Pages that are shared stay as they are while their requests live, so the groups hold until the set of
         requests changes."""
-        if not self.cache.can_share or self._page_table is None or any(len(e.tokens) != 1 for e in entries):
+        if not self._key_bytes or not self.cache.can_share or self._page_table is None or any(len(e.tokens) != 1 for e in entries):
             return []
         reqs = (self.cache.changes, tuple(e.req_id for e in entries))
         if reqs != self._groups_of[0]:

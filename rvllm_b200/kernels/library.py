@@ -325,12 +325,13 @@ class CudaKernels:
         softmax denominator; `gate` (float [tokens, heads]): multiplies each head's output; `distance_bias` (a
         `parts.distance.DistanceBias`): added to a score by the distance between query and key, after the cap.
 
-        A step whose sequences share beginnings (`meta.shared`) goes to `shared_prefix_attention`.
+        A step whose sequences share beginnings (`meta.shared`) goes to `shared_prefix_attention` where that gains (`reads_prefixes_once`).
         bfloat16 with a head size that is a multiple of 16 and pages of a power of two go to the
         tensor-core flash kernel (one token per sequence: the decode tiling, keys split over CTAs
         when the batch alone cannot fill the GPU); everything else goes to the plain kernel."""
         page = cache_layer.shape[3]
-        if meta.shared is not None and meta.max_q_len == 1 and window is None and distance_bias is None and num_heads // num_kv_heads <= TILE_ROWS:
+        if meta.shared is not None and meta.max_q_len == 1 and window is None and distance_bias is None and num_heads // num_kv_heads <= TILE_ROWS \
+                and self.reads_prefixes_once(q.dtype, num_kv_heads, head_dim, page, cache_layer.shape[0], meta.num_seqs):
             return self.shared_prefix_attention(q, cache_layer, meta, meta.shared.layout(num_heads, num_kv_heads), num_heads, num_kv_heads,
                                                 head_dim, scale, softcap, sinks, gate, meta.max_own_len)
         extras = softcap is not None or sinks is not None or gate is not None or distance_bias is not None
@@ -525,6 +526,23 @@ class CudaKernels:
         self._entries[key] = fn
         return fn
 
+    @staticmethod
+    def _prefixes_on_tensor_cores(dtype, num_kv_heads: int, head_dim: int, page: int, pages: int, num_seqs: int) -> bool:
+        """Whether the tcgen05 kernel takes a step's shared beginnings."""
+        return dtype == torch.bfloat16 and head_dim in (64, 128) and page & (page - 1) == 0 and page >= 8 and \
+            pages * 2 * num_kv_heads * page < 2 ** 31 and num_seqs <= 2048
+
+    def reads_prefixes_once(self, dtype, num_kv_heads: int, head_dim: int, page: int, pages: int, num_seqs: int) -> bool:
+        """Whether `paged_attention` gives a step's shared beginnings to `shared_prefix_attention`: in float32, and in bfloat16 on the
+        tcgen05 kernel.  Other bfloat16 heads and pages would have them on the plain kernel's multiply-adds, while the tensor-core decode kernel
+        takes each sequence for itself.  us each for itself / shared, 64 sequences, 32 heads on 32, 32 on 8 and 16 on 1: heads of 96 behind
+        2,048 with 600 keys of their own 360 / 647, 97 / 239 and 25 / 95, with 16 285 / 126, 79 / 96 and 23 / 56, behind 8,192 with 16 1,688 /
+        339, 290 / 309 and 59 / 179; heads of 80, 256 and 32 alike.  (What gains there is one query head on a kv head with next to
+        no keys of its own.)  In float32 both are multiply-adds."""
+        if dtype == torch.float32:
+            return head_dim % 4 == 0 and head_dim <= 256
+        return self._prefixes_on_tensor_cores(dtype, num_kv_heads, head_dim, page, pages, num_seqs)
+
     def shared_prefix_attention(self, q, cache_layer, meta: AttentionMeta, shared: SharedPrefixes, num_heads, num_kv_heads, head_dim,
                                 scale: float, softcap: Optional[float] = None, sinks: Optional[torch.Tensor] = None,
                                 gate: Optional[torch.Tensor] = None, max_own: Optional[int] = None) -> torch.Tensor:
@@ -575,8 +593,7 @@ class CudaKernels:
                 if t is not None and t.get_device() != here:
                     raise KernelError(f"shared_prefix_attention: sinks or gate on {t.device}, the current device is cuda:{here}")
         group = num_heads // num_kv_heads
-        fast = dt == 1 and head_dim in (64, 128) and page & (page - 1) == 0 and page >= 8 and pages * 2 * num_kv_heads * page < 2 ** 31 \
-            and B <= 2048
+        fast = self._prefixes_on_tensor_cores(dtype, num_kv_heads, head_dim, page, pages, B)
         tiles, items = shared.capacity
         if items == 0 or B == 0 or group > TILE_ROWS or not (fast or (head_dim % 4 == 0 and head_dim <= 256)):
             whole = meta

@@ -236,6 +236,22 @@ def test_without_groups_it_is_the_paged_attention():
     assert alone.capacity == (0, 0) and torch.equal(run(s, shared=alone), want)
 
 
+@pytest.mark.parametrize("dtype,hd,page,once", [(torch.bfloat16, 96, 16, False), (torch.bfloat16, 80, 16, False), (torch.bfloat16, 256, 16, False),
+                                                (torch.bfloat16, 128, 4, False), (torch.bfloat16, 128, 16, True), (torch.float32, 96, 16, True)])
+def test_which_steps_paged_attention_reads_once(dtype, hd, page, once, monkeypatch):
+    """Heads and pages that the tensor-core kernel of shared beginnings does not take stay with the one that takes each sequence for itself."""
+    s = make([(6, 96)], 1, 8, 2, hd, page, dtype, seed=hd, own=(1, 50), stale="0")
+    calls, original = [], lib().shared_prefix_attention
+    monkeypatch.setattr(lib(), "shared_prefix_attention", lambda *a, **kw: (calls.append(1), original(*a, **kw))[1])
+    call = lambda: lib().paged_attention(s["q"], s["cache"], s["meta"], 8, 2, hd, hd ** -0.5, None)  # noqa: E731
+    want = call()
+    s["meta"].shared = StepPrefixes(s["plan"], 7, "cuda")
+    got = call()
+    assert len(calls) == once and (once or torch.equal(got, want))
+    exact, tol = plain(s, hd ** -0.5)
+    assert float(((got.cpu().to(F64) - exact).abs() / tol).max()) <= 1.0
+
+
 def test_pages_that_do_not_exist_are_not_read():
     """Entries beyond the cache or negative inside the prefix: no result is promised, and nothing outside the cache is touched."""
     for dtype in (torch.bfloat16, torch.float32):

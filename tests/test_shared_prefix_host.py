@@ -384,6 +384,41 @@ def test_when_a_step_reads_shared_beginnings_once():
     assert not worth(full, 2, 128, 5) and worth(full, 2, 256, 5) and worth(full, 64, 64, 5)
 
 
+def runner(needs, dtype, page=16, num_pages=300, max_seqs=8):
+    """A step function over a cache without tensors, whose device tables are taken to exist, and the kernel library's own rules."""
+    from rvllm_b200.cache import CacheManager
+    from rvllm_b200.engine.step import ModelRunner
+    from rvllm_b200.kernels.library import CudaKernels
+    cache = CacheManager(needs, num_pages, page, max_seqs, dtype, "cpu", allocate=False)
+    r = ModelRunner(None, cache, CudaKernels.__new__(CudaKernels), 4096, "cpu")
+    r._page_table = torch.zeros(1)
+    r._worth_sharing = lambda groups, keys: True
+    return r
+
+
+def decoded(r, tokens=64, n=3):
+    """(entries, starts) of a decode step of n requests that share their first `tokens` tokens."""
+    from rvllm_b200.engine import StepEntry
+    r.cache.admit(0); r.cache.append(0, tokens)
+    for i in range(1, n):
+        r.cache.admit(i); r.cache.share(i, 0, tokens)
+    return [StepEntry(i, [1], (0,)) for i in range(n)], [r.cache.append(i, 1) for i in range(n)]
+
+
+def test_heads_whose_shared_beginnings_are_read_once():
+    """bfloat16 heads and pages that the tensor-core kernel does not take stay with the decode kernel that does take them."""
+    from rvllm_b200.parts import KvCacheNeed
+    bf, f32 = torch.bfloat16, torch.float32
+    for dtype, head, page, shares in ((bf, 128, 16, True), (bf, 64, 8, True), (bf, 96, 16, False), (bf, 80, 16, False), (bf, 256, 16, False),
+                                      (bf, 32, 16, False), (bf, 128, 4, False), (bf, 64, 24, False), (f32, 96, 16, True), (f32, 20, 4, True),
+                                      (f32, 260, 16, False), (f32, 18, 16, False)):
+        r = runner({0: KvCacheNeed(2, head, None)}, dtype, page)
+        groups = r._shared_groups(*decoded(r, 96))
+        assert groups == ([([0, 1, 2], 96)] if shares else []), (dtype, head, page)
+    both = runner({0: KvCacheNeed(2, 96, None), 1: KvCacheNeed(1, 128, None)}, bf)
+    assert both._key_bytes == 2 * 128 * 2 and both._shared_groups(*decoded(both)) == [([0, 1, 2], 64)]
+
+
 def test_pieces_of_the_own_keys():
     """The parts' sums stay small however many sequences there are and however long they are; a few sequences have a warp a chunk."""
     from rvllm_b200.kernels.library import CudaKernels
