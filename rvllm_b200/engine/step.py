@@ -367,7 +367,10 @@ class ModelRunner:
 
     # ---- beginnings that requests share ----------------------------------------------------------
     def _reads_once(self, need) -> bool:
-        """Whether the attention of a cache group reads beginnings that sequences share once."""
+        """Whether the attention of a cache group may read beginnings that sequences share once (one row for key and value, values of
+        another size than keys and windows have kernels of their own, which read each sequence for itself)."""
+        if need.planes != 2 or need.flat_pages or need.window is not None or need.chunk is not None:
+            return False
         rule = getattr(self.kernels, "reads_prefixes_once", None)
         return rule is not None and rule(self.cache.dtype, need.num_kv_heads, need.head_dim, self.cache.page_size, self.cache.num_pages, self.cache.max_seqs)
 
@@ -505,6 +508,8 @@ class ModelRunner:
                     m.shared, m.max_own_len = shared, self._longest_own(starts, groups)
             hidden = self.model.forward(ctx, self.cache)
             logits = self.model.compute_logits(hidden, ctx) if ctx.logit_rows.numel() else None
+            if groups and not shared.used:
+                self._key_bytes = 0
         for e in entries:
             self.cache.release_passed(e.req_id)
         self.steps_run += 1
@@ -552,7 +557,9 @@ class ModelRunner:
                     m.shared, m.max_own_len = shared, own_limit
             hidden = self.model.forward(ctx, self.cache)
             logits = self.model.compute_logits(hidden, ctx)
-            if state is None:
+            if groups and not shared.used:
+                self._key_bytes = 0            # no layer reads beginnings once (their attention is another): no graphs of such steps
+            elif state is None:
                 self._graphs[bucket] = self._capture(*bucket)
             return logits
         host, dev, graph, out, launches, shared = state

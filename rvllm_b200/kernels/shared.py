@@ -163,6 +163,11 @@ class StepPrefixes:
         self.num_seqs, self.device, self.most_groups, self.num_sms = num_seqs, device, most_groups, num_sms
         self._layouts = {}
 
+    @property
+    def used(self) -> bool:
+        """Whether any layer has asked for a layout."""
+        return bool(self._layouts)
+
     @staticmethod
     def _own(groups):
         """A copy: the caller may go on with its lists."""

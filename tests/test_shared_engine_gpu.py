@@ -153,6 +153,24 @@ def test_an_identifier_that_is_used_again(monkeypatch):
     assert float((logits[0] - logits[1]).abs().max()) <= 2e-4 * float(logits[1].abs().max())
 
 
+@pytest.mark.parametrize("eager", [True, False])
+def test_layers_that_read_no_beginning_once_get_no_graphs_of_their_own(eager, monkeypatch):
+    """Where no layer's attention asks for the groups of a step, later steps make none."""
+    from rvllm_b200 import SamplingParams
+    llm = make(folder_for(SHAPED), "float32", enforce_eager=eager)
+    k, r = llm.engine.kernels, llm.engine.runner
+    original = k.paged_attention
+
+    def each_for_itself(q, cache, meta, *args, **kw):
+        meta.shared = None
+        return original(q, cache, meta, *args, **kw)
+    monkeypatch.setattr(k, "paged_attention", each_for_itself)
+    a, _ = stems(515, seed=3)
+    llm.generate([a, a, a], SamplingParams(max_tokens=6, ignore_eos=True))
+    assert not r._key_bytes and all(own == 0 for _, _, own in r._graphs)
+    assert eager or r._graphs
+
+
 # ------------------------------------------------------------------------------------------------------------ step tables
 def windowed():
     return dict(plain_windows={"architectures": ["Qwen2ForCausalLM"], "hidden_size": 64, "num_hidden_layers": 4, "num_attention_heads": 4,

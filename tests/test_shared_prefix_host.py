@@ -419,6 +419,17 @@ def test_heads_whose_shared_beginnings_are_read_once():
     assert both._key_bytes == 2 * 128 * 2 and both._shared_groups(*decoded(both)) == [([0, 1, 2], 64)]
 
 
+def test_caches_that_no_attention_reads_once_make_no_groups():
+    """A row that is key and value at once, and pages of unlike rows: the pages are shared, the steps are those of any batch."""
+    from rvllm_b200.parts import KvCacheNeed
+    for dtype in (torch.bfloat16, torch.float32):
+        for need in (KvCacheNeed(1, 576, None, planes=1), KvCacheNeed(1, 64, None, planes=1), KvCacheNeed(2, 64, None, 2, 128)):
+            r = runner({0: need}, dtype)
+            assert r.cache.can_share and r._shared_groups(*decoded(r)) == []
+        mixed = runner({0: KvCacheNeed(1, 128, None, planes=1), 1: KvCacheNeed(2, 64, None)}, dtype)
+        assert mixed._shared_groups(*decoded(mixed)) == [([0, 1, 2], 64)]
+
+
 def test_pieces_of_the_own_keys():
     """The parts' sums stay small however many sequences there are and however long they are; a few sequences have a warp a chunk."""
     from rvllm_b200.kernels.library import CudaKernels
