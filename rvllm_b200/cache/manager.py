@@ -318,16 +318,22 @@ class CacheManager:
         """No page lost, held twice or free while held; tables agree with the pools."""
         for gi, g in enumerate(self.groups):
             g.pool.check()
-            held = {}
+            held: Dict[int, List[Hashable]] = {}         # page -> the requests whose tables have it
             for req, r in self.requests.items():
                 for p in r.tables[gi]:
                     if p < 0:
                         continue
-                    if p in held and not (g.pool.holds(p, held[p]) and g.pool.holds(p, req)):
-                        raise SchedulerError(f"page {p} of group {gi} is in the tables of {held[p]!r} and {req!r}")
-                    held[p] = req
+                    there = held.setdefault(p, [])
+                    if there and there[-1] == req:
+                        raise SchedulerError(f"page {p} of group {gi} is in the table of {req!r} twice")
+                    if there and not (g.pool.holds(p, there[-1]) and g.pool.holds(p, req)):
+                        raise SchedulerError(f"page {p} of group {gi} is in the tables of {there[-1]!r} and {req!r}")
+                    there.append(req)
                     if not g.pool.holds(p, req):
                         raise SchedulerError(f"page {p} of group {gi}: table of {req!r}, pool says {g.pool.owner(p)!r}")
+            for p, there in held.items():
+                if g.pool.num_holders(p) != len(there):
+                    raise SchedulerError(f"page {p} of group {gi} has {g.pool.num_holders(p)} holders and is in the tables of {there!r}")
             if len(held) + g.pool.num_free != g.pool.num_pages:
                 raise SchedulerError(f"group {gi}: {len(held)} held + {g.pool.num_free} free != {g.pool.num_pages}")
         self.slots.check()

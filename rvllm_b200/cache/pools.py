@@ -39,6 +39,9 @@ class PagePool:
     def holds(self, page: int, owner: Hashable) -> bool:
         return self._owner[page] == owner or owner in self._others.get(page, ())
 
+    def num_holders(self, page: int) -> int:
+        return (self._owner[page] is not None) + len(self._others.get(page, ()))
+
     def allocate(self, n: int, owner: Hashable) -> List[int]:
         if n > len(self._free):
             raise KvExhausted(n, len(self._free))

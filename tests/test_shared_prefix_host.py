@@ -115,6 +115,29 @@ def test_a_shared_page_is_free_when_its_last_holder_gives_it_back():
     assert m.num_free_pages() == [16, 16]
 
 
+def test_a_page_twice_in_one_table_is_found():
+    """A page that several requests hold is in their tables once each: not in one twice, and in no fewer than hold it."""
+    from rvllm_b200 import SchedulerError
+    m = manager()
+    m.admit("a"); m.append("a", 12)
+    m.admit("b"); m.share("b", "a", 8)
+    m.check()
+    for req in ("a", "b"):
+        table = m.requests[req].tables[0]
+        kept = list(table)
+        for at in range(1, len(table)):
+            table[at] = table[0]
+            with pytest.raises(SchedulerError, match="twice"):
+                m.check()
+            table[:] = kept
+    table = m.requests["b"].tables[0]
+    gone = table.pop()                               # b gives it up without saying so: its holder would keep the page for good
+    with pytest.raises(SchedulerError, match="holders"):
+        m.check()
+    table.append(gone)
+    m.check()
+
+
 def test_what_cannot_be_shared_is_refused():
     from rvllm_b200 import SchedulerError
     from rvllm_b200.parts import KvCacheNeed, StateNeed
