@@ -330,8 +330,8 @@ class CudaKernels:
         tensor-core flash kernel (one token per sequence: the decode tiling, keys split over CTAs
         when the batch alone cannot fill the GPU); everything else goes to the plain kernel."""
         page = cache_layer.shape[3]
-        if meta.shared is not None and meta.max_q_len == 1 and window is None and distance_bias is None and num_heads // num_kv_heads <= TILE_ROWS \
-                and self.reads_prefixes_once(q.dtype, num_kv_heads, head_dim, page, cache_layer.shape[0], meta.num_seqs):
+        if meta.shared is not None and meta.max_q_len == 1 and window is None and distance_bias is None and scale > 0 \
+                and num_heads // num_kv_heads <= TILE_ROWS and self.reads_prefixes_once(q.dtype, num_kv_heads, head_dim, page, cache_layer.shape[0], meta.num_seqs):
             return self.shared_prefix_attention(q, cache_layer, meta, meta.shared.layout(num_heads, num_kv_heads), num_heads, num_kv_heads,
                                                 head_dim, scale, softcap, sinks, gate, meta.max_own_len)
         extras = softcap is not None or sinks is not None or gate is not None or distance_bias is not None

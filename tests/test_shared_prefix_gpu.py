@@ -252,6 +252,17 @@ def test_which_steps_paged_attention_reads_once(dtype, hd, page, once, monkeypat
     assert float(((got.cpu().to(F64) - exact).abs() / tol).max()) <= 1.0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+def test_scales_that_only_paged_attention_takes(dtype, scale):
+    """A scale that is not positive (some configurations allow any number) is no reason for a step with shared beginnings to fail."""
+    s = make([(6, 96)], 1, 8, 2, 64, 16, dtype, seed=2, own=(1, 50), stale="0")
+    call = lambda: lib().paged_attention(s["q"], s["cache"], s["meta"], 8, 2, 64, scale, None)  # noqa: E731
+    want = call()
+    s["meta"].shared = StepPrefixes(s["plan"], 7, "cuda")
+    assert torch.equal(call(), want)
+
+
 def test_pages_that_do_not_exist_are_not_read():
     """Entries beyond the cache or negative inside the prefix: no result is promised, and nothing outside the cache is touched."""
     for dtype in (torch.bfloat16, torch.float32):
