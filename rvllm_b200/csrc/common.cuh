@@ -28,6 +28,8 @@
 // Two rules for what runs before rv_pdl_wait(): it reads only what no kernel of the step writes
 // (weights, the step's metadata), and it writes no global memory at all - a buffer handed out by a
 // stream-ordered allocator may still be in use, under another name, by a kernel running ahead.
+// (The one kernel that writes metadata, step_tables.cu, is followed by a launch without the attribute,
+// which starts when it is complete: what is launched early behind that one finds its tables written.)
 static int g_rv_pdl = 0;
 RV_EXPORT void rv_set_pdl(int on) { g_rv_pdl = on; }
 

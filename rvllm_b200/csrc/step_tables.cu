@@ -124,15 +124,18 @@ step_tables_kernel(const TableParams p) {
         if (b == p.num_seqs - 1) p.cu_seqlens[p.num_seqs] = (int)(tokens + (unsigned)q);
         p.ctx_lens[b] = real ? (int)((unsigned)start + (unsigned)q) : 0;
     }
-    // The step's other kernels may read this metadata before they wait for their predecessor, so nothing behind this kernel may
-    // start before all of it is written: it gives no early signal, and what it wrote is out when a CTA ends.
-    __threadfence();
+    // (no early signal: the step's other kernels may read this metadata before they wait for their predecessor, see below)
 }
 
-// The arguments, packed by the caller in the order of TableParams, then the stream.
+// Nothing, launched without the early attribute: it starts when the tables are complete, and a kernel behind it may read them before its
+// own wait.  A launch that asks to start early right behind the tables would be promised them only after that wait.
+__global__ void tables_settled_kernel() {}
+
+// The arguments, packed by the caller in the order of TableParams, then the stream, and whether the next launch on it may be an early one.
 struct TableArgs {
     TableParams p;
     cudaStream_t stream;
+    int settle;
 };
 
 RV_EXPORT int rv_step_tables(const TableArgs* a) {
@@ -148,5 +151,8 @@ RV_EXPORT int rv_step_tables(const TableArgs* a) {
     else if (per == 2) RV_LAUNCH_ST = rv_launch(step_tables_kernel<2>, grid, dim3(TABLE_THREADS), 0, a->stream, p);
     else if (per == 4) RV_LAUNCH_ST = rv_launch(step_tables_kernel<4>, grid, dim3(TABLE_THREADS), 0, a->stream, p);
     else RV_LAUNCH_ST = rv_launch(step_tables_kernel<8>, grid, dim3(TABLE_THREADS), 0, a->stream, p);
+    const int st = rv_launch_status();
+    if (st != RV_OK || !a->settle || !g_rv_pdl) return st;
+    RV_LAUNCH_ST = rv_launch_alone(tables_settled_kernel, dim3(1), dim3(32), 0, a->stream);
     return rv_launch_status();
 }

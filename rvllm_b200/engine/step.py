@@ -345,7 +345,8 @@ class ModelRunner:
         tables, slots, positions, token_seq, cu, ctx_dev = dev[sent:sent + sum(built)].split_with_sizes(built)
         made = StepTables(tables.view(G, B, MB), slots.view(G, T), positions, token_seq, cu, ctx_dev)
         self.kernels.step_tables(self._page_table, dev[:B], dev[o_held:o_tok].view(G, B), dev[o_start:o_q], dev[o_q:o_held], dev[o_new:max(at, o_new + 1)],
-                                 self._spans, T, MB, cache.page_size, out=made)
+                                 self._spans, T, MB, cache.page_size, out=made,
+                                 settle=late is None and (pad_to is None or not entries))    # (otherwise `late_tokens` or a graph is next)
         for r in held:
             r.on_device = [len(t) for t in r.tables]
         ctx = StepContext()

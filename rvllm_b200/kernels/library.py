@@ -58,7 +58,7 @@ def _need(t: torch.Tensor, name: str, dtype=None, dims=None):
 # arguments of the entry points that take them as one block (the structures of the same names in csrc/)
 _SHARED_ARGS = struct.Struct("=15q12i2f")       # shared_attention_tcgen05.cu
 _PLAIN_ARGS = struct.Struct("=14q12i2f")       # shared_prefix.cu
-_TABLE_ARGS = struct.Struct("=13q8iq")         # step_tables.cu
+_TABLE_ARGS = struct.Struct("=13q8iqi")        # step_tables.cu
 
 
 class AttentionMeta:
@@ -665,7 +665,7 @@ class CudaKernels:
 
     def step_tables(self, page_table: torch.Tensor, rows: torch.Tensor, held: torch.Tensor, starts: torch.Tensor, q_lens: torch.Tensor,
                     new_pages: torch.Tensor, spans: torch.Tensor, num_tokens: int, max_blocks: int, page_size: int,
-                    out: Optional[StepTables] = None) -> StepTables:
+                    out: Optional[StepTables] = None, settle: bool = True) -> StepTables:
         """The block tables, slot map and positions of a step from its requests' lengths; all tensors int32 on the device.
 
         page_table [groups, table rows, table width]: the pages of every request, kept by the caller and brought up to date
@@ -676,7 +676,11 @@ class CudaKernels:
         of a group (0: none); blocks that no later token can see are -1 in its block tables.
 
         `num_tokens` = the sum of q_lens and `max_blocks` >= the most blocks of a sequence, as the caller knows them.  With `out`
-        the tables are written into tensors of the caller (those a captured graph reads)."""
+        the tables are written into tensors of the caller (those a captured graph reads).
+
+        Kernels that are launched early read tables before they wait for what runs in front of them, so an empty launch without the early
+        attribute follows.  `settle` False leaves it out: for a caller whose next launch on the stream is not an early one (a graph,
+        `late_tokens`, any kernel of torch)."""
         here = torch._C._cuda_getDevice()
         given = (page_table, rows, held, starts, q_lens, new_pages, spans)
         for t in given:
@@ -711,7 +715,7 @@ class CudaKernels:
             page_table.data_ptr(), rows.data_ptr(), held.data_ptr(), starts.data_ptr(), q_lens.data_ptr(), new_pages.data_ptr(), spans.data_ptr(),
             out.block_tables.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.token_seq.data_ptr(),
             out.cu_seqlens.data_ptr(), out.ctx_lens.data_ptr(), G, B, R, width, new_pages.shape[0], num_tokens, max_blocks, page_size,
-            torch._C._cuda_getCurrentRawStream(here)))
+            torch._C._cuda_getCurrentRawStream(here), settle))
         _check("step_tables", st)
         return out
 

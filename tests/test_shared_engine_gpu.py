@@ -223,3 +223,23 @@ def test_tables_of_the_device_are_those_of_the_host(model):
                 assert torch.equal(x, y)
         for e in entries:
             eng.cache.release_passed(e.req_id)
+
+
+def test_tables_are_settled_where_kernels_follow_that_start_early(monkeypatch):
+    """Steps without a graph, and the padded batch that a capture runs first, launch kernels right behind the tables; a replayed graph, and
+    tokens that the host has not read, come with a boundary of their own."""
+    from rvllm_b200.engine import StepEntry
+    eng = make(folder_for(SHAPED), "float32", share_prefixes=False).engine
+    k, seen = eng.kernels, []
+    original = k.step_tables
+    monkeypatch.setattr(k, "step_tables", lambda *a, **kw: (seen.append(kw["settle"]), original(*a, **kw))[1])
+    step = lambda n, t=1, late=None: eng.runner.step([StepEntry(i, list(range(1, t + 1)), (t - 1,)) for i in range(n)], late_tokens=late)  # noqa: E731
+    step(2, 5)
+    assert seen == [True]                            # portions
+    step(2)
+    assert seen == [True, True, True]                # the first of its size: eagerly, then a batch of padding rows
+    step(2)
+    assert seen[3:] == [False]                       # replayed
+    ids = torch.tensor([3, 4], dtype=torch.int32, device="cuda")
+    step(2, late=(ids, [0, 1]))
+    assert seen[4:] == [False]

@@ -514,6 +514,32 @@ def test_step_tables_captured():
     assert out.ctx_lens.tolist() == [5, 4] and table[0].tolist()[1][:2] == [3, 6]
 
 
+def test_attention_right_behind_the_tables():
+    """Tables that change from call to call, read by the launch right behind, which starts early where the library launches it so."""
+    s = make([], 40, 32, 8, 128, 16, torch.bfloat16, seed=3, own=(300, 900), stale="0")
+    B, real, ctx = 40, s["meta"].block_tables, s["meta"].ctx_lens
+    MB, W = real.shape[1], real.shape[1] + 1
+    q_lens, held, spans = i32([1] * B), i32([[0] * B]), i32([[0, 0]])
+    orders = [torch.randperm(B, generator=torch.Generator().manual_seed(i)) for i in range(6)]
+    table = torch.full((1, B, W), -1, dtype=torch.int32, device="cuda")
+    want = lib().paged_attention(s["q"], s["cache"], s["meta"], 32, 8, 128, 128 ** -0.5, None)
+    steps = []
+    for order in orders:                             # sequence i of a step is sequence order[i] of the cache
+        lens = [s["ctx"][int(b)] for b in order]
+        new = torch.cat([real[int(b), :(n + 15) // 16] for b, n in zip(order, lens)])
+        steps.append((order.cuda(), s["q"][order.cuda()].contiguous(), i32([n - 1 for n in lens]), new.contiguous()))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for order, q, starts, new in steps:
+            t = lib().step_tables(table, i32(list(range(B))), held, starts, q_lens, new, spans, B, MB, 16)
+            meta = AttentionMeta(t.block_tables[0], t.cu_seqlens, t.ctx_lens, t.token_seq, t.slot_mapping[0], B, 1, int(max(s["ctx"])), 16, B)
+            got.append((order, lib().paged_attention(q, s["cache"], meta, 32, 8, 128, 128 ** -0.5, None)))
+    torch.cuda.synchronize()
+    for order, out in got:
+        assert torch.equal(out, want[order])
+
+
 def test_step_tables_refusals():
     good = dict(page_table=torch.zeros((1, 2, 4), dtype=torch.int32, device="cuda"), rows=i32([0, 1]), held=i32([[0, 0]]), starts=i32([0, 0]),
                 q_lens=i32([1, 1]), new_pages=i32([1, 2]), spans=i32([[0, 0]]), num_tokens=2, max_blocks=4, page_size=16)
