@@ -499,6 +499,32 @@ def test_step_tables_with_lengths_past_31_bits():
         assert room[at:].eq(123456789).all()
 
 
+@pytest.mark.parametrize("rows,held,starts,q", [
+    ([2, 9], [-4, 0], [40, -3], [30, 5]), ([-7, 2 ** 31 - 1], [0, 0], [5, 5], [3, 3]), ([0, 3], [99, -99], [0, 47], [1, 1]),
+    ([1, 2], [0, 0], [4000, 46], [5, 9]), ([3, 0], [3, 3], [-50, 100], [90, -90]), ([-2 ** 31, 3], [-2 ** 31, 2 ** 31 - 1], [-2 ** 31, 0], [-2 ** 31, 48])])
+def test_step_tables_write_inside_their_tensors(rows, held, starts, q):
+    """Rows, held entries, starts and lengths out of range: the page table and every output lie between guards, and these stay as they are;
+    so do the rows of the page table that no sequence of the step owns."""
+    from rvllm_b200.kernels import StepTables
+    R, W, MB, T = 4, 3, 5, 20
+    shapes = [(1, R, W), (1, 2, MB), (1, T), (T,), (T,), (3,), (2,)]
+    room = torch.full((sum(math.prod(s) + 64 for s in shapes) + 64,), 123456789, dtype=torch.int32, device="cuda")
+    views, at = [], 64
+    for s in shapes:
+        views.append(room[at:at + math.prod(s)].view(s))
+        at += math.prod(s) + 64
+    views[0].zero_()
+    lib().step_tables(views[0], i32(rows), i32([held]), i32(starts), i32(q), i32([5, 6]), i32([[0, 0]]), T, MB, 16, out=StepTables(*views[1:]))
+    at = 0
+    for s in shapes:
+        assert room[at:at + 64].eq(123456789).all()
+        at += math.prod(s) + 64
+    assert room[at:].eq(123456789).all()
+    others = [r for r in range(R) if r not in rows]
+    assert views[0][0, others].eq(0).all() and views[0].ge(-1).all() and views[0].le(6).all()
+    assert views[1].ge(-1).all() and views[1].le(6).all()
+
+
 def test_step_tables_captured():
     table = torch.zeros((1, 2, 8), dtype=torch.int32, device="cuda")
     rows, held, starts, q, new, spans = i32([1, 0]), i32([[0, 0]]), i32([0, 0]), i32([1, 1]), i32([3, 4]), i32([[0, 0]])
