@@ -227,7 +227,7 @@ __device__ __forceinline__ void prefix_part(const PlainParams& p, float* sh, int
 }
 
 // A piece of the keys behind the prefix of one sequence, against up to eight of its heads: a warp has a row, its lanes the keys of the
-// tile for the scores and hd / 32 columns for the sums; the next tile's words wait in registers.
+// tile for the scores and hd / 32 columns for the sums; the next tile's words wait in registers.  Warps beyond the heads of a group only load.
 template <typename T, int DPL>
 __device__ __forceinline__ void own_part(const PlainParams& p, float* sh, int cta) {
     constexpr int R = PLAIN_THREADS / 32;
@@ -295,6 +295,7 @@ __device__ __forceinline__ void own_part(const PlainParams& p, float* sh, int ct
         __syncthreads();
         fetch(key0 + PLAIN_TILE, page);
         page = page_of(key0 + 2 * PLAIN_TILE + mine);
+        if (warp >= rows) continue;                         // (it brings its keys, and has no row to put them to)
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int d = 0; d < p.hd; d += 4) {
