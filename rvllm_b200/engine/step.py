@@ -33,12 +33,22 @@ from ..kernels.shared import StepPrefixes, StepTables
 SHARED_MOST_GROUPS = 8         # groups of a captured step: those that save the most
 # A decode step reads shared beginnings once, instead of as many times as requests hold them, where that is the faster way:
 # * bfloat16: the keys and values it saves a layer are this many bytes and half of those that it reads sequence by sequence.  32 heads of
-#   128 on 8, shared against each for itself: 16 requests with 16 keys of their own behind 256 (15.7 MB saved) 8.3 and 8.5 us, behind
-#   512 9.0 and 10.0, 8 behind 2,048 (59 MB) 10.7 and 12.8, 64 with 1,024 of their own (268 MB) behind 512 (132 MB) 53 and 55,
-#   behind 2,048 58 and 94, with 16 behind 8,192 25 and 225;
+#   128 on 8, each for itself and shared, us: 16 requests with 16 keys of their own behind 256 (15.7 MB saved) 9.1 and 8.7, behind
+#   512 10.5 and 9.4, 8 behind 2,048 (59 MB) 13.3 and 11.1, 64 with 1,024 of their own (268 MB) behind 512 (132 MB) 59 and 54,
+#   behind 2,048 94 and 59, with 16 behind 8,192 226 and 26;
 SHARED_MIN_BYTES = 24 << 20
-# * float32: some beginning is this long (28 heads of 128 on 4: 4 requests with 16 keys of their own behind 64 12.3 and 8.0 us, behind
-#   256 12.6 and 17.2, 16 behind 1,024 32 and 104), or the bytes saved are half of the above (64 behind 64: 15.5 and 46).
+#   ... and twice as many in a graph, which is launched for any groups that fit it (1 to 4 us a layer that a layout of the very groups does
+#   without), unless it has this many (sequence, kv head) pairs, where reading each for itself costs more, or one kv head, where it has
+#   few CTAs.  Each for itself and shared in a graph, us: 16 behind 512 10.4 and 11.0, 2 behind 8,192 (34 MB) 15.5 and 17.7, with 800 of
+#   their own 16.1 and 21.5; 64 behind 128 (33 MB) 16.4 and 12.3, 28 heads on 4 64 behind 256 (33 MB) 18.0 and 12.7, 16 on one
+#   32 behind 2,048 (33 MB) 16.5 and 12.0.  (336 sizes of 8 to 170 MB saved, six layouts of heads: 1.7 % above the
+#   better of the two in all, 8 % above each for itself at worst; with the one threshold 3.4 and 34 %.)
+SHARED_GRAPH_MIN_BYTES = 48 << 20
+SHARED_GRAPH_MANY_PAIRS = 256
+# * float32: some beginning is this long (28 heads of 128 on 4: 4 requests with 16 keys of their own behind 64 8.3 and 12.5 us, behind
+#   256 17.0 and 12.9, 16 behind 1,024 105 and 31; in a graph 15.7, 17.1 and 33), or the bytes saved are half of the above (64 behind
+#   64: 46 and 15.4, in a graph 18.8).  What it does not ask for is the heads on a kv head: with one, own keys take longer shared than each
+#   for itself (16 heads of 64 on 16, 64 requests with 800 of their own behind 512 241 and 257).
 SHARED_MIN_TOKENS_F32 = 256
 
 
@@ -84,7 +94,10 @@ class ModelRunner:
         self._eager_prefixes: Optional[StepPrefixes] = None
         # bytes of a key and its value in the largest of the groups whose shared beginnings are read once (0: there is no such group)
         needs = [g.need for g in cache.groups if self._reads_once(g.need)]
-        self._key_bytes = max((n.num_kv_heads * n.row_elements for n in needs), default=0) * torch.empty((), dtype=cache.dtype).element_size()
+        widest = max(needs, key=lambda n: n.num_kv_heads * n.row_elements, default=None)
+        self._kv_heads = widest.num_kv_heads if widest else 0
+        self._key_bytes = self._kv_heads * widest.row_elements * torch.empty((), dtype=cache.dtype).element_size() if widest else 0
+        self._least_saved = SHARED_MIN_BYTES
         self._page_table = None
         if cache.groups and self.device.type == "cuda" and hasattr(kernels, "step_tables"):
             G = len(cache.groups)
@@ -375,9 +388,9 @@ class ModelRunner:
         rule = getattr(self.kernels, "reads_prefixes_once", None)
         return rule is not None and rule(self.cache.dtype, need.num_kv_heads, need.head_dim, self.cache.page_size, self.cache.num_pages, self.cache.max_seqs)
 
-    def _shared_groups(self, entries, starts):
-        """(places, tokens) per group of entries that begin with the same cached tokens, for a step of decoded tokens; none where it
-        would not pay.  Pages that are shared stay as they are while their requests live, so the groups hold until the set of
+    def _shared_groups(self, entries, starts, graph: bool = False):
+        """(places, tokens) per group of entries that begin with the same cached tokens, for a step of decoded tokens (`graph`: one that
+        runs from a captured graph); none where it would not pay.  Pages that are shared stay as they are while their requests live, so the groups hold until the set of
         requests changes."""
         if not self._key_bytes or not self.cache.can_share or self._page_table is None or any(len(e.tokens) != 1 for e in entries):
             return []
@@ -386,6 +399,8 @@ class ModelRunner:
             groups = sorted(self.cache.shared_groups(reqs[1]), key=lambda g: -(len(g[0]) - 1) * g[1])[:SHARED_MOST_GROUPS]
             self._groups_of = (reqs, groups)
         groups = self._groups_of[1]
+        few = graph and 1 < self._kv_heads and len(entries) * self._kv_heads < SHARED_GRAPH_MANY_PAIRS
+        self._least_saved = SHARED_GRAPH_MIN_BYTES if few else SHARED_MIN_BYTES
         return groups if groups and self._worth_sharing(groups, sum(starts) + len(starts)) else []
 
     def _worth_sharing(self, groups, keys: int) -> bool:
@@ -394,7 +409,7 @@ class ModelRunner:
         own = keys - sum(len(m) * t for m, t in groups)
         if self.cache.dtype == torch.float32:
             return max(t for _, t in groups) >= SHARED_MIN_TOKENS_F32 or saved * self._key_bytes >= SHARED_MIN_BYTES // 2
-        return saved * self._key_bytes >= SHARED_MIN_BYTES + own * self._key_bytes // 2
+        return saved * self._key_bytes >= getattr(self, "_least_saved", SHARED_MIN_BYTES) + own * self._key_bytes // 2
 
     def _eager_shared(self, groups, num_seqs: int) -> StepPrefixes:
         last = self._eager_prefixes
@@ -542,7 +557,7 @@ class ModelRunner:
 
     def _step_graph(self, entries, starts, bucket: int, late=None) -> torch.Tensor:
         ctx_limit = self._ctx_bucket(max(starts) + 1)
-        groups = self._shared_groups(entries, starts)
+        groups = self._shared_groups(entries, starts, graph=True)
         # a step that reads shared beginnings once is another graph, laid out for the keys behind them
         own_limit = self._ctx_bucket(self._longest_own(starts, groups)) if groups else 0
         bucket = (bucket, ctx_limit, own_limit)

@@ -453,6 +453,27 @@ def test_caches_that_no_attention_reads_once_make_no_groups():
         assert mixed._shared_groups(*decoded(mixed)) == [([0, 1, 2], 64)]
 
 
+def test_when_a_graph_reads_shared_beginnings_once():
+    """A captured step, which is launched for any groups that fit it, asks for more: at 8 key/value heads of 128 in bfloat16."""
+    from rvllm_b200.engine.step import ModelRunner
+    from rvllm_b200.parts import KvCacheNeed
+
+    def shares(n, tokens, graph, need=KvCacheNeed(8, 128, None)):
+        r = runner({0: need}, torch.bfloat16, num_pages=2000, max_seqs=64)
+        del r._worth_sharing
+        assert type(r)._worth_sharing is ModelRunner._worth_sharing
+        return bool(r._shared_groups(*decoded(r, tokens, n), graph=graph))
+    for n, tokens, eager, graph in ((16, 256, False, False), (16, 512, True, False), (2, 8192, True, False), (8, 2048, True, True), (16, 1024, True, True),
+                                    (64, 128, True, True), (32, 256, True, True)):
+        assert shares(n, tokens, False) == eager and shares(n, tokens, True) == graph, (n, tokens)
+    one = KvCacheNeed(1, 128, None)
+    assert shares(32, 2048, True, one) and not shares(32, 1024, True, one)
+    r = runner({0: KvCacheNeed(8, 128, None)}, torch.bfloat16, num_pages=2000)    # the one does not stay for the other
+    del r._worth_sharing
+    step = decoded(r, 8192, 2)
+    assert [bool(r._shared_groups(*step, graph=g)) for g in (True, False, True, False)] == [False, True, False, True]
+
+
 def test_pieces_of_the_own_keys():
     """The parts' sums stay small however many sequences there are and however long they are; a few sequences have a warp a chunk."""
     from rvllm_b200.kernels.library import CudaKernels
