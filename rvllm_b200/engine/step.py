@@ -396,9 +396,9 @@ class ModelRunner:
             return []
         reqs = (self.cache.changes, tuple(e.req_id for e in entries))
         if reqs != self._groups_of[0]:
-            groups = sorted(self.cache.shared_groups(reqs[1]), key=lambda g: -(len(g[0]) - 1) * g[1])[:SHARED_MOST_GROUPS]
+            groups = sorted(self.cache.shared_groups(reqs[1]), key=lambda g: -(len(g[0]) - 1) * g[1])
             self._groups_of = (reqs, groups)
-        groups = self._groups_of[1]
+        groups = self._groups_of[1][:SHARED_MOST_GROUPS] if graph else self._groups_of[1]
         few = graph and 1 < self._kv_heads and len(entries) * self._kv_heads < SHARED_GRAPH_MANY_PAIRS
         self._least_saved = SHARED_GRAPH_MIN_BYTES if few else SHARED_MIN_BYTES
         return groups if groups and self._worth_sharing(groups, sum(starts) + len(starts)) else []

@@ -474,6 +474,23 @@ def test_when_a_graph_reads_shared_beginnings_once():
     assert [bool(r._shared_groups(*step, graph=g)) for g in (True, False, True, False)] == [False, True, False, True]
 
 
+def test_only_graphs_are_laid_out_for_so_many_groups():
+    """Of eleven prompts' samples a graph takes the eight that save the most, a step by itself all."""
+    from rvllm_b200.engine import StepEntry
+    from rvllm_b200.parts import KvCacheNeed
+    r = runner({0: KvCacheNeed(8, 128, None)}, torch.bfloat16, num_pages=2000, max_seqs=40)
+    names = []
+    for g in range(11):
+        r.cache.admit((g, 0)); r.cache.append((g, 0), 16 * (g + 1))
+        for i in (1, 2):
+            r.cache.admit((g, i)); r.cache.share((g, i), (g, 0), 16 * (g + 1))
+        names += [(g, i) for i in range(3)]
+    entries, starts = [StepEntry(n, [1], (0,)) for n in names], [r.cache.append(n, 1) for n in names]
+    for graph, n in ((True, 8), (False, 11), (True, 8)):
+        groups = r._shared_groups(entries, starts, graph=graph)
+        assert [t for _, t in groups] == [16 * (g + 1) for g in range(10, 10 - n, -1)]
+
+
 def test_pieces_of_the_own_keys():
     """The parts' sums stay small however many sequences there are and however long they are; a few sequences have a warp a chunk."""
     from rvllm_b200.kernels.library import CudaKernels
