@@ -177,6 +177,11 @@ class CacheManager:
         """True where a request's first pages say all there is to know about its first tokens."""
         return bool(self.groups) and not self._has_window and not self._state_needs
 
+    @property
+    def any_shared(self) -> bool:
+        """Whether any page has several holders."""
+        return self.can_share and self.groups[0].pool.any_shared
+
     def share(self, req: Hashable, donor: Hashable, num_tokens: int) -> None:
         """The pages of `donor`'s first `num_tokens` tokens (a multiple of the page size) become the first pages of `req`, which has
         none yet.  The caller knows that both begin with these tokens and that the donor's are in the cache."""
@@ -198,7 +203,7 @@ class CacheManager:
         """Which of the requests `reqs` begin with the same pages: (places in `reqs`, tokens) per group, each request in one group at
         most.  Where a few of those that share a beginning share more among themselves, the grouping that saves the most keys is taken
         (looked for up to 64 beginnings within one another)."""
-        if not self.can_share:
+        if not self.any_shared:
             return []
         tables = [self.requests[r].tables[0] for r in reqs]
 
@@ -208,11 +213,18 @@ class CacheManager:
                 return 0, []
             first = tables[members[0]]
             common = min(len(tables[m]) for m in members)
+            run = first[depth:common]                # whole runs of pages are compared at a time
             for m in members[1:]:
-                t, n = tables[m], depth
-                while n < common and t[n] == first[n]:
-                    n += 1
-                common = n
+                t, lo = tables[m], depth
+                if t[lo:common] == run:
+                    continue
+                while lo < common:
+                    mid = (lo + common) // 2
+                    if t[lo:mid + 1] == first[lo:mid + 1]:
+                        lo = mid + 1
+                    else:
+                        common = mid
+                run = first[depth:common]
             parts: Dict[int, List[int]] = {}
             for m in members:
                 if len(tables[m]) > common:

@@ -39,6 +39,10 @@ class PagePool:
     def holds(self, page: int, owner: Hashable) -> bool:
         return self._owner[page] == owner or owner in self._others.get(page, ())
 
+    @property
+    def any_shared(self) -> bool:
+        return bool(self._others)
+
     def num_holders(self, page: int) -> int:
         return (self._owner[page] is not None) + len(self._others.get(page, ()))
 

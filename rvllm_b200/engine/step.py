@@ -392,7 +392,7 @@ class ModelRunner:
         """(places, tokens) per group of entries that begin with the same cached tokens, for a step of decoded tokens (`graph`: one that
         runs from a captured graph); none where it would not pay.  Pages that are shared stay as they are while their requests live, so the groups hold until the set of
         requests changes."""
-        if not self._key_bytes or not self.cache.can_share or self._page_table is None or any(len(e.tokens) != 1 for e in entries):
+        if not self._key_bytes or not self.cache.any_shared or self._page_table is None or any(len(e.tokens) != 1 for e in entries):
             return []
         reqs = (self.cache.changes, tuple(e.req_id for e in entries))
         if reqs != self._groups_of[0]:

@@ -186,6 +186,49 @@ def test_groups_that_save_the_most():
     assert m2.shared_groups(["a"]) == [] and m2.shared_groups([]) == []
 
 
+@pytest.mark.parametrize("seed", range(6))
+def test_groups_against_a_plain_search(seed):
+    """Which pages two requests have in common, compared one by one, at lengths around those of runs that are compared at a time."""
+    rng = random.Random(seed)
+    m = manager(num_pages=4000, page=2, max_seqs=64)
+    m.admit(0); m.append(0, 2 * rng.choice((1, 2, 3, 31, 64)) + 1)
+    for i in range(1, 30):
+        m.admit(i)
+        donor = rng.randrange(i)
+        whole = m.num_tokens(donor) // 2
+        if whole and rng.random() < 0.8:
+            m.share(i, donor, 2 * rng.choice((1, whole, rng.randint(1, whole))))
+        m.append(i, rng.randint(1, 40))
+    names = rng.sample(range(30), rng.randint(2, 30))
+    common = lambda a, b: next((k for k, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b)))  # noqa: E731
+    tables = [m.block_table(n, 0) for n in names]
+    seen = set()
+    for ms, tokens in m.shared_groups(names):
+        assert len(ms) > 1 and not seen & set(ms)
+        seen |= set(ms)
+        assert tokens == 2 * min(common(tables[ms[0]], tables[i]) for i in ms[1:]) > 0
+    best = max(common(a, b) for i, a in enumerate(tables) for b in tables[:i])
+    assert bool(seen) == (best > 0)
+
+
+def test_nothing_is_looked_for_where_no_page_is_shared(monkeypatch):
+    from rvllm_b200.engine import StepEntry
+    from rvllm_b200.parts import KvCacheNeed
+    r = runner({0: KvCacheNeed(2, 128, None)}, torch.bfloat16)
+    looked = []
+    original = r.cache.shared_groups
+    monkeypatch.setattr(r.cache, "shared_groups", lambda reqs: (looked.append(tuple(reqs)), original(reqs))[1])
+    for i in range(3):
+        r.cache.admit(i); r.cache.append(i, 64)
+    entries = [StepEntry(i, [1], (0,)) for i in range(3)]
+    assert r._shared_groups(entries, [64] * 3) == [] and not looked
+    r.cache.admit(3); r.cache.share(3, 1, 64)
+    entries.append(StepEntry(3, [1], (0,)))
+    assert r._shared_groups(entries, [64] * 4) == [([1, 3], 64)] and looked == [(0, 1, 2, 3)]
+    r.cache.free(1)                                  # its pages have one holder again
+    assert r._shared_groups(entries[:1] + entries[2:], [64] * 3) == [] and len(looked) == 1
+
+
 def test_beginnings_within_one_another():
     """1,500 requests, each of which goes on from the one before: a chain as deep as the step is wide."""
     n = 1500
