@@ -83,8 +83,9 @@ class LLM:
 
     def capture_graphs(self, max_context: Optional[int] = None) -> int:
         """Capture the CUDA graphs of the decode steps now (every batch bucket, contexts up to
-        `max_context`, default max_model_len) instead of at the first step that needs each."""
-        return self.engine.runner.capture_decode_graphs(max_context)
+        `max_context`, default max_model_len; with `share_prefixes` also those of steps that read shared
+        beginnings once) instead of at the first step that needs each."""
+        return self.engine.runner.capture_decode_graphs(max_context, share_prefixes=self.config.share_prefixes)
 
     def _new_scheduler(self) -> Scheduler:
         ec = self.config

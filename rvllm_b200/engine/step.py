@@ -399,8 +399,7 @@ class ModelRunner:
             groups = sorted(self.cache.shared_groups(reqs[1]), key=lambda g: -(len(g[0]) - 1) * g[1])
             self._groups_of = (reqs, groups)
         groups = self._groups_of[1][:SHARED_MOST_GROUPS] if graph else self._groups_of[1]
-        few = graph and 1 < self._kv_heads and len(entries) * self._kv_heads < SHARED_GRAPH_MANY_PAIRS
-        self._least_saved = SHARED_GRAPH_MIN_BYTES if few else SHARED_MIN_BYTES
+        self._least_saved = self._graph_least(len(entries)) if graph else SHARED_MIN_BYTES
         return groups if groups and self._worth_sharing(groups, sum(starts) + len(starts)) else []
 
     def _worth_sharing(self, groups, keys: int) -> bool:
@@ -410,6 +409,18 @@ class ModelRunner:
         if self.cache.dtype == torch.float32:
             return max(t for _, t in groups) >= SHARED_MIN_TOKENS_F32 or saved * self._key_bytes >= SHARED_MIN_BYTES // 2
         return saved * self._key_bytes >= getattr(self, "_least_saved", SHARED_MIN_BYTES) + own * self._key_bytes // 2
+
+    def _may_share(self, num_seqs: int, context: int) -> bool:
+        """Whether a graph of so many sequences in contexts up to `context` ever reads shared beginnings once: in a step of all of them that
+        differ in their last tokens only."""
+        if not self._key_bytes or not self.cache.can_share or self._page_table is None or num_seqs < 2:
+            return False
+        self._least_saved = self._graph_least(num_seqs)
+        return self._worth_sharing([(list(range(num_seqs)), context - 1)], num_seqs * context)
+
+    def _graph_least(self, num_seqs: int) -> int:
+        few = 1 < self._kv_heads and num_seqs * self._kv_heads < SHARED_GRAPH_MANY_PAIRS
+        return SHARED_GRAPH_MIN_BYTES if few else SHARED_MIN_BYTES
 
     def _eager_shared(self, groups, num_seqs: int) -> StepPrefixes:
         last = self._eager_prefixes
@@ -618,10 +629,12 @@ class ModelRunner:
             self._graph_event.record()
         return host, dev, graph, out, launches, shared
 
-    def capture_decode_graphs(self, max_context: Optional[int] = None, batch_sizes: Optional[Sequence[int]] = None) -> int:
+    def capture_decode_graphs(self, max_context: Optional[int] = None, batch_sizes: Optional[Sequence[int]] = None,
+                              share_prefixes: bool = False) -> int:
         """Capture the decode graphs ahead of time, for every batch bucket (or the given ones) and
         every context bucket up to `max_context` (default: max_model_len), so that no step of a
-        running service pays for a capture.  A graph is captured on a batch of padding rows, which
+        running service pays for a capture.  With `share_prefixes` also those of steps that read shared
+        beginnings once, for every length of the keys behind them.  A graph is captured on a batch of padding rows, which
         write nothing, so live requests are not disturbed.  Returns the number of graphs captured."""
         if not self.graph_batch_sizes or self.device.type != "cuda" or not getattr(self.model, "graph_safe", True):
             return 0
@@ -644,6 +657,15 @@ class ModelRunner:
                     ctx = self.pack([], [], pad_to=bucket, buffers=self._graph_buffers(bucket), ctx_limit=ctx_limit)
                     self.model.compute_logits(self.model.forward(ctx, self.cache), ctx)
                     self._graphs[(bucket, ctx_limit, 0)] = self._capture(bucket, ctx_limit)
+                    made += 1
+                for own_limit in ctx_buckets if share_prefixes else ():
+                    if own_limit > ctx_limit or (bucket, ctx_limit, own_limit) in self._graphs or not self._may_share(bucket, ctx_limit):
+                        continue
+                    state = self._capture(bucket, ctx_limit, own_limit)
+                    if not state[-1].used:
+                        self._key_bytes = 0            # no layer reads beginnings once
+                        break
+                    self._graphs[(bucket, ctx_limit, own_limit)] = state
                     made += 1
         return made
 

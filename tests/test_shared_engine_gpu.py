@@ -153,6 +153,29 @@ def test_an_identifier_that_is_used_again(monkeypatch):
     assert float((logits[0] - logits[1]).abs().max()) <= 2e-4 * float(logits[1].abs().max())
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_graphs_made_ahead_serve_steps_that_share(dtype, monkeypatch):
+    """After `capture_graphs` no step of requests that share beginnings captures anything, at any length of what lies behind them."""
+    from rvllm_b200 import SamplingParams
+    llm = make(folder_for(SHAPED), dtype, num_blocks=600, max_model_len=1024, max_num_batched_tokens=1024)
+    made = llm.capture_graphs()
+    r = llm.engine.runner
+    keys = set(r._graphs)
+    assert made == len(keys) and (4, 768, 512) in keys and (4, 768, 768) in keys and (4, 768, 0) in keys and (1, 512, 512) not in keys
+    assert not any(own > ctx for _, ctx, own in keys) and llm.capture_graphs() == 0
+    calls = counted(llm, monkeypatch)
+    replayed = []
+    original = r._step_graph
+    monkeypatch.setattr(r, "_step_graph", lambda e, s, b, late=None: (replayed.append(r._shared_groups(e, s, graph=True)), original(e, s, b, late))[1])
+    a, _ = stems(515, seed=5)
+    long = (a * 12)[:700]
+    sp = SamplingParams(max_tokens=5, ignore_eos=True)
+    for prompts in ([a, a, a], [long, long[:690] + [1]], [a + long[:650], a + [3], long[::-1]]):
+        llm.generate(prompts, sp)
+    assert sum(bool(g) for g in replayed) >= 8 and set(r._graphs) == keys
+    assert not calls, "a step ran without its graph"
+
+
 @pytest.mark.parametrize("eager", [True, False])
 def test_layers_that_read_no_beginning_once_get_no_graphs_of_their_own(eager, monkeypatch):
     """Where no layer's attention asks for the groups of a step, later steps make none."""
