@@ -37,7 +37,11 @@ def _staged(host: np.ndarray, device) -> torch.Tensor:
     """The array in memory that a copy to `device` reads without making the host wait for the stream (which as a rule is at work on the
     step before).  Pinned memory from torch's host allocator, which does not hand it out again before the copy has been done."""
     t = torch.from_numpy(host)
-    return t.pin_memory() if torch.device(device).type == "cuda" else t
+    if torch.device(device).type != "cuda":
+        return t
+    if torch.cuda.is_current_stream_capturing():
+        raise KernelError("shared prefixes: groups are laid out and changed outside a capture (a replay would copy memory that is given back)")
+    return t.pin_memory()
 
 
 class SharedPrefixes:
@@ -81,8 +85,9 @@ class SharedPrefixes:
         return self._lay_out(groups, self.capacity)[:2]
 
     def write(self, laid_out) -> None:
-        host, (self.num_tiles, self.num_items) = laid_out
+        host, used = laid_out
         self.device_ints.copy_(_staged(host, self.device_ints.device), non_blocking=True)
+        self.num_tiles, self.num_items = used
 
     @staticmethod
     def ints(num_seqs: int, capacity: Tuple[int, int]) -> int:

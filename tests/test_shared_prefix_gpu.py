@@ -348,6 +348,23 @@ def test_groups_are_sent_while_the_device_is_busy():
     assert layout.own_start.tolist() == want[0][4:68].tolist()
 
 
+def test_groups_are_not_changed_inside_a_capture():
+    s = make([(12, 130)], 0, 16, 4, 128, 16, torch.bfloat16, seed=1, own=(1, 30))
+    shared, step = SharedPrefixes(s["plan"], 12, 16, 4, "cuda", capacity=(6, 80)), StepPrefixes(s["plan"], 12, "cuda", 4)
+    want = run(s, shared=shared).clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: shared.refill([]), lambda: SharedPrefixes(s["plan"], 12, 16, 4, "cuda"), lambda: step.layout(16, 4)):
+            with pytest.raises(KernelError, match="capture"):
+                call()
+        out = run(s, shared=shared)
+    graph.replay()
+    assert torch.equal(out, want)
+    shared.refill([([0, 1], 64)])                    # the refused calls left nothing behind
+    assert shared.own_start.tolist() == [64, 64] + [0] * 10 and step.layout(16, 4).own_start.tolist() == [130] * 12
+
+
 def test_on_another_stream_and_twice_at_once():
     a = make([(30, 600)], 2, 32, 8, 128, 16, torch.bfloat16, seed=11, own=(1, 100))
     b = make([(30, 333)], 2, 32, 8, 128, 16, torch.bfloat16, seed=12, own=(1, 100))
