@@ -10,7 +10,7 @@
 //   positions, token_seq, cu_seqlens, ctx_lens                   as the step's kernels read them.
 // A sequence without a row (-1) stands for no request: its context length is 0, its entries and slots are -1.
 //
-// One launch, no order between its CTAs: where a sequence's pages begin in the list, and its tokens in the step, are sums over
+// One launch for the tables, no order between its CTAs: where a sequence's pages begin in the list, and its tokens in the step, are sums over
 // the sequences before it, which every CTA forms for itself (integers: any order gives the same), and an entry that is new in
 // this step is read from the list, never from the row that another CTA may be writing.  A CTA takes 1, 2, 4 or 8 neighbouring
 // sequences of one group, with 256, 128, 64 or 32 threads each: one while the CTAs find room at once (four an SM), more where the
@@ -19,7 +19,7 @@
 // What bounds it is latency - a launch, the lengths, the sums, the entries, each behind the other - and from a few hundred sequences on
 // the sums, not the bytes.  GPU time in graphs with 1 / 2 / 4 / 8 sequences a CTA, us: 64 decoded tokens in contexts up to 32,767 (0.6 MB)
 // 4.5 / 6.5 / 8.7 / 14; 800 in contexts up to 8,000 7.2 / 5.7 / 6.7 / 8.7; 2,000 21 / 15.9 / 9.7 / 11.2; 1,024 in two groups with
-// portions (18 MB) 16.9 / 13.5 / 12.3 / 18.7, which is 1.5 TB/s.
+// portions (18 MB) 16.9 / 13.5 / 12.3 / 18.7, which is 1.5 TB/s.  The empty launch behind it (see there) takes 0.8 us more, and the host 2.7.
 #include "common.cuh"
 
 #define TABLE_THREADS 256

@@ -626,7 +626,8 @@ class CudaKernels:
             COUNTERS['launches'] += 1
             return out
         # own keys in pieces of 64 or more; the ranges of the prefixes, cut for the tensor cores, in as many parts of 64 keys as two CTAs
-        # an SM take (a tile of 64 keys takes a CTA 5 us; 16 sequences behind 777 keys, 28 heads on 4: 25.9 us in ranges of two, 21.1 of one)
+        # an SM take (a tile of 64 keys takes a CTA 5 us; 16 sequences behind 777 keys, 28 heads on 4: 25.9 us in ranges of two, 21.1 of one; a
+        # layout with a capacity, whose ranges in use the host does not know here, is not cut: 31.6)
         splits = max(1, min(64, -(-max_own // 64), 4 * self.num_sms // (B * num_kv_heads)))
         own_rows = splits * B * num_heads
         row_blocks = -(-shared.widest * group // 32)
