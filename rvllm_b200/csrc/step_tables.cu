@@ -152,7 +152,7 @@ RV_EXPORT int rv_step_tables(const TableArgs* a) {
     else if (per == 4) RV_LAUNCH_ST = rv_launch(step_tables_kernel<4>, grid, dim3(TABLE_THREADS), 0, a->stream, p);
     else RV_LAUNCH_ST = rv_launch(step_tables_kernel<8>, grid, dim3(TABLE_THREADS), 0, a->stream, p);
     const int st = rv_launch_status();
-    if (st != RV_OK || !a->settle || !g_rv_pdl) return st;
+    if (st != RV_OK || !a->settle) return st;            // (whether others are launched early is not for this library's switch to say)
     RV_LAUNCH_ST = rv_launch_alone(tables_settled_kernel, dim3(1), dim3(32), 0, a->stream);
     return rv_launch_status();
 }

@@ -716,7 +716,7 @@ class CudaKernels:
             page_table.data_ptr(), rows.data_ptr(), held.data_ptr(), starts.data_ptr(), q_lens.data_ptr(), new_pages.data_ptr(), spans.data_ptr(),
             out.block_tables.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.token_seq.data_ptr(),
             out.cu_seqlens.data_ptr(), out.ctx_lens.data_ptr(), G, B, R, width, new_pages.shape[0], num_tokens, max_blocks, page_size,
-            torch._C._cuda_getCurrentRawStream(here), settle))
+            torch._C._cuda_getCurrentRawStream(here), settle and self.pdl and self._pdl_allowed))
         _check("step_tables", st)
         return out
 

@@ -557,6 +557,28 @@ def test_step_tables_captured():
     assert out.ctx_lens.tolist() == [5, 4] and table[0].tolist()[1][:2] == [3, 6]
 
 
+def test_tables_are_settled_while_any_library_launches_early(monkeypatch):
+    """The switch of a single source file says how its own kernels are launched, not whether those behind the tables are launched early."""
+    import struct
+    k = lib()
+    k.set_pdl(True)
+    one = (torch.zeros((1, 2, 4), dtype=torch.int32, device="cuda"), i32([0]), i32([[0]]), i32([0]), i32([1]), i32([1]), i32([[0, 0]]), 1, 4, 16)
+    k.step_tables(*one)
+    seen, original = [], k._entries["tables"]
+    monkeypatch.setitem(k._entries, "tables", lambda block: (seen.append(struct.unpack_from("=i", block, 13 * 8 + 8 * 4 + 8)[0]), original(block))[1])
+    monkeypatch.setattr(k, "pdl", True)
+    for alone in ((), ("step_tables.cu",)):
+        monkeypatch.setattr(k, "no_pdl_for", alone)
+        k._lib("step_tables.cu").rv_set_pdl(0 if alone else 1)
+        k.step_tables(*one)
+        k.step_tables(*one, settle=False)
+    monkeypatch.setattr(k, "pdl", False)
+    k.step_tables(*one)
+    k._lib("step_tables.cu").rv_set_pdl(1)
+    torch.cuda.synchronize()
+    assert seen == [1, 0, 1, 0, 0]
+
+
 def test_attention_right_behind_the_tables():
     """Tables that change from call to call, read by the launch right behind, which starts early where the library launches it so."""
     s = make([], 40, 32, 8, 128, 16, torch.bfloat16, seed=3, own=(300, 900), stale="0")
