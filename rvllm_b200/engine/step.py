@@ -19,6 +19,7 @@ requests' pages that stays there; otherwise the host writes them out.
 """
 from __future__ import annotations
 
+import gc
 from dataclasses import dataclass, field
 from typing import Dict, Hashable, List, Optional, Sequence
 
@@ -617,9 +618,16 @@ class ModelRunner:
         torch.cuda.synchronize(self.device)
         graph = torch.cuda.CUDAGraph()
         before = COUNTERS["launches"]
-        with torch.cuda.graph(graph, pool=self._graph_pool):
-            hidden = self.model.forward(ctx, self.cache)
-            out = self.model.compute_logits(hidden, ctx)
+        # no garbage collection meanwhile: it may be that of an engine with graphs of its own, and destroying these ends the capture
+        collects = gc.isenabled()
+        gc.disable()
+        try:
+            with torch.cuda.graph(graph, pool=self._graph_pool):
+                hidden = self.model.forward(ctx, self.cache)
+                out = self.model.compute_logits(hidden, ctx)
+        finally:
+            if collects:
+                gc.enable()
         launches = COUNTERS["launches"] - before
         COUNTERS["launches"] = before          # captured, not run
         if self._graph_pool is None:

@@ -16,6 +16,14 @@ SHAPED = {"architectures": ["LlamaForCausalLM"], "hidden_size": 256, "num_hidden
 
 
 @pytest.fixture(autouse=True)
+def collected():
+    """Engines with their graphs are gone when a test ends, not in the middle of a later one's capture."""
+    import gc
+    yield
+    gc.collect()
+
+
+@pytest.fixture(autouse=True)
 def share_little(monkeypatch):
     from rvllm_b200.engine.step import ModelRunner
     monkeypatch.setattr(ModelRunner, "_worth_sharing", lambda self, groups, keys: True)
@@ -174,6 +182,23 @@ def test_graphs_made_ahead_serve_steps_that_share(dtype, monkeypatch):
         llm.generate(prompts, sp)
     assert sum(bool(g) for g in replayed) >= 8 and set(r._graphs) == keys
     assert not calls, "a step ran without its graph"
+
+
+def test_no_garbage_is_collected_during_a_capture(monkeypatch):
+    """That of an engine that is gone may hold graphs, whose end would end the capture (many are captured ahead for steps that share)."""
+    import gc
+    llm = make(folder_for(SHAPED), "float32", max_model_len=512)
+    model, seen = llm.engine.model, []
+    original = model.forward
+    monkeypatch.setattr(model, "forward", lambda *a: (seen.append((torch.cuda.is_current_stream_capturing(), gc.isenabled())), original(*a))[1])
+    for enabled in (True, False):
+        (gc.enable if enabled else gc.disable)()
+        try:
+            llm.engine.runner._graphs.clear()
+            assert llm.capture_graphs() > 0 and gc.isenabled() == enabled
+        finally:
+            gc.enable()
+    assert {c for c, _ in seen} == {True, False} and not any(c and g for c, g in seen)
 
 
 @pytest.mark.parametrize("eager", [True, False])
