@@ -608,6 +608,8 @@ class CudaKernels:
         out = torch.empty_like(q)
         sinks_at, gate_at = 0 if sinks is None else sinks.data_ptr(), 0 if gate is None else gate.data_ptr()
         stream, cap = torch._C._cuda_getCurrentRawStream(here), softcap or 0.0
+        if shared.written_on != stream:
+            shared.wait_for_write()
         if fast:
             # one buffer: the prefixes' sums, their maxima and denominators, and those of the own keys
             piece, pieces, own_ctas = self._own_pieces(B * num_kv_heads * -(-group // 8), max_own)

@@ -71,7 +71,9 @@ class SharedPrefixes:
         # the most ranges of a row tile, the fewest keys that any sequence has before its own begin (0: one has no prefix), key tiles of
         # a range, sequences of a row tile
         self.most_parts, self.shortest, self.longest, self.widest = sizes
+        self._event, self.written_on = None, None
         self.device_ints = _staged(host, device).to(device, non_blocking=True)
+        self._note_write()
 
     def refill(self, groups) -> None:
         """Other groups of the same step size, into the same array (on the current stream).  It takes a capacity given when the object
@@ -88,6 +90,21 @@ class SharedPrefixes:
         host, used = laid_out
         self.device_ints.copy_(_staged(host, self.device_ints.device), non_blocking=True)
         self.num_tiles, self.num_items = used
+        self._note_write()
+
+    def _note_write(self) -> None:
+        device = self.device_ints.device
+        if device.type == "cuda":
+            stream = torch.cuda.current_stream(device)
+            self._event = self._event or torch.cuda.Event()
+            self._event.record(stream)
+            self.written_on = stream.cuda_stream
+
+    def wait_for_write(self) -> None:
+        """For a call on another stream than the array was written on: the current stream waits for the copy, the host does not.  (A capture
+        cannot wait for what is outside it; `torch.cuda.graph` begins one when the device is idle.)"""
+        if self._event is not None and not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(self.device_ints.device).wait_event(self._event)
 
     @staticmethod
     def ints(num_seqs: int, capacity: Tuple[int, int]) -> int:

@@ -382,6 +382,28 @@ def test_on_another_stream_and_twice_at_once():
             assert torch.equal(g, w)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_a_layout_that_is_still_on_its_way_to_another_stream(dtype):
+    """Made, and changed, on a busy stream and used at once on another: the call waits for the copy on the device."""
+    s = make([(12, 130)], 1, 16, 4, 128, 16, dtype, seed=1, own=(1, 30))
+    exact = SharedPrefixes(s["plan"], 13, 16, 4, "cuda")
+    roomy = SharedPrefixes([], 13, 16, 4, "cuda", capacity=(6, 80))
+    roomy.refill(s["plan"])
+    want = [run(s, shared=exact).clone(), run(s, shared=roomy).clone()]
+    roomy.refill([])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    torch.cuda._sleep(100_000_000)                   # about a twentieth of a second
+    late = SharedPrefixes(s["plan"], 13, 16, 4, "cuda")
+    roomy.refill(s["plan"])
+    with torch.cuda.stream(side):
+        got = [run(s, shared=late), run(s, shared=roomy)]
+    torch.cuda.synchronize()
+    lib().raise_on_abort()
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+
+
 def test_refusals():
     s = make([(4, 50)], 1, 8, 2, 64, 16, torch.bfloat16, own=(1, 20))
     nh, nkv, hd = s["dims"]
